@@ -222,6 +222,62 @@ smoe_status smoe_ffn_run(const smoe_geom* g, const smoe_weights* w, const smoe_h
                          int32_t n_tokens, float* out, int32_t add_shared, void* workspace, size_t workspace_bytes,
                          const smoe_trace* trace, void* hip_stream);
 
+/* ---------------------------------------------------------------------------------------------- dense layers
+ * The dense operators of a layer round the block: the ends of a block on one residual stream, and the dense product.  No
+ * counterpart in the reference's MoE block.  Rows are of three types (GGUF's numbers); `ld` is the distance of two rows in
+ * values (ignored for one row; an input's may be 0: one row for every token). */
+enum { SMOE_F32 = 0, SMOE_F16 = 1, SMOE_BF16 = 30 };
+
+/* The norm after a block, its gate and the residual scales, and the norm before the next block.  Per token, on rows of
+ * n_embd values (rs(v) = 1 / sqrt(mean(v^2) + eps)):
+ *   z   = y, or with post (the norm after the block) y rs(y) post;
+ *   out = res_scale R + y_scale g z,  g = 1, or the gate's value, or (SMOE_GATE_SIGMOID) its sigmoid;
+ *   x   = out rs(out) pre,  from the f32 out (not its rounding to R's type); without pre, unit weight. */
+enum { SMOE_GATE_NONE = 0, SMOE_GATE_SIGMOID = 1 };
+typedef struct {
+    const float* pre;  /* [n_embd] weight of the norm before the next block, or NULL: 1 */
+    const float* post; /* [n_embd] weight of the norm after the block, or NULL: no such norm */
+    float eps;
+    float res_scale, y_scale;
+    int32_t gate_act;  /* SMOE_GATE_*: what the gate's values go through */
+} smoe_ends;
+
+/* One call does a block's end and the next one's start: R (r_type) and the block's output y (y_type) -> out (r_type), the
+ * new stream, and x (x_type), the next block's input.  y and out NULL: x = R rs(R) pre alone (the scales are not used);
+ * x NULL: out alone.  The gate's value of token t, channel d is gate[t gate_ld + d gate_step] (f32; NULL: none): one per
+ * channel with gate_ld 0, per token with gate_step 0.  out and x may each be R's or y's own rows (the same address, row
+ * stride and value size) and share no other byte with an input or each other.  n_embd 1 .. 16384; rows that start
+ * 16-byte aligned and n_embd % 8 == 0 take wide accesses.  Rows past n_tokens are left as they are. */
+smoe_status smoe_block_ends(const smoe_ends* e, int32_t n_embd, int32_t n_tokens, const void* R, int32_t r_type,
+                            int64_t r_ld, const void* y, int32_t y_type, int64_t y_ld, const float* gate, int64_t gate_ld,
+                            int64_t gate_step, void* out, int64_t out_ld, void* x, int32_t x_type, int64_t x_ld,
+                            void* hip_stream);
+
+/* The dense product with its epilogue: y = act(x w' + bias) [* (x w2' + bias2)] [+ residual], x [T][n_in] and the weights
+ * [n_out][n_in] both bf16 or both fp16, sums in f32, the activation in f32, one rounding to y's type.  GELU is the tanh
+ * form, RELU2 relu squared.  With w2 the activation's result is multiplied by the second product (SwiGLU: SMOE_ACT_SILU). */
+enum { SMOE_ACT_NONE = 0, SMOE_ACT_SILU = 1, SMOE_ACT_GELU = 2, SMOE_ACT_RELU = 3, SMOE_ACT_RELU2 = 4, SMOE_ACT_SIGMOID = 5 };
+typedef struct {
+    int32_t n_in;      /* a multiple of 8, at most 65536 */
+    int32_t n_out;     /* 1 .. 2^24 */
+    int32_t w_type;    /* SMOE_BF16 or SMOE_F16: x, w and w2 */
+    int32_t act;       /* SMOE_ACT_* */
+    const void* w;     /* [n_out][n_in], 16-byte aligned */
+    const void* w2;    /* the same, or NULL */
+    const float* bias; /* [n_out], or NULL */
+    const float* bias2;
+} smoe_linear;
+
+/* Workspace bytes of smoe_linear_run for up to max_tokens tokens (0 on a bad shape). */
+size_t smoe_linear_workspace_bytes(const smoe_linear* L, int32_t max_tokens);
+
+/* x 16-byte aligned, x_ld a multiple of 8 (at most 2^21); residual of y's type, NULL for none; y may be residual's own
+ * rows (the same address and row stride) and share no other byte with an input.  `workspace`: 256-byte aligned, read by no
+ * later call; concurrent calls need distinct ones.  Every result is the same bits in every run. */
+smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, int32_t n_tokens, const void* residual,
+                            int64_t r_ld, void* y, int32_t y_type, int64_t y_ld, void* workspace, size_t workspace_bytes,
+                            void* hip_stream);
+
 /* ---------------------------------------------------------------------------------------------- GGUF models */
 
 /* A model in GGUF v3 files, read on the host: every shard of a split model (`<stem>-NNNNN-of-MMMMM.gguf`, any
@@ -381,6 +437,24 @@ smoe_status smoe_router_topk(const float* logits, int32_t n_tokens, int32_t n_ex
  * 1 <= k < n_expert <= 1024. */
 smoe_status smoe_router_margin(const float* logits, int32_t n_tokens, int32_t n_expert, int32_t k, float* stats,
                                int32_t* ids, void* hip_stream);
+
+/* The load of the router over a batch: logits [T][n_expert] f32 (rows logits_ld apart), the experts ids [T][k] that were
+ * selected from them, and the tokens that count (mask [T], a byte each, nonzero: counts; NULL: all), n of them:
+ *   p = softmax(logits), lse = log sum exp(logits); counts[e] = pairs of such tokens with ids e; f_e = counts[e] / (n k);
+ *   mean_p[e] = mean p_e; balance = n_expert sum_e f_e mean_p[e]; z = mean lse^2;
+ *   loss = {balance_coef balance + z_coef z, balance, z, n}.
+ * With dlogits (rows dlogits_ld apart; may be logits) loss[0]'s gradient to the logits, the counts taken as constants:
+ *   dlogits_tj = (balance_coef n_expert p_tj (f_j - sum_e f_e p_te) + 2 z_coef lse_t p_tj) / n, 0 for other tokens,
+ * and with dbias [n_expert] its sum over the tokens (the gradient to smoe_weights' logit_bias).  A token repeated in ids
+ * counts each time, an id outside [0, n_expert) not at all.  No token counts (n = 0): every result is 0.  Logits of -inf
+ * have p = 0; a counted row of them alone has p = 0 and lse = 0; other tokens' values, NaN or not, reach nothing.
+ * n_expert 1 .. 1024, k 1 .. 64, at most 2^24 pairs; zero tokens launch nothing.  The same bits in every run.  No
+ * counterpart in the reference, which does not train. */
+size_t smoe_router_balance_workspace_bytes(int32_t max_tokens, int32_t n_expert);
+smoe_status smoe_router_balance(const float* logits, int64_t logits_ld, const int32_t* ids, const uint8_t* mask,
+                                int32_t n_tokens, int32_t n_expert, int32_t k, float balance_coef, float z_coef, float* loss,
+                                int32_t* counts, float* mean_p, float* dlogits, int64_t dlogits_ld, float* dbias,
+                                void* workspace, size_t workspace_bytes, void* hip_stream);
 
 /* x [n] f32 -> bf16 bits, round to nearest even, NaN quieted.
  * Replaces f32_to_bf16_bulk (metal/include/strata/metal/elementwise.hpp:27). */

@@ -53,6 +53,17 @@ class _Trace(C.Structure):
                                           "stage_events", "xq", "hq", "parts", "shared", "overflow", "egate", "eup",
                                           "sgu", "shq")]
 
+
+class _Ends(C.Structure):
+    _fields_ = [("pre", C.c_void_p), ("post", C.c_void_p), ("eps", C.c_float), ("res_scale", C.c_float),
+                ("y_scale", C.c_float), ("gate_act", C.c_int32)]
+
+
+class _Linear(C.Structure):
+    _fields_ = [("n_in", C.c_int32), ("n_out", C.c_int32), ("w_type", C.c_int32), ("act", C.c_int32), ("w", C.c_void_p),
+                ("w2", C.c_void_p), ("bias", C.c_void_p), ("bias2", C.c_void_p)]
+
+
 class _Hc(C.Structure):
     _fields_ = [("hc", C.c_int32), ("hc_lr", C.c_int32), ("eps", C.c_float), ("norm", C.c_void_p),
                 ("down", C.c_void_p), ("up", C.c_void_p), ("inject", C.c_void_p)]
@@ -90,6 +101,12 @@ def lib():
             "smoe_hc_write": (i32, [vp, i32, vp, vp, vp, i32, vp, vp]),
             "smoe_ffn_workspace_bytes": (C.c_size_t, [vp, vp, i32]),
             "smoe_ffn_run": (i32, [vp, vp, vp, vp, i32, vp, i32, vp, C.c_size_t, vp, vp]),
+            "smoe_block_ends": (i32, [vp, i32, i32, vp, i32, i64, vp, i32, i64, vp, i64, i64, vp, i64, vp, i32, i64, vp]),
+            "smoe_linear_workspace_bytes": (C.c_size_t, [vp, i32]),
+            "smoe_linear_run": (i32, [vp, vp, i64, i32, vp, i64, vp, i32, i64, vp, C.c_size_t, vp]),
+            "smoe_router_balance_workspace_bytes": (C.c_size_t, [i32, i32]),
+            "smoe_router_balance": (i32, [vp, i64, vp, vp, i32, i32, i32, f32, f32, vp, vp, vp, vp, i64, vp, vp, C.c_size_t,
+                                          vp]),
             "smoe_router_topk": (i32, [vp, i32, i32, i32, vp, vp, vp]),
             "smoe_router_margin": (i32, [vp, i32, i32, i32, vp, vp, vp]),
             "smoe_f32_to_bf16": (i32, [vp, i64, vp, vp]),
@@ -530,7 +547,255 @@ class FfnLayer:
     __call__ = run
 
 
+# ------------------------------------------------------------------------------------------------ dense layers
+
+F32, F16, BF16 = 0, 1, 30  # SMOE_F32, SMOE_F16, SMOE_BF16
+GATE_NONE, GATE_SIGMOID = 0, 1
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_RELU, ACT_RELU2, ACT_SIGMOID = range(6)
+
+
+_ELEM: Dict = {}
+
+
+def _elem_type(dtype) -> int:
+    """The SMOE_F32 / F16 / BF16 number of a torch dtype (int16: bf16 bits, as elsewhere in this module), or -1."""
+    if not _ELEM:
+        import torch
+        _ELEM.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int16: BF16})
+    return _ELEM.get(dtype, -1)
+
+
+def _rows(t, name: str, n: int, tokens: int = -1, device: int = -1):
+    """(type, row stride) of a (tokens, n) tensor on GPU `device` whose rows are contiguous, at any stride."""
+    import torch
+    if not isinstance(t, torch.Tensor):
+        raise SmoeError(-1, f"{name} is not a tensor")
+    code = _elem_type(t.dtype)
+    if code < 0:
+        raise SmoeError(-3, f"{name} is {t.dtype}, needs float32, float16 or bfloat16 (or int16: bf16 bits)")
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != n or (tokens >= 0 and shape[0] != tokens):
+        raise SmoeError(-2, f"{name} has shape {tuple(shape)}, needs ({'tokens' if tokens < 0 else tokens}, {n})")
+    ld, step = t.stride()
+    if step != 1 and n > 1:
+        raise SmoeError(-5, f"{name}'s rows are not contiguous")
+    _on_device(t, name, device)
+    return code, ld
+
+
+def _on_device(t, name: str, device: int = -1):
+    """Refuse a tensor that is on no GPU, or not on the call's."""
+    at = t.get_device()
+    if at < 0:
+        raise SmoeError(-1, f"{name} is on {t.device}, not a GPU")
+    if device >= 0 and at != device:
+        raise SmoeError(-1, f"{name} is on {t.device}, the call's other tensors on cuda:{device}")
+
+
+def _current(device: int, stream) -> Optional[int]:
+    """The current stream's handle, when a call on `device` runs on it; None: under _on, which makes them current."""
+    import torch
+    if stream is None and torch.cuda.current_device() == device:
+        return torch._C._cuda_getCurrentRawStream(device)
+    return None
+
+
+def _on(device: int, stream):
+    """The call's device, and its stream if one is given, current: its outputs and workspace are allocated for them."""
+    import torch
+    if stream is None:
+        return torch.cuda.device(device)
+    if stream.device_index != device:
+        raise SmoeError(-1, f"the stream is on cuda:{stream.device_index}, the call's tensors on cuda:{device}")
+    return torch.cuda.stream(stream)
+
+
+def _vector(t, name: str, n: int):
+    import torch
+    return t if t is None else _need(t, name, torch.float32, shape=(n,))
+
+
+class BlockEnds:
+    """The ends of a block on one residual stream (smoe_block_ends), where HyperConnection has them on several: the norm
+    after the block (weight `post`, None: no such norm), its gate, the residual scales, and the norm before the next block
+    (weight `pre`, None: 1).  Between two blocks `post` is the one's and `pre` the next one's.  The weights are f32 [n_embd]
+    tensors.  A call's rows are (tokens, n_embd) tensors of float32, float16 or bfloat16 with any row stride; the gate is
+    float32 and broadcasts to them (one per channel, per token, or both)."""
+
+    def __init__(self, n_embd: int, pre=None, post=None, res_scale: float = 1.0, y_scale: float = 1.0, eps: float = 1e-6,
+                 gate_act: int = GATE_NONE):
+        self.n_embd, self.pre, self.post = n_embd, _vector(pre, "pre", n_embd), _vector(post, "post", n_embd)
+        self._c = _Ends(_ptr(pre), _ptr(post), eps, res_scale, y_scale, gate_act)
+        self._ref = C.byref(self._c)
+
+    def _run(self, R, y, gate, out, x, x_dtype, form, stream):
+        import torch
+        n = self.n_embd
+        rt, r_ld = _rows(R, "R", n)
+        T, dev = R.shape[0], R.get_device()
+        st = _current(dev, stream)
+        if st is None:
+            with _on(dev, stream):
+                return self._run(R, y, gate, out, x, x_dtype, form, None)
+        for t, name in ((self.pre, "pre"), (self.post, "post")):
+            if t is not None:
+                _on_device(t, name, dev)
+        yt = y_ld = o_ld = xt = x_ld = g_ld = g_step = 0
+        yp = gp = op = xp = None
+        if y is not None:
+            yt, y_ld = _rows(y, "y", n, T, dev)
+            yp = y.data_ptr()
+            if out is None:
+                out = torch.empty((T, n), dtype=R.dtype, device=R.device)
+            ot, o_ld = _rows(out, "out", n, T, dev)
+            if ot != rt:
+                raise SmoeError(-1, f"out is {out.dtype}, needs {R.dtype}")
+            op = out.data_ptr()
+            if gate is not None:
+                if gate.dtype != torch.float32:
+                    raise SmoeError(-1, f"gate is {gate.dtype}, needs torch.float32")
+                _on_device(gate, "gate", dev)
+                try:
+                    g_ld, g_step = gate.expand(T, n).stride()
+                except RuntimeError:
+                    raise SmoeError(-2, f"gate has shape {tuple(gate.shape)}, does not broadcast to ({T}, {n})") from None
+                gp = gate.data_ptr()
+        if form:
+            if x is None:
+                x = torch.empty((T, n), dtype=x_dtype or R.dtype, device=R.device)
+            xt, x_ld = _rows(x, "x", n, T, dev)
+            xp = x.data_ptr()
+        _check(lib().smoe_block_ends(self._ref, n, T, R.data_ptr(), rt, r_ld, yp, yt, y_ld, gp, g_ld, g_step, op, o_ld, xp,
+                                     xt, x_ld, st))
+        return out, x
+
+    def read(self, R, x=None, x_dtype=None, stream=None):
+        """x = R rs(R) pre, a block's input from the stream (x_dtype None: R's)."""
+        return self._run(R, None, None, None, x, x_dtype, True, stream)[1]
+
+    def write(self, R, y, gate=None, out=None, stream=None):
+        """out = res_scale R + y_scale g z, the block's output back onto the stream; `out` may be R."""
+        return self._run(R, _given(y, "y"), gate, out, None, None, False, stream)[0]
+
+    def join(self, R, y, gate=None, out=None, x=None, x_dtype=None, stream=None):
+        """write, then read of the new stream (in f32, before its rounding), in one pass: (out, x)."""
+        return self._run(R, _given(y, "y"), gate, out, x, x_dtype, True, stream)
+
+
+def _given(t, name: str):
+    if t is None:
+        raise SmoeError(-6, f"{name} is None")
+    return t
+
+
+class Linear:
+    """The dense product with its epilogue (smoe_linear_run): y = act(x w' + bias) [* (x w2' + bias2)] [+ residual].
+    `w` and `w2` are (n_out, n_in) tensors of bfloat16 (or int16: bf16 bits) or float16, the biases f32 [n_out].  The
+    weights stay the caller's tensors."""
+
+    def __init__(self, n_in: int, n_out: int, w, bias=None, w2=None, bias2=None, act: int = ACT_NONE):
+        for t, name in ((w, "w"), (w2, "w2")):
+            if t is not None:
+                _need(t, name, w.dtype)
+                if t.numel() != n_in * n_out:
+                    raise SmoeError(-2, f"{name} has {t.numel()} elements, needs {n_out} x {n_in}")
+                _on_device(t, name, w.get_device())
+        self.n_in, self.n_out, self.dtype = n_in, n_out, w.dtype
+        self.tensors = (w, w2, _vector(bias, "bias", n_out), _vector(bias2, "bias2", n_out))
+        for t, name in ((bias, "bias"), (bias2, "bias2")):
+            if t is not None:
+                _on_device(t, name, w.get_device())
+        self._type = _elem_type(w.dtype)
+        self._c = _Linear(n_in, n_out, self._type, act, w.data_ptr(), _ptr(w2), _ptr(bias), _ptr(bias2))
+        self._ref = C.byref(self._c)
+        self._sizes: Dict = {}
+        if lib().smoe_linear_workspace_bytes(self._ref, 0) == 0:
+            raise SmoeError(-1, lib().smoe_last_error().decode())
+
+    def workspace_bytes(self, max_tokens: int) -> int:
+        return int(lib().smoe_linear_workspace_bytes(self._ref, max_tokens))
+
+    def _bytes(self, T: int) -> int:
+        """workspace_bytes, kept per batch size."""
+        n = self._sizes.get(T)
+        if n is None:
+            n = self._sizes[T] = self.workspace_bytes(T) if T > 0 else 0
+        return n
+
+    def run(self, x, residual=None, y=None, y_dtype=None, stream=None):
+        """y (tokens, n_out) of `y_dtype` (None: residual's, else x's); `y` may be residual."""
+        import torch
+        w, N = self.tensors[0], self.n_out
+        dev = w.get_device()
+        xt, x_ld = _rows(x, "x", self.n_in, -1, dev)
+        if xt != self._type:
+            raise SmoeError(-1, f"x is {x.dtype}, the weights {self.dtype}")
+        st = _current(dev, stream)
+        if st is None:
+            with _on(dev, stream):
+                return self.run(x, residual, y, y_dtype)
+        T = x.shape[0]
+        rp, rt, r_ld = None, -1, 0
+        if residual is not None:
+            rt, r_ld = _rows(residual, "residual", N, T, dev)
+            rp = residual.data_ptr()
+        if y is None:
+            y = torch.empty((T, N), dtype=y_dtype or (x if residual is None else residual).dtype, device=x.device)
+        yt, y_ld = _rows(y, "y", N, T, dev)
+        if rt >= 0 and rt != yt:
+            raise SmoeError(-1, f"residual is {residual.dtype}, y {y.dtype}")
+        # a workspace of the call's own: calls on several streams, captured or not, share none
+        n = self._bytes(T)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n > 256 else None
+        _check(lib().smoe_linear_run(self._ref, x.data_ptr(), x_ld, T, rp, r_ld, y.data_ptr(), yt, y_ld, _ptr(ws), n, st))
+        return y
+
+    __call__ = run
+
+
 # ------------------------------------------------------------------------------------------------ stages
+
+def router_balance(logits, ids, mask=None, balance_coef: float = 1.0, z_coef: float = 0.0, grad: bool = False, stream=None):
+    """The router's load over a batch (smoe_router_balance): a dict of loss [4] = (balance_coef balance + z_coef z, balance,
+    z, tokens counted), counts [E] (int32) and mean_p [E]; with `grad` also dlogits [T][E] and dbias [E], the gradients of
+    loss[0] to the logits and to a bias added to them.  logits (T, E) f32 with any row stride, ids (T, k) int32 as
+    router_topk selects them, mask (T,) bool or uint8: the tokens that count."""
+    import torch
+    if logits.dim() != 2:
+        raise SmoeError(-1, "logits must be (tokens, experts)")
+    T, E = logits.shape
+    if logits.dtype != torch.float32:
+        raise SmoeError(-1, f"logits is {logits.dtype}, needs torch.float32")
+    _, ld = _rows(logits, "logits", E)
+    dev = logits.get_device()
+    st = _current(dev, stream)
+    if st is None:
+        with _on(dev, stream):
+            return router_balance(logits, ids, mask, balance_coef, z_coef, grad)
+    _need(ids, "ids", torch.int32)
+    _on_device(ids, "ids", dev)
+    if ids.dim() != 2 or ids.shape[0] != T:
+        raise SmoeError(-2, f"ids has shape {tuple(ids.shape)}, needs ({T}, k)")
+    if mask is not None:
+        _need(mask, "mask", torch.uint8 if mask.dtype == torch.uint8 else torch.bool, shape=(T,))
+        _on_device(mask, "mask", dev)
+    new = torch.zeros if T == 0 else torch.empty
+    # loss, mean_p and dbias are views of one allocation
+    f = new(4 + (2 if grad else 1) * E, dtype=torch.float32, device=logits.device)
+    out = dict(loss=f[:4], counts=new(E, dtype=torch.int32, device=logits.device), mean_p=f[4:4 + E])
+    dp = bp = None
+    if grad:
+        out["dlogits"], out["dbias"] = new((T, E), dtype=torch.float32, device=logits.device), f[4 + E:]
+        dp, bp = out["dlogits"].data_ptr(), out["dbias"].data_ptr()
+    n = lib().smoe_router_balance_workspace_bytes(T, E)
+    if n == 0 and T > 0:
+        raise SmoeError(-1, lib().smoe_last_error().decode())
+    ws = torch.empty(n, dtype=torch.uint8, device=logits.device)
+    base = f.data_ptr()
+    _check(lib().smoe_router_balance(logits.data_ptr(), ld, ids.data_ptr(), _ptr(mask), T, E, ids.shape[1], balance_coef,
+                                     z_coef, base, out["counts"].data_ptr(), base + 16, dp, E, bp, ws.data_ptr(), n, st))
+    return out
+
 
 def router_topk(logits, k: int, stream=None):
     import torch

@@ -41,7 +41,8 @@ COMMON = [
 ]
 
 SOURCES = ["smoe_decode.hip", "smoe_prefill.hip", "smoe_iq2.hip", "smoe_iq2_mm.hip", "smoe_hc.hip", "smoe_native.hip",
-           "smoe_cache.hip", "smoe_synth.hip", "smoe_api.cpp", "smoe_gguf.cpp"]
+           "smoe_cache.hip", "smoe_ends.hip", "smoe_linear.hip", "smoe_balance.hip", "smoe_synth.hip", "smoe_api.cpp",
+           "smoe_dense.cpp", "smoe_gguf.cpp"]
 
 
 def _compile(src: str) -> str:
@@ -60,7 +61,7 @@ def _compile(src: str) -> str:
 # on it (and on a sanitized build of the test checker) under the clang sanitizer runtime.  Never loaded by the
 # product path.
 LIB_ASAN = os.path.join(LIBDIR, "libsmoe_asan.so")
-HOST_SOURCES = ["smoe_api.cpp", "smoe_gguf.cpp"]
+HOST_SOURCES = ["smoe_api.cpp", "smoe_dense.cpp", "smoe_gguf.cpp"]
 SANITIZE = [f for opt in ("-fsanitize=address", "-fsanitize=undefined", "-fno-sanitize-recover=undefined",
                           "-fno-omit-frame-pointer") for f in ("-Xarch_host", opt)]
 

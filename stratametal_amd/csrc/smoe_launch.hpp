@@ -192,6 +192,47 @@ hipError_t launch_grouped_prep(const uint8_t* xq, int64_t n_blocks, int natural,
                                const int32_t* counts, int cap_groups, int cap_entries, int n_tok, int n_rows,
                                int4* items, int32_t* etok, int32_t* edst, hipStream_t s);
 
+// the ends of a block on one residual stream (smoe_ends.hip); rows of any stride, types of smoe_types.hpp; y NULL: out is R,
+// not written; x NULL: not formed
+struct EndsArgs {
+    const void *R, *y;
+    void *out, *x;
+    const float *gate, *post, *pre;
+    int64_t r_ld, y_ld, out_ld, x_ld, gate_ld, gate_step;
+    int r_type, y_type, x_type, gate_sigmoid;
+    int n, n_tokens;
+    float eps, res_scale, y_scale;
+};
+hipError_t launch_block_ends(const EndsArgs& a, hipStream_t s);
+
+// the dense product (smoe_linear.hip): y = act(x w' + bias) [* (x w2' + bias2)] [+ residual]; part: the K slices' sums
+struct LinearArgs {
+    const void *x, *w, *w2, *residual;
+    const float *bias, *bias2;
+    void* y;
+    float* part;
+    int64_t x_ld, r_ld, y_ld;
+    int n_in, n_out, n_tokens;
+    int w_type, y_type, act;
+};
+size_t linear_part_bytes(int64_t n_tokens, int n_in, int n_out, bool pair);
+hipError_t launch_linear(const LinearArgs& a, hipStream_t s);
+
+// the router's balance loss (smoe_balance.hip); dlogits and dbias may be NULL
+struct BalanceArgs {
+    const float* logits;
+    const int32_t* ids;
+    const uint8_t* mask;
+    float *loss, *mean_p, *dlogits, *dbias;
+    int32_t* counts;
+    int64_t ld, ld_d;
+    int n_tokens, n_expert, k;
+    float balance_coef, z_coef;
+    void* work;
+};
+size_t balance_work_bytes(int64_t n_tokens, int n_expert);
+hipError_t launch_balance(const BalanceArgs& a, hipStream_t s);
+
 hipError_t launch_synth_blocks(int type, uint64_t seed, uint64_t stream_id, int64_t n_blocks, float sigma, uint8_t* out,
                                hipStream_t s);
 hipError_t launch_synth_bf16(uint64_t seed, uint64_t stream_id, int64_t n, float sigma, uint16_t* out, hipStream_t s);

@@ -25,6 +25,7 @@
 // C[4 q + r][j] in register r: a lane holds four consecutive rows of one column, which the epilogues store as one
 // piece (measured: down 82 -> 72 us at the benchmark's prefill 512, whose stores had been one dword per row).
 #include "smoe_device.hpp"
+#include "smoe_dma.hpp"
 #include "smoe_gemv.hpp"
 #include "smoe_items.hpp"
 #include "smoe_launch.hpp"
@@ -187,7 +188,6 @@ constexpr int kWgRows = 256;
 // the stores of the one before run (a down K loop is only n_ff / 128 units).
 constexpr int kDownRbw = 2;
 constexpr int kWaves = 8;
-constexpr uint32_t kOob = 0x80000000u;
 constexpr int kRing = 148480;           // bytes of the stage ring
 constexpr int kDummy = kRing;           // 1 KB landing slot of the padding instructions
 constexpr int kLds = kRing + 1024;
@@ -244,25 +244,6 @@ struct Shape {
     static_assert(kStages - 2 <= 6, "wait_stages cases");
 };
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
-
-// Raw buffer resource over [base, base + bytes) (no swizzle, no stride; out-of-range lanes read nothing).
-__device__ __forceinline__ i32x4 buffer_rsrc(const void* base, uint32_t bytes) {
-    const uint64_t b = reinterpret_cast<uint64_t>(base);
-    return i32x4{(int)(uint32_t)b, (int)(uint32_t)(b >> 32), (int)bytes, 0x00020000};
-}
-__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const lds_u8*)p; }
-// M0 is written one instruction before the load that reads it (one wait state for LDS DMA).
-__device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, i32x4 rsrc, uint32_t soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff),
-                 "s"(rsrc), "s"(soff)
-                 : "memory", "m0");
-}
-template <int N>
-__device__ __forceinline__ void vmcnt() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 // Wait until this wave's loads of all but the `after` newest stages are done.
 template <int SLOTS>
 __device__ __forceinline__ void wait_stages(int after) {

@@ -159,4 +159,26 @@ constexpr bool junction_apart(int64_t T, int E, int H, bool f32) {
                        T * E >= (H >= 2560 ? 2048 : H >= 2048 ? 4096 : 8192));
 }
 
+// The ends of a block: waves to a row, and slots of eight values to a lane.
+struct EndsShape {
+    int waves, slots;
+};
+constexpr int kEndsMaxRow = 16384;
+constexpr EndsShape ends_shape(int64_t T, int n) {
+    return n <= 512 ? EndsShape{1, 1} : n <= 2048 ? EndsShape{4, 1} : n <= 4096 ? EndsShape{4, 2}
+           : n <= 8192 ? EndsShape{4, 4} : EndsShape{16, 2};
+}
+constexpr int64_t ends_groups(int64_t T, int n) { return ends_shape(T, n).waves == 1 ? (T + 3) / 4 : T; }
+
+// The router's balance loss: work-groups of four rows at a time, and of the counts.
+constexpr int64_t balance_groups(int64_t T) { return T < 4 ? 1 : (T + 3) / 4 < 512 ? (T + 3) / 4 : 512; }
+constexpr int64_t balance_count_groups(int64_t T) { return T < 2048 ? 1 : T / 1024 < 16 ? T / 1024 : 16; }
+
+// The dense product: a row of x or w, rows of w, and the distance of x's rows (a tile of 256 rows stays within 31-bit
+// offsets).
+constexpr int kLinearMaxIn = 65536, kLinearMaxOut = 1 << 24;
+constexpr int64_t kLinearMaxLd = (int64_t)1 << 21;
+constexpr int64_t kLinearSplitTokens = 0;
+constexpr bool linear_grid_fits(int64_t T, int64_t N, bool pair) { return (T + 63) / 64 <= 65535; }
+
 }  // namespace smoe

@@ -1,0 +1,65 @@
+// stratametal_amd/csrc/smoe_types.hpp - rows of f32, fp16 or bf16 values for the dense operators round the block: the
+// element types, eight values to and from registers, and the exponential their activations take.
+#pragma once
+
+#include "smoe_device.hpp"
+
+namespace smoe {
+
+// smoe.h's SMOE_F32, SMOE_F16, SMOE_BF16 (GGUF's type numbers)
+enum ElemType : int { kF32 = 0, kF16 = 1, kBf16 = 30 };
+__host__ __device__ constexpr int elem_bytes(int type) { return type == kF32 ? 4 : 2; }
+
+// One value to and from f32; the conversion instructions round to nearest even, as the hardware's fp16 does.
+__device__ __forceinline__ float elem_to_f32(uint32_t bits, int type) {
+    return type == kF32 ? u2f(bits)
+                        : type == kBf16 ? bf16_to_f32(bits) : (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+__device__ __forceinline__ uint16_t f32_to_half_bits(float v, int type) {
+    return type == kBf16 ? (uint16_t)f32_to_bf16(v) : __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b, int type) {
+    return (uint32_t)f32_to_half_bits(a, type) | (uint32_t)f32_to_half_bits(b, type) << 16;
+}
+
+// Eight consecutive values as loaded: 32 bytes of f32, or 16 of a 16-bit type (the first half).
+struct Raw8 {
+    uint4 a, b;
+};
+__device__ __forceinline__ float raw8_value(const Raw8& r, int j, int type) {  // j constant after unrolling
+    const uint32_t q[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    if (type == kF32) return u2f(q[j]);
+    return elem_to_f32(j & 1 ? q[j >> 1] >> 16 : q[j >> 1] & 0xFFFFu, type);
+}
+
+// Eight values to `p` (16-byte aligned).
+__device__ __forceinline__ void store8(void* p, const float (&v)[8], int type) {
+    uint4* o = reinterpret_cast<uint4*>(p);
+    if (type == kF32) {
+        o[0] = make_uint4(f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3]));
+        o[1] = make_uint4(f2u(v[4]), f2u(v[5]), f2u(v[6]), f2u(v[7]));
+    } else {
+        o[0] = make_uint4(pack_half2(v[0], v[1], type), pack_half2(v[2], v[3], type), pack_half2(v[4], v[5], type),
+                          pack_half2(v[6], v[7], type));
+    }
+}
+__device__ __forceinline__ void store1(void* p, int64_t i, float v, int type) {
+    if (type == kF32) static_cast<float*>(p)[i] = v;
+    else static_cast<uint16_t*>(p)[i] = f32_to_half_bits(v, type);
+}
+
+// e^x = 2^t, t = x log2 e with the product's rounding error and log2 e's low part carried as a first-order factor
+// 1 + ln2 * rest, so that the error stays at the hardware exponential's own rounding for every |x| (t alone would be off
+// by |x| 2^-24).  x past the range gives 0 or inf.
+__device__ __forceinline__ float exp_fast(float x) {
+    constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596300e-8f;
+    const float xc = __builtin_fminf(__builtin_fmaxf(x, -150.0f), 150.0f);  // (the rest of an infinite product is NaN)
+    const float t = xc * kLog2e;
+    const float rest = __builtin_fmaf(xc, kLog2eLow, __builtin_fmaf(xc, kLog2e, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    const float r = __builtin_fmaf(e, rest * 0.693147181f, e);
+    return e == __builtin_inff() ? e : x != x ? x : r;
+}
+__device__ __forceinline__ float sigmoid_fast(float x) { return 1.0f / (1.0f + exp_fast(-x)); }
+
+}  // namespace smoe
