@@ -98,8 +98,6 @@ smoe_status smoe_block_ends(const smoe_ends* e, int32_t n_embd, int32_t n_tokens
             return fail(SMOE_EINVAL, "block_ends: an output overlaps the gate or a norm's weight");
     }
     if (overlap(so, sx)) return fail(SMOE_EINVAL, "block_ends: out and x overlap");
-    if (smoe::ends_groups(n_tokens, n_embd) >= smoe::kGridGroups)
-        return fail(SMOE_EINVAL, "block_ends: the tokens exceed a launch's grid: split them");
     smoe::EndsArgs a{};
     a.R = R, a.y = y, a.out = out, a.x = x;
     a.gate = gate, a.post = y ? e->post : nullptr, a.pre = x ? e->pre : nullptr;

@@ -10,56 +10,64 @@
 
 namespace smoe {
 
+enum { kEndsNoGate = 0, kEndsGateOnce = 1, kEndsGateRow = 2 };  // a gate for every row, or a row's own
+
 namespace {
 
-// A row's values in a lane's slots, as loaded.  VEC: slot m is the 8 values of chunk l + L m (L lanes to a row); else
-// value j of slot m is element l + L (8 m + j).  Those past the row hold its last ones (every load is in bounds).
+// A row's values in a lane's slots of four, as loaded.  VEC: slot m is the 4 values of chunk l + L m (L lanes to a row: a
+// load or store of the wave is one run of bytes for every type); else value j of slot m is element l + L (4 m + j).  Those
+// past the row hold its last ones (every load is in bounds).
 template <bool VEC>
 __device__ __forceinline__ int slot_at(int l, int L, int m, int j) {
-    return VEC ? 8 * (l + L * m) + j : l + L * (8 * m + j);
+    return VEC ? 4 * (l + L * m) + j : l + L * (4 * m + j);
 }
 template <bool VEC, int L, int NV>
-__device__ __forceinline__ void load_row(const void* p, int type, int n, int l, Raw8 (&raw)[NV]) {
-    if constexpr (VEC) {
-        const int last = (n >> 3) - 1;
-        if (type == kF32) {
+__device__ __forceinline__ void load_row(const void* p, int type, int n, int l, uint4 (&raw)[NV]) {
+    if (type == kF32) {
 #pragma unroll
-            for (int m = 0; m < NV; ++m) {
-                const uint4* q = static_cast<const uint4*>(p) + 2 * min(l + L * m, last);
-                raw[m].a = q[0];
-                raw[m].b = q[1];
+        for (int m = 0; m < NV; ++m) {
+            if constexpr (VEC) {
+                raw[m] = static_cast<const uint4*>(p)[min(l + L * m, (n >> 2) - 1)];
+            } else {
+                const uint32_t* q = static_cast<const uint32_t*>(p);
+                raw[m] = make_uint4(q[min(l + L * (4 * m), n - 1)], q[min(l + L * (4 * m + 1), n - 1)],
+                                    q[min(l + L * (4 * m + 2), n - 1)], q[min(l + L * (4 * m + 3), n - 1)]);
             }
-        } else {
-#pragma unroll
-            for (int m = 0; m < NV; ++m) raw[m].a = static_cast<const uint4*>(p)[min(l + L * m, last)];
         }
     } else {
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
-            uint32_t v[8];
-            if (type == kF32) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = static_cast<const uint32_t*>(p)[min(slot_at<false>(l, L, m, j), n - 1)];
-                raw[m].a = make_uint4(v[0], v[1], v[2], v[3]);
-                raw[m].b = make_uint4(v[4], v[5], v[6], v[7]);
+            if constexpr (VEC) {
+                const uint2 q = static_cast<const uint2*>(p)[min(l + L * m, (n >> 2) - 1)];
+                raw[m].x = q.x, raw[m].y = q.y;
             } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = static_cast<const uint16_t*>(p)[min(slot_at<false>(l, L, m, j), n - 1)];
-                raw[m].a = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+                const uint16_t* q = static_cast<const uint16_t*>(p);
+                raw[m] = make_uint4(q[min(l + L * (4 * m), n - 1)], q[min(l + L * (4 * m + 1), n - 1)],
+                                    q[min(l + L * (4 * m + 2), n - 1)], q[min(l + L * (4 * m + 3), n - 1)]);
             }
         }
     }
 }
+template <bool VEC, int NV>
+__device__ __forceinline__ void row_values(const uint4 (&raw)[NV], int type, float (&v)[NV][4]) {
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+        const uint32_t q[4] = {raw[m].x, raw[m].y, raw[m].z, raw[m].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[m][j] = type == kF32 ? u2f(q[j]) : elem_to_f32(!VEC ? q[j] : j & 1 ? q[j >> 1] >> 16 : q[j >> 1] & 0xFFFFu, type);
+    }
+}
 template <bool VEC, int L, int NV>
-__device__ __forceinline__ void store_row(void* p, int type, int n, int l, const float (&v)[NV][8]) {
+__device__ __forceinline__ void store_row(void* p, int type, int n, int l, const float (&v)[NV][4]) {
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
         if constexpr (VEC) {
             const int c = l + L * m;
-            if (8 * c < n) store8(static_cast<uint8_t*>(p) + (size_t)c * (8 * elem_bytes(type)), v[m], type);
+            if (4 * c < n) store4(static_cast<uint8_t*>(p) + (size_t)c * (4 * elem_bytes(type)), v[m], type);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 const int d = slot_at<false>(l, L, m, j);
                 if (d < n) store1(p, d, v[m][j], type);
             }
@@ -83,14 +91,14 @@ __device__ __forceinline__ float row_sum(float v, float* s) {
 
 // 1 / sqrt(mean v^2 + eps) of a row.  The squares are summed in f32: a row whose mean square leaves f32's safe range is
 // summed again with its values scaled by 2^-80 or 2^80 (one branch for the row: its lanes all hold the same q).
-// s: 2 WAVES floats of LDS, used once.
+// s: 2 WAVES floats of LDS, used once between two other barriers.
 template <int WAVES, bool VEC, int L, int NV>
-__device__ __forceinline__ float row_scale(const float (&v)[NV][8], int n, int l, float eps, float* s) {
+__device__ __forceinline__ float row_scale(const float (&v)[NV][4], int n, int l, float eps, float* s) {
     float acc = 0.0f;
 #pragma unroll
     for (int m = 0; m < NV; ++m)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 4; ++j)
             if (slot_at<VEC>(l, L, m, j) < n) acc = __builtin_fmaf(v[m][j], v[m][j], acc);
     const float q = row_sum<WAVES>(acc, s) / (float)n + eps;
     if (!(q > 0x1p120f || q < 0x1p-100f)) return 1.0f / __builtin_sqrtf(q);
@@ -99,90 +107,144 @@ __device__ __forceinline__ float row_scale(const float (&v)[NV][8], int n, int l
 #pragma unroll
     for (int m = 0; m < NV; ++m)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 4; ++j)
             if (slot_at<VEC>(l, L, m, j) < n) acc = __builtin_fmaf(v[m][j] * f, v[m][j] * f, acc);
     return f / __builtin_sqrtf(row_sum<WAVES>(acc, s + WAVES) / (float)n + eps * f * f);
 }
 
 }  // namespace
 
-// WAVES waves to a row of up to 512 WAVES NV values: four rows to a work-group of one-wave rows, else one.
-template <int WAVES, int NV, bool VEC>
+// WAVES waves to a row of up to 256 WAVES NV values: four rows at a time to a work-group of one-wave rows, else one.  A
+// work-group takes every gridDim.x-th set of rows; the next row's values are loaded before this one's are worked on, and
+// what no row changes (y_scale post g of a gate per channel, and pre) stays in registers.
+template <int WAVES, int NV, bool VEC, int GATE>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_block_ends(const EndsArgs a) {
     constexpr int L = 64 * WAVES, ROWS = WAVES == 1 ? 4 : 1;
-    __shared__ float sum_s[4 * WAVES];
+    constexpr bool AHEAD = NV < 4;  // (four slots and the next row's do not fit the 128 registers of 16 waves)
+    __shared__ float sum_s[2][4 * WAVES];  // (two rows' in turn: a wave may be one row ahead of another's last read)
     const int l = threadIdx.x % L, n = a.n;
-    const int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / L;
-    if (t >= a.n_tokens) return;  // (one-wave rows only, and they meet no barrier)
     const bool write = a.y != nullptr;
-    Raw8 rr[NV], yr[NV];
-    load_row<VEC, L, NV>(static_cast<const uint8_t*>(a.R) + t * a.r_ld * elem_bytes(a.r_type), a.r_type, n, l, rr);
-    if (write) load_row<VEC, L, NV>(static_cast<const uint8_t*>(a.y) + t * a.y_ld * elem_bytes(a.y_type), a.y_type, n, l, yr);
-    float v[NV][8];
-    if (!write) {
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / L;
+    if (t >= a.n_tokens) return;  // (one-wave rows only, and they meet no barrier)
+    uint4 rr[NV], yr[NV], gr[NV];
+    const auto load = [&](int64_t row) {
+        row = row < a.n_tokens ? row : a.n_tokens - 1;
+        load_row<VEC, L, NV>(static_cast<const uint8_t*>(a.R) + row * a.r_ld * elem_bytes(a.r_type), a.r_type, n, l, rr);
+        if (write) load_row<VEC, L, NV>(static_cast<const uint8_t*>(a.y) + row * a.y_ld * elem_bytes(a.y_type), a.y_type, n, l, yr);
+    };
+    const auto load_gate = [&](int64_t row) {  // of a row: strided or one value
+        row = row < a.n_tokens ? row : a.n_tokens - 1;
+        const float* g = a.gate + row * a.gate_ld;
+        if (VEC && a.gate_vec) {
+            load_row<VEC, L, NV>(g, kF32, n, l, gr);
+        } else {
 #pragma unroll
-        for (int m = 0; m < NV; ++m)
+            for (int m = 0; m < NV; ++m) {
+                float w[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[m][j] = raw8_value(rr[m], j, a.r_type);
-    } else {
-        float z[NV][8];
-#pragma unroll
-        for (int m = 0; m < NV; ++m)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[m][j] = raw8_value(yr[m], j, a.y_type);
-        if (a.post) {
-            const float rs = row_scale<WAVES, VEC, L, NV>(z, n, l, a.eps, sum_s);
-#pragma unroll
-            for (int m = 0; m < NV; ++m)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) z[m][j] = (z[m][j] * rs) * a.post[min(slot_at<VEC>(l, L, m, j), n - 1)];
-        }
-        if (a.gate) {
-            const float* g = a.gate + t * a.gate_ld;
-#pragma unroll
-            for (int m = 0; m < NV; ++m)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float w = g[min(slot_at<VEC>(l, L, m, j), n - 1) * a.gate_step];
-                    z[m][j] = z[m][j] * (a.gate_sigmoid ? sigmoid_fast(w) : w);
-                }
-        }
-#pragma unroll
-        for (int m = 0; m < NV; ++m)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                v[m][j] = __builtin_fmaf(a.y_scale, z[m][j], a.res_scale * raw8_value(rr[m], j, a.r_type));
-        store_row<VEC, L, NV>(static_cast<uint8_t*>(a.out) + t * a.out_ld * elem_bytes(a.r_type), a.r_type, n, l, v);
-    }
-    if (a.x) {
-        const float rs = row_scale<WAVES, VEC, L, NV>(v, n, l, a.eps, sum_s + 2 * WAVES);
-#pragma unroll
-        for (int m = 0; m < NV; ++m)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[m][j] = v[m][j] * rs;
-                if (a.pre) v[m][j] = v[m][j] * a.pre[min(slot_at<VEC>(l, L, m, j), n - 1)];
+                for (int j = 0; j < 4; ++j) w[j] = g[min(slot_at<VEC>(l, L, m, j), n - 1) * a.gate_step];
+                gr[m] = make_uint4(f2u(w[0]), f2u(w[1]), f2u(w[2]), f2u(w[3]));
             }
-        store_row<VEC, L, NV>(static_cast<uint8_t*>(a.x) + t * a.x_ld * elem_bytes(a.x_type), a.x_type, n, l, v);
+        }
+    };
+    uint4 cr[NV], pr[NV];
+    load(t);
+    if constexpr (GATE != kEndsNoGate) load_gate(t);
+    if (a.post) load_row<VEC, L, NV>(a.post, kF32, n, l, cr);
+    if (a.pre) load_row<VEC, L, NV>(a.pre, kF32, n, l, pr);
+    float c[NV][4], w[NV][4];
+#pragma unroll
+    for (int m = 0; m < NV; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[m][j] = w[m][j] = 1.0f;
+    if (a.post) row_values<VEC, NV>(cr, kF32, c);
+    if (a.pre) row_values<VEC, NV>(pr, kF32, w);
+#pragma unroll
+    for (int m = 0; m < NV; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[m][j] = a.y_scale * c[m][j];
+    const auto gated = [&](float (&v)[NV][4]) {
+        float g[NV][4];
+        row_values<VEC, NV>(gr, kF32, g);
+#pragma unroll
+        for (int m = 0; m < NV; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[m][j] = v[m][j] * (a.gate_sigmoid ? sigmoid_fast(g[m][j]) : g[m][j]);
+    };
+    if constexpr (GATE == kEndsGateOnce) gated(c);
+    for (int it = 0; t < a.n_tokens; t += step, ++it) {
+        float* s = sum_s[it & 1];
+        if (!AHEAD && it > 0) {
+            load(t);
+            if constexpr (GATE == kEndsGateRow) load_gate(t);
+        }
+        float v[NV][4], z[NV][4];
+        row_values<VEC, NV>(rr, a.r_type, v);
+        if (write) row_values<VEC, NV>(yr, a.y_type, z);
+        if constexpr (GATE == kEndsGateRow) {
+            float g[NV][4];
+#pragma unroll
+            for (int m = 0; m < NV; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) g[m][j] = c[m][j];
+            gated(g);
+            if (AHEAD && t + step < a.n_tokens) {
+                load(t + step);
+                load_gate(t + step);
+            }
+            const float rs = a.post ? row_scale<WAVES, VEC, L, NV>(z, n, l, a.eps, s) : 1.0f;
+#pragma unroll
+            for (int m = 0; m < NV; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[m][j] = __builtin_fmaf(z[m][j] * rs, g[m][j], a.res_scale * v[m][j]);
+        } else {
+            if (AHEAD && t + step < a.n_tokens) load(t + step);
+            if (write) {
+                const float rs = a.post ? row_scale<WAVES, VEC, L, NV>(z, n, l, a.eps, s) : 1.0f;
+#pragma unroll
+                for (int m = 0; m < NV; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[m][j] = __builtin_fmaf(z[m][j] * rs, c[m][j], a.res_scale * v[m][j]);
+            }
+        }
+        if (write)
+            store_row<VEC, L, NV>(static_cast<uint8_t*>(a.out) + t * a.out_ld * elem_bytes(a.r_type), a.r_type, n, l, v);
+        if (a.x) {
+            const float rs = row_scale<WAVES, VEC, L, NV>(v, n, l, a.eps, s + 2 * WAVES);
+#pragma unroll
+            for (int m = 0; m < NV; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[m][j] = (v[m][j] * rs) * w[m][j];
+            store_row<VEC, L, NV>(static_cast<uint8_t*>(a.x) + t * a.x_ld * elem_bytes(a.x_type), a.x_type, n, l, v);
+        }
     }
 }
 
-hipError_t launch_block_ends(const EndsArgs& a, hipStream_t s) {
-    const auto al = [](const void* p, int64_t ld, int type) {
-        return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * elem_bytes(type))) & 15) == 0;
+hipError_t launch_block_ends(const EndsArgs& args, hipStream_t s) {
+    EndsArgs a = args;
+    const auto al = [](const void* p, int64_t ld, int type) {  // rows of 4-value vectors
+        return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * elem_bytes(type))) & (4 * elem_bytes(type) - 1)) == 0;
     };
-    const bool vec = a.n % 8 == 0 && al(a.R, a.r_ld, a.r_type) && al(a.y, a.y_ld, a.y_type) &&
+    const bool vec = a.n % 4 == 0 && al(a.R, a.r_ld, a.r_type) && al(a.y, a.y_ld, a.y_type) &&
                      al(a.out, a.out_ld, a.r_type) && al(a.x, a.x_ld, a.x_type) && al(a.post, 0, kF32) && al(a.pre, 0, kF32);
+    a.gate_vec = a.gate_step == 1 && al(a.gate, a.gate_ld, kF32);
+    const int mode = !a.gate ? kEndsNoGate : a.gate_ld == 0 ? kEndsGateOnce : kEndsGateRow;
     const EndsShape sh = ends_shape(a.n_tokens, a.n);
     const dim3 grid((unsigned)ends_groups(a.n_tokens, a.n)), block(sh.waves == 1 ? 256 : 64 * sh.waves);
-#define SMOE_ENDS(W, V)                                                                    \
-    if (sh.waves == W && sh.slots == V) {                                                  \
-        if (vec) hipLaunchKernelGGL((k_block_ends<W, V, true>), grid, block, 0, s, a);     \
-        else hipLaunchKernelGGL((k_block_ends<W, V, false>), grid, block, 0, s, a);        \
-        return hipGetLastError();                                                          \
+#define SMOE_ENDS_K(W, V, G)                                                               \
+    if (vec) hipLaunchKernelGGL((k_block_ends<W, V, true, G>), grid, block, 0, s, a);      \
+    else hipLaunchKernelGGL((k_block_ends<W, V, false, G>), grid, block, 0, s, a)
+#define SMOE_ENDS(W, V)                                          \
+    if (sh.waves == W && sh.slots == V) {                        \
+        if (mode == kEndsNoGate) { SMOE_ENDS_K(W, V, 0); }       \
+        else if (mode == kEndsGateOnce) { SMOE_ENDS_K(W, V, 1); }\
+        else { SMOE_ENDS_K(W, V, 2); }                           \
+        return hipGetLastError();                                \
     }
-    SMOE_ENDS(1, 1) SMOE_ENDS(1, 2) SMOE_ENDS(1, 4) SMOE_ENDS(4, 1) SMOE_ENDS(4, 2) SMOE_ENDS(4, 4) SMOE_ENDS(16, 2)
+    SMOE_ENDS(1, 1) SMOE_ENDS(1, 2) SMOE_ENDS(4, 1) SMOE_ENDS(4, 2) SMOE_ENDS(8, 2) SMOE_ENDS(16, 2) SMOE_ENDS(16, 4)
 #undef SMOE_ENDS
+#undef SMOE_ENDS_K
     return hipErrorInvalidValue;
 }
 

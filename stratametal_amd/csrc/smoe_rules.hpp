@@ -159,20 +159,28 @@ constexpr bool junction_apart(int64_t T, int E, int H, bool f32) {
                        T * E >= (H >= 2560 ? 2048 : H >= 2048 ? 4096 : 8192));
 }
 
-// The ends of a block: waves to a row, and slots of eight values to a lane.
+// The ends of a block: waves to a row, and slots of four values to a lane.
 struct EndsShape {
     int waves, slots;
 };
 constexpr int kEndsMaxRow = 16384;
 constexpr EndsShape ends_shape(int64_t T, int n) {
-    return n <= 512 ? EndsShape{1, 1} : n <= 2048 ? EndsShape{4, 1} : n <= 4096 ? EndsShape{4, 2}
-           : n <= 8192 ? EndsShape{4, 4} : EndsShape{16, 2};
+    return n <= 256 ? EndsShape{1, 1} : n <= 512 ? EndsShape{1, 2} : n <= 1024 ? EndsShape{4, 1} : n <= 2048 ? EndsShape{4, 2}
+           : n <= 4096 ? EndsShape{8, 2} : n <= 8192 ? EndsShape{16, 2} : EndsShape{16, 4};
 }
-constexpr int64_t ends_groups(int64_t T, int n) { return ends_shape(T, n).waves == 1 ? (T + 3) / 4 : T; }
+// Work-groups: as many as the chip holds at a time (16 waves to a CU), each taking rows in turn.
+constexpr int64_t ends_groups(int64_t T, int n) {
+    const int w = ends_shape(T, n).waves;
+    const int64_t sets = w == 1 ? (T + 3) / 4 : T, most = 256 * (16 / (w == 1 ? 4 : w));
+    return sets < most ? sets : most;
+}
 
-// The router's balance loss: work-groups of four rows at a time, and of the counts.
-constexpr int64_t balance_groups(int64_t T) { return T < 4 ? 1 : (T + 3) / 4 < 512 ? (T + 3) / 4 : 512; }
-constexpr int64_t balance_count_groups(int64_t T) { return T < 2048 ? 1 : T / 1024 < 16 ? T / 1024 : 16; }
+// The router's balance loss: one work-group for a few tokens; the ids counted by every work-group or, from many on,
+// first; at most 1024 work-groups of rows (k_balance_sums).
+constexpr bool balance_one(int64_t T, int k) { return T <= 64 && T * k <= 4096; }
+constexpr bool balance_counts_apart(int64_t T, int k) { return T * k > 16384; }
+constexpr int64_t balance_groups(int64_t T) { return T < 4 ? 1 : (T + 3) / 4 < 1024 ? (T + 3) / 4 : 1024; }
+constexpr int64_t balance_count_groups(int64_t T) { return T < 512 ? 1 : T / 256 < 16 ? T / 256 : 16; }
 
 // The dense product: a row of x or w, rows of w, and the distance of x's rows (a tile of 256 rows stays within 31-bit
 // offsets).

@@ -22,26 +22,10 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b, int type) {
     return (uint32_t)f32_to_half_bits(a, type) | (uint32_t)f32_to_half_bits(b, type) << 16;
 }
 
-// Eight consecutive values as loaded: 32 bytes of f32, or 16 of a 16-bit type (the first half).
-struct Raw8 {
-    uint4 a, b;
-};
-__device__ __forceinline__ float raw8_value(const Raw8& r, int j, int type) {  // j constant after unrolling
-    const uint32_t q[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
-    if (type == kF32) return u2f(q[j]);
-    return elem_to_f32(j & 1 ? q[j >> 1] >> 16 : q[j >> 1] & 0xFFFFu, type);
-}
-
-// Eight values to `p` (16-byte aligned).
-__device__ __forceinline__ void store8(void* p, const float (&v)[8], int type) {
-    uint4* o = reinterpret_cast<uint4*>(p);
-    if (type == kF32) {
-        o[0] = make_uint4(f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3]));
-        o[1] = make_uint4(f2u(v[4]), f2u(v[5]), f2u(v[6]), f2u(v[7]));
-    } else {
-        o[0] = make_uint4(pack_half2(v[0], v[1], type), pack_half2(v[2], v[3], type), pack_half2(v[4], v[5], type),
-                          pack_half2(v[6], v[7], type));
-    }
+// Four values to `p` (aligned to them).
+__device__ __forceinline__ void store4(void* p, const float (&v)[4], int type) {
+    if (type == kF32) *static_cast<uint4*>(p) = make_uint4(f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3]));
+    else *static_cast<uint2*>(p) = make_uint2(pack_half2(v[0], v[1], type), pack_half2(v[2], v[3], type));
 }
 __device__ __forceinline__ void store1(void* p, int64_t i, float v, int type) {
     if (type == kF32) static_cast<float*>(p)[i] = v;
