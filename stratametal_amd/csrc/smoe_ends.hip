@@ -22,40 +22,39 @@ __device__ __forceinline__ int slot_at(int l, int L, int m, int j) {
     return VEC ? 4 * (l + L * m) + j : l + L * (4 * m + j);
 }
 template <bool VEC, int L, int NV>
-__device__ __forceinline__ void load_row(const void* p, int type, int n, int l, uint4 (&raw)[NV]) {
+__device__ __forceinline__ void load_row(const void* p, int type, int n, int l, u32x4 (&raw)[NV]) {
     if (type == kF32) {
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
             if constexpr (VEC) {
-                raw[m] = static_cast<const uint4*>(p)[min(l + L * m, (n >> 2) - 1)];
+                raw[m] = static_cast<const u32x4*>(p)[min(l + L * m, (n >> 2) - 1)];
             } else {
                 const uint32_t* q = static_cast<const uint32_t*>(p);
-                raw[m] = make_uint4(q[min(l + L * (4 * m), n - 1)], q[min(l + L * (4 * m + 1), n - 1)],
-                                    q[min(l + L * (4 * m + 2), n - 1)], q[min(l + L * (4 * m + 3), n - 1)]);
+                raw[m] = u32x4{q[min(l + L * (4 * m), n - 1)], q[min(l + L * (4 * m + 1), n - 1)],
+                               q[min(l + L * (4 * m + 2), n - 1)], q[min(l + L * (4 * m + 3), n - 1)]};
             }
         }
     } else {
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
             if constexpr (VEC) {
-                const uint2 q = static_cast<const uint2*>(p)[min(l + L * m, (n >> 2) - 1)];
-                raw[m].x = q.x, raw[m].y = q.y;
+                raw[m].xy = static_cast<const u32x2*>(p)[min(l + L * m, (n >> 2) - 1)];
             } else {
                 const uint16_t* q = static_cast<const uint16_t*>(p);
-                raw[m] = make_uint4(q[min(l + L * (4 * m), n - 1)], q[min(l + L * (4 * m + 1), n - 1)],
-                                    q[min(l + L * (4 * m + 2), n - 1)], q[min(l + L * (4 * m + 3), n - 1)]);
+                raw[m] = u32x4{q[min(l + L * (4 * m), n - 1)], q[min(l + L * (4 * m + 1), n - 1)],
+                               q[min(l + L * (4 * m + 2), n - 1)], q[min(l + L * (4 * m + 3), n - 1)]};
             }
         }
     }
 }
 template <bool VEC, int NV>
-__device__ __forceinline__ void row_values(const uint4 (&raw)[NV], int type, float (&v)[NV][4]) {
+__device__ __forceinline__ void row_values(const u32x4 (&raw)[NV], int type, float (&v)[NV][4]) {
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
-        const uint32_t q[4] = {raw[m].x, raw[m].y, raw[m].z, raw[m].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            v[m][j] = type == kF32 ? u2f(q[j]) : elem_to_f32(!VEC ? q[j] : j & 1 ? q[j >> 1] >> 16 : q[j >> 1] & 0xFFFFu, type);
+            v[m][j] = type == kF32 ? u2f(raw[m][j])
+                                   : elem_to_f32(!VEC ? raw[m][j] : j & 1 ? raw[m][j >> 1] >> 16 : raw[m][j >> 1] & 0xFFFFu, type);
     }
 }
 template <bool VEC, int L, int NV>
@@ -127,7 +126,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_block_ends(co
     const int64_t step = (int64_t)gridDim.x * ROWS;
     int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / L;
     if (t >= a.n_tokens) return;  // (one-wave rows only, and they meet no barrier)
-    uint4 rr[NV], yr[NV], gr[NV];
+    u32x4 rr[NV], yr[NV], gr[NV];
     const auto load = [&](int64_t row) {
         row = row < a.n_tokens ? row : a.n_tokens - 1;
         load_row<VEC, L, NV>(static_cast<const uint8_t*>(a.R) + row * a.r_ld * elem_bytes(a.r_type), a.r_type, n, l, rr);
@@ -144,11 +143,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_block_ends(co
                 float w[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = g[min(slot_at<VEC>(l, L, m, j), n - 1) * a.gate_step];
-                gr[m] = make_uint4(f2u(w[0]), f2u(w[1]), f2u(w[2]), f2u(w[3]));
+                gr[m] = u32x4{f2u(w[0]), f2u(w[1]), f2u(w[2]), f2u(w[3])};
             }
         }
     };
-    uint4 cr[NV], pr[NV];
+    u32x4 cr[NV], pr[NV];
     load(t);
     if constexpr (GATE != kEndsNoGate) load_gate(t);
     if (a.post) load_row<VEC, L, NV>(a.post, kF32, n, l, cr);

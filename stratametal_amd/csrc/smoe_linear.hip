@@ -26,16 +26,39 @@ __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
                                                        0);
 }
 
+// 1 / (1 + e^-x), the quotient by the hardware's reciprocal (1 ulp).  e^-x = 2^t, t = -x log2 e: t's rounding is at most
+// |x| 2^-24 of e^-x, so as much of a small sigmoid(x), and of a large one its part e^-x of that.
+__device__ __forceinline__ float act_sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f));
+}
 // smoe.h's SMOE_ACT_*
 __device__ __forceinline__ float activate(float a, int act) {
     switch (act) {
-        case 1: return a * sigmoid_fast(a);
+        case 1: return a * act_sigmoid(a);
         // 0.5 a (1 + tanh u) = a sigmoid(2 u), u = sqrt(2 / pi) (a + 0.044715 a^3)
-        case 2: return a * sigmoid_fast(1.59576912f * a * __builtin_fmaf(0.044715f * a, a, 1.0f));
+        case 2: return a * act_sigmoid(1.59576912f * a * __builtin_fmaf(0.044715f * a, a, 1.0f));
         case 3: return a > 0.0f || a != a ? a : 0.0f;
         case 4: return a > 0.0f || a != a ? a * a : 0.0f;
-        case 5: return sigmoid_fast(a);
+        case 5: return act_sigmoid(a);
         default: return a;
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void activate_all(float (&v)[N][4], int act) {
+    const auto each = [&](auto which) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[k][j] = activate(v[k][j], decltype(which)::value);
+    };
+    switch (act) {
+        case 1: each(std::integral_constant<int, 1>{}); break;
+        case 2: each(std::integral_constant<int, 2>{}); break;
+        case 3: each(std::integral_constant<int, 3>{}); break;
+        case 4: each(std::integral_constant<int, 4>{}); break;
+        case 5: each(std::integral_constant<int, 5>{}); break;
+        default: break;
     }
 }
 
@@ -80,6 +103,54 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, bool vec, int64_t t
         for (int i = 0; i < 4; ++i)
             if (o + i < a.n_out) store1(y, i, v[i], a.y_type);
     }
+}
+
+// The same for tokens t, t + PER, ... (those below t_end) of one lane's outputs, all of them there, rows of vectors; b and c
+// are their biases.
+template <int BATCH, int PER, bool PAIR>
+__device__ __forceinline__ void finish_batch(const LinearArgs& a, int64_t t, int64_t t_end, int o, const float (&b)[4],
+                                             const float (&c)[4], const f32x4 (&g)[BATCH], const f32x4 (&u)[BATCH]) {
+    const bool f32 = a.y_type == kF32;
+    u32x4 r[BATCH];
+    if (a.residual && f32) {
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+            r[k] = *reinterpret_cast<const u32x4*>(static_cast<const float*>(a.residual) + min(t + k * PER, t_end - 1) * a.r_ld + o);
+    } else if (a.residual) {
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+            r[k].xy = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.residual) + min(t + k * PER, t_end - 1) * a.r_ld + o);
+    }
+    float v[BATCH][4];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[k][j] = g[k][j] + b[j];
+    activate_all(v, a.act);
+    if constexpr (PAIR) {
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[k][j] = v[k][j] * (u[k][j] + c[j]);
+    }
+    if (a.residual) {
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[k][j] += f32 ? u2f(r[k][j]) : elem_to_f32(j & 1 ? r[k][j >> 1] >> 16 : r[k][j >> 1] & 0xFFFFu, a.y_type);
+        }
+    }
+    const auto put = [&](auto type) {
+        constexpr int E = decltype(type)::value;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+            if (t + k * PER < t_end)
+                store4(static_cast<uint8_t*>(a.y) + ((t + k * PER) * a.y_ld + o) * elem_bytes(E), v[k], E);
+    };
+    if (f32) put(std::integral_constant<int, kF32>{});
+    else if (a.y_type == kBf16) put(std::integral_constant<int, kBf16>{});
+    else put(std::integral_constant<int, kF16>{});
 }
 
 // y and residual rows take 4-value vectors.
@@ -132,34 +203,18 @@ __device__ __forceinline__ void tile_of(int i, int n, int tiles_o, int tiles_t, 
     o = in / rows;
 }
 
-// A tile of BM = 16 MT WM weight rows by BN = 16 NT WN tokens per work-group of WM WN waves, MT x NT fragments of 16 x 16
-// to a wave; K in steps of 64 through a ring of STAGES LDS buffers, filled by loads that write LDS directly.  A row's step is
-// eight 16-byte pieces, piece c of row r at place c ^ (r & 7), so that the 16 rows of a fragment's read spread over the
-// banks.  PAIR: the tile's 16-row sets are w's and w2's in turn, so that a lane holds both sums of its outputs.
-// blockIdx.y: a slice of K, whose sums go to `part` ([slice][w, w2][token][n_out]) for k_linear_join.
-template <int MT, int NT, int WM, int WN, int STAGES, bool PAIR, bool F16>
-__global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a, int tiles_o, int tiles_t) {
-    constexpr int WAVES = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
-    constexpr int OUTS = PAIR ? BM / 2 : BM;           // outputs of the tile
-    constexpr int WS = BM / 8 / WAVES, XS = BN / 8 / WAVES, SLOTS = WS + XS;  // a wave's loads of a step, 8 rows each
-    constexpr int STEP = (BM + BN) * 128;              // bytes of a step
-    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole loads");
-    static_assert(!PAIR || (MT % 2 == 0 && WAVES % 4 == 0), "sets in pairs, a wave's loads all of one matrix");
-    static_assert(STAGES >= 2 && STAGES <= 4, "wait_steps");
-    __shared__ __align__(1024) uint8_t lds[STAGES * STEP];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN;
-    int to, tt;
-    tile_of(blockIdx.x, gridDim.x, tiles_o, tiles_t, to, tt);
-    const int o0 = to * OUTS, t0 = tt * BN;
-    const int n_o = min(OUTS, a.n_out - o0), n_t = min(BN, a.n_tokens - t0);
+// A wave's loads of a step: load i brings rows 8 (i WAVES + wave) .. + 7 of the tile's weights (i < BM / 8 / WAVES, buffer
+// rw), then of its tokens (rx), lane l piece (l & 7) ^ (l >> 3) of row l >> 3, from byte off[i] on at K = 0 (past the buffer
+// for a row past the matrix).  PAIR: the tile's 16-row sets are w's and w2's in turn, and a wave's loads all of one of them.
+template <int BM, int BN, int WAVES, bool PAIR, int SLOTS>
+__device__ __forceinline__ void tile_loads(const LinearArgs& a, int o0, int t0, int n_o, int n_t, int wave, int lane, i32x4& rw,
+                                           i32x4& rx, uint32_t (&off)[SLOTS]) {
+    constexpr int WS = BM / 8 / WAVES;
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && SLOTS == WS + BN / 8 / WAVES, "whole loads");
+    static_assert(!PAIR || WAVES % 4 == 0, "a wave's loads all of one matrix");
     const uint32_t wrow = 2u * a.n_in;
-    // load i of the wave: rows 8 (i WAVES + wave) .. + 7 of the weights, then of the tokens; lane: row l >> 3, place l & 7
-    const void* wm_at = PAIR && (wave & 2) ? a.w2 : a.w;
-    const i32x4 rw = uniform_rsrc(static_cast<const uint8_t*>(wm_at) + (size_t)o0 * wrow, n_o * wrow);
-    const i32x4 rx = uniform_rsrc(static_cast<const uint8_t*>(a.x) + (size_t)t0 * a.x_ld * 2,
-                                  (uint32_t)((n_t - 1) * a.x_ld * 2) + wrow);
-    uint32_t off[SLOTS];
+    rw = uniform_rsrc(static_cast<const uint8_t*>(PAIR && (wave & 2) ? a.w2 : a.w) + (size_t)o0 * wrow, n_o * wrow);
+    rx = uniform_rsrc(static_cast<const uint8_t*>(a.x) + (size_t)t0 * a.x_ld * 2, (uint32_t)((n_t - 1) * a.x_ld * 2) + wrow);
     const int piece = (lane & 7) ^ (lane >> 3);
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
@@ -168,6 +223,90 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a
         if (i < WS) off[i] = o < n_o ? o * wrow + 16u * piece : kOob;
         else off[i] = row < n_t ? (uint32_t)(row * a.x_ld * 2) + 16u * piece : kOob;
     }
+}
+
+// A wave's MT x NT fragments of sums, outputs from o0 and tokens from t0 (those below t_end) on, through the epilogue, NG
+// sets of 16 tokens at a time through the wave's own piece of LDS, so that a token's outputs lie in consecutive lanes: a
+// lane's outputs are the same four of every token it takes, its bias is loaded once, and the residual's loads and the
+// stores of BATCH tokens go together (one at a time the epilogue of a 256 x 256 tile took 36 us).
+template <int MT>
+constexpr int kStoreRow = 64 * MT + 16;  // bytes of a token's sums, and 16 that spread the tokens over the banks
+template <int MT, int NG>
+constexpr int kStoreBytes = 16 * NG * kStoreRow<MT>;
+template <int MT, int NT, int NG, bool PAIR>
+__device__ __forceinline__ void tile_store(const LinearArgs& a, const f32x4 (&acc)[MT][NT], uint8_t* mine, int o0, int t0,
+                                           int t_end, int lane) {
+    constexpr int ROW = kStoreRow<MT>;
+    constexpr int QUADS = 4 * MT / (PAIR ? 2 : 1);  // quads of outputs of a token
+    constexpr int PER = 64 / QUADS;                 // tokens of an access
+    constexpr int BATCH = 16 * NG / PER < 8 ? 16 * NG / PER : 8;
+    static_assert(!PAIR || MT % 2 == 0, "sets in pairs");
+    static_assert(NT % NG == 0 && 64 % QUADS == 0 && 16 * NG / PER % BATCH == 0, "whole batches");
+    const int q = lane % QUADS, o = o0 + 4 * q;
+    const bool vec = rows_vec(a) && o + 4 <= a.n_out && gridDim.y == 1;
+    float b[4], c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int oc = min(o + j, a.n_out - 1);
+        b[j] = a.bias ? a.bias[oc] : 0.0f;
+        c[j] = PAIR && a.bias2 ? a.bias2[oc] : 0.0f;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n += NG) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                *reinterpret_cast<f32x4*>(mine + (16 * i + (lane & 15)) * ROW + m * 64 + (lane >> 4) * 16) = acc[m][n + i];
+        const uint8_t* at = mine + (lane / QUADS) * ROW + (PAIR ? (q >> 2) * 128 + (q & 3) * 16 : q * 16);
+        const int t1 = t0 + n * 16 + lane / QUADS;
+        if (vec) {
+#pragma unroll 1
+            for (int i = 0; i < 16 * NG / PER; i += BATCH) {
+                f32x4 g[BATCH], u[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    g[k] = *reinterpret_cast<const f32x4*>(at + (i + k) * PER * ROW);
+                    u[k] = PAIR ? *reinterpret_cast<const f32x4*>(at + (i + k) * PER * ROW + 64) : g[k];
+                }
+                finish_batch<BATCH, PER, PAIR>(a, t1 + i * PER, t_end, o, b, c, g, u);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < 16 * NG / PER; ++i) {
+                const f32x4 g = *reinterpret_cast<const f32x4*>(at + i * PER * ROW);
+                const f32x4 u = *reinterpret_cast<const f32x4*>(at + i * PER * ROW + (PAIR ? 64 : 0));
+                const int t = t1 + i * PER;
+                if (t >= t_end || o >= a.n_out) continue;
+                if (gridDim.y > 1) put_part<PAIR>(a, blockIdx.y, t, o, g, u);
+                else finish4<PAIR>(a, false, t, o, {g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]});
+            }
+        }
+    }
+}
+
+// A tile of BM = 16 MT WM weight rows by BN = 16 NT WN tokens per work-group of WM WN waves, MT x NT fragments of 16 x 16
+// to a wave; K in steps of 64 through a ring of STAGES LDS buffers, filled by loads that write LDS directly.  A row's step is
+// eight 16-byte pieces, piece c of row r at place c ^ (r & 7), so that the 16 rows of a fragment's read spread over the
+// banks.  blockIdx.y: a slice of K, whose sums go to `part` ([slice][w, w2][token][n_out]) for k_linear_join.
+template <int MT, int NT, int WM, int WN, int STAGES, bool PAIR, bool F16>
+__global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a, int tiles_o, int tiles_t) {
+    constexpr int WAVES = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
+    constexpr int OUTS = PAIR ? BM / 2 : BM;           // outputs of the tile
+    constexpr int WS = BM / 8 / WAVES, XS = BN / 8 / WAVES, SLOTS = WS + XS;  // a wave's loads of a step, 8 rows each
+    constexpr int STEP = (BM + BN) * 128;              // bytes of a step
+    static_assert(STAGES >= 2 && STAGES <= 4, "wait_steps");
+    __shared__ __align__(1024) uint8_t lds[STAGES * STEP];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    int to, tt;
+    tile_of(blockIdx.x, gridDim.x, tiles_o, tiles_t, to, tt);
+    const int o0 = to * OUTS, t0 = tt * BN;
+    const int n_o = min(OUTS, a.n_out - o0), n_t = min(BN, a.n_tokens - t0);
+    i32x4 rw, rx;
+    uint32_t off[SLOTS];
+    tile_loads<BM, BN, WAVES, PAIR>(a, o0, t0, n_o, n_t, wave, lane, rw, rx, off);
+    const int piece = (lane & 7) ^ (lane >> 3);
     const int all = (a.n_in + 63) / 64;
     const int u0 = (int)((int64_t)all * blockIdx.y / gridDim.y), u1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
     const auto load = [&](int u) {
@@ -208,32 +347,123 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a
                 for (int n = 0; n < NT; ++n) acc[m][n] = mfma16<F16>(av[m], bv[n], acc[m][n]);
         }
     }
-    // The epilogue by 16 tokens at a time through the wave's own piece of LDS, so that a token's outputs lie in consecutive
-    // lanes (and the fragments' registers are named by constants in a short loop).
-    constexpr int ROW = 64 * MT + 16;                  // bytes of a token's sums, and 16 that spread the tokens over the banks
-    constexpr int QUADS = 4 * MT / (PAIR ? 2 : 1);     // quads of outputs of a token
-    static_assert(WAVES * 16 * ROW <= STAGES * STEP, "the waves' pieces");
+    constexpr int NG = WAVES * kStoreBytes<MT, NT> <= STAGES * STEP ? NT : NT / 2;
+    static_assert(WAVES * kStoreBytes<MT, NG> <= STAGES * STEP, "the waves' pieces");
     __syncthreads();
-    uint8_t* mine = lds + wave * 16 * ROW;
-    const bool vec = rows_vec(a);
+    tile_store<MT, NT, NG, PAIR>(a, acc, lds + wave * kStoreBytes<MT, NG>, o0 + wm * (16 * MT / (PAIR ? 2 : 1)), t0 + wn * NT * 16, t0 + n_t,
+                             lane);
+}
+
+// c[n] += a b[n] for eight fragments, in place in accumulation registers (left to itself the compiler rotates 256 of them
+// through copies and their wait states, a third of the loop).  The two wait states before are those of a VALU write that an
+// operand may come from; settle() passes those of a read of the sums.
+template <bool F16>
+__device__ __forceinline__ void mfma16_row(f32x4 (&c)[8], const u32x4& a, const u32x4 (&b)[8]) {
+#define SMOE_ROW(OP)                                                                                               \
+    asm volatile("s_nop 1\n\t" OP " %0, %8, %9, %0\n\t" OP " %1, %8, %10, %1\n\t" OP " %2, %8, %11, %2\n\t" OP     \
+                 " %3, %8, %12, %3\n\t" OP " %4, %8, %13, %4\n\t" OP " %5, %8, %14, %5\n\t" OP " %6, %8, %15, %6\n\t" \
+                 OP " %7, %8, %16, %7"                                                                            \
+                 : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7])  \
+                 : "v"(a), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "v"(b[4]), "v"(b[5]), "v"(b[6]), "v"(b[7]))
+    if constexpr (F16) SMOE_ROW("v_mfma_f32_16x16x32_f16");
+    else SMOE_ROW("v_mfma_f32_16x16x32_bf16");
+#undef SMOE_ROW
+}
+
+__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
+// The same product in tiles of 256 weight rows by 256 tokens, four waves (one to a SIMD) of 128 by 128: 64 fragments of
+// sums in 256 accumulation registers, so that 128 matrix instructions share 32 fragment reads of LDS (eight waves of 128 by
+// 64 need 48, which with the loads' writes keeps the LDS as long busy as the matrix cores).  A step of 64 of K is two
+// halves; while a half's 64 instructions run, the fragments of the next half are read, and in the second half, past the
+// step's one barrier, the loads of the step after the next are issued into the buffer that the barrier freed.
+template <bool PAIR, bool F16>
+__global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int tiles_o, int tiles_t) {
+    constexpr int MT = 8, NT = 8, WAVES = 4, BM = 256, BN = 256, OUTS = PAIR ? 128 : 256;
+    constexpr int WS = 8, SLOTS = 16, STEP = (BM + BN) * 128;
+    constexpr int LDS = 2 * STEP > WAVES * kStoreBytes<MT, 4> ? 2 * STEP : WAVES * kStoreBytes<MT, 4>;
+    __shared__ __align__(1024) uint8_t lds[LDS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    int to, tt;
+    tile_of(blockIdx.x, gridDim.x, tiles_o, tiles_t, to, tt);
+    const int o0 = to * OUTS, t0 = tt * BN;
+    const int n_o = min(OUTS, a.n_out - o0), n_t = min(BN, a.n_tokens - t0);
+    uint32_t off[SLOTS];
+    i32x4 rw, rx;
+    tile_loads<BM, BN, WAVES, PAIR>(a, o0, t0, n_o, n_t, wave, lane, rw, rx, off);
+    const int steps = (a.n_in + 63) / 64;
+    const int piece = (lane & 7) ^ (lane >> 3);
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 1024);
+    const auto load = [&](int u, int i) {
+        dma16(base + (u & 1) * STEP + (i < WS ? i * WAVES * 1024 : BM * 128 + (i - WS) * WAVES * 1024),
+              u * 64 + 8 * piece < a.n_in ? off[i] + 128u * u : kOob, i < WS ? rw : rx, 0);
+    };
+    f32x4 acc[MT][NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-            *reinterpret_cast<f32x4*>(mine + fr * ROW + m * 64 + (lane >> 4) * 16) = acc[m][n];
-#pragma unroll 1
-        for (int i = lane; i < 16 * QUADS; i += 64) {
-            const int tr = i / QUADS, q = i % QUADS;
-            const int t = (wn * NT + n) * 16 + tr, o = o0 + wm * (4 * QUADS) + 4 * q;
-            const uint8_t* at = mine + tr * ROW + (PAIR ? (q >> 2) * 128 + (q & 3) * 16 : q * 16);
-            const f32x4 g = *reinterpret_cast<const f32x4*>(at), u = *reinterpret_cast<const f32x4*>(at + (PAIR ? 64 : 0));
-            if (t < n_t && o < a.n_out) {
-                if (gridDim.y == 1)
-                    finish4<PAIR>(a, vec, t0 + t, o, {g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]});
-                else put_part<PAIR>(a, blockIdx.y, t0 + t, o, g, u);
-            }
-        }
+        for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int fr = lane & 15;
+    u32x4 av[2][MT], bv[2][NT];
+    const uint8_t* wb = lds + (wm * MT * 16 + fr) * 128;
+    const uint8_t* xb = lds + (BM + wn * NT * 16 + fr) * 128;
+    // fragment i of half h of step u: the tokens, which the half's first instructions all need, then the weights' rows
+    const auto read = [&](int u, int h, int i) {
+        const int at = (u & 1) * STEP + ((4 * h + (lane >> 4)) ^ (fr & 7)) * 16;
+        if (i < NT) bv[h][i] = *reinterpret_cast<const u32x4*>(xb + at + i * 2048);
+        else av[h][i - NT] = *reinterpret_cast<const u32x4*>(wb + at + (i - NT) * 2048);
+    };
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) load(0, i);
+    if (steps > 1) {
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) load(1, i);
+        vmcnt<SLOTS>();
+    } else {
+        vmcnt<0>();
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT + NT; ++i) read(0, 0, i);
+    const auto step = [&](int u, auto next, auto after) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (m < 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) read(u, 1, 4 * m + i);
+            }
+            mfma16_row<F16>(acc[m], av[0][m], bv[0]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (decltype(next)::value) {
+            // every wave has read step u, and step u + 1 is there
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if constexpr (decltype(after)::value) {
+                load(u + 2, 2 * m);
+                load(u + 2, 2 * m + 1);
+            }
+            if (decltype(next)::value && m < 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) read(u + 1, 0, 4 * m + i);
+            }
+            mfma16_row<F16>(acc[m], av[1][m], bv[1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    int u = 0;
+    for (; u + 2 < steps; ++u) step(u, std::true_type{}, std::true_type{});
+    if (u + 1 < steps) step(u++, std::true_type{}, std::false_type{});
+    step(u, std::false_type{}, std::false_type{});
+    settle();
+    __syncthreads();
+    tile_store<MT, NT, 4, PAIR>(a, acc, lds + wave * kStoreBytes<MT, 4>, o0 + wm * (16 * MT / (PAIR ? 2 : 1)), t0 + wn * NT * 16, t0 + n_t,
+                             lane);
 }
 
 // A few tokens: 16 outputs to a work-group (PAIR: of both matrices), its WAVES waves each every WAVES-th 64 of K, straight
@@ -357,8 +587,12 @@ hipError_t launch_linear_as(const LinearArgs& a, const LinearPlan& p, hipStream_
     SMOE_FEW(1, 4) SMOE_FEW(1, 8) SMOE_FEW(1, 16) SMOE_FEW(2, 4) SMOE_FEW(2, 8)
 #undef SMOE_FEW
     if (p.kind == kLinearTile) {
-        if (p.a == 256) e = launch_tile<8, 4, 2, 4, 2, PAIR, F16>(a, p.slices, s);
-        else if (p.a == 128 && p.b == 128) e = launch_tile<4, 4, 2, 2, 2, PAIR, F16>(a, p.slices, s);
+        if (p.a == 256) {
+            const int tiles_o = (a.n_out + (PAIR ? 127 : 255)) / (PAIR ? 128 : 256), tiles_t = (a.n_tokens + 255) / 256;
+            hipLaunchKernelGGL((k_linear_big<PAIR, F16>), dim3(tiles_o * tiles_t), dim3(256), 0, s, a, tiles_o, tiles_t);
+            e = hipGetLastError();
+        }
+        if (p.a == 128 && p.b == 128) e = launch_tile<4, 4, 2, 2, 2, PAIR, F16>(a, p.slices, s);
         else if (p.a == 128 && p.b == 64) e = launch_tile<4, 2, 2, 2, 3, PAIR, F16>(a, p.slices, s);
         else if (p.a == 64 && p.b == 64) e = launch_tile<2, 2, 2, 2, 4, PAIR, F16>(a, p.slices, s);
     }
