@@ -8,6 +8,7 @@
 #include "smoe_types.hpp"
 
 #include <type_traits>
+#include <utility>
 
 namespace smoe {
 
@@ -354,35 +355,52 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a
                              lane);
 }
 
-// c[n] += a b[n] for eight fragments, in place in accumulation registers (left to itself the compiler rotates 256 of them
-// through copies and their wait states, a third of the loop).  The two wait states before are those of a VALU write that an
-// operand may come from; settle() passes those of a read of the sums.
+// c += a b, in place in accumulation registers: left to itself the compiler rotates k_linear_big's 256 of them through copies
+// and their wait states, a third of the loop.  Nothing but LDS reads may write a and b shortly before, and settle() comes
+// between the last of these and a read of a sum: the hardware does not wait for either by itself.
 template <bool F16>
-__device__ __forceinline__ void mfma16_row(f32x4 (&c)[8], const u32x4& a, const u32x4 (&b)[8]) {
-#define SMOE_ROW(OP)                                                                                               \
-    asm volatile("s_nop 1\n\t" OP " %0, %8, %9, %0\n\t" OP " %1, %8, %10, %1\n\t" OP " %2, %8, %11, %2\n\t" OP     \
-                 " %3, %8, %12, %3\n\t" OP " %4, %8, %13, %4\n\t" OP " %5, %8, %14, %5\n\t" OP " %6, %8, %15, %6\n\t" \
-                 OP " %7, %8, %16, %7"                                                                            \
-                 : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7])  \
-                 : "v"(a), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "v"(b[4]), "v"(b[5]), "v"(b[6]), "v"(b[7]))
-    if constexpr (F16) SMOE_ROW("v_mfma_f32_16x16x32_f16");
-    else SMOE_ROW("v_mfma_f32_16x16x32_bf16");
-#undef SMOE_ROW
+__device__ __forceinline__ void mfma16_in_place(f32x4& c, const u32x4& a, const u32x4& b) {
+    if constexpr (F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-
+// The same with a load into LDS (dma16, to `lds` + AT) round it: the matrix instruction is the wait state between m0's write
+// and its use.
+template <bool F16, int AT>
+__device__ __forceinline__ void mfma16_dma(f32x4& c, const u32x4& a, const u32x4& b, uint32_t lds, uint32_t voff, i32x4 rsrc) {
+#define SMOE_MFMA_DMA(OP)                                                                                          \
+    asm volatile("s_add_u32 m0, %3, %4\n\t" OP " %0, %1, %2, %0\n\tbuffer_load_dwordx4 %5, %6, 0 offen lds"         \
+                 : "+a"(c)                                                                                          \
+                 : "v"(a), "v"(b), "s"(lds), "n"(AT), "v"(voff), "s"(rsrc)                                         \
+                 : "memory", "m0", "scc")
+    if constexpr (F16) SMOE_MFMA_DMA("v_mfma_f32_16x16x32_f16");
+    else SMOE_MFMA_DMA("v_mfma_f32_16x16x32_bf16");
+#undef SMOE_MFMA_DMA
+}
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 // The same product in tiles of 256 weight rows by 256 tokens, four waves (one to a SIMD) of 128 by 128: 64 fragments of
 // sums in 256 accumulation registers, so that 128 matrix instructions share 32 fragment reads of LDS (eight waves of 128 by
 // 64 need 48, which with the loads' writes keeps the LDS as long busy as the matrix cores).  A step of 64 of K is two
-// halves; while a half's 64 instructions run, the fragments of the next half are read, and in the second half, past the
-// step's one barrier, the loads of the step after the next are issued into the buffer that the barrier freed.
+// halves; while a half's 64 instructions run, the fragments of the next half are read.  LDS is a ring of five tiles of 256
+// rows, of w and of x in turn: in a step's first half the weights of the step after the next go where the step before had
+// its tokens, in its second half, past the one barrier, the tokens where this step had its weights, so that the loads are
+// spread evenly: a wave issues in order, and waits where they back up (all of them in the second half: 7 % slower).
+enum { kNone = 0, kAll = 1, kLast = 2 };  // what a step loads
+// f(0), f(1), ... as compile-time constants
+template <int N, class F, int... I>
+__device__ __forceinline__ void each_of_impl(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each_of(F&& f) {
+    each_of_impl<N>(f, std::make_integer_sequence<int, N>{});
+}
 template <bool PAIR, bool F16>
 __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int tiles_o, int tiles_t) {
     constexpr int MT = 8, NT = 8, WAVES = 4, BM = 256, BN = 256, OUTS = PAIR ? 128 : 256;
-    constexpr int WS = 8, SLOTS = 16, STEP = (BM + BN) * 128;
-    constexpr int LDS = 2 * STEP > WAVES * kStoreBytes<MT, 4> ? 2 * STEP : WAVES * kStoreBytes<MT, 4>;
-    __shared__ __align__(1024) uint8_t lds[LDS];
+    constexpr int WS = 8, SLOTS = 16, TILE = 256 * 128, RING = 5;
+    static_assert(WAVES * kStoreBytes<MT, 4> <= RING * TILE, "the waves' pieces of the epilogue");
+    __shared__ __align__(1024) uint8_t lds[RING * TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
     int to, tt;
@@ -395,9 +413,20 @@ __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int t
     const int steps = (a.n_in + 63) / 64;
     const int piece = (lane & 7) ^ (lane >> 3);
     const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 1024);
-    const auto load = [&](int u, int i) {
-        dma16(base + (u & 1) * STEP + (i < WS ? i * WAVES * 1024 : BM * 128 + (i - WS) * WAVES * 1024),
-              u * 64 + 8 * piece < a.n_in ? off[i] + 128u * u : kOob, i < WS ? rw : rx, 0);
+    // load i of step u's weights (i < 8), then of its tokens, into the ring's tile `at` (a byte offset); the buffers' bases
+    // move on by a step's 128 bytes (rw, rx: those of the next step to be loaded)
+    const auto load = [&](int u, int i, uint32_t at) {
+        dma16(base + at + i % WS * WAVES * 1024, u * 64 + 8 * piece < a.n_in ? off[i] : kOob, i < WS ? rw : rx, 0);
+    };
+    const auto move_on = [](i32x4& r) {
+        const uint64_t p = ((uint64_t)(uint32_t)r[1] << 32 | (uint32_t)r[0]) + 128;
+        r[0] = (int)(uint32_t)p;
+        r[1] = (int)(uint32_t)(p >> 32);
+        r[2] -= 128;
+    };
+    const auto later = [](uint32_t at, int tiles) {  // the ring's tile `tiles` (1 .. 4) after
+        at += tiles * TILE;
+        return at >= RING * TILE ? at - RING * TILE : at;
     };
     f32x4 acc[MT][NT];
 #pragma unroll
@@ -406,19 +435,24 @@ __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int t
         for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int fr = lane & 15;
     u32x4 av[2][MT], bv[2][NT];
+    // fragment i of half h of the step whose weights are the ring's tile `at`: the tokens, which the half's first
+    // instructions all need, then the weights' rows
     const uint8_t* wb = lds + (wm * MT * 16 + fr) * 128;
-    const uint8_t* xb = lds + (BM + wn * NT * 16 + fr) * 128;
-    // fragment i of half h of step u: the tokens, which the half's first instructions all need, then the weights' rows
-    const auto read = [&](int u, int h, int i) {
-        const int at = (u & 1) * STEP + ((4 * h + (lane >> 4)) ^ (fr & 7)) * 16;
-        if (i < NT) bv[h][i] = *reinterpret_cast<const u32x4*>(xb + at + i * 2048);
-        else av[h][i - NT] = *reinterpret_cast<const u32x4*>(wb + at + (i - NT) * 2048);
+    const uint8_t* xb = lds + (wn * NT * 16 + fr) * 128;
+    const auto read = [&](uint32_t at, int h, int i) {
+        const int k = ((4 * h + (lane >> 4)) ^ (fr & 7)) * 16;
+        if (i < NT) bv[h][i] = *reinterpret_cast<const u32x4*>(xb + later(at, 1) + k + i * 2048);
+        else av[h][i - NT] = *reinterpret_cast<const u32x4*>(wb + at + k + (i - NT) * 2048);
     };
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) load(0, i);
+    for (int i = 0; i < SLOTS; ++i) load(0, i, i < WS ? 0 : TILE);
+    move_on(rw);
+    move_on(rx);
     if (steps > 1) {
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) load(1, i);
+        for (int i = 0; i < SLOTS; ++i) load(1, i, i < WS ? 2 * TILE : 3 * TILE);
+        move_on(rw);
+        move_on(rx);
         vmcnt<SLOTS>();
     } else {
         vmcnt<0>();
@@ -426,40 +460,54 @@ __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int t
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MT + NT; ++i) read(0, 0, i);
-    const auto step = [&](int u, auto next, auto after) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (m < 4) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) read(u, 1, 4 * m + i);
+    // One step; LOADS: of the step after the next, none, all of its 64 values, or the last ones there are.  A wave issues in
+    // order and a matrix instruction takes 16 cycles, time for three others: what else there is goes in between, one by one.
+    const auto half = [&](auto loads, int u, int h, uint32_t to_at, auto&& fill) {
+        constexpr int LOADS = decltype(loads)::value;
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(base + to_at);
+        const auto one = [&](auto at) {
+            constexpr int I = decltype(at)::value, M = I / NT, N = I % NT;
+            fill(at);
+            if constexpr (LOADS != kNone && I % 8 == 2) {
+                const uint32_t v = off[h * WS + I / 8];
+                mfma16_dma<F16, I / 8 * WAVES * 1024>(acc[M][N], av[h][M], bv[h][N], dst,
+                                                      LOADS == kAll || (u + 2) * 64 + 8 * piece < a.n_in ? v : kOob, h ? rx : rw);
+            } else {
+                mfma16_in_place<F16>(acc[M][N], av[h][M], bv[h][N]);
             }
-            mfma16_row<F16>(acc[m], av[0][m], bv[0]);
             __builtin_amdgcn_sched_barrier(0);
-        }
-        if constexpr (decltype(next)::value) {
-            // every wave has read step u, and step u + 1 is there
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        };
+        each_of<MT * NT>(one);
+    };
+    const auto step = [&](int u, uint32_t at, auto next, auto loads) {
+        constexpr bool NEXT = decltype(next)::value;
+        constexpr int LOADS = decltype(loads)::value;
+        const uint32_t at1 = later(at, 2);
+        half(loads, u, 0, later(at, 4), [&](auto i) {
+            constexpr int I = decltype(i)::value;
+            if constexpr (I % 3 == 0 && I / 3 < 16) read(at, 1, I / 3);
+        });
+        if constexpr (LOADS != kNone) move_on(rw);
+        if constexpr (NEXT) {
+            // every wave has read this step, and the next one is there (of the one after, its weights may be on their way)
+            if constexpr (LOADS != kNone) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if constexpr (decltype(after)::value) {
-                load(u + 2, 2 * m);
-                load(u + 2, 2 * m + 1);
-            }
-            if (decltype(next)::value && m < 4) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) read(u + 1, 0, 4 * m + i);
-            }
-            mfma16_row<F16>(acc[m], av[1][m], bv[1]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        half(loads, u, 1, at, [&](auto i) {
+            constexpr int I = decltype(i)::value;
+            if constexpr (NEXT && I % 3 == 0 && I / 3 < 16) read(at1, 0, I / 3);
+        });
+        if constexpr (LOADS != kNone) move_on(rx);
+        return at1;
     };
     int u = 0;
-    for (; u + 2 < steps; ++u) step(u, std::true_type{}, std::true_type{});
-    if (u + 1 < steps) step(u++, std::true_type{}, std::false_type{});
-    step(u, std::false_type{}, std::false_type{});
+    uint32_t at = 0;
+    for (; u + 3 < steps; ++u) at = step(u, at, std::true_type{}, std::integral_constant<int, kAll>{});
+    if (u + 2 < steps) at = step(u++, at, std::true_type{}, std::integral_constant<int, kLast>{});
+    if (u + 1 < steps) at = step(u++, at, std::true_type{}, std::integral_constant<int, kNone>{});
+    step(u, at, std::false_type{}, std::integral_constant<int, kNone>{});
     settle();
     __syncthreads();
     tile_store<MT, NT, 4, PAIR>(a, acc, lds + wave * kStoreBytes<MT, 4>, o0 + wm * (16 * MT / (PAIR ? 2 : 1)), t0 + wn * NT * 16, t0 + n_t,
