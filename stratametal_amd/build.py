@@ -45,21 +45,9 @@ SOURCES = ["smoe_decode.hip", "smoe_prefill.hip", "smoe_iq2.hip", "smoe_iq2_mm.h
            "smoe_dense.cpp", "smoe_gguf.cpp"]
 
 
-# smoe_linear.hip's K loops only add to their sums, and k_linear_big's 256 sums of a lane take all accumulation registers
-WITHOUT = {"smoe_linear.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form")}
-
-
-def _flags(src: str):
-    gone = WITHOUT.get(src)
-    if not gone:
-        return COMMON
-    i = next(i for i in range(len(COMMON) - 1) if tuple(COMMON[i:i + 2]) == gone)
-    return COMMON[:i] + COMMON[i + 2:]
-
-
 def _compile(src: str) -> str:
     obj = os.path.join(BUILD, os.path.splitext(src)[0] + ".o")
-    cmd = [HIPCC, *_flags(src), "-c", os.path.join(CSRC, src), "-o", obj]
+    cmd = [HIPCC, *COMMON, "-c", os.path.join(CSRC, src), "-o", obj]
     if src.endswith(".cpp"):
         cmd[1:1] = ["-x", "hip"]
     out = subprocess.run(cmd, capture_output=True, text=True)

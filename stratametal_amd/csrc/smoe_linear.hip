@@ -183,14 +183,6 @@ __device__ __forceinline__ void put_part(const LinearArgs& a, int slice, int64_t
 
 }  // namespace
 
-// The K loop's ring of STAGES LDS buffers: a wave waits until its loads of all but the `after` newest steps are done.
-template <int SLOTS, int STAGES>
-__device__ __forceinline__ void wait_steps(int after) {
-    if (STAGES > 2 && after >= STAGES - 2) vmcnt<(STAGES - 2) * SLOTS>();
-    else if (STAGES > 3 && after == STAGES - 3) vmcnt<(STAGES - 3) * SLOTS>();
-    else vmcnt<0>();
-}
-
 // The tile of work-group i of n: consecutive work-groups go to the 8 XCDs in turn, so XCD x takes the x-th eighth of the
 // tiles; in it, bands of kBand token tiles are walked output tile by output tile, so that the tiles at work together share
 // rows of both matrices in that XCD's L2.
@@ -286,18 +278,33 @@ __device__ __forceinline__ void tile_store(const LinearArgs& a, const f32x4 (&ac
     }
 }
 
+// f(0), f(1), ... as compile-time constants
+template <int N, class F, int... I>
+__device__ __forceinline__ void each_of_impl(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+    (void)f;
+}
+template <int N, class F>
+__device__ __forceinline__ void each_of(F&& f) {
+    each_of_impl<N>(f, std::make_integer_sequence<int, N>{});
+}
+
 // A tile of BM = 16 MT WM weight rows by BN = 16 NT WN tokens per work-group of WM WN waves, MT x NT fragments of 16 x 16
-// to a wave; K in steps of 64 through a ring of STAGES LDS buffers, filled by loads that write LDS directly.  A row's step is
+// to a wave; K in steps of 64 through a ring of RING LDS buffers, filled by loads that write LDS directly.  A row's step is
 // eight 16-byte pieces, piece c of row r at place c ^ (r & 7), so that the 16 rows of a fragment's read spread over the
-// banks.  blockIdx.y: a slice of K, whose sums go to `part` ([slice][w, w2][token][n_out]) for k_linear_join.
-template <int MT, int NT, int WM, int WN, int STAGES, bool PAIR, bool F16>
+// banks.  A step is two halves: while a half's products run, the fragments of the next half are read and half of the loads
+// of the step RING (weights: past the middle) or RING - 1 (tokens) later are issued; one barrier, in the middle.  (A step's
+// fragments read after its barrier: 0.67 us a step of 128 x 128 whatever the ring.)  Steps past the end load nothing: their
+// offsets lie past the buffers, zeros go to LDS, and the count of loads under way stays the same.
+// blockIdx.y: a slice of K, whose sums go to `part` ([slice][w, w2][token][n_out]) for k_linear_join.
+template <int MT, int NT, int WM, int WN, int RING, bool PAIR, bool F16>
 __global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a, int tiles_o, int tiles_t) {
     constexpr int WAVES = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
     constexpr int OUTS = PAIR ? BM / 2 : BM;           // outputs of the tile
     constexpr int WS = BM / 8 / WAVES, XS = BN / 8 / WAVES, SLOTS = WS + XS;  // a wave's loads of a step, 8 rows each
     constexpr int STEP = (BM + BN) * 128;              // bytes of a step
-    static_assert(STAGES >= 2 && STAGES <= 4, "wait_steps");
-    __shared__ __align__(1024) uint8_t lds[STAGES * STEP];
+    static_assert((RING - 1) * SLOTS <= 63, "vmcnt");
+    __shared__ __align__(1024) uint8_t lds[RING * STEP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     int to, tt;
@@ -307,16 +314,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a
     i32x4 rw, rx;
     uint32_t off[SLOTS];
     tile_loads<BM, BN, WAVES, PAIR>(a, o0, t0, n_o, n_t, wave, lane, rw, rx, off);
-    const int piece = (lane & 7) ^ (lane >> 3);
     const int all = (a.n_in + 63) / 64;
     const int u0 = (int)((int64_t)all * blockIdx.y / gridDim.y), u1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
-    const auto load = [&](int u) {
-        const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds) + (u - u0) % STAGES * STEP + wave * 1024);
-        const bool in = u * 64 + 8 * piece < a.n_in;  // (a last short step: zeros past the row)
-#pragma unroll
-        for (int i = 0; i < SLOTS; ++i)  // (a row past the matrix stays past the buffer)
-            dma16(base + (i < WS ? i * WAVES * 1024 : BM * 128 + (i - WS) * WAVES * 1024),
-                  in ? off[i] + 128u * u : kOob, i < WS ? rw : rx, 0);
+    const int k_end = min(a.n_in, u1 * 64), k_lane = 8 * ((lane & 7) ^ (lane >> 3));
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 1024);
+    const auto load = [&](int u, int i, uint32_t at) {  // load i of step u into the ring's step `at` (a byte offset)
+        dma16(base + at + (i < WS ? i * WAVES * 1024 : BM * 128 + (i - WS) * WAVES * 1024),
+              u * 64 + k_lane < k_end ? off[i] + 128u * u : kOob, i < WS ? rw : rx, 0);
     };
     f32x4 acc[MT][NT];
 #pragma unroll
@@ -324,32 +328,53 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i)
-        if (u0 + i < u1) load(u0 + i);
+    for (int r = 0; r < RING; ++r)
+#pragma unroll
+        for (int i = 0; i < (r < RING - 1 ? SLOTS : WS); ++i) load(u0 + r, i, r * STEP);
+    vmcnt<(RING - 2) * SLOTS + WS>();
+    __syncthreads();
     const int fr = lane & 15;
+    const uint8_t* wb = lds + (wm * MT * 16 + fr) * 128;
+    const uint8_t* xb = lds + (BM + wn * NT * 16 + fr) * 128;
+    uint4 av[2][MT], bv[2][NT];
+    const auto read = [&](uint32_t at, int h, int i) {  // fragment i of half h: the tokens, then the weights
+        const int k = ((4 * h + (lane >> 4)) ^ (fr & 7)) * 16;
+        if (i < NT) bv[h][i] = *reinterpret_cast<const uint4*>(xb + at + k + i * 2048);
+        else av[h][i - NT] = *reinterpret_cast<const uint4*>(wb + at + k + (i - NT) * 2048);
+    };
+#pragma unroll
+    for (int i = 0; i < MT + NT; ++i) read(0, 0, i);
+    uint32_t at = 0, before = (RING - 1) * STEP;  // of this step and the one before
     for (int u = u0; u < u1; ++u) {
-        wait_steps<SLOTS, STAGES>(u1 - 1 - u);
-        __syncthreads();  // step u is in LDS, and every wave is done with the buffer that the next load overwrites
-        if (u + STAGES - 1 < u1) load(u + STAGES - 1);
-        const uint8_t* step = lds + (u - u0) % STAGES * STEP;
-        const uint8_t* wb = step + (wm * MT * 16 + fr) * 128;
-        const uint8_t* xb = step + (BM + wn * NT * 16 + fr) * 128;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const int at = ((4 * kk + (lane >> 4)) ^ (fr & 7)) * 16;
-            uint4 av[MT], bv[NT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) av[m] = *reinterpret_cast<const uint4*>(wb + m * 2048 + at);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) bv[n] = *reinterpret_cast<const uint4*>(xb + n * 2048 + at);
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) acc[m][n] = mfma16<F16>(av[m], bv[n], acc[m][n]);
-        }
+        const uint32_t next = at + STEP == RING * STEP ? 0 : at + STEP;
+        const auto half = [&](auto which) {
+            constexpr int H = decltype(which)::value, L = H ? WS : XS, F = MT * NT, FR = MT + NT;
+            each_of<F>([&](auto idx) {
+                constexpr int I = decltype(idx)::value;
+                // what goes before product I: the I-th shares of the loads and of the next half's fragments
+                each_of<(I + 1) * L / F - I * L / F>([&](auto j) {
+                    constexpr int l = I * L / F + decltype(j)::value;
+                    if constexpr (H) load(u + RING, l, at);
+                    else load(u + RING - 1, WS + l, before);
+                });
+                each_of<(I + 1) * FR / F - I * FR / F>([&](auto j) { read(H ? next : at, 1 - H, I * FR / F + decltype(j)::value); });
+                acc[I / NT][I % NT] = mfma16<F16>(av[H][I / NT], bv[H][I % NT], acc[I / NT][I % NT]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        half(std::integral_constant<int, 0>{});
+        // every wave has read this step, and the next one is there
+        vmcnt<(RING - 2) * SLOTS>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        half(std::integral_constant<int, 1>{});
+        before = at;
+        at = next;
     }
-    constexpr int NG = WAVES * kStoreBytes<MT, NT> <= STAGES * STEP ? NT : NT / 2;
-    static_assert(WAVES * kStoreBytes<MT, NG> <= STAGES * STEP, "the waves' pieces");
+    vmcnt<0>();
+    constexpr int NG = WAVES * kStoreBytes<MT, NT> <= RING * STEP ? NT : NT / 2;
+    static_assert(WAVES * kStoreBytes<MT, NG> <= RING * STEP, "the waves' pieces");
     __syncthreads();
     tile_store<MT, NT, NG, PAIR>(a, acc, lds + wave * kStoreBytes<MT, NG>, o0 + wm * (16 * MT / (PAIR ? 2 : 1)), t0 + wn * NT * 16, t0 + n_t,
                              lane);
@@ -385,16 +410,6 @@ __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" :
 // rows, of w and of x in turn: in a step's first half the weights of the step after the next go where the step before had
 // its tokens, in its second half, past the one barrier, the tokens where this step had its weights, so that the loads are
 // spread evenly: a wave issues in order, and waits where they back up (all of them in the second half: 7 % slower).
-enum { kNone = 0, kAll = 1, kLast = 2 };  // what a step loads
-// f(0), f(1), ... as compile-time constants
-template <int N, class F, int... I>
-__device__ __forceinline__ void each_of_impl(F&& f, std::integer_sequence<int, I...>) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, class F>
-__device__ __forceinline__ void each_of(F&& f) {
-    each_of_impl<N>(f, std::make_integer_sequence<int, N>{});
-}
 template <bool PAIR, bool F16>
 __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int tiles_o, int tiles_t) {
     constexpr int MT = 8, NT = 8, WAVES = 4, BM = 256, BN = 256, OUTS = PAIR ? 128 : 256;
@@ -410,20 +425,20 @@ __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int t
     uint32_t off[SLOTS];
     i32x4 rw, rx;
     tile_loads<BM, BN, WAVES, PAIR>(a, o0, t0, n_o, n_t, wave, lane, rw, rx, off);
-    const int steps = (a.n_in + 63) / 64;
-    const int piece = (lane & 7) ^ (lane >> 3);
+    const int all = (a.n_in + 63) / 64;
+    const int u0 = (int)((int64_t)all * blockIdx.y / gridDim.y), u1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
     const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 1024);
-    // load i of step u's weights (i < 8), then of its tokens, into the ring's tile `at` (a byte offset); the buffers' bases
-    // move on by a step's 128 bytes (rw, rx: those of the next step to be loaded)
-    const auto load = [&](int u, int i, uint32_t at) {
-        dma16(base + at + i % WS * WAVES * 1024, u * 64 + 8 * piece < a.n_in ? off[i] : kOob, i < WS ? rw : rx, 0);
-    };
-    const auto move_on = [](i32x4& r) {
-        const uint64_t p = ((uint64_t)(uint32_t)r[1] << 32 | (uint32_t)r[0]) + 128;
+    // values of K that are left from the lane's first one on; the buffers' bases move on by a step's 128 bytes
+    int w_left = min(a.n_in, u1 * 64) - 8 * ((lane & 7) ^ (lane >> 3)), x_left = w_left;
+    const auto move_on = [](i32x4& r, int& left, int steps) {
+        const uint64_t p = ((uint64_t)(uint32_t)r[1] << 32 | (uint32_t)r[0]) + 128u * steps;
         r[0] = (int)(uint32_t)p;
         r[1] = (int)(uint32_t)(p >> 32);
-        r[2] -= 128;
+        r[2] -= 128 * steps;
+        left -= 64 * steps;
     };
+    move_on(rw, w_left, u0);
+    move_on(rx, x_left, u0);
     const auto later = [](uint32_t at, int tiles) {  // the ring's tile `tiles` (1 .. 4) after
         at += tiles * TILE;
         return at >= RING * TILE ? at - RING * TILE : at;
@@ -445,103 +460,76 @@ __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int t
         else av[h][i - NT] = *reinterpret_cast<const u32x4*>(wb + at + k + (i - NT) * 2048);
     };
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) load(0, i, i < WS ? 0 : TILE);
-    move_on(rw);
-    move_on(rx);
-    if (steps > 1) {
+    for (int r = 0; r < 2; ++r) {
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) load(1, i, i < WS ? 2 * TILE : 3 * TILE);
-        move_on(rw);
-        move_on(rx);
-        vmcnt<SLOTS>();
-    } else {
-        vmcnt<0>();
+        for (int i = 0; i < SLOTS; ++i)
+            dma16(base + (i < WS ? 2 * r : 2 * r + 1) * TILE + i % WS * WAVES * 1024, w_left > 0 ? off[i] : kOob, i < WS ? rw : rx, 0);
+        move_on(rw, w_left, 1);
+        move_on(rx, x_left, 1);
     }
+    vmcnt<SLOTS>();
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MT + NT; ++i) read(0, 0, i);
-    // One step; LOADS: of the step after the next, none, all of its 64 values, or the last ones there are.  A wave issues in
-    // order and a matrix instruction takes 16 cycles, time for three others: what else there is goes in between, one by one.
-    const auto half = [&](auto loads, int u, int h, uint32_t to_at, auto&& fill) {
-        constexpr int LOADS = decltype(loads)::value;
-        const uint32_t dst = __builtin_amdgcn_readfirstlane(base + to_at);
-        const auto one = [&](auto at) {
-            constexpr int I = decltype(at)::value, M = I / NT, N = I % NT;
-            fill(at);
-            if constexpr (LOADS != kNone && I % 8 == 2) {
-                const uint32_t v = off[h * WS + I / 8];
-                mfma16_dma<F16, I / 8 * WAVES * 1024>(acc[M][N], av[h][M], bv[h][N], dst,
-                                                      LOADS == kAll || (u + 2) * 64 + 8 * piece < a.n_in ? v : kOob, h ? rx : rw);
-            } else {
-                mfma16_in_place<F16>(acc[M][N], av[h][M], bv[h][N]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        each_of<MT * NT>(one);
-    };
-    const auto step = [&](int u, uint32_t at, auto next, auto loads) {
-        constexpr bool NEXT = decltype(next)::value;
-        constexpr int LOADS = decltype(loads)::value;
-        const uint32_t at1 = later(at, 2);
-        half(loads, u, 0, later(at, 4), [&](auto i) {
-            constexpr int I = decltype(i)::value;
-            if constexpr (I % 3 == 0 && I / 3 < 16) read(at, 1, I / 3);
-        });
-        if constexpr (LOADS != kNone) move_on(rw);
-        if constexpr (NEXT) {
-            // every wave has read this step, and the next one is there (of the one after, its weights may be on their way)
-            if constexpr (LOADS != kNone) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
-            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-        }
-        half(loads, u, 1, at, [&](auto i) {
-            constexpr int I = decltype(i)::value;
-            if constexpr (NEXT && I % 3 == 0 && I / 3 < 16) read(at1, 0, I / 3);
-        });
-        if constexpr (LOADS != kNone) move_on(rx);
-        return at1;
-    };
-    int u = 0;
+    // A wave issues in order and a matrix instruction takes 16 cycles, time for three others: what else there is goes in
+    // between, one by one.  (One loop for all steps, whose loads past the end are of zeros from past the buffers: between
+    // versions of it the compiler would copy the sums.)
     uint32_t at = 0;
-    for (; u + 3 < steps; ++u) at = step(u, at, std::true_type{}, std::integral_constant<int, kAll>{});
-    if (u + 2 < steps) at = step(u++, at, std::true_type{}, std::integral_constant<int, kLast>{});
-    if (u + 1 < steps) at = step(u++, at, std::true_type{}, std::integral_constant<int, kNone>{});
-    step(u, at, std::false_type{}, std::integral_constant<int, kNone>{});
+    for (int u = u0; u < u1; ++u) {
+        const uint32_t next = later(at, 2);
+        const auto half = [&](auto which) {
+            constexpr int H = decltype(which)::value;
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(base + (H ? at : later(at, 4)));
+            each_of<MT * NT>([&](auto idx) {
+                constexpr int I = decltype(idx)::value, M = I / NT, N = I % NT;
+                if constexpr (I % 3 == 0 && I / 3 < MT + NT) read(H ? next : at, 1 - H, I / 3);
+                if constexpr (I % 8 == 2)
+                    mfma16_dma<F16, I / 8 * WAVES * 1024>(acc[M][N], av[H][M], bv[H][N], dst,
+                                                          (H ? x_left : w_left) > 0 ? off[H * WS + I / 8] : kOob, H ? rx : rw);
+                else
+                    mfma16_in_place<F16>(acc[M][N], av[H][M], bv[H][N]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            if constexpr (H) move_on(rx, x_left, 1);
+            else move_on(rw, w_left, 1);
+        };
+        half(std::integral_constant<int, 0>{});
+        // every wave has read this step, and the next one is there (of the one after, its weights may be on their way)
+        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        half(std::integral_constant<int, 1>{});
+        at = next;
+    }
+    vmcnt<0>();
     settle();
     __syncthreads();
     tile_store<MT, NT, 4, PAIR>(a, acc, lds + wave * kStoreBytes<MT, 4>, o0 + wm * (16 * MT / (PAIR ? 2 : 1)), t0 + wn * NT * 16, t0 + n_t,
                              lane);
 }
 
-// A few tokens: 16 outputs to a work-group (PAIR: of both matrices), its WAVES waves each every WAVES-th 64 of K, straight
-// from memory to the matrix instruction's layout: lane l holds row (or token) l & 15, values 8 (l >> 4) .. of a 32-value
-// step.  Bound by the weights' bytes: up to LOADS of a lane's weight loads are on their way together.  Tokens in NT sets of 16
-// (lanes past the last token hold its values, and their results are dropped); the waves' sums meet in LDS, in wave order.
-template <int NT, int WAVES, bool PAIR, bool F16>
-__global__ __launch_bounds__(64 * WAVES) void k_linear_few(const LinearArgs a) {
-    constexpr int SETS = PAIR ? 2 : 1, BLOCKS = 4;  // blocks of 64 of K on their way
-    __shared__ f32x4 sum_s[WAVES][SETS * NT][64];
+// Up to 16 tokens: 16 outputs to a work-group of eight waves, each every eighth 64 of K, straight from memory to the matrix
+// instruction's layout: lane l holds row (or token) l & 15, values 8 (l >> 4) .. of a 32-value piece.  Bound by the weights'
+// bytes: four blocks of 64 of K of a wave are on their way together.  Lanes past the last token hold its values, and their
+// results are dropped; the waves' sums meet in LDS, in wave order.
+template <bool PAIR, bool F16>
+__global__ __launch_bounds__(512) void k_linear_few(const LinearArgs a) {
+    constexpr int SETS = PAIR ? 2 : 1, WAVES = 8, BLOCKS = 4;
+    __shared__ f32x4 sum_s[WAVES][SETS][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int o0 = blockIdx.x * 16;
-    const int row = min(o0 + (lane & 15), a.n_out - 1), kq = 8 * (lane >> 4);
+    const int o0 = blockIdx.x * 16, kq = 8 * (lane >> 4);
+    const size_t row = (size_t)min(o0 + (lane & 15), a.n_out - 1) * a.n_in;
     const uint16_t* wp[SETS];
-    wp[0] = static_cast<const uint16_t*>(a.w) + (size_t)row * a.n_in;
-    if constexpr (PAIR) wp[1] = static_cast<const uint16_t*>(a.w2) + (size_t)row * a.n_in;
-    const uint16_t* xp[NT];
+    wp[0] = static_cast<const uint16_t*>(a.w) + row;
+    if constexpr (PAIR) wp[1] = static_cast<const uint16_t*>(a.w2) + row;
+    const uint16_t* xp = static_cast<const uint16_t*>(a.x) + min(lane & 15, a.n_tokens - 1) * a.x_ld;
+    f32x4 acc[SETS];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-        xp[n] = static_cast<const uint16_t*>(a.x) + min(16 * n + (lane & 15), a.n_tokens - 1) * a.x_ld;
-    const int all = (a.n_in + 63) / 64;
-    const int u0 = (int)((int64_t)all * blockIdx.y / gridDim.y), u1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
-    f32x4 acc[SETS][NT];
-#pragma unroll
-    for (int i = 0; i < SETS; ++i)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[i][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < SETS; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int u = u0 + wave; u < u1; u += BLOCKS * WAVES) {
-        uint4 wv[BLOCKS][2][SETS], xv[BLOCKS][2][NT];
+    const int blocks = (a.n_in + 63) / 64;
+    for (int u = wave; u < blocks; u += BLOCKS * WAVES) {
+        uint4 wv[BLOCKS][2][SETS], xv[BLOCKS][2];
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
@@ -549,42 +537,32 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(const LinearArgs a) {
                 const int k = min((u + b * WAVES) * 64 + 32 * h + kq, a.n_in - 8);
 #pragma unroll
                 for (int i = 0; i < SETS; ++i) wv[b][h][i] = *reinterpret_cast<const uint4*>(wp[i] + k);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) xv[b][h][n] = *reinterpret_cast<const uint4*>(xp[n] + k);
+                xv[b][h] = *reinterpret_cast<const uint4*>(xp + k);
             }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                // (past the slice or the row: zeros of both, whatever the last values are)
-                const bool in = u + b * WAVES < u1 && (u + b * WAVES) * 64 + 32 * h + kq < a.n_in;
+                // (past the row: zeros of both, whatever the last values are)
+                const bool in = (u + b * WAVES) * 64 + 32 * h + kq < a.n_in;
+                const uint4 x = in ? xv[b][h] : zero;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint4 x = in ? xv[b][h][n] : zero;
-#pragma unroll
-                    for (int i = 0; i < SETS; ++i) acc[i][n] = mfma16<F16>(in ? wv[b][h][i] : zero, x, acc[i][n]);
-                }
+                for (int i = 0; i < SETS; ++i) acc[i] = mfma16<F16>(in ? wv[b][h][i] : zero, x, acc[i]);
             }
     }
 #pragma unroll
+    for (int i = 0; i < SETS; ++i) sum_s[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
     for (int i = 0; i < SETS; ++i)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sum_s[wave][i * NT + n][lane] = acc[i][n];
-    __syncthreads();
-    const bool vec = rows_vec(a);
-    for (int n = wave; n < NT; n += WAVES) {
-        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-#pragma unroll
-        for (int i = 0; i < SETS; ++i) {
-            s[i] = sum_s[0][i * NT + n][lane];
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w) s[i] = s[i] + sum_s[w][i * NT + n][lane];
-        }
-        const int t = 16 * n + (lane & 15), o = o0 + 4 * (lane >> 4);
-        if (t >= a.n_tokens || o >= a.n_out) continue;
-        if (gridDim.y == 1) finish4<PAIR>(a, vec, t, o, {s[0][0], s[0][1], s[0][2], s[0][3]}, {s[1][0], s[1][1], s[1][2], s[1][3]});
-        else put_part<PAIR>(a, blockIdx.y, t, o, s[0], s[1]);
-    }
+        for (int w = 1; w < WAVES; ++w) acc[i] = acc[i] + sum_s[w][i][lane];
+    const int t = lane & 15, o = o0 + 4 * (lane >> 4);
+    if (t >= a.n_tokens || o >= a.n_out) return;
+    const f32x4 g = acc[0], u = acc[SETS - 1];
+    finish4<PAIR>(a, rows_vec(a), t, o, {g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]});
 }
 
 // The slices' sums added in order, and the epilogue: four outputs of a token to a thread.
@@ -625,25 +603,21 @@ hipError_t launch_tile(const LinearArgs& a, int slices, hipStream_t s) {
 }
 template <bool PAIR, bool F16>
 hipError_t launch_linear_as(const LinearArgs& a, const LinearPlan& p, hipStream_t s) {
+    if (p.kind == kLinearFew) {
+        hipLaunchKernelGGL((k_linear_few<PAIR, F16>), dim3((a.n_out + 15) / 16), dim3(512), 0, s, a);
+        return hipGetLastError();
+    }
     hipError_t e = hipErrorInvalidValue;
-    const dim3 few((a.n_out + 15) / 16, p.slices);
-#define SMOE_FEW(N, W) \
-    if (p.kind == kLinearFew && p.a == N && p.b == W) { \
-        hipLaunchKernelGGL((k_linear_few<N, W, PAIR, F16>), few, dim3(64 * W), 0, s, a); \
-        e = hipGetLastError(); \
+    if (p.kind == kLinear256) {
+        const int tiles_o = (a.n_out + (PAIR ? 127 : 255)) / (PAIR ? 128 : 256), tiles_t = (a.n_tokens + 255) / 256;
+        hipLaunchKernelGGL((k_linear_big<PAIR, F16>), dim3(tiles_o * tiles_t, p.slices), dim3(256), 0, s, a, tiles_o, tiles_t);
+        e = hipGetLastError();
     }
-    SMOE_FEW(1, 4) SMOE_FEW(1, 8) SMOE_FEW(1, 16) SMOE_FEW(2, 4) SMOE_FEW(2, 8)
-#undef SMOE_FEW
-    if (p.kind == kLinearTile) {
-        if (p.a == 256) {
-            const int tiles_o = (a.n_out + (PAIR ? 127 : 255)) / (PAIR ? 128 : 256), tiles_t = (a.n_tokens + 255) / 256;
-            hipLaunchKernelGGL((k_linear_big<PAIR, F16>), dim3(tiles_o * tiles_t), dim3(256), 0, s, a, tiles_o, tiles_t);
-            e = hipGetLastError();
-        }
-        if (p.a == 128 && p.b == 128) e = launch_tile<4, 4, 2, 2, 2, PAIR, F16>(a, p.slices, s);
-        else if (p.a == 128 && p.b == 64) e = launch_tile<4, 2, 2, 2, 3, PAIR, F16>(a, p.slices, s);
-        else if (p.a == 64 && p.b == 64) e = launch_tile<2, 2, 2, 2, 4, PAIR, F16>(a, p.slices, s);
-    }
+    // tiles of 64 x 32, 64 x 64, 128 x 64 and 128 x 128: two work-groups to a CU but for the last
+    if (p.kind == kLinear64x32) e = launch_tile<2, 1, 2, 2, 6, PAIR, F16>(a, p.slices, s);
+    if (p.kind == kLinear64) e = launch_tile<2, 2, 2, 2, 5, PAIR, F16>(a, p.slices, s);
+    if (p.kind == kLinear128x64) e = launch_tile<4, 2, 2, 2, 3, PAIR, F16>(a, p.slices, s);
+    if (p.kind == kLinear128) e = launch_tile<4, 4, 2, 2, 3, PAIR, F16>(a, p.slices, s);
     if (e != hipSuccess || p.slices == 1) return e;
     const int64_t quads = (int64_t)a.n_tokens * ((a.n_out + 3) / 4);
     hipLaunchKernelGGL(k_linear_join<PAIR>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a, p.slices);

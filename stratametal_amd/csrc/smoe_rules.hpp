@@ -186,20 +186,19 @@ constexpr int64_t balance_count_groups(int64_t T) { return T < 512 ? 1 : T / 256
 // offsets).
 constexpr int kLinearMaxIn = 65536, kLinearMaxOut = 1 << 24;
 constexpr int64_t kLinearMaxLd = (int64_t)1 << 21;
-// Which kernel: the rows' (kLinearFew: a token sets of 16, b waves) or a tile of a weight rows by b tokens; K in slices.
-enum LinearKind { kLinearFew, kLinearTile };
+// Which kernel, and in how many slices of K.
+enum LinearKind { kLinearFew, kLinear64x32, kLinear64, kLinear128x64, kLinear128, kLinear256 };
 struct LinearPlan {
     LinearKind kind;
-    int a, b, slices;
+    int slices;
 };
 constexpr int64_t kLinearSplitTokens = 1024;  // no batch beyond is sliced
 inline LinearPlan linear_plan(int64_t T, int K, int64_t N, bool pair) {
-    if (T <= 16) return {kLinearFew, 1, 8, 1};
-    if (T <= 32) return {kLinearFew, 2, 8, 1};
+    if (T <= 4) return {kLinearFew, 1};
     const int64_t rows = pair ? 2 * N : N;
-    if (((rows + 255) / 256) * ((T + 255) / 256) >= 200) return {kLinearTile, 256, 256, 1};
-    if (((rows + 127) / 128) * ((T + 127) / 128) >= 200) return {kLinearTile, 128, 128, 1};
-    return {kLinearTile, 64, 64, 1};
+    if (((rows + 255) / 256) * ((T + 255) / 256) >= 200) return {kLinear256, 1};
+    if (((rows + 127) / 128) * ((T + 127) / 128) >= 200) return {kLinear128, 1};
+    return {kLinear64, 1};
 }
 // (at most the smallest tiles' work-groups, in one dimension)
 inline bool linear_grid_fits(int64_t T, int64_t N, bool pair) {
