@@ -268,8 +268,9 @@ typedef struct {
     const float* bias2;
 } smoe_linear;
 
-/* Workspace bytes of smoe_linear_run for up to max_tokens tokens (0 on a bad shape). */
-size_t smoe_linear_workspace_bytes(const smoe_linear* L, int32_t max_tokens);
+/* Workspace bytes of smoe_linear_run for n_tokens tokens (0 on a bad shape).  A smaller batch may need more, where its
+ * tiles are few and K is sliced: size a workspace of several batch sizes by the largest of theirs. */
+size_t smoe_linear_workspace_bytes(const smoe_linear* L, int32_t n_tokens);
 
 /* x 16-byte aligned, x_ld a multiple of 8 (at most 2^21); residual of y's type, NULL for none; y may be residual's own
  * rows (the same address and row stride) and share no other byte with an input.  `workspace`: 256-byte aligned, read by no

@@ -712,14 +712,14 @@ class Linear:
         if lib().smoe_linear_workspace_bytes(self._ref, 0) == 0:
             raise SmoeError(-1, lib().smoe_last_error().decode())
 
-    def workspace_bytes(self, max_tokens: int) -> int:
-        return int(lib().smoe_linear_workspace_bytes(self._ref, max_tokens))
+    def workspace_bytes(self, n_tokens: int) -> int:
+        return int(lib().smoe_linear_workspace_bytes(self._ref, n_tokens))
 
     def _bytes(self, T: int) -> int:
         """workspace_bytes, kept per batch size."""
         n = self._sizes.get(T)
         if n is None:
-            n = self._sizes[T] = self.workspace_bytes(T) if T > 0 else 0
+            n = self._sizes[T] = self.workspace_bytes(T)
         return n
 
     def run(self, x, residual=None, y=None, y_dtype=None, stream=None):

@@ -124,19 +124,14 @@ static smoe_status check_linear(const smoe_linear* L) {
     return SMOE_OK;
 }
 
-size_t smoe_linear_workspace_bytes(const smoe_linear* L, int32_t max_tokens) {
+size_t smoe_linear_workspace_bytes(const smoe_linear* L, int32_t n_tokens) {
     if (check_linear(L) != SMOE_OK) return 0;
-    if (max_tokens < 0) {
+    if (n_tokens < 0) {
         fail(SMOE_EINVAL, "linear: negative token count");
         return 0;
     }
     ok();
-    size_t most = 0;
-    for (int64_t t = 1; t <= max_tokens && t <= smoe::kLinearSplitTokens; ++t) {
-        const size_t b = smoe::linear_part_bytes(t, L->n_in, L->n_out, L->w2 != nullptr);
-        most = b > most ? b : most;
-    }
-    return most + 256;
+    return 256 + (n_tokens ? smoe::linear_part_bytes(n_tokens, L->n_in, L->n_out, L->w2 != nullptr) : 0);
 }
 
 smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, int32_t n_tokens, const void* residual,
@@ -166,7 +161,8 @@ smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, i
                            rows_of(L->w2, L->w_type, 1, 0, wb), rows_of(L->bias, SMOE_F32, 1, 0, L->n_out),
                            rows_of(L->bias2, SMOE_F32, 1, 0, L->n_out)})
         if (overlap(sy, in)) return fail(SMOE_EINVAL, "linear: y overlaps x, a weight or a bias");
-    if (!smoe::linear_grid_fits(n_tokens, L->n_out, L->w2 != nullptr))
+    const smoe::LinearPlan plan = smoe::linear_plan(n_tokens, L->n_in, L->n_out, L->w2 != nullptr);
+    if (smoe::linear_groups(plan, n_tokens, L->n_out, L->w2 != nullptr) >= smoe::kGridGroups)
         return fail(SMOE_EINVAL, "linear: the product exceeds a launch's grid: split it");
     const size_t need = smoe::linear_part_bytes(n_tokens, L->n_in, L->n_out, L->w2 != nullptr);
     if (need) {

@@ -69,13 +69,15 @@ def test_linear(want, kw):
 def test_linear_workspace():
     L = S.lib()
 
-    def size(T, **kw):
-        return L.smoe_linear_workspace_bytes(C.byref(S._Linear(kw.get("n_in", 8192), kw.get("n_out", 64), S.BF16, 0, A, None,
-                                                               None, None)), T)
+    def size(T, n_in=8192, n_out=64):
+        return L.smoe_linear_workspace_bytes(C.byref(S._Linear(n_in, n_out, S.BF16, 0, A, None, None, None)), T)
 
     assert size(0) > 0 and size(1) > 0 and size(-1) == 0 and size(4, n_in=9) == 0
-    sizes = [size(t) for t in range(0, 600)]
-    assert sizes == sorted(sizes)  # enough for every smaller batch
+    need = size(100)  # few tiles: K is sliced
+    assert need > 256
+    assert linear(n_in=8192, n_out=64, T=100, w=A, ws=None) == ENULL
+    assert linear(n_in=8192, n_out=64, T=100, ws=E + 8) == EALIGN
+    assert linear(n_in=8192, n_out=64, T=100, wsb=need - 257) == ESIZE
 
 
 def balance(l=A, ld=None, ids=B, mask=None, T=8, n=16, k=4, cb=1.0, cz=0.0, loss=D, counts=D + 256, p=D + 8192, d=None, dld=None,
