@@ -595,7 +595,7 @@ def _on_device(t, name: str, device: int = -1):
 def _current(device: int, stream) -> Optional[int]:
     """The current stream's handle, when a call on `device` runs on it; None: under _on, which makes them current."""
     import torch
-    if stream is None and torch.cuda.current_device() == device:
+    if stream is None and torch._C._cuda_getDevice() == device:
         return torch._C._cuda_getCurrentRawStream(device)
     return None
 
@@ -625,8 +625,12 @@ class BlockEnds:
     def __init__(self, n_embd: int, pre=None, post=None, res_scale: float = 1.0, y_scale: float = 1.0, eps: float = 1e-6,
                  gate_act: int = GATE_NONE):
         self.n_embd, self.pre, self.post = n_embd, _vector(pre, "pre", n_embd), _vector(post, "post", n_embd)
+        weights = [t for t in (pre, post) if t is not None]
+        self._device = weights[0].get_device() if weights else -1
+        for t in weights:
+            _on_device(t, "post", self._device)
         self._c = _Ends(_ptr(pre), _ptr(post), eps, res_scale, y_scale, gate_act)
-        self._ref = C.byref(self._c)
+        self._ref, self._call = C.byref(self._c), lib().smoe_block_ends
 
     def _run(self, R, y, gate, out, x, x_dtype, form, stream):
         import torch
@@ -637,37 +641,49 @@ class BlockEnds:
         if st is None:
             with _on(dev, stream):
                 return self._run(R, y, gate, out, x, x_dtype, form, None)
-        for t, name in ((self.pre, "pre"), (self.post, "post")):
-            if t is not None:
-                _on_device(t, name, dev)
+        if self._device >= 0 and self._device != dev:
+            raise SmoeError(-1, f"the norms' weights are on cuda:{self._device}, the call's tensors on cuda:{dev}")
         yt = y_ld = o_ld = xt = x_ld = g_ld = g_step = 0
         yp = gp = op = xp = None
         if y is not None:
             yt, y_ld = _rows(y, "y", n, T, dev)
             yp = y.data_ptr()
             if out is None:
-                out = torch.empty((T, n), dtype=R.dtype, device=R.device)
-            ot, o_ld = _rows(out, "out", n, T, dev)
-            if ot != rt:
-                raise SmoeError(-1, f"out is {out.dtype}, needs {R.dtype}")
+                out, o_ld = torch.empty((T, n), dtype=R.dtype, device=R.device), n
+            else:
+                ot, o_ld = _rows(out, "out", n, T, dev)
+                if ot != rt:
+                    raise SmoeError(-1, f"out is {out.dtype}, needs {R.dtype}")
             op = out.data_ptr()
             if gate is not None:
-                if gate.dtype != torch.float32:
-                    raise SmoeError(-1, f"gate is {gate.dtype}, needs torch.float32")
-                _on_device(gate, "gate", dev)
-                try:
-                    g_ld, g_step = gate.expand(T, n).stride()
-                except RuntimeError:
-                    raise SmoeError(-2, f"gate has shape {tuple(gate.shape)}, does not broadcast to ({T}, {n})") from None
+                g_ld, g_step = self._gate(gate, T, dev)
                 gp = gate.data_ptr()
         if form:
             if x is None:
-                x = torch.empty((T, n), dtype=x_dtype or R.dtype, device=R.device)
-            xt, x_ld = _rows(x, "x", n, T, dev)
+                dtype = x_dtype or R.dtype
+                xt = _elem_type(dtype)
+                if xt < 0:
+                    raise SmoeError(-3, f"x_dtype is {dtype}, needs float32, float16 or bfloat16 (or int16: bf16 bits)")
+                x, x_ld = torch.empty((T, n), dtype=dtype, device=R.device), n
+            else:
+                xt, x_ld = _rows(x, "x", n, T, dev)
             xp = x.data_ptr()
-        _check(lib().smoe_block_ends(self._ref, n, T, R.data_ptr(), rt, r_ld, yp, yt, y_ld, gp, g_ld, g_step, op, o_ld, xp,
-                                     xt, x_ld, st))
+        _check(self._call(self._ref, n, T, R.data_ptr(), rt, r_ld, yp, yt, y_ld, gp, g_ld, g_step, op, o_ld, xp, xt, x_ld,
+                          st))
         return out, x
+
+    def _gate(self, gate, T: int, dev: int):
+        """(token stride, channel stride) of a gate broadcast to (T, n_embd)."""
+        import torch
+        if gate.dtype != torch.float32:
+            raise SmoeError(-1, f"gate is {gate.dtype}, needs torch.float32")
+        _on_device(gate, "gate", dev)
+        if gate.dim() == 1 and gate.shape[0] == self.n_embd:
+            return 0, gate.stride(0)
+        try:
+            return gate.expand(T, self.n_embd).stride()
+        except RuntimeError:
+            raise SmoeError(-2, f"gate has shape {tuple(gate.shape)}, does not broadcast to ({T}, {self.n_embd})") from None
 
     def read(self, R, x=None, x_dtype=None, stream=None):
         """x = R rs(R) pre, a block's input from the stream (x_dtype None: R's)."""
@@ -707,7 +723,7 @@ class Linear:
                 _on_device(t, name, w.get_device())
         self._type = _elem_type(w.dtype)
         self._c = _Linear(n_in, n_out, self._type, act, w.data_ptr(), _ptr(w2), _ptr(bias), _ptr(bias2))
-        self._ref = C.byref(self._c)
+        self._ref, self._call = C.byref(self._c), lib().smoe_linear_run
         self._sizes: Dict = {}
         if lib().smoe_linear_workspace_bytes(self._ref, 0) == 0:
             raise SmoeError(-1, lib().smoe_last_error().decode())
@@ -740,14 +756,19 @@ class Linear:
             rt, r_ld = _rows(residual, "residual", N, T, dev)
             rp = residual.data_ptr()
         if y is None:
-            y = torch.empty((T, N), dtype=y_dtype or (x if residual is None else residual).dtype, device=x.device)
-        yt, y_ld = _rows(y, "y", N, T, dev)
+            dtype = y_dtype or (x if residual is None else residual).dtype
+            yt = _elem_type(dtype)
+            if yt < 0:
+                raise SmoeError(-3, f"y_dtype is {dtype}, needs float32, float16 or bfloat16 (or int16: bf16 bits)")
+            y, y_ld = torch.empty((T, N), dtype=dtype, device=x.device), N
+        else:
+            yt, y_ld = _rows(y, "y", N, T, dev)
         if rt >= 0 and rt != yt:
             raise SmoeError(-1, f"residual is {residual.dtype}, y {y.dtype}")
         # a workspace of the call's own: calls on several streams, captured or not, share none
         n = self._bytes(T)
         ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n > 256 else None
-        _check(lib().smoe_linear_run(self._ref, x.data_ptr(), x_ld, T, rp, r_ld, y.data_ptr(), yt, y_ld, _ptr(ws), n, st))
+        _check(self._call(self._ref, x.data_ptr(), x_ld, T, rp, r_ld, y.data_ptr(), yt, y_ld, _ptr(ws), n, st))
         return y
 
     __call__ = run

@@ -8,7 +8,7 @@
 // waves through LDS in wave order, the work-groups' partial rows in k_balance_sums in a fixed order and in 64 bits; the
 // counts are integers: every result is the same bits in every run.
 //   k_balance_one                                    a few tokens: one work-group does it all
-//   k_balance_rows, k_balance_sums                   up to kCountPairs pairs: each work-group counts the ids for itself
+//   k_balance_rows, k_balance_sums                   some pairs: each work-group that needs the counts counts for itself
 //   k_balance_counts, k_balance_rows, k_balance_sums a batch
 #include "smoe_gemv.hpp"
 #include "smoe_launch.hpp"
@@ -424,7 +424,7 @@ void launch_rows(const BalanceArgs& a, int G, int C, const Work& w, hipStream_t 
 hipError_t launch_balance(const BalanceArgs& a, hipStream_t s) {
     const int T = a.n_tokens, E = a.n_expert;
     const int G = (int)balance_groups(T);
-    const int C = balance_counts_apart(T, a.k) ? (int)balance_count_groups(T) : 0;
+    const int C = balance_counts_apart(T, a.k, a.dlogits != nullptr) ? (int)balance_count_groups(T) : 0;
     Work w;
     work_layout(T, E, static_cast<uint8_t*>(a.work), &w);
     const bool one = balance_one(T, a.k);

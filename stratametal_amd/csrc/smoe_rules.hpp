@@ -175,12 +175,19 @@ constexpr int64_t ends_groups(int64_t T, int n) {
     return sets < most ? sets : most;
 }
 
-// The router's balance loss: one work-group for a few tokens; the ids counted by every work-group or, from many on,
-// first; at most 1024 work-groups of rows (k_balance_sums).
+// The router's balance loss: one work-group for a few tokens (64 tokens of 512 experts 15.7 us with gradients, in two launches
+// 18.9; 256 tokens 38 and 19.5).
 constexpr bool balance_one(int64_t T, int k) { return T <= 64 && T * k <= 4096; }
-constexpr bool balance_counts_apart(int64_t T, int k) { return T * k > 16384; }
-constexpr int64_t balance_groups(int64_t T) { return T < 4 ? 1 : (T + 3) / 4 < 1024 ? (T + 3) / 4 : 1024; }
-constexpr int64_t balance_count_groups(int64_t T) { return T < 512 ? 1 : T / 256 < 16 ? T / 256 : 16; }
+// The pairs counted first, by a launch of their own, or by every work-group that needs them: with gradients those of the rows
+// (us apart and not: 2560 pairs 18.7 and 19.5 with a mask, 17.6 and 17.0 without, 5120 19.5 and 23.2, 10240 20.5 and
+// 28.8), else those of the sums, few and large (10240 pairs 16.4 and 15.5).
+constexpr bool balance_counts_apart(int64_t T, int k, bool grad) { return T * k > (grad ? 3000 : 12000); }
+// Work-groups of four rows at a time, at most 1024 (k_balance_sums): each leaves a row of partial sums (4096 tokens of 512
+// experts 27.5 us with 256 or 512 of them, 31.8 with 1024, 30.4 with 128; 32768 of 1024 99, 77.5, 79.8, 151).
+constexpr int64_t balance_groups(int64_t T) { return T < 4 ? 1 : (T + 3) / 4 < 512 ? (T + 3) / 4 : 512; }
+// Work-groups of the counts, whose rows every reader adds up (4096 tokens 29.8 us with 8, 31.7 with 16; 32768 84 and 80,
+// with 64 95).
+constexpr int64_t balance_count_groups(int64_t T) { return T < 1024 ? 1 : T / 512 < 16 ? T / 512 : 16; }
 
 // The dense product: a row of x or w, rows of w, and the distance of x's rows (a tile of 256 rows stays within 31-bit
 // offsets).

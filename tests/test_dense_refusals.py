@@ -103,7 +103,7 @@ def test_binding_refuses_bad_tensors():
     x = torch.zeros((4, 64))
     g = torch.zeros((4, 2), dtype=torch.int32)
     e = object.__new__(S.BlockEnds)
-    e.n_embd, e.pre, e.post = 64, None, None
+    e.n_embd, e.pre, e.post, e._device = 64, None, None, -1
     for fn, why in [
         (lambda: S.BlockEnds(64, pre=x), "shape"), (lambda: S.BlockEnds(4, post=torch.zeros(4)), "not a GPU"),
         (lambda: e.read(x.double()), "float64"), (lambda: e.read(x[:, :32]), "shape"), (lambda: e.read(x[0]), "shape"),
