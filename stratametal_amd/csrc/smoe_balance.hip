@@ -102,7 +102,7 @@ struct Rows {
     float* dlogits;
     int64_t ld, ld_d;
     int T, E;
-    float cb, cz;
+    float cz;
     float next[NJ];
     uint8_t next_on;
 
@@ -137,8 +137,11 @@ struct Rows {
                 if (col(j) < E) d[col(j)] = g[j];
         }
     }
-    __device__ __forceinline__ double run(int64_t t, int64_t step, const float (&f)[NJ], float inv_n, float (&psum)[NJ],
+    // bf: cb E f / n.  A row's e^(v - top) is 2^(v log2 e - c), c = top log2 e as rounded, which every p and lse share; a top
+    // whose c is near f32's end takes v - top first.
+    __device__ __forceinline__ double run(int64_t t, int64_t step, const float (&bf)[NJ], float inv_n, float (&psum)[NJ],
                                           float (&dsum)[NJ]) {
+        constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
         double zsum = 0.0;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) psum[j] = dsum[j] = 0.0f;
@@ -160,31 +163,38 @@ struct Rows {
 #pragma unroll
             for (int j = 1; j < NJ; ++j) top = __builtin_fmaxf(top, v[j]);
             top = wave_max_fast(top);
-            const float shift = top == -__builtin_inff() ? 0.0f : top;  // a row of -inf alone: every e^v is 0
+            float c = top * kLog2e;
+            if (__builtin_fabsf(top) > 1e30f) {  // (the same in every lane)
+                const float shift = top == -__builtin_inff() ? 0.0f : top;  // a row of -inf alone: every e^v is 0
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) v[j] = v[j] - shift;
+                c = 0.0f;
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                v[j] = exp_fast(v[j] - shift);
+                v[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j], kLog2e, -c));
                 sum += v[j];
             }
             sum = wave_sum_xor_fast(sum);
             const bool none = sum == 0.0f;
             const float inv = none ? 0.0f : 1.0f / sum;
-            const float lse = none ? 0.0f : top + __builtin_logf(sum);
+            const float log_sum = __builtin_logf(sum);
+            const float lse = none ? 0.0f : __builtin_fabsf(top) > 1e30f ? top + log_sum : __builtin_fmaf(c, kLn2, log_sum);
             zsum += (double)lse * (double)lse;
             float fp = 0.0f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 v[j] = v[j] * inv;
                 psum[j] += v[j];
-                if constexpr (GRAD) fp = __builtin_fmaf(f[j], v[j], fp);
+                if constexpr (GRAD) fp = __builtin_fmaf(bf[j], v[j], fp);
             }
             if constexpr (GRAD) {
                 fp = wave_sum_xor_fast(fp);
-                const float zc = 2.0f * cz * lse, bc = cb * (float)E;
+                const float k = __builtin_fmaf(2.0f * cz * inv_n, lse, -fp);
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    v[j] = v[j] * __builtin_fmaf(bc, f[j] - fp, zc) * inv_n;
+                    v[j] = v[j] * (bf[j] + k);
                     dsum[j] += v[j];
                 }
                 store(t, v);
@@ -241,10 +251,10 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void k_balance_rows(const Balanc
     __shared__ double z_s[kRowWaves];
     const int wave = threadIdx.x >> 6, tid = threadIdx.x, E = a.n_expert;
     const int64_t step = (int64_t)gridDim.x * kRowWaves, t = (int64_t)blockIdx.x * kRowWaves + wave;
-    Rows<NJ, GRAD, VEC> r{a.logits, a.mask, a.dlogits, a.ld, a.ld_d, a.n_tokens, E, a.balance_coef, a.z_coef, {}, 1};
+    Rows<NJ, GRAD, VEC> r{a.logits, a.mask, a.dlogits, a.ld, a.ld_d, a.n_tokens, E, a.z_coef, {}, 1};
     r.load(t);
     if (blockIdx.x == 0 && tid == 0) *w.ticket = 0;
-    float f[NJ], psum[NJ], dsum[NJ];
+    float bf[NJ], psum[NJ], dsum[NJ];
     float inv_n = 0.0f;
     if constexpr (GRAD) {
         int32_t* hist = reinterpret_cast<int32_t*>(&col_s[0][0]);
@@ -257,12 +267,12 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void k_balance_rows(const Balanc
         }
         const int n = hist[E];
         inv_n = n > 0 ? 1.0f / (float)n : 0.0f;
-        const float inv_nk = inv_n / (float)a.k;
+        const float scale = inv_n / (float)a.k * (a.balance_coef * (float)E) * inv_n;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) f[j] = (float)hist[min(r.col(j), E - 1)] * inv_nk;
+        for (int j = 0; j < NJ; ++j) bf[j] = (float)hist[min(r.col(j), E - 1)] * scale;
         __syncthreads();
     }
-    const double zsum = r.run(t, step, f, inv_n, psum, dsum);
+    const double zsum = r.run(t, step, bf, inv_n, psum, dsum);
     // the waves' column sums, in wave order
     const auto fold = [&](const float (&v)[NJ], float* out) {
 #pragma unroll
@@ -353,17 +363,18 @@ __global__ __launch_bounds__(64 * kOneWaves) void k_balance_one(const BalanceArg
     __shared__ int32_t hist[64 * NJ + 1];
     __shared__ double z_s[kOneWaves], b_s[kOneWaves];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = threadIdx.x, E = a.n_expert;
-    Rows<NJ, GRAD, VEC> r{a.logits, a.mask, a.dlogits, a.ld, a.ld_d, a.n_tokens, E, a.balance_coef, a.z_coef, {}, 1};
+    Rows<NJ, GRAD, VEC> r{a.logits, a.mask, a.dlogits, a.ld, a.ld_d, a.n_tokens, E, a.z_coef, {}, 1};
     r.load(wave);
     histogram(a.ids, a.mask, 0, a.n_tokens, E, a.k, hist);
     const int n = hist[E];
-    const float inv_n = n > 0 ? 1.0f / (float)n : 0.0f, inv_nk = inv_n / (float)a.k;
-    float f[NJ], psum[NJ], dsum[NJ];
+    const float inv_n = n > 0 ? 1.0f / (float)n : 0.0f;
+    float bf[NJ], psum[NJ], dsum[NJ];
     if constexpr (GRAD) {
+        const float scale = inv_n / (float)a.k * (a.balance_coef * (float)E) * inv_n;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) f[j] = (float)hist[min(r.col(j), E - 1)] * inv_nk;
+        for (int j = 0; j < NJ; ++j) bf[j] = (float)hist[min(r.col(j), E - 1)] * scale;
     }
-    const double zsum = r.run(wave, kOneWaves, f, inv_n, psum, dsum);
+    const double zsum = r.run(wave, kOneWaves, bf, inv_n, psum, dsum);
     const double over = n > 0 ? 1.0 / (double)n : 0.0;
     const auto put = [&](const float (&v)[NJ]) {
 #pragma unroll

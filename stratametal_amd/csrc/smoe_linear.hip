@@ -63,7 +63,20 @@ __device__ __forceinline__ void activate_all(float (&v)[N][4], int act) {
     }
 }
 
-// Four outputs o .. o + 3 of token t (those below n_out): g the sums of w, u of w2.
+// Output o of token t: g the sum of w, u of w2.
+template <bool PAIR>
+__device__ __forceinline__ void finish1(const LinearArgs& a, int64_t t, int o, float g, float u) {
+    float v = activate(a.bias ? g + a.bias[o] : g, a.act);
+    if constexpr (PAIR) v = v * (a.bias2 ? u + a.bias2[o] : u);
+    if (a.residual) {
+        const int64_t at = t * a.r_ld + o;
+        v += a.y_type == kF32 ? static_cast<const float*>(a.residual)[at]
+                              : elem_to_f32(static_cast<const uint16_t*>(a.residual)[at], a.y_type);
+    }
+    store1(a.y, t * a.y_ld + o, v, a.y_type);
+}
+
+// Four outputs o .. o + 3 of token t (those below n_out).
 template <bool PAIR>
 __device__ __forceinline__ void finish4(const LinearArgs& a, bool vec, int64_t t, int o, const float (&g)[4],
                                         const float (&u)[4]) {
@@ -155,7 +168,7 @@ __device__ __forceinline__ void finish_batch(const LinearArgs& a, int64_t t, int
 }
 
 // y and residual rows take 4-value vectors.
-__device__ __forceinline__ bool rows_vec(const LinearArgs& a) {
+__host__ __device__ __forceinline__ bool rows_vec(const LinearArgs& a) {
     const uintptr_t m = (a.y_type == kF32 ? 16 : 8) - 1;
     return ((reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.residual)) & m) == 0 &&
            ((a.y_ld | (a.residual ? a.r_ld : 0)) & 3) == 0;
@@ -236,7 +249,7 @@ __device__ __forceinline__ void tile_store(const LinearArgs& a, const f32x4 (&ac
     static_assert(!PAIR || MT % 2 == 0, "sets in pairs");
     static_assert(NT % NG == 0 && 64 % QUADS == 0 && 16 * NG / PER % BATCH == 0, "whole batches");
     const int q = lane % QUADS, o = o0 + 4 * q;
-    const bool vec = rows_vec(a) && o + 4 <= a.n_out && gridDim.y == 1;
+    const bool vec = rows_vec(a) && a.n_out % 4 == 0 && gridDim.y == 1;
     float b[4], c[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -255,7 +268,7 @@ __device__ __forceinline__ void tile_store(const LinearArgs& a, const f32x4 (&ac
         const int t1 = t0 + n * 16 + lane / QUADS;
         if (vec) {
 #pragma unroll 1
-            for (int i = 0; i < 16 * NG / PER; i += BATCH) {
+            for (int i = 0; i < 16 * NG / PER && o < a.n_out; i += BATCH) {
                 f32x4 g[BATCH], u[BATCH];
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
@@ -264,15 +277,22 @@ __device__ __forceinline__ void tile_store(const LinearArgs& a, const f32x4 (&ac
                 }
                 finish_batch<BATCH, PER, PAIR>(a, t1 + i * PER, t_end, o, b, c, g, u);
             }
-        } else {
+        } else if (gridDim.y > 1) {
 #pragma unroll 1
             for (int i = 0; i < 16 * NG / PER; ++i) {
-                const f32x4 g = *reinterpret_cast<const f32x4*>(at + i * PER * ROW);
-                const f32x4 u = *reinterpret_cast<const f32x4*>(at + i * PER * ROW + (PAIR ? 64 : 0));
                 const int t = t1 + i * PER;
-                if (t >= t_end || o >= a.n_out) continue;
-                if (gridDim.y > 1) put_part<PAIR>(a, blockIdx.y, t, o, g, u);
-                else finish4<PAIR>(a, false, t, o, {g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]});
+                if (t < t_end && o < a.n_out)
+                    put_part<PAIR>(a, blockIdx.y, t, o, *reinterpret_cast<const f32x4*>(at + i * PER * ROW),
+                                   *reinterpret_cast<const f32x4*>(at + i * PER * ROW + (PAIR ? 64 : 0)));
+            }
+        } else {  // rows that take no vectors: lanes take consecutive outputs
+            constexpr int OUTS = 4 * QUADS;
+#pragma unroll 4
+            for (int i = lane; i < 16 * NG * OUTS; i += 64) {
+                const int tr = i / OUTS, oc = i % OUTS, t = t0 + n * 16 + tr;
+                const uint8_t* v = mine + tr * ROW + 4 * (PAIR ? oc / 16 * 32 + oc % 16 : oc);
+                if (t < t_end && o0 + oc < a.n_out)
+                    finish1<PAIR>(a, t, o0 + oc, *reinterpret_cast<const float*>(v), *reinterpret_cast<const float*>(v + (PAIR ? 64 : 0)));
             }
         }
     }
@@ -565,26 +585,30 @@ __global__ __launch_bounds__(512) void k_linear_few(const LinearArgs a) {
     finish4<PAIR>(a, rows_vec(a), t, o, {g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]});
 }
 
-// The slices' sums added in order, and the epilogue: four outputs of a token to a thread.
-template <bool PAIR>
+// The slices' sums added in order, and the epilogue: four outputs of a token to a thread, or one where rows take no vectors.
+template <bool PAIR, bool VEC>
 __global__ __launch_bounds__(256) void k_linear_join(const LinearArgs a, int slices) {
-    const int quads = (a.n_out + 3) / 4;
+    const int per = VEC ? (a.n_out + 3) / 4 : a.n_out;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)a.n_tokens * quads) return;
-    const int64_t t = i / quads;
-    const int o = (int)(i % quads) * 4;
-    float g[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
-    for (int s = 0; s < slices; ++s) {
-        const f32x4 q = *part_at<PAIR>(a, s, 0, t, o);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) g[j] += q[j];
-        if constexpr (PAIR) {
-            const f32x4 p = *part_at<PAIR>(a, s, 1, t, o);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) u[j] += p[j];
+    if (i >= (int64_t)a.n_tokens * per) return;
+    const int64_t t = i / per;
+    const int o = (int)(i % per) * (VEC ? 4 : 1);
+    if constexpr (VEC) {
+        f32x4 g = *part_at<PAIR>(a, 0, 0, t, o), u = *part_at<PAIR>(a, 0, PAIR, t, o);
+        for (int s = 1; s < slices; ++s) {
+            g = g + *part_at<PAIR>(a, s, 0, t, o);
+            if constexpr (PAIR) u = u + *part_at<PAIR>(a, s, 1, t, o);
         }
+        finish4<PAIR>(a, true, t, o, {g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]});
+    } else {
+        const auto one = [&](int s, int which) { return reinterpret_cast<const float*>(part_at<PAIR>(a, s, which, t, o))[o & 3]; };
+        float g = one(0, 0), u = one(0, PAIR);
+        for (int s = 1; s < slices; ++s) {
+            g += one(s, 0);
+            if constexpr (PAIR) u += one(s, 1);
+        }
+        finish1<PAIR>(a, t, o, g, u);
     }
-    finish4<PAIR>(a, rows_vec(a), t, o, g, u);
 }
 
 size_t linear_part_bytes(int64_t T, int K, int N, bool pair) {
@@ -619,8 +643,11 @@ hipError_t launch_linear_as(const LinearArgs& a, const LinearPlan& p, hipStream_
     if (p.kind == kLinear128x64) e = launch_tile<4, 2, 2, 2, 3, PAIR, F16>(a, p.slices, s);
     if (p.kind == kLinear128) e = launch_tile<4, 4, 2, 2, 3, PAIR, F16>(a, p.slices, s);
     if (e != hipSuccess || p.slices == 1) return e;
-    const int64_t quads = (int64_t)a.n_tokens * ((a.n_out + 3) / 4);
-    hipLaunchKernelGGL(k_linear_join<PAIR>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a, p.slices);
+    const bool vec = rows_vec(a) && a.n_out % 4 == 0;
+    const int64_t n = (int64_t)a.n_tokens * (vec ? a.n_out / 4 : a.n_out);
+    const dim3 grid((unsigned)((n + 255) / 256));
+    if (vec) hipLaunchKernelGGL((k_linear_join<PAIR, true>), grid, dim3(256), 0, s, a, p.slices);
+    else hipLaunchKernelGGL((k_linear_join<PAIR, false>), grid, dim3(256), 0, s, a, p.slices);
     return hipGetLastError();
 }
 }  // namespace

@@ -206,32 +206,33 @@ struct LinearTile {
     double step, shared; // us of a step of 64 of K, alone on a CU and with the others
 };
 constexpr LinearTile kLinearTiles[] = {{},
-                                       {64, 32, 2, 0.7, 0.22, 0.57},
-                                       {64, 64, 2, 1.4, 0.27, 0.52},
-                                       {128, 64, 2, 1.9, 0.40, 0.72},
-                                       {128, 128, 1, 2.7, 0.61, 0.61},
-                                       {256, 256, 1, 11.1, 1.27, 1.27}};
-// A product's time in us, from its sizes: the rounds of work-groups over the 256 CUs times their steps, and where K is
-// sliced the launch and the bytes that join the sums; the rows' kernel reads 2048 of K at a time.  Fitted to 254 shapes (9
-// of 256 to 8192 by 512 to 16384, 1 to 2500 tokens, one matrix and pairs), each by every kernel in 1 to 8 slices: the least of
-// it is on average 1.3 % longer than the shape's shortest (of a choice of kernel and slices by the tiles' number alone,
-// 12 %).  us, by few, 64 x 32, 64 x 64, 128 x 64, 128 x 128 and 256 x 256: 1 token 2048 x 2048 5.3, 8.2, 9.7, -, -, -; 8
-// tokens 2048 x 8192 9.9, 8.7, 10.1, -, -, -; 16 tokens 8192 x 2048 18.4, 24.8, 29.6 and in four slices 12.9, 13.9; 128
-// tokens 2048 x 8192 -, -, 12.9, 18.7, 23.3, 74; 301 tokens 2568 x 5003 -, -, 28.7, 28.1, 36.5, 99 and 24.9 in two slices of
-// 128 x 128; 4096 tokens 4096 x 4096 -, -, 232, 191, 157, 102.
+                                       {64, 32, 2, 0.8, 0.18, 0.42},
+                                       {64, 64, 2, 1.5, 0.23, 0.48},
+                                       {128, 64, 2, 1.8, 0.40, 0.71},
+                                       {128, 128, 1, 2.4, 0.62, 0.62},
+                                       {256, 256, 1, 11.3, 1.24, 1.24}};
+// A product's time in us, from its sizes: the rounds of work-groups over the 256 CUs times their steps, or the bytes of w and
+// x at 6 bytes a ps where those take longer, and where K is sliced the launch and the bytes that join the sums; the rows'
+// kernel reads 2048 of K at a time.  Fitted to 254 shapes (9 of 256 to 8192 by 512 to 16384, 1 to 2500 tokens, one matrix
+// and pairs), each timed by every kernel in 1 to 8 slices: the kernel of the least of it takes on average 0.8 % longer than
+// the shape's fastest, at most 18 %.  us, by few, 64 x 32, 64 x 64, 128 x 64, 128 x 128 and 256 x 256: 1 token 2048 x 2048
+// 5.3, 8.2, 9.7, -, -, -; 8 tokens 2048 x 8192 9.9, 8.7, 10.1, -, -, -; 16 tokens 8192 x 2048 18.4, 24.8, 29.6 and in four
+// slices -, 12.9, 13.9; 128 tokens 2048 x 8192 -, -, 12.9, 18.7, 23.3, -; 301 tokens 2568 x 5003 -, -, 28.7, 28.1, 36.5, 99,
+// in two slices of 128 x 128 24.9; 4096 tokens 4096 x 4096 -, -, 232, 191, 157, 102.
 inline double linear_time(LinearKind kind, int slices, int64_t T, int64_t K, int64_t N, bool pair) {
     const int64_t rows = pair ? 2 * N : N;
+    const double w_bytes = (double)rows * (double)K * 2, x_bytes = (double)T * (double)K * 2;
     if (kind == kLinearFew) {
-        const double wg = (double)((N + 15) / 16), trips = (double)((K + 2047) / 2048) * 1.8 * (wg > 512 ? wg / 512 : 1);
-        const double bytes = (double)rows * K * 2 / 6.1e6;
-        return 3.6 + (trips > bytes ? trips : bytes) * (1 + 0.02 * (double)(T - 1));
+        const double wg = (double)((N + 15) / 16), trips = (double)((K + 2047) / 2048) * 3.4 * (wg > 512 ? wg / 512 : 1);
+        return 3.4 + (trips > w_bytes / 6.0e6 ? trips : w_bytes / 6.0e6) * (1 + 0.003 * (double)(T - 1));
     }
     const LinearTile& t = kLinearTiles[kind];
     const int64_t wg = (rows + t.rows - 1) / t.rows * ((T + t.tokens - 1) / t.tokens) * slices;
     const int64_t steps = ((K + 63) / 64 + slices - 1) / slices;
     const int64_t at_once = wg <= 256 ? 1 : t.per_cu, rounds = (wg + 256 * at_once - 1) / (256 * at_once);
-    const double join = slices > 1 ? 4.1 + 0.26e-6 * 4 * (double)(slices * T * rows) : 0;
-    return 1.9 + (double)rounds * (t.fixed + (double)steps * (at_once == 1 ? t.step : t.shared)) + join;
+    const double work = (double)rounds * (t.fixed + (double)steps * (at_once == 1 ? t.step : t.shared));
+    const double bytes = t.fixed + (w_bytes + x_bytes) / 6.4e6;
+    return 2.4 + (work > bytes ? work : bytes) + (slices > 1 ? 2.9 + 0.31e-6 * 4 * (double)(slices * T * rows) : 0);
 }
 constexpr int64_t kLinearFewTokens = 16;
 inline LinearPlan linear_plan(int64_t T, int64_t K, int64_t N, bool pair) {

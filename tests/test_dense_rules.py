@@ -1,0 +1,98 @@
+"""The dense operators' rules of stratametal_amd/csrc/smoe_rules.hpp at sizes whose sides were measured (the figures stand
+beside the rules), and their bounds; and what k_linear_big's hand-written matrix instructions need of the code round them."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+from test_dispatch_rules import ROOT, ask  # noqa: F401
+
+HIPCC = "/opt/rocm/bin/hipcc"
+FEW, T6432, T64, T12864, T128, T256 = range(6)
+
+
+def test_linear_plan(ask):  # noqa: F811
+    """tokens, n_in, n_out, pair -> a kernel and slices within a tenth of the fastest measured."""
+    cases = [(1, 2048, 2048, 0, {(FEW, 1)}), (1, 4096, 4096, 0, {(FEW, 1)}), (1, 2048, 8192, 1, {(FEW, 1), (T6432, 1), (T64, 1)}),
+             (12, 2048, 8192, 0, {(T6432, 1)}), (16, 8192, 2048, 0, {(T6432, 4), (T6432, 8)}), (128, 2048, 8192, 0, {(T64, 1)}),
+             (12, 4096, 4096, 1, {(FEW, 1), (T6432, 1), (T6432, 4), (T64, 1), (T12864, 4), (T128, 4)}),
+             (512, 4096, 4096, 0, {(T12864, 1), (T128, 2)}), (4096, 4096, 4096, 0, {(T256, 1)}),
+             (4096, 2048, 8192, 1, {(T256, 1)}), (4096, 8192, 8192, 0, {(T256, 1)})]
+    got = ask([e for T, K, N, p, _ in cases for e in (f"linear_plan({T}, {K}, {N}, {p}).kind", f"linear_plan({T}, {K}, {N}, {p}).slices")])
+    for i, c in enumerate(cases):
+        assert (got[2 * i], got[2 * i + 1]) in c[-1], (c, got[2 * i:2 * i + 2])
+
+
+def test_linear_plan_bounds(ask):  # noqa: F811
+    """Any size has a kernel that takes it: the rows' kernel at most 16 tokens, no slice without steps, grids that fit."""
+    sizes = [(T, K, N, p) for T in (1, 2, 16, 17, 500, 70000, 2 ** 31 - 1) for K in (8, 64, 72, 200, 8192, 65536)
+             for N in (1, 63, 5003, 2 ** 24) for p in (0, 1)]
+    got = ask([e for T, K, N, p in sizes for e in
+               (f"linear_plan({T}, {K}, {N}, {p}).kind", f"linear_plan({T}, {K}, {N}, {p}).slices",
+                f"linear_groups(linear_plan({T}, {K}, {N}, {p}), {T}, {N}, {p})")])
+    for i, (T, K, N, p) in enumerate(sizes):
+        kind, slices, groups = got[3 * i:3 * i + 3]
+        assert kind > FEW or (T <= 16 and slices == 1)
+        assert slices in (1, 2, 4, 8) and (slices == 1 or (K // 64 >= 2 * slices and groups * slices <= 1100))
+        assert groups >= 1
+
+
+def test_balance_rules(ask):  # noqa: F811
+    tokens = list(range(1, 700)) + [1024, 2048, 4096, 32768, 2 ** 24]
+    got = ask([e for T in tokens for e in (f"balance_groups({T})", f"balance_count_groups({T})", f"balance_one({T}, 10)")])
+    groups, counts, one = got[::3], got[1::3], got[2::3]
+    assert groups == sorted(groups) and groups[0] == 1 and max(groups) <= 1024 and max(g * 4 - T for g, T in zip(groups, tokens)) < 4
+    assert counts == sorted(counts) and counts[0] == 1 and max(counts) <= 64
+    assert all(o == (T <= 64) for o, T in zip(one, tokens))
+
+
+def test_ends_shapes(ask):  # noqa: F811
+    """A row's slots hold it, and few lanes more."""
+    widths = [1, 8, 256, 257, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384]
+    got = ask([e for n in widths for e in (f"ends_shape(9, {n}).waves", f"ends_shape(9, {n}).slots", f"ends_groups(100000, {n})")])
+    for i, n in enumerate(widths):
+        waves, slots, groups = got[3 * i:3 * i + 3]
+        assert n <= 256 * waves * slots and (n > 64 * waves * slots or n <= 256), n
+        assert groups * (waves if waves > 1 else 4) == 256 * 16
+
+
+@pytest.mark.skipif(shutil.which(HIPCC) is None, reason="no hipcc")
+def test_big_tile_code(tmp_path):
+    """k_linear_big writes its matrix instructions itself, and the hardware waits for neither a VALU write of their operands
+    nor a read of their results: in the code between the first and the last of them no sum is moved, no VALU instruction
+    writes an operand's register less than 16 instructions before it is read as one, and two long waits precede the reads."""
+    from stratametal_amd import build as B
+    out = str(tmp_path / "linear.s")
+    subprocess.run([HIPCC, *B.COMMON, "-S", "--cuda-device-only", os.path.join(B.CSRC, "smoe_linear.hip"), "-o", out], check=True,
+                   capture_output=True)
+    text = open(out).read()
+
+    def regs(operand):
+        r = set()
+        for a, b in re.findall(r"\bv\[(\d+):(\d+)\]", operand):
+            r |= set(range(int(a), int(b) + 1))
+        return r | {int(a) for a in re.findall(r"\bv(\d+)\b", operand)}
+
+    seen = 0
+    for m in re.finditer(r"^(_ZN4smoe12k_linear_bigI\S+?):(.*?)\.Lfunc_end", text, re.S | re.M):
+        lines = [x.strip().split(";")[0].strip() for x in m.group(2).split("\n")]
+        lines = [x for x in lines if x and not x.startswith((";", "."))]
+        mfma = [i for i, x in enumerate(lines) if x.startswith("v_mfma")]
+        assert len(mfma) == 128 and not any("accvgpr" in x for x in lines[mfma[0]:mfma[-1]])
+        loop = lines[mfma[0]:mfma[-1] + 1] * 2
+        written = {}
+        for i, x in enumerate(loop):
+            op, _, rest = x.partition(" ")
+            ops = rest.split(",")
+            if op.startswith("v_mfma"):
+                for r in regs(ops[1]) | regs(ops[2]):
+                    assert i - written.get(r, -99) >= 16, (x, r)
+            elif op.startswith("v_") and not op.startswith("v_cmp"):
+                written.update({r: i for r in regs(ops[0])})
+        after = lines[mfma[-1] + 1:]
+        first_read = next(i for i, x in enumerate(after) if re.search(r"\ba(\[|\d)", x))
+        assert sum(x.startswith("s_nop 15") for x in after[:first_read]) == 2
+        seen += 1
+    assert seen == 4
