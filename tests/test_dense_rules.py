@@ -39,6 +39,16 @@ def test_linear_plan_bounds(ask):  # noqa: F811
         assert groups >= 1
 
 
+def test_tile_cases_reach_every_kernel(ask):  # noqa: F811
+    from test_gpu_linear import SIZES, TILES
+    sizes = [(T, K, N, p) for T, K, N in SIZES for p in (0, 1)] + [(T, K, N, int(p)) for T, K, N, p, _, _ in TILES]
+    got = ask([e for T, K, N, p in sizes for e in (f"linear_plan({T}, {K}, {N}, {p}).kind", f"linear_plan({T}, {K}, {N}, {p}).slices > 1")])
+    seen = {(k, s, bool(c[3])) for k, s, c in zip(got[::2], got[1::2], sizes)}
+    assert {(FEW, 0, p) for p in (False, True)} <= seen
+    assert {(k, 0, p) for k in (T6432, T64, T12864, T128, T256) for p in (False, True)} <= seen
+    assert {k for k, s, _ in seen if s} >= {T6432, T64, T12864, T128, T256}
+
+
 def test_balance_rules(ask):  # noqa: F811
     tokens = list(range(1, 700)) + [1024, 2048, 4096, 32768, 2 ** 24]
     got = ask([e for T in tokens for e in (f"balance_groups({T})", f"balance_count_groups({T})", f"balance_one({T}, 10)")])

@@ -47,6 +47,27 @@ def test_gated_pair(T, K, N, w, y):
     check(L, x, None, "silu", L.run(x, y_dtype=TYPES[y]), y)
 
 
+# sizes on every tile, whole and in slices of K, odd ones and with a short last step among them (test_dense_rules.py holds
+# them to that): tokens, n_in, n_out, pair, residual and y's type
+TILES = [(3000, 136, 2100, True, None, "bf16"), (2999, 200, 2099, True, "f32", "f32"), (1300, 1032, 4099, True, None, "fp16"),
+         (4096, 520, 4096, False, "f32", "f32"), (640, 8192, 2048, False, "bf16", "bf16"), (640, 8192, 2048, True, None, "f32"),
+         (900, 8192, 500, True, "fp16", "fp16"), (1300, 1032, 4099, False, "bf16", "bf16"), (520, 5000, 777, False, None, "f32"),
+         (256, 2048, 512, False, "f32", "f32"), (600, 3000, 1000, True, "bf16", "bf16"), (700, 4104, 1500, False, None, "f32"),
+         (1500, 72, 1203, True, "f32", "f32"), (300, 4096, 300, True, None, "bf16"), (500, 8192, 1000, False, "f32", "f32"),
+         (257, 8200, 1003, False, "f32", "f32"), (9, 8200, 1003, False, "f32", "f32"), (33, 1032, 6000, True, None, "f32"),
+         (257, 2056, 1501, True, "bf16", "bf16"), (700, 4104, 1500, True, "f32", "f32"), (600, 3000, 999, False, "fp16", "fp16")]
+
+
+@pytest.mark.parametrize("i", range(len(TILES)))
+@pytest.mark.parametrize("w", ["bf16", "fp16"])
+def test_tiles(i, w):
+    T, K, N, pair, residual, y = TILES[i]
+    say(f"case: linear tiles {TILES[i]} {w}")
+    act = "silu" if pair else "gelu"
+    x, r, L = make(40 + i, T, K, N, w, pair=pair, act=act, residual=residual)
+    check(L, x, r, act, L.run(x, residual=r, y_dtype=TYPES[y]), y)
+
+
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("pair", [False, True])
 @pytest.mark.parametrize("T", [1, 5, 40, 300])
