@@ -167,6 +167,34 @@ __device__ __forceinline__ void finish_batch(const LinearArgs& a, int64_t t, int
     else put(std::integral_constant<int, kF16>{});
 }
 
+// The same of one output, rows of any alignment.
+template <int BATCH, int PER, bool PAIR>
+__device__ __forceinline__ void finish_column(const LinearArgs& a, int64_t t, int64_t t_end, int o, const float (&g)[BATCH],
+                                              const float (&u)[BATCH]) {
+    const bool f32 = a.y_type == kF32;
+    const float b = a.bias ? a.bias[o] : 0.0f, c = PAIR && a.bias2 ? a.bias2[o] : 0.0f;
+    uint32_t r[BATCH];
+    if (a.residual) {
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const int64_t at = min(t + k * PER, t_end - 1) * a.r_ld + o;
+            r[k] = f32 ? static_cast<const uint32_t*>(a.residual)[at] : static_cast<const uint16_t*>(a.residual)[at];
+        }
+    }
+    static_assert(BATCH % 4 == 0, "activate_all");
+    float v[BATCH / 4][4];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) v[k / 4][k % 4] = g[k] + b;
+    activate_all(v, a.act);
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+        float w = v[k / 4][k % 4];
+        if constexpr (PAIR) w = w * (u[k] + c);
+        if (a.residual) w += f32 ? u2f(r[k]) : elem_to_f32(r[k], a.y_type);
+        if (t + k * PER < t_end) store1(a.y, (t + k * PER) * a.y_ld + o, w, a.y_type);
+    }
+}
+
 // y and residual rows take 4-value vectors.
 __host__ __device__ __forceinline__ bool rows_vec(const LinearArgs& a) {
     const uintptr_t m = (a.y_type == kF32 ? 16 : 8) - 1;
@@ -285,14 +313,23 @@ __device__ __forceinline__ void tile_store(const LinearArgs& a, const f32x4 (&ac
                     put_part<PAIR>(a, blockIdx.y, t, o, *reinterpret_cast<const f32x4*>(at + i * PER * ROW),
                                    *reinterpret_cast<const f32x4*>(at + i * PER * ROW + (PAIR ? 64 : 0)));
             }
-        } else {  // rows that take no vectors: lanes take consecutive outputs
-            constexpr int OUTS = 4 * QUADS;
-#pragma unroll 4
-            for (int i = lane; i < 16 * NG * OUTS; i += 64) {
-                const int tr = i / OUTS, oc = i % OUTS, t = t0 + n * 16 + tr;
-                const uint8_t* v = mine + tr * ROW + 4 * (PAIR ? oc / 16 * 32 + oc % 16 : oc);
-                if (t < t_end && o0 + oc < a.n_out)
-                    finish1<PAIR>(a, t, o0 + oc, *reinterpret_cast<const float*>(v), *reinterpret_cast<const float*>(v + (PAIR ? 64 : 0)));
+        } else {  // rows that take no vectors: lanes take consecutive outputs of a token, a lane the same one of several
+            constexpr int OUTS = 4 * QUADS, W = OUTS < 64 ? OUTS : 64, PER1 = 64 / W, ALL = 16 * NG / PER1;
+            constexpr int B = ALL < 16 ? ALL : 16;
+            const int t2 = t0 + n * 16 + lane / W;
+#pragma unroll 1
+            for (int oc = lane % W; oc < OUTS && o0 + oc < a.n_out; oc += W) {
+                const uint8_t* v = mine + lane / W * ROW + 4 * (PAIR ? oc / 16 * 32 + oc % 16 : oc);
+#pragma unroll 1
+                for (int i = 0; i < ALL; i += B) {
+                    float g[B], u[B];
+#pragma unroll
+                    for (int k = 0; k < B; ++k) {
+                        g[k] = *reinterpret_cast<const float*>(v + (i + k) * PER1 * ROW);
+                        u[k] = PAIR ? *reinterpret_cast<const float*>(v + (i + k) * PER1 * ROW + 64) : 0.0f;
+                    }
+                    finish_column<B, PER1, PAIR>(a, t2 + i * PER1, t_end, o0 + oc, g, u);
+                }
             }
         }
     }

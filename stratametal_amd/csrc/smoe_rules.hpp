@@ -204,21 +204,22 @@ struct LinearTile {
     int per_cu;          // work-groups that a CU's LDS holds
     double fixed;        // us of a work-group beside its steps
     double step, shared; // us of a step of 64 of K, alone on a CU and with the others
+    double astride;      // as much longer with rows that start inside a 128-byte line: a step's piece of one is of two lines
 };
 constexpr LinearTile kLinearTiles[] = {{},
-                                       {64, 32, 2, 0.8, 0.18, 0.42},
-                                       {64, 64, 2, 1.5, 0.23, 0.48},
-                                       {128, 64, 2, 1.8, 0.40, 0.71},
-                                       {128, 128, 1, 2.4, 0.62, 0.62},
-                                       {256, 256, 1, 11.3, 1.24, 1.24}};
+                                       {64, 32, 2, 0.8, 0.18, 0.42, 1.0},
+                                       {64, 64, 2, 1.5, 0.23, 0.48, 1.3},
+                                       {128, 64, 2, 1.8, 0.40, 0.71, 1.4},
+                                       {128, 128, 1, 2.4, 0.62, 0.62, 1.1},
+                                       {256, 256, 1, 11.3, 1.24, 1.24, 1.0}};
 // A product's time in us, from its sizes: the rounds of work-groups over the 256 CUs times their steps, or the bytes of w and
 // x at 6 bytes a ps where those take longer, and where K is sliced the launch and the bytes that join the sums; the rows'
 // kernel reads 2048 of K at a time.  Fitted to 254 shapes (9 of 256 to 8192 by 512 to 16384, 1 to 2500 tokens, one matrix
-// and pairs), each timed by every kernel in 1 to 8 slices: the kernel of the least of it takes on average 0.8 % longer than
-// the shape's fastest, at most 18 %.  us, by few, 64 x 32, 64 x 64, 128 x 64, 128 x 128 and 256 x 256: 1 token 2048 x 2048
+// and pairs), each timed by every kernel in 1 to 8 slices: the kernel of the least of it takes on average 0.9 % longer than
+// the shape's fastest, at most 25 %.  us, by few, 64 x 32, 64 x 64, 128 x 64, 128 x 128 and 256 x 256: 1 token 2048 x 2048
 // 5.3, 8.2, 9.7, -, -, -; 8 tokens 2048 x 8192 9.9, 8.7, 10.1, -, -, -; 16 tokens 8192 x 2048 18.4, 24.8, 29.6 and in four
-// slices -, 12.9, 13.9; 128 tokens 2048 x 8192 -, -, 12.9, 18.7, 23.3, -; 301 tokens 2568 x 5003 -, -, 28.7, 28.1, 36.5, 99,
-// in two slices of 128 x 128 24.9; 4096 tokens 4096 x 4096 -, -, 232, 191, 157, 102.
+// slices -, 12.9, 13.9; 128 tokens 2048 x 8192 -, -, 12.9, 18.7, 23.3, -; 301 tokens 2560 x 5004 -, -, 21.2, 20.4, 24.3, - and in
+// two slices -, -, -, 24.4, 21.1, 37, the same of 2568 -, -, 30.0, 27.8, 30.9, - and -, -, -, 28.9, 24.1, 40; 4096 tokens 4096 x 4096 -, -, 232, 191, 157, 102.
 inline double linear_time(LinearKind kind, int slices, int64_t T, int64_t K, int64_t N, bool pair) {
     const int64_t rows = pair ? 2 * N : N;
     const double w_bytes = (double)rows * (double)K * 2, x_bytes = (double)T * (double)K * 2;
@@ -230,7 +231,8 @@ inline double linear_time(LinearKind kind, int slices, int64_t T, int64_t K, int
     const int64_t wg = (rows + t.rows - 1) / t.rows * ((T + t.tokens - 1) / t.tokens) * slices;
     const int64_t steps = ((K + 63) / 64 + slices - 1) / slices;
     const int64_t at_once = wg <= 256 ? 1 : t.per_cu, rounds = (wg + 256 * at_once - 1) / (256 * at_once);
-    const double work = (double)rounds * (t.fixed + (double)steps * (at_once == 1 ? t.step : t.shared));
+    const double step = (at_once == 1 ? t.step : t.shared) * (K % 64 ? t.astride : 1);
+    const double work = (double)rounds * (t.fixed + (double)steps * step);
     const double bytes = t.fixed + (w_bytes + x_bytes) / 6.4e6;
     return 2.4 + (work > bytes ? work : bytes) + (slices > 1 ? 2.9 + 0.31e-6 * 4 * (double)(slices * T * rows) : 0);
 }
