@@ -199,7 +199,7 @@ struct EndsArgs {
     void *out, *x;
     const float *gate, *post, *pre;
     int64_t r_ld, y_ld, out_ld, x_ld, gate_ld, gate_step;
-    int r_type, y_type, x_type, gate_sigmoid, gate_vec;
+    int r_type, y_type, x_type, gate_sigmoid, gate_unit;
     int n, n_tokens;
     float eps, res_scale, y_scale;
 };

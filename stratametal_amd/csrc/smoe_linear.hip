@@ -147,13 +147,18 @@ __device__ __forceinline__ void finish_batch(const LinearArgs& a, int64_t t, int
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[k][j] = v[k][j] * (u[k][j] + c[j]);
     }
-    if (a.residual) {
+    const auto add = [&](auto type) {  // the residual, of one type for all
+        constexpr int E = decltype(type)::value;
 #pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
+        for (int k = 0; k < BATCH; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                v[k][j] += f32 ? u2f(r[k][j]) : elem_to_f32(j & 1 ? r[k][j >> 1] >> 16 : r[k][j >> 1] & 0xFFFFu, a.y_type);
-        }
+                v[k][j] += E == kF32 ? u2f(r[k][j]) : elem_to_f32(j & 1 ? r[k][j >> 1] >> 16 : r[k][j >> 1] & 0xFFFFu, E);
+    };
+    if (a.residual) {
+        if (f32) add(std::integral_constant<int, kF32>{});
+        else if (a.y_type == kBf16) add(std::integral_constant<int, kBf16>{});
+        else add(std::integral_constant<int, kF16>{});
     }
     const auto put = [&](auto type) {
         constexpr int E = decltype(type)::value;

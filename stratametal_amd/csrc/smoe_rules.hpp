@@ -159,19 +159,20 @@ constexpr bool junction_apart(int64_t T, int E, int H, bool f32) {
                        T * E >= (H >= 2560 ? 2048 : H >= 2048 ? 4096 : 8192));
 }
 
-// The ends of a block: waves to a row, and slots of four values to a lane.
+// The ends of a block: lanes to a row, and slots of four values to a lane.
 struct EndsShape {
-    int waves, slots;
+    int lanes, slots;
 };
 constexpr int kEndsMaxRow = 16384;
-constexpr EndsShape ends_shape(int64_t T, int n) {
-    return n <= 256 ? EndsShape{1, 1} : n <= 512 ? EndsShape{1, 2} : n <= 1024 ? EndsShape{4, 1} : n <= 2048 ? EndsShape{4, 2}
-           : n <= 4096 ? EndsShape{8, 2} : n <= 8192 ? EndsShape{16, 2} : EndsShape{16, 4};
+constexpr EndsShape ends_shape(int n) {
+    return n <= 64 ? EndsShape{16, 1} : n <= 128 ? EndsShape{32, 1} : n <= 256 ? EndsShape{64, 1} : n <= 512 ? EndsShape{64, 2}
+           : n <= 1024 ? EndsShape{256, 1} : n <= 2048 ? EndsShape{256, 2} : n <= 4096 ? EndsShape{512, 2}
+           : n <= 8192 ? EndsShape{1024, 2} : EndsShape{1024, 4};
 }
 // Work-groups: as many as the chip holds at a time (16 waves to a CU), each taking rows in turn.
 constexpr int64_t ends_groups(int64_t T, int n) {
-    const int w = ends_shape(T, n).waves;
-    const int64_t sets = w == 1 ? (T + 3) / 4 : T, most = 256 * (16 / (w == 1 ? 4 : w));
+    const int lanes = ends_shape(n).lanes, rows = lanes < 256 ? 256 / lanes : 1;
+    const int64_t sets = (T + rows - 1) / rows, most = 256 * 1024 / (lanes < 256 ? 256 : lanes);
     return sets < most ? sets : most;
 }
 

@@ -52,6 +52,7 @@ __device__ __forceinline__ float exp_fast(float x) {
     const float r = __builtin_fmaf(e, rest * 0.693147181f, e);
     return e == __builtin_inff() ? e : x != x ? x : r;
 }
-__device__ __forceinline__ float sigmoid_fast(float x) { return 1.0f / (1.0f + exp_fast(-x)); }
+// (the quotient by the hardware's reciprocal: 1 ulp)
+__device__ __forceinline__ float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x)); }
 
 }  // namespace smoe

@@ -60,12 +60,14 @@ def test_balance_rules(ask):  # noqa: F811
 
 def test_ends_shapes(ask):  # noqa: F811
     """A row's slots hold it, and few lanes more."""
-    widths = [1, 8, 256, 257, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384]
-    got = ask([e for n in widths for e in (f"ends_shape(9, {n}).waves", f"ends_shape(9, {n}).slots", f"ends_groups(100000, {n})")])
+    widths = [1, 8, 64, 65, 128, 129, 256, 257, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384]
+    got = ask([e for n in widths for e in (f"ends_shape({n}).lanes", f"ends_shape({n}).slots", f"ends_groups(100000, {n})",
+                                           f"ends_groups(5, {n})")])
     for i, n in enumerate(widths):
-        waves, slots, groups = got[3 * i:3 * i + 3]
-        assert n <= 256 * waves * slots and (n > 64 * waves * slots or n <= 256), n
-        assert groups * (waves if waves > 1 else 4) == 256 * 16
+        lanes, slots, groups, few = got[4 * i:4 * i + 4]
+        assert n <= 4 * lanes * slots and (n > 2 * lanes * slots or n <= 64), n
+        assert groups * max(lanes, 256) == 256 * 1024
+        assert few == (5 if lanes >= 256 else (5 * lanes + 255) // 256)
 
 
 @pytest.mark.skipif(shutil.which(HIPCC) is None, reason="no hipcc")
