@@ -490,13 +490,14 @@ __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int t
     const int all = (a.n_in + 63) / 64;
     const int u0 = (int)((int64_t)all * blockIdx.y / gridDim.y), u1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
     const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds) + wave * 1024);
-    // values of K that are left from the lane's first one on; the buffers' bases move on by a step's 128 bytes
+    // values of K that are left from the lane's first one on; the buffers' bases move on by a step's 128 bytes, their sizes
+    // stay (less 128 a step, that of a tile of one row would fall below 0 past the end, and kOob be in range): which lanes
+    // load rests on w_left, x_left and off alone
     int w_left = min(a.n_in, u1 * 64) - 8 * ((lane & 7) ^ (lane >> 3)), x_left = w_left;
     const auto move_on = [](i32x4& r, int& left, int steps) {
         const uint64_t p = ((uint64_t)(uint32_t)r[1] << 32 | (uint32_t)r[0]) + 128u * steps;
         r[0] = (int)(uint32_t)p;
         r[1] = (int)(uint32_t)(p >> 32);
-        r[2] -= 128 * steps;
         left -= 64 * steps;
     };
     move_on(rw, w_left, u0);

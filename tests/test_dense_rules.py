@@ -47,6 +47,10 @@ def test_tile_cases_reach_every_kernel(ask):  # noqa: F811
     assert {(FEW, 0, p) for p in (False, True)} <= seen
     assert {(k, 0, p) for k in (T6432, T64, T12864, T128, T256) for p in (False, True)} <= seen
     assert {k for k, s, _ in seen if s} >= {T6432, T64, T12864, T128, T256}
+    # last tiles of 256 rows with one row, whole and in slices: the loads past the end of K stay out of range of its buffer
+    ones = {(k, s, bool(c[3])) for k, s, c in zip(got[::2], got[1::2], sizes)
+            if k == T256 and c[0] % 256 == 1 and c[2] % (128 if c[3] else 256) == 1}
+    assert ones == {(T256, 0, True), (T256, 1, False)}
 
 
 def test_balance_rules(ask):  # noqa: F811

@@ -56,7 +56,9 @@ TILES = [(3000, 136, 2100, True, None, "bf16"), (2999, 200, 2099, True, "f32", "
          (1500, 72, 1203, True, "f32", "f32"), (300, 4096, 300, True, None, "bf16"), (500, 8192, 1000, False, "f32", "f32"),
          (257, 8200, 1003, False, "f32", "f32"), (9, 8200, 1003, False, "f32", "f32"), (33, 1032, 6000, True, None, "f32"),
          (257, 2056, 1501, True, "bf16", "bf16"), (700, 4104, 1500, True, "f32", "f32"), (600, 3000, 999, False, "fp16", "fp16"),
-         (257, 2048, 5001, False, "bf16", "bf16"), (300, 1024, 2001, True, None, "f32")]
+         (257, 2048, 5001, False, "bf16", "bf16"), (300, 1024, 2001, True, None, "f32"),
+         # a last tile of one row and one token
+         (2817, 200, 2433, True, "f32", "f32"), (513, 8192, 2305, False, None, "bf16"), (1281, 520, 4097, True, None, "fp16")]
 
 
 @pytest.mark.parametrize("i", range(len(TILES)))
