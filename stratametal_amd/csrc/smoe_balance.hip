@@ -11,7 +11,7 @@
 //   k_balance_rows, k_balance_sums                   some pairs: each work-group that needs the counts counts for itself
 //   k_balance_counts, k_balance_rows, k_balance_sums a batch
 // Bound by the logits' and the gradient's bytes in a large batch (32768 tokens of 1024 experts 72 us among other calls, 268 MB),
-// by the launches' chains of latencies else: 4096 tokens of 512 experts, 10 each, 24.5 us, 64 tokens without gradients 11.
+// by the launches' chains of latencies else: 4096 tokens of 512 experts, 10 each, 24.5 us, 64 tokens without gradients 10.
 #include "smoe_gemv.hpp"
 #include "smoe_launch.hpp"
 #include "smoe_rules.hpp"
