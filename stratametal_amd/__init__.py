@@ -806,25 +806,23 @@ def router_balance(logits, ids, mask=None, balance_coef: float = 1.0, z_coef: fl
     if mask is not None:
         _need(mask, "mask", torch.uint8 if mask.dtype == torch.uint8 else torch.bool, shape=(T,))
         _on_device(mask, "mask", dev)
-    # loss, mean_p and dbias are views of one allocation
-    at = logits.device
-    sizes = (4, E, E) if grad else (4, E)
-    f = torch.empty_strided((sum(sizes),), (1,), dtype=torch.float32, device=at)
-    counts = torch.empty_strided((E,), (1,), dtype=torch.int32, device=at)
-    if T == 0:
-        f.zero_(), counts.zero_()
-    base, parts = f.data_ptr(), f.split_with_sizes(sizes)
-    out = dict(loss=parts[0], counts=counts, mean_p=parts[1])
+    at, new, f32 = logits.device, torch.empty_strided, torch.float32
+    loss, counts = new((4,), (1,), dtype=f32, device=at), new((E,), (1,), dtype=torch.int32, device=at)
+    mean_p = new((E,), (1,), dtype=f32, device=at)
+    out = dict(loss=loss, counts=counts, mean_p=mean_p)
     dp = bp = None
     if grad:
-        out["dlogits"], out["dbias"] = _new(T, E, torch.float32, at), parts[2]
-        dp, bp = out["dlogits"].data_ptr(), base + 4 * (4 + E)
+        out["dlogits"], out["dbias"] = _new(T, E, f32, at), new((E,), (1,), dtype=f32, device=at)
+        dp, bp = out["dlogits"].data_ptr(), out["dbias"].data_ptr()
+    if T == 0:
+        for t in out.values():
+            t.zero_()
     n = lib().smoe_router_balance_workspace_bytes(T, E)
     if n == 0 and T > 0:
         raise SmoeError(-1, lib().smoe_last_error().decode())
-    ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=at)
+    ws = new((n,), (1,), dtype=torch.uint8, device=at)
     _check(lib().smoe_router_balance(logits.data_ptr(), ld, ids.data_ptr(), _ptr(mask), T, E, ids.shape[1], balance_coef,
-                                     z_coef, base, counts.data_ptr(), base + 16, dp, E, bp, ws.data_ptr(), n, st))
+                                     z_coef, loss.data_ptr(), counts.data_ptr(), mean_p.data_ptr(), dp, E, bp, ws.data_ptr(), n, st))
     return out
 
 

@@ -132,3 +132,17 @@ def test_row_strides_and_gradient_in_place():
                                          got["loss"].data_ptr(), got["counts"].data_ptr(), got["mean_p"].data_ptr(),
                                          ls.data_ptr(), E + 11, None, ws.data_ptr(), n, S._stream()))
     assert torch.equal(ls, want["dlogits"]) and bool(torch.isnan(wide[:, :3]).all()) and bool(torch.isnan(wide[:, 3 + E:]).all())
+
+
+def test_results_share_no_memory():
+    """Each result is a tensor of its own: one may be changed in place, by differentiable operands too."""
+    say("case: balance results apart")
+    l, ids, _ = make(4, 33, 40, 3)
+    o = run(l, ids, None, 0.01, 0.001)
+    assert len({t.untyped_storage().data_ptr() for t in o.values()}) == len(o)
+    w = torch.ones(4, device="cuda", requires_grad=True)
+    keep = {k: t.clone() for k, t in o.items()}
+    o["loss"].mul_(w).sum().backward()
+    assert torch.equal(w.grad, keep["loss"])
+    for k in ("counts", "mean_p", "dlogits", "dbias"):
+        assert torch.equal(o[k], keep[k])
