@@ -359,9 +359,8 @@ __device__ __forceinline__ void each_of(F&& f) {
 // fragments read after its barrier: 0.67 us a step of 128 x 128 whatever the ring.)  Steps past the end load nothing: their
 // offsets lie past the buffers, zeros go to LDS, and the count of loads under way stays the same.
 // blockIdx.y: a slice of K, whose sums go to `part` ([slice][w, w2][token][n_out]) for k_linear_join.
-// Few tokens are bound by the weights' bytes (one token by two matrices of 8192 x 2048, 67 MB in tiles of 64 x 32: 12 us among
-// other calls, 30 us behind a fill of 512 MiB that leaves every cache dirty), some hundred by how few work-groups there are
-// (301 tokens, 5003 x 2568, tiles of 128 x 128 in two slices of K: 17 us and 6 to join them, 0.45 PFLOP/s).
+// Some ten tokens are bound by the weights' bytes, some hundred by how few work-groups there are (301 tokens, 5003 x 2568,
+// tiles of 128 x 128 in two slices of K: 17 us and 6 to join them, 0.45 PFLOP/s).
 template <int MT, int NT, int WM, int WN, int RING, bool PAIR, bool F16>
 __global__ __launch_bounds__(64 * WM * WN) void k_linear_tile(const LinearArgs a, int tiles_o, int tiles_t) {
     constexpr int WAVES = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
@@ -576,49 +575,84 @@ __global__ __launch_bounds__(256, 1) void k_linear_big(const LinearArgs a, int t
                              lane);
 }
 
-// Up to 16 tokens: 16 outputs to a work-group of eight waves, each every eighth 64 of K, straight from memory to the matrix
-// instruction's layout: lane l holds row (or token) l & 15, values 8 (l >> 4) .. of a 32-value piece.  Bound by the weights'
-// bytes: four blocks of 64 of K of a wave are on their way together.  Lanes past the last token hold its values, and their
-// results are dropped; the waves' sums meet in LDS, in wave order.  One token by 2048 x 2048 5.3 us, 8 tokens by 2048 x 8192
-// 9.9 (the tiles 8.2 and 8.7).
-template <bool PAIR, bool F16>
+// v[j] of lane p of a quad becomes its lane j's v[p].
+__device__ __forceinline__ void turn_quads(u32x4 (&v)[4], int lane) {
+    const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const auto pair = [&](int i, int j, bool second, auto ctrl) {
+            constexpr int CTRL = decltype(ctrl)::value;
+            const uint32_t a = v[i][d], b = v[j][d];
+            const uint32_t pa = __builtin_amdgcn_mov_dpp((int)a, CTRL, 0xF, 0xF, true);
+            const uint32_t pb = __builtin_amdgcn_mov_dpp((int)b, CTRL, 0xF, 0xF, true);
+            v[i][d] = second ? pb : a;
+            v[j][d] = second ? b : pa;
+        };
+        pair(0, 1, odd, std::integral_constant<int, 0xB1>{});  // lanes 1, 0, 3, 2
+        pair(2, 3, odd, std::integral_constant<int, 0xB1>{});
+        pair(0, 2, high, std::integral_constant<int, 0x4E>{});  // lanes 2, 3, 0, 1
+        pair(1, 3, high, std::integral_constant<int, 0x4E>{});
+    }
+}
+
+// Up to 16 tokens: 16 outputs to a work-group of eight waves, each every eighth 128 of K, straight from memory to the matrix
+// instruction's layout: lane l holds row (or token) l & 15, 8 values of each 32-value quarter l >> 4 of a block at a time.
+// That layout's own loads would have neighbouring lanes on different rows, four lines to a quad, and the L1 serve 15 bytes a
+// cycle; so the quads load 64 bytes of one row, of four rows in turn, and exchange them (turn_quads): 16 tokens by 2048 x
+// 8192 11.3 us for 16.9, by 2048 x 2048 4.9 for 6.3.  BLOCKS blocks of a wave are on their way together (linear_few_blocks).
+// Lanes past the last token hold its values, and their results are dropped; the waves' sums meet in LDS, in wave order.
+// Bound by the weights' bytes (one token by two matrices of 8192 x 2048, 67 MB, 14.5 us from HBM in turn, 4.6 TB/s; 12 where the
+// caches hold part of them, 25 behind a fill that leaves the caches dirty), in few work-groups by what a CU takes in.
+template <int BLOCKS, bool PAIR, bool F16>
 __global__ __launch_bounds__(512) void k_linear_few(const LinearArgs a) {
-    constexpr int SETS = PAIR ? 2 : 1, WAVES = 8, BLOCKS = 4;
+    constexpr int SETS = PAIR ? 2 : 1, WAVES = 8;
     __shared__ f32x4 sum_s[WAVES][SETS][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int o0 = blockIdx.x * 16, kq = 8 * (lane >> 4);
-    const size_t row = (size_t)min(o0 + (lane & 15), a.n_out - 1) * a.n_in;
+    const int o0 = blockIdx.x * 16, row = lane & 12, kl = 8 * (4 * (lane >> 4) + (lane & 3)), kq = 32 * (lane >> 4);
+    const size_t first = (size_t)o0 * a.n_in;
     const uint16_t* wp[SETS];
-    wp[0] = static_cast<const uint16_t*>(a.w) + row;
-    if constexpr (PAIR) wp[1] = static_cast<const uint16_t*>(a.w2) + row;
-    const uint16_t* xp = static_cast<const uint16_t*>(a.x) + min(lane & 15, a.n_tokens - 1) * a.x_ld;
+    wp[0] = static_cast<const uint16_t*>(a.w) + first;
+    if constexpr (PAIR) wp[1] = static_cast<const uint16_t*>(a.w2) + first;
+    const uint16_t* xp = static_cast<const uint16_t*>(a.x);
+    uint32_t w_at[4], x_at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        w_at[j] = (uint32_t)(min(row + j, a.n_out - 1 - o0) * a.n_in);
+        x_at[j] = (uint32_t)(min(row + j, a.n_tokens - 1) * (int)a.x_ld);
+    }
     f32x4 acc[SETS];
 #pragma unroll
     for (int i = 0; i < SETS; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    const int blocks = (a.n_in + 63) / 64;
+    const u32x4 zero = {0, 0, 0, 0};
+    const int blocks = (a.n_in + 127) / 128;
     for (int u = wave; u < blocks; u += BLOCKS * WAVES) {
-        uint4 wv[BLOCKS][2][SETS], xv[BLOCKS][2];
+        u32x4 wv[BLOCKS][SETS][4], xv[BLOCKS][4];
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b)
+        for (int b = 0; b < BLOCKS; ++b) {
+            const uint32_t k = min((u + b * WAVES) * 128 + kl, a.n_in - 8);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = min((u + b * WAVES) * 64 + 32 * h + kq, a.n_in - 8);
+            for (int j = 0; j < 4; ++j) {
 #pragma unroll
-                for (int i = 0; i < SETS; ++i) wv[b][h][i] = *reinterpret_cast<const uint4*>(wp[i] + k);
-                xv[b][h] = *reinterpret_cast<const uint4*>(xp + k);
+                for (int i = 0; i < SETS; ++i) wv[b][i][j] = *reinterpret_cast<const u32x4*>(wp[i] + (w_at[j] + k));
+                xv[b][j] = *reinterpret_cast<const u32x4*>(xp + (x_at[j] + k));
             }
+        }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b)
+        for (int b = 0; b < BLOCKS; ++b) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int i = 0; i < SETS; ++i) turn_quads(wv[b][i], lane);
+            turn_quads(xv[b], lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
                 // (past the row: zeros of both, whatever the last values are)
-                const bool in = (u + b * WAVES) * 64 + 32 * h + kq < a.n_in;
-                const uint4 x = in ? xv[b][h] : zero;
+                const bool in = (u + b * WAVES) * 128 + kq + 8 * j < a.n_in;
+                const u32x4 x = in ? xv[b][j] : zero;
 #pragma unroll
-                for (int i = 0; i < SETS; ++i) acc[i] = mfma16<F16>(in ? wv[b][h][i] : zero, x, acc[i]);
+                for (int i = 0; i < SETS; ++i)
+                    acc[i] = mfma16<F16>(__builtin_bit_cast(uint4, in ? wv[b][i][j] : zero), __builtin_bit_cast(uint4, x), acc[i]);
             }
+        }
     }
 #pragma unroll
     for (int i = 0; i < SETS; ++i) sum_s[wave][i][lane] = acc[i];
@@ -677,7 +711,9 @@ hipError_t launch_tile(const LinearArgs& a, int slices, hipStream_t s) {
 template <bool PAIR, bool F16>
 hipError_t launch_linear_as(const LinearArgs& a, const LinearPlan& p, hipStream_t s) {
     if (p.kind == kLinearFew) {
-        hipLaunchKernelGGL((k_linear_few<PAIR, F16>), dim3((a.n_out + 15) / 16), dim3(512), 0, s, a);
+        const dim3 grid((a.n_out + 15) / 16);
+        if (linear_few_blocks(a.n_in) == 1) hipLaunchKernelGGL((k_linear_few<1, PAIR, F16>), grid, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((k_linear_few<2, PAIR, F16>), grid, dim3(512), 0, s, a);
         return hipGetLastError();
     }
     hipError_t e = hipErrorInvalidValue;

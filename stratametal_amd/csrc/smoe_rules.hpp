@@ -213,20 +213,31 @@ constexpr LinearTile kLinearTiles[] = {{},
                                        {128, 64, 2, 1.8, 0.40, 0.71, 1.4},
                                        {128, 128, 1, 2.4, 0.62, 0.62, 1.1},
                                        {256, 256, 1, 11.3, 1.24, 1.24, 1.0}};
-// A product's time in us, from its sizes: the rounds of work-groups over the 256 CUs times their steps, or the bytes of w and
-// x at 6 bytes a ps where those take longer, and where K is sliced the launch and the bytes that join the sums; the rows'
-// kernel reads 2048 of K at a time.  Fitted to 254 shapes (9 of 256 to 8192 by 512 to 16384, 1 to 2500 tokens, one matrix
-// and pairs), each timed by every kernel in 1 to 8 slices: the kernel of the least of it takes on average 0.9 % longer than
-// the shape's fastest, at most 25 %.  us, by few, 64 x 32, 64 x 64, 128 x 64, 128 x 128 and 256 x 256: 1 token 2048 x 2048
-// 5.3, 8.2, 9.7, -, -, -; 8 tokens 2048 x 8192 9.9, 8.7, 10.1, -, -, -; 16 tokens 8192 x 2048 18.4, 24.8, 29.6 and in four
-// slices -, 12.9, 13.9; 128 tokens 2048 x 8192 -, -, 12.9, 18.7, 23.3, -; 301 tokens 2560 x 5004 -, -, 21.2, 20.4, 24.3, - and in
-// two slices -, -, -, 24.4, 21.1, 37, the same of 2568 -, -, 30.0, 27.8, 30.9, - and -, -, -, 28.9, 24.1, 40; 4096 tokens 4096 x 4096 -, -, 232, 191, 157, 102.
+// The rows' kernel: blocks of 128 of K that each of a work-group's eight waves has on its way: one where two would not come
+// out even (1 and 2, us, 1 token, n_in x n_out: 512 x 512 2.9 and 3.3, 1024 x 16384 7.9 and 9.9, 2568 x 5003 8.4 and 9.2;
+// 2048 x 2048 5.1 and 4.9, 4096 x 4096 8.6 and 8.2, 8192 x 2048 11.4 and 10.3).
+constexpr int linear_few_blocks(int64_t K) {
+    const int64_t each = (K + 1023) / 1024;  // a wave's blocks
+    return each == 1 || each == 3 ? 1 : 2;
+}
+// A product's time in us, from its sizes (n_in x n_out below): the rounds of work-groups over the 256 CUs times their
+// steps, or the bytes of w and x at 6 bytes a ps where those take longer, and where K is sliced the launch and the bytes
+// that join the sums; the rows' kernel takes in the weights by each CU's rate.  Fitted to 254 shapes (9 of 256 to 8192 by
+// 512 to 16384, 1 to 2500 tokens, one matrix and pairs), each timed by every kernel in 1 to 8 slices: the kernel of the
+// least of it takes on average 0.9 % longer than the shape's fastest, at most 25 %; the rows' kernel anew to 36 of 1 and
+// 16 tokens, its choice within 5 % but for one matrix 8192 x 512 (tiles in slices 10.6 for 9.6).  us, by few, 64 x 32, 64
+// x 64, 128 x 64, 128 x 128 and 256 x 256: 1 token 2048 x 2048 4.9, 8.2, 9.7, -, -, -; 9 tokens 2048 x 8192 8.2, 8.6,
+// 10.1, -, -, -; 16 tokens 8192 x 2048 11.3, 24.1, 29.6 and in four slices -, 12.0, 13.9, by two matrices 21.4, 27.9 and
+// in four slices 18.6; 128 tokens 2048 x 8192 -, -, 12.9, 18.7, 23.3, -; 301 tokens 2560 x 5004 -, -, 21.2, 20.4, 24.3, -
+// and in two slices -, -, -, 24.4, 21.1, 37, the same of 2568 -, -, 30.0, 27.8, 30.9, - and -, -, -, 28.9, 24.1, 40; 4096
+// tokens 4096 x 4096 -, -, 232, 191, 157, 102.
 inline double linear_time(LinearKind kind, int slices, int64_t T, int64_t K, int64_t N, bool pair) {
     const int64_t rows = pair ? 2 * N : N;
     const double w_bytes = (double)rows * (double)K * 2, x_bytes = (double)T * (double)K * 2;
     if (kind == kLinearFew) {
-        const double wg = (double)((N + 15) / 16), trips = (double)((K + 2047) / 2048) * 3.4 * (wg > 512 ? wg / 512 : 1);
-        return 3.4 + (trips > w_bytes / 6.0e6 ? trips : w_bytes / 6.0e6) * (1 + 0.003 * (double)(T - 1));
+        const int64_t wg = (N + 15) / 16;
+        const double cus = w_bytes / ((double)(wg < 256 ? wg : 256) * (pair ? 31e3 : 36e3));  // what a CU takes in
+        return 2.9 + (cus > w_bytes / 6.4e6 ? cus : w_bytes / 6.4e6) * (1 + 0.002 * (double)(T - 1));
     }
     const LinearTile& t = kLinearTiles[kind];
     const int64_t wg = (rows + t.rows - 1) / t.rows * ((T + t.tokens - 1) / t.tokens) * slices;

@@ -16,7 +16,7 @@ FEW, T6432, T64, T12864, T128, T256 = range(6)
 def test_linear_plan(ask):  # noqa: F811
     """tokens, n_in, n_out, pair -> a kernel and slices within a tenth of the fastest measured."""
     cases = [(1, 2048, 2048, 0, {(FEW, 1)}), (1, 4096, 4096, 0, {(FEW, 1)}), (1, 2048, 8192, 1, {(FEW, 1), (T6432, 1), (T64, 1)}),
-             (12, 2048, 8192, 0, {(T6432, 1)}), (16, 8192, 2048, 0, {(T6432, 4), (T6432, 8)}), (128, 2048, 8192, 0, {(T64, 1)}),
+             (12, 2048, 8192, 0, {(FEW, 1)}), (16, 8192, 2048, 0, {(FEW, 1)}), (16, 8192, 2048, 1, {(T6432, 4)}), (128, 2048, 8192, 0, {(T64, 1)}),
              (12, 4096, 4096, 1, {(FEW, 1), (T6432, 1), (T6432, 4), (T64, 1), (T12864, 4), (T128, 4)}),
              (512, 4096, 4096, 0, {(T12864, 1), (T128, 2)}), (4096, 4096, 4096, 0, {(T256, 1)}),
              (4096, 2048, 8192, 1, {(T256, 1)}), (4096, 8192, 8192, 0, {(T256, 1)})]
@@ -40,11 +40,14 @@ def test_linear_plan_bounds(ask):  # noqa: F811
 
 
 def test_tile_cases_reach_every_kernel(ask):  # noqa: F811
-    from test_gpu_linear import SIZES, TILES
+    from test_gpu_linear import FEW as ROWS, SIZES, TILES
     sizes = [(T, K, N, p) for T, K, N in SIZES for p in (0, 1)] + [(T, K, N, int(p)) for T, K, N, p, _, _ in TILES]
     got = ask([e for T, K, N, p in sizes for e in (f"linear_plan({T}, {K}, {N}, {p}).kind", f"linear_plan({T}, {K}, {N}, {p}).slices > 1")])
     seen = {(k, s, bool(c[3])) for k, s, c in zip(got[::2], got[1::2], sizes)}
     assert {(FEW, 0, p) for p in (False, True)} <= seen
+    kinds = ask([f"linear_plan({T}, {K}, {N}, {p}).kind" for T, K, N in ROWS for p in (0, 1)])
+    blocks = ask([f"linear_few_blocks({K})" for _, K, _ in ROWS for p in (0, 1)])
+    assert {(b, p) for k, b, p in zip(kinds, blocks, (0, 1) * len(ROWS)) if k == FEW} == {(1, 0), (1, 1), (2, 0), (2, 1)}
     assert {(k, 0, p) for k in (T6432, T64, T12864, T128, T256) for p in (False, True)} <= seen
     assert {k for k, s, _ in seen if s} >= {T6432, T64, T12864, T128, T256}
     # last tiles of 256 rows with one row, whole and in slices: the loads past the end of K stay out of range of its buffer

@@ -71,6 +71,18 @@ def test_tiles(i, w):
     check(L, x, r, act, L.run(x, residual=r, y_dtype=TYPES[y]), y)
 
 
+# rows in one and in two blocks of 128 at a time, whole and short last ones, few outputs and tokens past a multiple of 16
+FEW = [(T, K, N) for K in (8, 72, 128, 1016, 1032, 2048, 2056, 2568, 4104) for T, N in ((1, 17), (3, 1), (16, 77))]
+
+
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("T,K,N", FEW)
+def test_few_tokens(T, K, N, pair):
+    say(f"case: linear few T={T} K={K} N={N} pair={pair}")
+    x, r, L = make(60 + T, T, K, N, pair=pair, act="silu", residual="f32")
+    check(L, x, r, "silu", L.run(x, residual=r), "f32")
+
+
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("pair", [False, True])
 @pytest.mark.parametrize("T", [1, 5, 40, 300])
