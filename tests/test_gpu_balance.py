@@ -134,6 +134,7 @@ def test_row_strides_and_gradient_in_place():
     assert torch.equal(ls, want["dlogits"]) and bool(torch.isnan(wide[:, :3]).all()) and bool(torch.isnan(wide[:, 3 + E:]).all())
 
 
+@pytest.mark.gpu
 def test_results_share_no_memory():
     """Each result is a tensor of its own: one may be changed in place, by differentiable operands too."""
     say("case: balance results apart")
