@@ -139,11 +139,12 @@ struct Rows {
                 if (col(j) < E) d[col(j)] = g[j];
         }
     }
-    // bf: cb E f / n.  A row's e^(v - top) is 2^(v log2 e - c), c = top log2 e as rounded, which every p and lse share; a top
-    // whose c is near f32's end takes v - top first.
+    // bf: cb E f / n.  A row's e^(v - top) is 2^(v log2 e - c), c = top log2 e as rounded: every e^v and their sum share a
+    // factor 2^d, d the rounding of c, that p is free of and lse takes back.  d grows with top (past 2^31 the factor itself
+    // leaves f32), so a row whose top is beyond kFar, where |d| is at most 1/16, takes v - top first.
     __device__ __forceinline__ double run(int64_t t, int64_t step, const float (&bf)[NJ], float inv_n, float (&psum)[NJ],
                                           float (&dsum)[NJ]) {
-        constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+        constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kFar = 0x1p20f;
         double zsum = 0.0;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) psum[j] = dsum[j] = 0.0f;
@@ -166,7 +167,8 @@ struct Rows {
             for (int j = 1; j < NJ; ++j) top = __builtin_fmaxf(top, v[j]);
             top = wave_max_fast(top);
             float c = top * kLog2e;
-            if (__builtin_fabsf(top) > 1e30f) {  // (the same in every lane)
+            const bool far = __builtin_fabsf(top) > kFar;  // (the same in every lane)
+            if (far) {
                 const float shift = top == -__builtin_inff() ? 0.0f : top;  // a row of -inf alone: every e^v is 0
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) v[j] = v[j] - shift;
@@ -182,7 +184,7 @@ struct Rows {
             const bool none = sum == 0.0f;
             const float inv = none ? 0.0f : 1.0f / sum;
             const float log_sum = __builtin_logf(sum);
-            const float lse = none ? 0.0f : __builtin_fabsf(top) > 1e30f ? top + log_sum : __builtin_fmaf(c, kLn2, log_sum);
+            const float lse = none ? 0.0f : far ? top + log_sum : __builtin_fmaf(c, kLn2, log_sum);
             zsum += (double)lse * (double)lse;
             float fp = 0.0f;
 #pragma unroll

@@ -147,3 +147,21 @@ def test_results_share_no_memory():
     assert torch.equal(w.grad, keep["loss"])
     for k in ("counts", "mean_p", "dlogits", "dbias"):
         assert torch.equal(o[k], keep[k])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top", [1e6, 1e7, 2e9, 1e10, 1e12, 1e20, 9e29, 1e31])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("T,E", [(20, 130), (300, 512)])
+def test_counted_rows_far_out(top, sign, T, E):
+    """Counted rows whose largest logit is far from zero: all of them alike, as a fill leaves them, or some steps of f32 apart
+    (p as of any row); by one work-group and by many, without gradients too."""
+    say(f"case: balance far rows top={sign * top} T={T} E={E}")
+    l, ids, _ = make(7, T, E, 4)
+    far = np.float32(sign * top)
+    l[1] = far
+    l[2::5] = far + np.float32(np.spacing(np.abs(far))) * np.round(3 * l[2::5])
+    l[3, ::2] = far if sign > 0 else -np.inf
+    want, bound = D.balance(l, ids, None, 0.5, 1e-8)
+    check(run(l, ids, None, 0.5, 1e-8), want, bound)
+    check(run(l, ids, None, 0.5, 1e-8, grad=False), want, bound)
