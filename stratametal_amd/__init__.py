@@ -712,15 +712,13 @@ def _given(t, name: str):
 
 class Linear:
     """The dense product with its epilogue (smoe_linear_run): y = act(x w' + bias) [* (x w2' + bias2)] [+ residual].
-    `w` and `w2` are (n_out, n_in) tensors of bfloat16 (or int16: bf16 bits) or float16, the biases f32 [n_out].  The
-    weights stay the caller's tensors."""
+    `w` and `w2` are (n_out, n_in) tensors (or flat ones of those rows) of bfloat16 (or int16: bf16 bits) or float16, the
+    biases f32 [n_out].  The weights stay the caller's tensors."""
 
     def __init__(self, n_in: int, n_out: int, w, bias=None, w2=None, bias2=None, act: int = ACT_NONE):
         for t, name in ((w, "w"), (w2, "w2")):
             if t is not None:
-                _need(t, name, w.dtype)
-                if t.numel() != n_in * n_out:
-                    raise SmoeError(-2, f"{name} has {t.numel()} elements, needs {n_out} x {n_in}")
+                _need(t, name, w.dtype, shape=(n_in * n_out,) if getattr(t, "ndim", 2) == 1 else (n_out, n_in))
                 _on_device(t, name, w.get_device())
         self.n_in, self.n_out, self.dtype = n_in, n_out, w.dtype
         self.tensors = (w, w2, _vector(bias, "bias", n_out), _vector(bias2, "bias2", n_out))

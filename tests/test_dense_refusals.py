@@ -116,3 +116,18 @@ def test_binding_refuses_bad_tensors():
         with pytest.raises(S.SmoeError) as err:
             fn()
         assert why in str(err.value), (why, str(err.value))
+
+
+def test_linear_refuses_weights_of_other_shapes():
+    """A weight's shape is (n_out, n_in), or flat: the same number of values in other rows is not the layer's."""
+    t = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16)  # noqa: E731
+    for fn, why in [
+        (lambda: S.Linear(64, 16, t(64, 16)), "w has shape (64, 16), needs (16, 64)"),
+        (lambda: S.Linear(64, 16, t(8, 128)), "shape"), (lambda: S.Linear(64, 16, t(2, 8, 64)), "shape"),
+        (lambda: S.Linear(64, 16, t(1023)), "shape"), (lambda: S.Linear(64, 16, t(17, 64)), "shape"),
+        # (as far as the refusal of host memory: the shape is right)
+        (lambda: S.Linear(64, 16, t(16, 64)), "not a GPU"), (lambda: S.Linear(64, 16, t(1024)), "not a GPU"),
+    ]:
+        with pytest.raises(S.SmoeError) as err:
+            fn()
+        assert why in str(err.value), (why, str(err.value))

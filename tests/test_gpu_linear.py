@@ -147,3 +147,15 @@ def test_same_bits_each_run():
         y = L.run(x, y_dtype=torch.float32)
         for _ in range(3):
             assert torch.equal(L.run(x, y_dtype=torch.float32), y)
+
+
+def test_weight_shapes():
+    """Flat weights are the (n_out, n_in) ones' rows; a second weight of another shape is refused as the first one is."""
+    say("case: linear weight shapes")
+    x, _, L = make(70, 5, 64, 16, pair=True, act="silu")
+    w, w2, b, b2 = L.tensors
+    flat = S.Linear(64, 16, w.reshape(-1), bias=b, w2=w2.reshape(-1), bias2=b2, act=S.ACT_SILU)
+    assert torch.equal(flat.run(x), L.run(x))
+    for bad in (w2.t().contiguous(), w2.reshape(8, 128), w2[:15]):
+        with pytest.raises(S.SmoeError, match="w2 has shape"):
+            S.Linear(64, 16, w, w2=bad)
