@@ -449,8 +449,9 @@ smoe_status smoe_router_margin(const float* logits, int32_t n_tokens, int32_t n_
  * and with dbias [n_expert] its sum over the tokens (the gradient to smoe_weights' logit_bias).  A token repeated in ids
  * counts each time, an id outside [0, n_expert) not at all.  No token counts (n = 0): every result is 0.  Logits of -inf
  * have p = 0; a counted row of them alone has p = 0 and lse = 0; other tokens' values, NaN or not, reach nothing.
- * n_expert 1 .. 1024, k 1 .. 64, at most 2^24 pairs; zero tokens launch nothing.  The same bits in every run.  No
- * counterpart in the reference, which does not train. */
+ * n_expert 1 .. 1024, k 1 .. 64, at most 2^24 pairs; zero tokens launch nothing.  dlogits may be logits' own rows (the same
+ * address and stride); else no output and not the workspace (256-byte aligned) shares a byte with an input or another of
+ * them.  The same bits in every run.  No counterpart in the reference, which does not train. */
 size_t smoe_router_balance_workspace_bytes(int32_t max_tokens, int32_t n_expert);
 smoe_status smoe_router_balance(const float* logits, int64_t logits_ld, const int32_t* ids, const uint8_t* mask,
                                 int32_t n_tokens, int32_t n_expert, int32_t k, float balance_coef, float z_coef, float* loss,

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <iterator>
 #include <string>
 
 #include "smoe_launch.hpp"
@@ -39,9 +40,17 @@ Span rows_of(const void* p, int32_t type, int64_t rows, int64_t ld, int64_t n) {
     const int64_t es = (int64_t)elem_size(type);
     return {p, rows, rows > 1 ? ld * es : n * es, n * es};
 }
-// Whether a written span shares a byte with another: columns of one matrix (the same step) that lie apart do not.
+Span bytes_of(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+// Whether a written span shares a byte with another: columns of one matrix (the same step) that lie apart do not, nor does
+// one row between the rows of a matrix.
 bool overlap(const Span& a, const Span& b) {
     if (!a.p || !b.p || a.hi() <= b.lo() || b.hi() <= a.lo()) return false;
+    if (a.rows == 1 && b.rows > 1) return overlap(b, a);
+    if (b.rows == 1 && a.step >= a.width) {
+        const int64_t from = (int64_t)(b.lo() - a.lo());  // of a's rows, the first that ends past b's start
+        const int64_t i = from < a.width ? 0 : (from - a.width) / a.step + 1;
+        return i < a.rows && i * a.step < from + b.width;
+    }
     if (a.step != b.step || a.step < a.width || a.step < b.width) return true;
     const int64_t at = ((int64_t)(b.lo() - a.lo()) % a.step + a.step) % a.step;  // b's rows within a's step
     return at < a.width || at + b.width > a.step;
@@ -217,10 +226,22 @@ smoe_status smoe_router_balance(const float* logits, int64_t logits_ld, const in
     if (workspace_bytes < need)
         return fail(SMOE_ESIZE, "router_balance workspace is " + std::to_string(workspace_bytes) + " bytes, needs " +
                                     std::to_string(need));
+    // (one work-group writes while others still read, and the ids and the mask are read by every launch)
     const Span sl = rows_of(logits, SMOE_F32, n_tokens, logits_ld, n_expert),
-               sd = rows_of(dlogits, SMOE_F32, n_tokens, dlogits_ld, n_expert);
+               sd = rows_of(dlogits, SMOE_F32, n_tokens, dlogits_ld, n_expert), ws = bytes_of(workspace, (int64_t)need);
+    const Span in[] = {sl, bytes_of(ids, (int64_t)n_tokens * k * 4), bytes_of(mask, n_tokens)};
+    const Span out[] = {sd, bytes_of(loss, 16), bytes_of(counts, 4 * n_expert), bytes_of(mean_p, 4 * n_expert),
+                        bytes_of(dbias, 4 * n_expert), ws};
     if (overlap(sd, sl) && !same(sd, sl))
-        return fail(SMOE_EINVAL, "router_balance: dlogits is logits' own rows or shares none with them");
+        return fail(SMOE_EINVAL, "router_balance: dlogits overlaps logits and is not their own rows");
+    for (const Span& o : out) {
+        for (const Span& i : in)
+            if (!(&o == &out[0] && &i == &in[0]) && overlap(o, i))
+                return fail(SMOE_EINVAL, "router_balance: an output or the workspace overlaps logits, ids or mask");
+        for (const Span* q = &o + 1; q < std::end(out); ++q)
+            if (overlap(o, *q))
+                return fail(SMOE_EINVAL, "router_balance: two outputs, or one and the workspace, overlap");
+    }
     smoe::BalanceArgs a{};
     a.logits = logits, a.ids = ids, a.mask = mask;
     a.loss = loss, a.mean_p = mean_p, a.dlogits = dlogits, a.dbias = dbias, a.counts = counts;

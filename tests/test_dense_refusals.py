@@ -10,6 +10,7 @@ import stratametal_amd as S
 A = 0x10000000  # addresses of buffers far apart, 256-byte aligned
 B, D, E, F, G = (A + (i << 34) for i in range(1, 6))
 OK, EINVAL, ESIZE, ETYPE, EALIGN, ENULL = 0, -1, -2, -3, -5, -6
+EDEVICE = -4
 BIG = float("inf")
 
 
@@ -131,3 +132,35 @@ def test_linear_refuses_weights_of_other_shapes():
         with pytest.raises(S.SmoeError) as err:
             fn()
         assert why in str(err.value), (why, str(err.value))
+
+
+@pytest.mark.parametrize("want,kw", [
+    # an output over an input
+    (EINVAL, dict(loss=B + 8)), (EINVAL, dict(counts=B + 64)), (EINVAL, dict(p=A + 448)), (EINVAL, dict(p=A - 60)),
+    (EINVAL, dict(d=B)), (EINVAL, dict(d=B - 8 * 64 + 4)), (EINVAL, dict(d=F, db=B + 124)),
+    (EINVAL, dict(mask=D + 12)), (EINVAL, dict(mask=D + 256 + 60)), (EINVAL, dict(mask=F, d=F)),
+    # two outputs
+    (EINVAL, dict(loss=D + 256)), (EINVAL, dict(counts=D + 12)), (EINVAL, dict(p=D + 256 + 60)), (EINVAL, dict(d=D)),
+    (EINVAL, dict(d=F, db=F + 64)), (EINVAL, dict(d=F, db=D + 8192)), (EINVAL, dict(d=A, db=A + 4)),
+    # columns of one matrix lie apart: the gradient beside the logits passes, its dbias over either does not
+    (EINVAL, dict(ld=40, d=A + 64, dld=40, db=A + 32 * 4)), (EINVAL, dict(ld=40, d=F, dld=40, db=F + 160 + 60)),
+    (EINVAL, dict(ld=40, d=F, dld=40, db=F + 160 - 60)), (EINVAL, dict(ld=40, p=A + 7 * 160 + 60)),
+    # the workspace
+    (EINVAL, dict(ws=A)), (EINVAL, dict(ws=B)), (EINVAL, dict(ws=D)), (EINVAL, dict(ws=D + 8192)), (EINVAL, dict(mask=E + 8)),
+    (EINVAL, dict(d=E + 64)), (EINVAL, dict(d=F, db=E)),
+])
+def test_balance_overlaps(want, kw):
+    """What one work-group writes while another reads it is refused; 8 tokens of 16 experts, 4 each."""
+    assert balance(**kw) == want
+    assert "overlap" in S.lib().smoe_last_error().decode()
+
+
+def test_apart_is_not_overlapping():
+    """What lies between a matrix's rows, or before and behind them, shares nothing with it: refused for another reason, that
+    comes after the overlaps (no GPU here), or not at all."""
+    if torch.cuda.is_available():
+        pytest.skip("the calls would run, on addresses that are nobody's")
+    for kw in (dict(ld=40, d=F, dld=40, db=F + 64), dict(ld=40, p=A + 3 * 160 + 96, loss=A + 5 * 160 + 64), dict(d=F, db=F + 512),
+               dict(d=F, db=F - 64), dict(ld=40, d=A + 64, dld=40, db=G), dict(p=A + 512), dict(ids=D + 16, counts=D + 144),
+               dict(ld=40, p=A + 7 * 160 + 64)):
+        assert balance(**kw) == EDEVICE, kw
