@@ -273,8 +273,8 @@ typedef struct {
 size_t smoe_linear_workspace_bytes(const smoe_linear* L, int32_t n_tokens);
 
 /* x 16-byte aligned, x_ld a multiple of 8 (at most 2^21); residual of y's type, NULL for none; y may be residual's own
- * rows (the same address and row stride) and share no other byte with an input.  `workspace`: 256-byte aligned, read by no
- * later call; concurrent calls need distinct ones.  Every result is the same bits in every run. */
+ * rows (the same address and row stride) and share no other byte with an input.  `workspace`: 256-byte aligned, apart from
+ * every operand, read by no later call; concurrent calls need distinct ones.  Every result is the same bits in every run. */
 smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, int32_t n_tokens, const void* residual,
                             int64_t r_ld, void* y, int32_t y_type, int64_t y_ld, void* workspace, size_t workspace_bytes,
                             void* hip_stream);

@@ -166,10 +166,11 @@ smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, i
     const Span sr = rows_of(residual, y_type, n_tokens, r_ld, L->n_out);
     const int64_t wb = (int64_t)L->n_out * L->n_in;
     if (overlap(sy, sr) && !same(sy, sr)) return fail(SMOE_EINVAL, "linear: y is residual's own rows or shares none with it");
-    for (const Span& in : {rows_of(x, L->w_type, n_tokens, x_ld, L->n_in), rows_of(L->w, L->w_type, 1, 0, wb),
-                           rows_of(L->w2, L->w_type, 1, 0, wb), rows_of(L->bias, SMOE_F32, 1, 0, L->n_out),
-                           rows_of(L->bias2, SMOE_F32, 1, 0, L->n_out)})
-        if (overlap(sy, in)) return fail(SMOE_EINVAL, "linear: y overlaps x, a weight or a bias");
+    const Span in[] = {rows_of(x, L->w_type, n_tokens, x_ld, L->n_in), rows_of(L->w, L->w_type, 1, 0, wb),
+                       rows_of(L->w2, L->w_type, 1, 0, wb), rows_of(L->bias, SMOE_F32, 1, 0, L->n_out),
+                       rows_of(L->bias2, SMOE_F32, 1, 0, L->n_out)};
+    for (const Span& i : in)
+        if (overlap(sy, i)) return fail(SMOE_EINVAL, "linear: y overlaps x, a weight or a bias");
     const smoe::LinearPlan plan = smoe::linear_plan(n_tokens, L->n_in, L->n_out, L->w2 != nullptr);
     if (smoe::linear_groups(plan, n_tokens, L->n_out, L->w2 != nullptr) >= smoe::kGridGroups)
         return fail(SMOE_EINVAL, "linear: the product exceeds a launch's grid: split it");
@@ -180,6 +181,10 @@ smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, i
         if (workspace_bytes < need)
             return fail(SMOE_ESIZE, "linear workspace is " + std::to_string(workspace_bytes) + " bytes, needs " +
                                         std::to_string(need));
+        const Span ws = bytes_of(workspace, (int64_t)need);
+        bool shared = overlap(ws, sy) || overlap(ws, sr);
+        for (const Span& i : in) shared = shared || overlap(ws, i);
+        if (shared) return fail(SMOE_EINVAL, "linear: the workspace overlaps y, residual, x, a weight or a bias");
     }
     smoe::LinearArgs a{};
     a.x = x, a.w = L->w, a.w2 = L->w2, a.residual = residual, a.bias = L->bias, a.bias2 = L->bias2, a.y = y;

@@ -164,3 +164,12 @@ def test_apart_is_not_overlapping():
                dict(d=F, db=F - 64), dict(ld=40, d=A + 64, dld=40, db=G), dict(p=A + 512), dict(ids=D + 16, counts=D + 144),
                dict(ld=40, p=A + 7 * 160 + 64)):
         assert balance(**kw) == EDEVICE, kw
+
+
+@pytest.mark.parametrize("kw", [dict(ws=A), dict(ws=B), dict(ws=D), dict(r=E + 4096), dict(b=E + 256), dict(w2=E + 16),
+                                dict(w2=F, b2=E + 256), dict(y=E + 1024, yt=S.BF16), dict(x=E + 64, T=40)])
+def test_linear_workspace_apart(kw):
+    """Where K is sliced the workspace is written while x, the weights and the residual are read: it shares no byte with them."""
+    kw = dict(dict(n_in=8192, n_out=64, T=100), **kw)
+    assert linear(**kw) == EINVAL
+    assert "workspace" in S.lib().smoe_last_error().decode()
