@@ -439,8 +439,9 @@ smoe_status smoe_router_topk(const float* logits, int32_t n_tokens, int32_t n_ex
 smoe_status smoe_router_margin(const float* logits, int32_t n_tokens, int32_t n_expert, int32_t k, float* stats,
                                int32_t* ids, void* hip_stream);
 
-/* The load of the router over a batch: logits [T][n_expert] f32 (rows logits_ld apart), the experts ids [T][k] that were
- * selected from them, and the tokens that count (mask [T], a byte each, nonzero: counts; NULL: all), n of them:
+/* The load of the router over a batch: logits [T][n_expert] f32 (rows logits_ld apart; 0: one row for every
+ * token), the experts ids [T][k] that were selected from them, and the tokens that count (mask [T], a byte each, nonzero:
+ * counts; NULL: all), n of them:
  *   p = softmax(logits), lse = log sum exp(logits); counts[e] = pairs of such tokens with ids e; f_e = counts[e] / (n k);
  *   mean_p[e] = mean p_e; balance = n_expert sum_e f_e mean_p[e]; z = mean lse^2;
  *   loss = {balance_coef balance + z_coef z, balance, z, n}.

@@ -221,7 +221,7 @@ smoe_status smoe_router_balance(const float* logits, int64_t logits_ld, const in
     if (n_tokens == 0) return ok();
     if (!logits || !ids || !loss || !counts || !mean_p || !workspace) return fail(SMOE_ENULL, "router_balance: NULL buffer");
     if (dbias && !dlogits) return fail(SMOE_ENULL, "router_balance: dbias without dlogits");
-    if (bad_ld(logits_ld, n_tokens, n_expert) || (dlogits && bad_ld(dlogits_ld, n_tokens, n_expert)))
+    if ((logits_ld != 0 && bad_ld(logits_ld, n_tokens, n_expert)) || (dlogits && bad_ld(dlogits_ld, n_tokens, n_expert)))
         return fail(SMOE_EINVAL, "router_balance: rows overlap");
     for (const void* p : {(const void*)logits, (const void*)ids, (const void*)loss, (const void*)counts, (const void*)mean_p,
                           (const void*)dlogits, (const void*)dbias})

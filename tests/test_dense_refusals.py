@@ -173,3 +173,12 @@ def test_linear_workspace_apart(kw):
     kw = dict(dict(n_in=8192, n_out=64, T=100), **kw)
     assert linear(**kw) == EINVAL
     assert "workspace" in S.lib().smoe_last_error().decode()
+
+
+def test_balance_row_strides():
+    """Logits of one row for every token pass (to the launch, which finds no GPU here); rows that overlap, a gradient of one
+    row and a gradient over the broadcast row do not."""
+    for kw in (dict(ld=-16), dict(ld=1), dict(d=F, dld=0), dict(ld=0, d=A), dict(ld=0, d=A, dld=0), dict(ld=0, d=A - 448)):
+        assert balance(**kw) == EINVAL, kw
+    if not torch.cuda.is_available():
+        assert balance(ld=0) == EDEVICE and balance(ld=0, d=A + 64) == EDEVICE

@@ -165,3 +165,17 @@ def test_counted_rows_far_out(top, sign, T, E):
     want, bound = D.balance(l, ids, None, 0.5, 1e-8)
     check(run(l, ids, None, 0.5, 1e-8), want, bound)
     check(run(l, ids, None, 0.5, 1e-8, grad=False), want, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E", [(1, 12), (40, 129), (300, 512)])
+def test_one_row_for_every_token(T, E):
+    """Logits broadcast over the tokens (row stride 0) give what their copies give."""
+    say(f"case: balance broadcast T={T} E={E}")
+    l, ids, mask = make(9, T, E, 4, 0.8)
+    one = torch.from_numpy(l[:1]).cuda().expand(T, E)
+    it, m = torch.from_numpy(ids).cuda(), torch.from_numpy(mask).cuda()
+    for grad in (False, True):
+        got = S.router_balance(one, it, mask=m, balance_coef=0.3, z_coef=0.2, grad=grad)
+        want = S.router_balance(one.contiguous(), it, mask=m, balance_coef=0.3, z_coef=0.2, grad=grad)
+        assert all(torch.equal(got[name], want[name]) for name in want)
