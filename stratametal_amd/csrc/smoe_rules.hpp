@@ -181,8 +181,10 @@ constexpr int64_t ends_groups(int64_t T, int n) {
 constexpr bool balance_one(int64_t T, int k) { return T <= 64 && T * k <= 4096; }
 // The pairs counted first, by a launch of their own, or by every work-group that needs them: with gradients those of the rows
 // (us apart and not: 2560 pairs 18.7 and 19.5 with a mask, 17.6 and 17.0 without, 5120 19.5 and 23.2, 10240 20.5 and
-// 28.8), else those of the sums, few and large (10240 pairs 16.4 and 15.5).
-constexpr bool balance_counts_apart(int64_t T, int k, bool grad) { return T * k > (grad ? 3000 : 12000); }
+// 28.8), else those of the sums, few and large (10240 pairs 16.4 and 15.5).  One work-group has no other to count for.
+constexpr bool balance_counts_apart(int64_t T, int k, bool grad) {
+    return !balance_one(T, k) && T * k > (grad ? 3000 : 12000);
+}
 // Work-groups of four rows at a time, at most 1024 (k_balance_sums): each leaves a row of partial sums (4096 tokens of 512
 // experts 27.5 us with 256 or 512 of them, 31.8 with 1024, 30.4 with 128; 32768 of 1024 99, 77.5, 79.8, 151).
 constexpr int64_t balance_groups(int64_t T) { return T < 4 ? 1 : (T + 3) / 4 < 512 ? (T + 3) / 4 : 512; }

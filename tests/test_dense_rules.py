@@ -65,6 +65,15 @@ def test_balance_rules(ask):  # noqa: F811
     assert all(o == (T <= 64) for o, T in zip(one, tokens))
 
 
+def test_balance_counts_only_where_read(ask):  # noqa: F811
+    """One work-group for a few tokens counts for itself: no launch of counts beside it."""
+    calls = [(T, k, g) for T in (1, 40, 47, 63, 64, 65, 300, 301, 4096) for k in (1, 8, 10, 46, 47, 63, 64) for g in ("true", "false")]
+    got = ask([e for T, k, g in calls for e in (f"balance_one({T}, {k})", f"balance_counts_apart({T}, {k}, {g})")])
+    for c, one, apart in zip(calls, got[::2], got[1::2]):
+        assert not (one and apart), c
+        assert one or bool(apart) == (c[0] * c[1] > (3000 if c[2] == "true" else 12000)), c
+
+
 def test_ends_shapes(ask):  # noqa: F811
     """A row's slots hold it, and few lanes more."""
     widths = [1, 8, 64, 65, 128, 129, 256, 257, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384]

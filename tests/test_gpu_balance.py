@@ -179,3 +179,13 @@ def test_one_row_for_every_token(T, E):
         got = S.router_balance(one, it, mask=m, balance_coef=0.3, z_coef=0.2, grad=grad)
         want = S.router_balance(one.contiguous(), it, mask=m, balance_coef=0.3, z_coef=0.2, grad=grad)
         assert all(torch.equal(got[name], want[name]) for name in want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k", [(64, 512, 64), (64, 64, 64), (50, 1000, 63), (65, 512, 64)])
+def test_few_tokens_of_many_experts(T, E, k):
+    """The most pairs of one work-group, and the first batch of several."""
+    say(f"case: balance few tokens T={T} E={E} k={k}")
+    l, ids, mask = make(T + k, T, E, k, 0.8)
+    want, bound = D.balance(l, ids, mask, 0.5, 0.1)
+    check(run(l, ids, mask, 0.5, 0.1), want, bound)
