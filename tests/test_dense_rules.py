@@ -86,6 +86,21 @@ def test_ends_shapes(ask):  # noqa: F811
         assert few == (5 if lanes >= 256 else (5 * lanes + 255) // 256)
 
 
+def test_row_loop_cases_reach_every_shape(ask):  # noqa: F811
+    """The sizes of test_gpu_ends_rows.py make every shape of the kernel take rows in turn, with vectors and without."""
+    from test_gpu_ends_rows import ROWS
+    got = ask([e for T, n in ROWS for e in (f"ends_shape({n}).lanes", f"ends_shape({n}).slots", f"ends_groups({T}, {n})")])
+    seen = set()
+    for i, (T, n) in enumerate(ROWS):
+        lanes, slots, groups = got[3 * i:3 * i + 3]
+        at_once = max(256 // lanes, 1)
+        sets = (T + at_once - 1) // at_once
+        assert 2 * groups < sets < 3 * groups, (T, n)  # some work-groups a third set, some two
+        seen.add((lanes, slots, n % 4 == 0))
+    shapes = ((16, 1), (32, 1), (64, 1), (64, 2), (256, 1), (256, 2), (512, 2), (1024, 2), (1024, 4))
+    assert seen == {(*s, v) for s in shapes for v in (True, False)}
+
+
 @pytest.mark.skipif(shutil.which(HIPCC) is None, reason="no hipcc")
 def test_big_tile_code(tmp_path):
     """k_linear_big writes its matrix instructions itself, and the hardware waits for neither a VALU write of their operands
