@@ -246,8 +246,9 @@ typedef struct {
  * new stream, and x (x_type), the next block's input.  y and out NULL: x = R rs(R) pre alone (the scales are not used);
  * x NULL: out alone.  The gate's value of token t, channel d is gate[t gate_ld + d gate_step] (f32; NULL: none): one per
  * channel with gate_ld 0, per token with gate_step 0.  out and x may each be R's or y's own rows (the same address, row
- * stride and value size) and share no other byte with an input or each other.  n_embd 1 .. 16384; rows that start
- * 16-byte aligned and n_embd % 8 == 0 take wide accesses.  Rows past n_tokens are left as they are. */
+ * stride and value size) and share no other byte with an input or each other.  n_embd 1 .. 16384; a multiple of 4 with
+ * rows (starts and strides) and norm weights aligned to four of their values takes wide accesses.  Rows past n_tokens are left
+ * as they are. */
 smoe_status smoe_block_ends(const smoe_ends* e, int32_t n_embd, int32_t n_tokens, const void* R, int32_t r_type,
                             int64_t r_ld, const void* y, int32_t y_type, int64_t y_ld, const float* gate, int64_t gate_ld,
                             int64_t gate_step, void* out, int64_t out_ld, void* x, int32_t x_type, int64_t x_ld,
@@ -447,7 +448,7 @@ smoe_status smoe_router_margin(const float* logits, int32_t n_tokens, int32_t n_
  *   loss = {balance_coef balance + z_coef z, balance, z, n}.
  * With dlogits (rows dlogits_ld apart; may be logits) loss[0]'s gradient to the logits, the counts taken as constants:
  *   dlogits_tj = (balance_coef n_expert p_tj (f_j - sum_e f_e p_te) + 2 z_coef lse_t p_tj) / n, 0 for other tokens,
- * and with dbias [n_expert] its sum over the tokens (the gradient to smoe_weights' logit_bias).  A token repeated in ids
+ * and with dbias [n_expert] its sum over the tokens (the gradient to a bias added to the logits, as smoe_weights' logit_bias).  A token repeated in ids
  * counts each time, an id outside [0, n_expert) not at all.  No token counts (n = 0): every result is 0.  Logits of -inf
  * have p = 0; a counted row of them alone has p = 0 and lse = 0; other tokens' values, NaN or not, reach nothing.
  * n_expert 1 .. 1024, k 1 .. 64, at most 2^24 pairs; zero tokens launch nothing.  dlogits may be logits' own rows (the same

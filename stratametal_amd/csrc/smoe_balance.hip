@@ -11,7 +11,9 @@
 //   k_balance_rows, k_balance_sums                   some pairs: each work-group that needs the counts counts for itself
 //   k_balance_counts, k_balance_rows, k_balance_sums a batch
 // Bound by the logits' and the gradient's bytes in a large batch (32768 tokens of 1024 experts 72 us among other calls, 268 MB),
-// by the launches' chains of latencies else: 4096 tokens of 512 experts, 10 each, 24.5 us, 64 tokens without gradients 10.
+// by the launches' chains of latencies else: 4096 tokens of 512 experts, 10 each, 24.5 us, without gradients 18, 64 tokens
+// without gradients 10.  Rows of more than 512 experts without vectors and with gradients spill in their loop (22 registers of
+// the 128): 32768 tokens of 1001 experts 200 us, of 1024 66, both among calls of their own kind.
 #include "smoe_gemv.hpp"
 #include "smoe_launch.hpp"
 #include "smoe_rules.hpp"
@@ -308,7 +310,7 @@ __global__ __launch_bounds__(1024) void k_balance_sums(const BalanceArgs a, int 
         n = count_of(w.tokens, 0, 1, C);
         cnt = count_of(w.counts, ec, E, C);
     }
-    double z = tid < G ? w.zsum[tid] : 0.0;  // (at most 1024 partial rows)
+    double z = tid < G ? w.zsum[tid] : 0.0;  // (balance_groups: at most 512 partial rows)
     double pa = 0.0, da = 0.0;
     for (int g = grp; g < G; g += 8 * kSumGroups) {
         float pv[8], dv[8];

@@ -137,10 +137,13 @@ __device__ __forceinline__ float row_scale(const float (&v)[NV][4], int n, int l
 // L lanes to a row of up to 4 L NV values: 256 / L rows at a time to a work-group, or from 256 lanes on one.  A work-group
 // takes every gridDim.x-th set of rows; the next row's values are loaded before this one's are worked on, and what no row
 // changes (y_scale post g of a gate per channel, and pre) stays in registers.  With four slots, or two and a gate of every
-// value, neither fits the 128 registers of 16 waves: a row's values are loaded when its turn comes, and the weights each time
-// where they are used.  4096 rows of 4096 f32 values in and out 45 us, 6.0 TB/s of the copy's 5.1 (from the caches in
-// part; 8192 rows 101 us, 5.3 TB/s); one row of 2048 3.5 us, a launch's latencies.  (Types chosen per value, not per row: a
-// bf16 batch with a gate of every value 155 us for 92.)
+// value, neither fits the 128 registers of 16 waves: a row's values are loaded when its turn comes, and the weights each
+// time where they are used.  Four slots spill all the same (16 to 101 registers, without vectors 70 to 379), as do two
+// without vectors and with a gate of every value (40): joins of 4096 rows of 16384 f32 values 226 us, 4.8 TB/s, with a
+// gate per channel 340, with one of every value 388, of 16383 394 to 1398; 8192 rows of 8192 207, 206 and 253 us, 5.2
+// TB/s.  4096 rows of 4096 f32 values in and out 45 us, 6.0 TB/s of the copy's 5.1 (from the caches in part; 8192 rows 101
+// us, 5.3 TB/s); one row of 2048 3.5 us, a launch's latencies.  (Types chosen per value, not per row: a bf16 batch with a
+// gate of every value 155 us for 92.)
 template <int L, int NV, bool VEC, int GATE>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void k_block_ends(const EndsArgs a) {
     constexpr int ROWS = L < 256 ? 256 / L : 1;

@@ -1,5 +1,5 @@
 // stratametal_amd/csrc/smoe_types.hpp - rows of f32, fp16 or bf16 values for the dense operators round the block: the
-// element types, eight values to and from registers, and the exponential their activations take.
+// element types, four values from registers, and the exponential their activations take.
 #pragma once
 
 #include "smoe_device.hpp"
