@@ -448,9 +448,10 @@ smoe_status smoe_router_margin(const float* logits, int32_t n_tokens, int32_t n_
  *   loss = {balance_coef balance + z_coef z, balance, z, n}.
  * With dlogits (rows dlogits_ld apart; may be logits) loss[0]'s gradient to the logits, the counts taken as constants:
  *   dlogits_tj = (balance_coef n_expert p_tj (f_j - sum_e f_e p_te) + 2 z_coef lse_t p_tj) / n, 0 for other tokens,
- * and with dbias [n_expert] its sum over the tokens (the gradient to a bias added to the logits, as smoe_weights' logit_bias).  A token repeated in ids
- * counts each time, an id outside [0, n_expert) not at all.  No token counts (n = 0): every result is 0.  Logits of -inf
- * have p = 0; a counted row of them alone has p = 0 and lse = 0; other tokens' values, NaN or not, reach nothing.
+ * and with dbias [n_expert] its sum over the tokens (the gradient to a bias added to the logits, as smoe_weights'
+ * logit_bias).  An expert repeated in a token's ids counts each time, an id outside [0, n_expert) not at all.  No token
+ * counts (n = 0): every result is 0.  Logits of -inf have p = 0; a counted row of them alone has p = 0 and lse = 0; other
+ * tokens' values, NaN or not, reach nothing.
  * n_expert 1 .. 1024, k 1 .. 64, at most 2^24 pairs; zero tokens launch nothing.  dlogits may be logits' own rows (the same
  * address and stride); else no output and not the workspace (256-byte aligned) shares a byte with an input or another of
  * them.  The same bits in every run.  No counterpart in the reference, which does not train. */

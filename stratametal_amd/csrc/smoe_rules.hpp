@@ -185,8 +185,8 @@ constexpr bool balance_one(int64_t T, int k) { return T <= 64 && T * k <= 4096; 
 constexpr bool balance_counts_apart(int64_t T, int k, bool grad) {
     return !balance_one(T, k) && T * k > (grad ? 3000 : 12000);
 }
-// Work-groups of four rows at a time, at most 512 (k_balance_sums takes up to 1024): each leaves a row of partial sums (4096 tokens of 512
-// experts 27.5 us with 256 or 512 of them, 31.8 with 1024, 30.4 with 128; 32768 of 1024 99, 77.5, 79.8, 151).
+// Work-groups of four rows at a time, at most 512 (k_balance_sums takes up to 1024): each leaves a row of partial sums (4096
+// tokens of 512 experts 27.5 us with 256 or 512 of them, 31.8 with 1024, 30.4 with 128; 32768 of 1024 99, 77.5, 79.8, 151).
 constexpr int64_t balance_groups(int64_t T) { return T < 4 ? 1 : (T + 3) / 4 < 512 ? (T + 3) / 4 : 512; }
 // Work-groups of the counts, whose rows every reader adds up (4096 tokens 29.8 us with 8, 31.7 with 16; 32768 84 and 80,
 // with 64 95).
