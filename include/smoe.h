@@ -280,6 +280,101 @@ smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, i
                             int64_t r_ld, void* y, int32_t y_type, int64_t y_ld, void* workspace, size_t workspace_bytes,
                             void* hip_stream);
 
+/* The same product with 4-bit weights: W[o][i] = scale[i / group][o] (code[o][i] - zero[i / group][o]), the codes 0 .. 15 two to
+ * a byte, the even i's low; the products are exact and summed in f32, a group's sum scaled once (no weight is rounded).
+ * x is bf16 or fp16. */
+typedef struct {
+    int32_t n_in;         /* a multiple of 32, at most 65536 */
+    int32_t n_out;        /* 1 .. 2^24 */
+    int32_t x_type;       /* SMOE_BF16 or SMOE_F16 */
+    int32_t act;          /* SMOE_ACT_* */
+    int32_t group;        /* values of n_in to a scale, a multiple of 32 (the last group of a row may be shorter) */
+    int32_t s_type;       /* the scales: SMOE_F32, SMOE_F16 or SMOE_BF16 */
+    const void* w;        /* [n_out][n_in / 2] bytes, 16-byte aligned */
+    const void* w2;       /* the same, or NULL */
+    const void* scales;   /* [ceil(n_in / group)][n_out] */
+    const void* scales2;
+    const uint8_t* zeros; /* [ceil(n_in / group)][n_out], or NULL: 8 */
+    const uint8_t* zeros2;
+    const float* bias;    /* [n_out], or NULL */
+    const float* bias2;
+} smoe_linear4;
+
+/* As smoe_linear_workspace_bytes and smoe_linear_run. */
+size_t smoe_linear4_workspace_bytes(const smoe_linear4* L, int32_t n_tokens);
+smoe_status smoe_linear4_run(const smoe_linear4* L, const void* x, int64_t x_ld, int32_t n_tokens, const void* residual,
+                             int64_t r_ld, void* y, int32_t y_type, int64_t y_ld, void* workspace, size_t workspace_bytes,
+                             void* hip_stream);
+
+/* ---------------------------------------------------------------------------------------------- attention
+ * The other half of a layer, in front of the block: rotary positions, a paged cache of keys and values, and attention over
+ * it.  No counterpart in the reference's MoE block. */
+
+/* Rotary positions: pair i of a head's first rot_dim values, (a, b), at position p becomes
+ *   scale (a cos w - b sin w, b cos w + a sin w),  w = 2 pi p turns[i],  i < rot_dim / 2;
+ * the head's other values are copied.  The call at -p is the transpose of the one at p (its gradient too). */
+enum { SMOE_ROPE_HALF = 0, SMOE_ROPE_PAIRS = 1 }; /* pair i: values (i, i + rot_dim / 2), or (2 i, 2 i + 1) */
+typedef struct {
+    int32_t head_dim;    /* even, at most 1024 */
+    int32_t rot_dim;     /* even, 2 .. head_dim */
+    int32_t layout;      /* SMOE_ROPE_* */
+    float scale;         /* of the turned values */
+    const double* turns; /* [rot_dim / 2] revolutions per position (device) */
+} smoe_rope;
+
+/* turns [rot_dim / 2] and the scale (both host) of f_i = base^(-2 i / rot_dim) radians per position, for contexts `factor`
+ * times as long as the trained ones:
+ *   NONE    f_i;  LINEAR  f_i / factor;  BASE  f_i with base factor^(rot_dim / (rot_dim - 2)) (rot_dim 2: f_i);
+ *   PARTS   f_i (g + (1 - g) / factor), g = (r - slow) / (fast - slow) within 0 .. 1, r = trained_len f_i / 2 pi the turns over
+ *           the trained length; scale 0.1 ln factor + 1 (the others 1). */
+enum { SMOE_ROPE_NONE = 0, SMOE_ROPE_LINEAR = 1, SMOE_ROPE_BASE = 2, SMOE_ROPE_PARTS = 3 };
+smoe_status smoe_rope_table(int32_t rot_dim, double base, int32_t scaling, double factor, double trained_len, double slow,
+                            double fast, double* turns, float* scale);
+
+/* x [n_tokens][n_heads][head_dim] of x_type, tokens x_ld values apart, turned to positions[n_tokens] into y of y_type (f32,
+ * fp16 or bf16 each; y may be x's own rows). */
+smoe_status smoe_rope_run(const smoe_rope* r, const int32_t* positions, int32_t n_tokens, int32_t n_heads, const void* x,
+                          int32_t x_type, int64_t x_ld, void* y, int32_t y_type, int64_t y_ld, void* hip_stream);
+
+/* A cache of keys and values in pages: token `off` of page p, head h at ((p * n_kv_heads + h) * page_size + off) * head_dim
+ * of k and of v.  Pages, heads and tokens together below 2^31. */
+typedef struct {
+    void *k, *v;        /* 16-byte aligned */
+    int32_t type;       /* SMOE_BF16 or SMOE_F16 */
+    int32_t n_pages;
+    int32_t page_size;  /* tokens, 1 .. 65536 */
+    int32_t n_kv_heads;
+    int32_t head_dim;   /* a multiple of 8, 8 .. 256 */
+} smoe_kv;
+
+/* A step's keys and values into the cache and its queries turned, one launch: k and v [n_tokens][n_kv_heads][head_dim] go to
+ * slots[n_tokens] (page * page_size + off; one outside the cache, as -1: that token is not stored), k turned to positions, and
+ * q [n_tokens][n_heads][head_dim], turned, to q_out of the cache's type.  q, k and v are of x_type (f32, fp16 or bf16), tokens
+ * q_ld, k_ld and v_ld values apart (columns of one matrix, say).  r NULL: nothing turns (then q is NULL too, and positions are
+ * not read); q NULL: the cache alone.  A call's slots are distinct (of two tokens' values for one slot it keeps either's).
+ * q_out may be q's own rows; no other output shares a byte with an input. */
+smoe_status smoe_kv_append(const smoe_kv* kv, const smoe_rope* r, const int32_t* positions, const int64_t* slots,
+                           int32_t n_tokens, int32_t x_type, const void* q, int64_t q_ld, int32_t n_heads, void* q_out,
+                           int64_t q_out_ld, const void* k, int64_t k_ld, const void* v, int64_t v_ld, void* hip_stream);
+
+/* Attention of each sequence's new tokens over its pages.  Sequence b has the query rows q_start[b] .. q_start[b + 1] - 1
+ * (n of them; q_start[n_seqs + 1] ascending from 0 .. n_tokens) and kv_len[b] keys, key j at token j % page_size of page
+ * pages[b][j / page_size].  Its i-th query has position p = kv_len - n + i and sees, `causal`, keys j <= p, and with a window
+ * (> 0) those with j > p - window; not causal, all keys (window 0).  With head h reading key head h / (n_heads / n_kv_heads):
+ *   out = sum_j w_j v_j,  w = softmax of scale q k_j over the keys it sees,  lse = ln sum_j exp(scale q k_j).
+ * A query that sees no key: zeros and -inf.  What a query does not see does not reach it, NaN or not; keys of a page outside
+ * the cache, and those past max_len, are not there (kv_len is read on the device; max_len, at most max_pages * page_size, is
+ * the longest that the launch is made for).  Scores and sums are f32; the weights are rounded to the cache's type for the
+ * second product.  q and out [n_tokens][n_heads][head_dim] of the cache's type, tokens q_ld and out_ld values apart (q 16-byte
+ * aligned, q_ld a multiple of 8); lse [n_tokens][n_heads] f32 or NULL.  Rows before the first sequence and behind the last one
+ * are left as they are.  `workspace` (256-byte aligned, apart from every operand): concurrent calls need distinct ones.  The
+ * same bits in every run. */
+size_t smoe_attend_workspace_bytes(const smoe_kv* kv, int32_t n_heads, int32_t n_tokens, int32_t n_seqs, int64_t max_len);
+smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t n_tokens, int32_t n_heads,
+                        const int32_t* q_start, const int32_t* kv_len, int32_t n_seqs, const int32_t* pages, int64_t pages_ld,
+                        int32_t max_pages, int64_t max_len, float scale, int32_t causal, int32_t window, void* out,
+                        int64_t out_ld, float* lse, void* workspace, size_t workspace_bytes, void* hip_stream);
+
 /* ---------------------------------------------------------------------------------------------- GGUF models */
 
 /* A model in GGUF v3 files, read on the host: every shard of a split model (`<stem>-NNNNN-of-MMMMM.gguf`, any

@@ -64,6 +64,21 @@ class _Linear(C.Structure):
                 ("w2", C.c_void_p), ("bias", C.c_void_p), ("bias2", C.c_void_p)]
 
 
+class _Linear4(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_in", "n_out", "x_type", "act", "group", "s_type")] + \
+               [(n, C.c_void_p) for n in ("w", "w2", "scales", "scales2", "zeros", "zeros2", "bias", "bias2")]
+
+
+class _Rope(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("layout", C.c_int32), ("scale", C.c_float),
+                ("turns", C.c_void_p)]
+
+
+class _Kv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_int32) for n in ("type", "n_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
 class _Hc(C.Structure):
     _fields_ = [("hc", C.c_int32), ("hc_lr", C.c_int32), ("eps", C.c_float), ("norm", C.c_void_p),
                 ("down", C.c_void_p), ("up", C.c_void_p), ("inject", C.c_void_p)]
@@ -104,6 +119,14 @@ def lib():
             "smoe_block_ends": (i32, [vp, i32, i32, vp, i32, i64, vp, i32, i64, vp, i64, i64, vp, i64, vp, i32, i64, vp]),
             "smoe_linear_workspace_bytes": (C.c_size_t, [vp, i32]),
             "smoe_linear_run": (i32, [vp, vp, i64, i32, vp, i64, vp, i32, i64, vp, C.c_size_t, vp]),
+            "smoe_linear4_workspace_bytes": (C.c_size_t, [vp, i32]),
+            "smoe_linear4_run": (i32, [vp, vp, i64, i32, vp, i64, vp, i32, i64, vp, C.c_size_t, vp]),
+            "smoe_rope_table": (i32, [i32, C.c_double, i32, C.c_double, C.c_double, C.c_double, C.c_double, vp, vp]),
+            "smoe_rope_run": (i32, [vp, vp, i32, i32, vp, i32, i64, vp, i32, i64, vp]),
+            "smoe_kv_append": (i32, [vp, vp, vp, vp, i32, i32, vp, i64, i32, vp, i64, vp, i64, vp, i64, vp]),
+            "smoe_attend_workspace_bytes": (C.c_size_t, [vp, i32, i32, i32, i64]),
+            "smoe_attend": (i32, [vp, vp, i64, i32, i32, vp, vp, i32, vp, i64, i32, i64, f32, i32, i32, vp, i64, vp, vp,
+                                  C.c_size_t, vp]),
             "smoe_router_balance_workspace_bytes": (C.c_size_t, [i32, i32]),
             "smoe_router_balance": (i32, [vp, i64, vp, vp, i32, i32, i32, f32, f32, vp, vp, vp, vp, i64, vp, vp, C.c_size_t,
                                           vp]),
@@ -776,6 +799,312 @@ class Linear:
         return y
 
     __call__ = run
+
+
+class Linear4:
+    """The product with 4-bit weights and group scales (smoe_linear4_run), with Linear's epilogue: y = act(x W' + bias)
+    [* (x W2' + bias2)] [+ residual], W[o][i] = scales[i // group][o] (code[o][i] - zeros[i // group][o]).  `w` and `w2` are
+    (n_out, n_in / 2) uint8 tensors of two codes to a byte, the even i's low; scales and scales2 (ceil(n_in / group), n_out) of
+    float32, float16 or bfloat16; zeros and zeros2 uint8 of that shape (None: 8); the biases f32 [n_out].  The weights stay the
+    caller's tensors; x is bfloat16 or float16."""
+
+    def __init__(self, n_in: int, n_out: int, w, scales, zeros=None, group: int = 128, bias=None, w2=None, scales2=None,
+                 zeros2=None, bias2=None, act: int = ACT_NONE):
+        import torch
+        if n_in < 32 or n_in % 32 or group < 32 or group % 32:
+            raise SmoeError(-1, "n_in and group must be multiples of 32")
+        groups = (-(-n_in // group), n_out)
+        given = [(w, "w", torch.uint8, (n_out, n_in // 2)), (scales, "scales", None, groups), (zeros, "zeros", torch.uint8, groups),
+                 (bias, "bias", torch.float32, (n_out,)), (w2, "w2", torch.uint8, (n_out, n_in // 2)),
+                 (scales2, "scales2", None, groups), (zeros2, "zeros2", torch.uint8, groups), (bias2, "bias2", torch.float32, (n_out,))]
+        _given(w, "w"), _given(scales, "scales")
+        if (w2 is None) != (scales2 is None):
+            raise SmoeError(-6, "w2 and scales2 go together")
+        for t, name, dtype, shape in given:
+            if t is not None:
+                _need(t, name, dtype or scales.dtype, shape=shape)
+                _on_device(t, name, w.get_device())
+        self.n_in, self.n_out, self.group = n_in, n_out, group
+        self.tensors = tuple(t for t, *_ in given)
+        self._act, self._cs = act, {}
+        self._device = w.get_device()
+        self._s_type = _elem_type(scales.dtype)
+        if self._s_type < 0:
+            raise SmoeError(-3, f"scales is {scales.dtype}, needs float32, float16 or bfloat16 (or int16: bf16 bits)")
+        self._layer(BF16)
+
+    def _layer(self, x_type: int):
+        """(the C layer for x of that type, its reference, its workspace bytes per batch size)"""
+        c = self._cs.get(x_type)
+        if c is None:
+            w, scales, zeros, bias, w2, scales2, zeros2, bias2 = (_ptr(t) for t in self.tensors)
+            layer = _Linear4(self.n_in, self.n_out, x_type, self._act, self.group, self._s_type, w, w2, scales, scales2, zeros, zeros2,
+                             bias, bias2)
+            if lib().smoe_linear4_workspace_bytes(C.byref(layer), 0) == 0:
+                raise SmoeError(-1, lib().smoe_last_error().decode())
+            c = self._cs[x_type] = (layer, C.byref(layer), {})
+        return c
+
+    def workspace_bytes(self, n_tokens: int, dtype=None) -> int:
+        return int(lib().smoe_linear4_workspace_bytes(self._layer(BF16 if dtype is None else _elem_type(dtype))[1], n_tokens))
+
+    def run(self, x, residual=None, y=None, y_dtype=None, stream=None):
+        """y (tokens, n_out) of `y_dtype` (None: residual's, else x's); `y` may be residual."""
+        import torch
+        N, dev = self.n_out, self._device
+        xt, x_ld = _rows(x, "x", self.n_in, -1, dev)
+        if xt == F32:
+            raise SmoeError(-3, f"x is {x.dtype}, needs float16 or bfloat16 (or int16: bf16 bits)")
+        st = _current(dev, stream)
+        if st is None:
+            with _on(dev, stream):
+                return self.run(x, residual, y, y_dtype)
+        T = x.shape[0]
+        rp, rt, r_ld = None, -1, 0
+        if residual is not None:
+            rt, r_ld = _rows(residual, "residual", N, T, dev)
+            rp = residual.data_ptr()
+        if y is None:
+            dtype = y_dtype or (x if residual is None else residual).dtype
+            yt = _elem_type(dtype)
+            if yt < 0:
+                raise SmoeError(-3, f"y_dtype is {dtype}, needs float32, float16 or bfloat16 (or int16: bf16 bits)")
+            y, y_ld = _new(T, N, dtype, x.device), N
+        else:
+            yt, y_ld = _rows(y, "y", N, T, dev)
+        if rt >= 0 and rt != yt:
+            raise SmoeError(-1, f"residual is {residual.dtype}, y {y.dtype}")
+        _, ref, sizes = self._layer(xt)
+        n = sizes.get(T)
+        if n is None:
+            n = sizes[T] = int(lib().smoe_linear4_workspace_bytes(ref, T))
+        ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=x.device) if n > 256 else None
+        _check(lib().smoe_linear4_run(ref, x.data_ptr(), x_ld, T, rp, r_ld, y.data_ptr(), yt, y_ld, _ptr(ws), n, st))
+        return y
+
+    __call__ = run
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+ROPE_HALF, ROPE_PAIRS = 0, 1
+_ROPE_SCALINGS = {"linear": 1, "ntk": 2, "parts": 3}
+
+
+def rope_table(rot_dim: int, base: float = 10000.0, scaling=None):
+    """(revolutions per position, a list of rot_dim / 2, and the scale on turned values) of smoe_rope_table.  `scaling`: None, or
+    (kind, factor, ...) for contexts `factor` times as long as the trained ones: "linear" and "ntk" (the base grows) read the
+    factor, "parts" also the trained length and the slow and fast ends in turns over it."""
+    kind, factor, trained, slow, fast = (tuple(scaling) + (0.0, 0.0, 0.0))[:5] if scaling else ("", 1.0, 0.0, 0.0, 0.0)
+    if scaling and kind not in _ROPE_SCALINGS:
+        raise SmoeError(-1, f"scaling is {kind!r}, needs one of {sorted(_ROPE_SCALINGS)}")
+    if rot_dim < 2 or rot_dim > 1024 or rot_dim % 2:
+        raise SmoeError(-1, "rot_dim must be even, 2 to 1024")
+    turns, scale = (C.c_double * (rot_dim // 2))(), C.c_float()
+    _check(lib().smoe_rope_table(rot_dim, base, _ROPE_SCALINGS.get(kind, 0), factor, trained, slow, fast, turns, C.byref(scale)))
+    return list(turns), scale.value
+
+
+def _heads(t, name: str, heads: int, dim: int, tokens: int = -1, device: int = -1):
+    """(type, token stride) of a (tokens, heads, dim) tensor whose tokens' values are contiguous, at any stride."""
+    import torch
+    if not isinstance(t, torch.Tensor):
+        raise SmoeError(-1, f"{name} is not a tensor")
+    code = _elem_type(t.dtype)
+    if code < 0:
+        raise SmoeError(-3, f"{name} is {t.dtype}, needs float32, float16 or bfloat16 (or int16: bf16 bits)")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (heads >= 0 and shape[1] != heads) or (tokens >= 0 and shape[0] != tokens):
+        raise SmoeError(-2, f"{name} has shape {tuple(shape)}, needs ({'tokens' if tokens < 0 else tokens}, "
+                            f"{'heads' if heads < 0 else heads}, {dim})")
+    ld, step, one = t.stride()
+    if one != 1 or (step != dim and shape[1] > 1):
+        raise SmoeError(-5, f"a token's values of {name} are not contiguous")
+    _on_device(t, name, device)
+    return code, ld
+
+
+def _new_heads(tokens: int, heads: int, dim: int, dtype, device):
+    import torch
+    return torch.empty_strided((tokens, heads, dim), (heads * dim, dim, 1), dtype=dtype, device=device)
+
+
+class Rotary:
+    """Rotary positions (smoe_rope_run): the first `rot_dim` (None: all) values of heads of `head_dim` turned in pairs that lie
+    half of them apart (ROPE_HALF) or side by side (ROPE_PAIRS), the frequencies from `base` and `scaling` (rope_table), or
+    `turns`, the revolutions per position of each pair, with `scale` on turned values.  Positions are int32 tensors; at -p a call
+    is the transpose of the one at p."""
+
+    def __init__(self, head_dim: int, rot_dim: Optional[int] = None, base: float = 10000.0, layout: int = ROPE_HALF, scaling=None,
+                 turns=None, scale: Optional[float] = None, device="cuda"):
+        import torch
+        rot_dim = head_dim if rot_dim is None else rot_dim
+        if turns is None:
+            turns, own_scale = rope_table(rot_dim, base, scaling)
+        else:
+            own_scale = 1.0
+        self.turns = torch.as_tensor(turns, dtype=torch.float64).to(device).contiguous()
+        if self.turns.shape != (rot_dim // 2,):
+            raise SmoeError(-2, f"turns has shape {tuple(self.turns.shape)}, needs ({rot_dim // 2},)")
+        _on_device(self.turns, "turns")
+        self.head_dim, self.rot_dim, self.scale = head_dim, rot_dim, own_scale if scale is None else scale
+        self._c = _Rope(head_dim, rot_dim, layout, self.scale, self.turns.data_ptr())
+        self._ref, self._device = C.byref(self._c), self.turns.get_device()
+        # (a call without tokens: the sizes alone are checked)
+        _check(lib().smoe_rope_run(self._ref, None, 0, 1, None, F32, 0, None, F32, 0, None))
+
+    def run(self, x, positions, y=None, y_dtype=None, stream=None):
+        """y (tokens, heads, head_dim) of `y_dtype` (None: x's); `y` may be x."""
+        import torch
+        xt, x_ld = _heads(x, "x", -1, self.head_dim, -1, self._device)
+        T, H, _ = x.shape
+        st = _current(self._device, stream)
+        if st is None:
+            with _on(self._device, stream):
+                return self.run(x, positions, y, y_dtype)
+        _need(positions, "positions", torch.int32, shape=(T,))
+        _on_device(positions, "positions", self._device)
+        if y is None:
+            dtype = y_dtype or x.dtype
+            yt, y_ld = _elem_type(dtype), H * self.head_dim
+            if yt < 0:
+                raise SmoeError(-3, f"y_dtype is {dtype}, needs float32, float16 or bfloat16 (or int16: bf16 bits)")
+            y = _new_heads(T, H, self.head_dim, dtype, x.device)
+        else:
+            yt, y_ld = _heads(y, "y", H, self.head_dim, T, self._device)
+        _check(lib().smoe_rope_run(self._ref, positions.data_ptr(), T, H, x.data_ptr(), xt, x_ld, y.data_ptr(), yt, y_ld, st))
+        return y
+
+    __call__ = run
+
+
+class PagedCache:
+    """A cache of keys and values in pages: `k` and `v` are (pages, key heads, tokens of a page, head_dim) tensors of bfloat16 (or
+    int16: bf16 bits) or float16.  They stay the caller's tensors."""
+
+    def __init__(self, k, v):
+        _given(k, "k"), _given(v, "v")
+        if getattr(k, "ndim", 0) != 4:
+            raise SmoeError(-2, "k must be (pages, key heads, tokens of a page, head_dim)")
+        for t, name in ((k, "k"), (v, "v")):
+            _need(t, name, k.dtype, shape=k.shape)
+            _on_device(t, name, k.get_device())
+        self.k, self.v = k, v
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self._type, self._device = _elem_type(k.dtype), k.get_device()
+        self._c = _Kv(k.data_ptr(), v.data_ptr(), self._type, *(int(k.shape[i]) for i in (0, 2, 1, 3)))
+        self._ref = C.byref(self._c)
+        self._sizes: Dict = {}
+        # (a call without tokens: the sizes alone are checked)
+        _check(lib().smoe_kv_append(self._ref, None, None, None, 0, F32, None, 0, 0, None, 0, None, 0, None, 0, None))
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=None, device="cuda"):
+        """A new cache (its pages' values are any until they are written)."""
+        import torch
+        k, v = (torch.empty((n_pages, n_kv_heads, page_size, head_dim), dtype=dtype or torch.bfloat16, device=device) for _ in "kv")
+        return cls(k, v)
+
+    def append(self, k, v, slots, rotary: Optional[Rotary] = None, positions=None, q=None, q_out=None, stream=None):
+        """Writes (tokens, key heads, head_dim) tensors k and v to `slots` (int64: page * page_size + place, one outside the cache
+        as -1: not stored), k turned to `positions` when `rotary` is given, and returns q (tokens, heads, head_dim) turned, of the
+        cache's type (None without q); `q_out` may be q.  A call's slots are distinct (smoe_kv_append)."""
+        import torch
+        dev, D, kv = self._device, self.head_dim, self.n_kv_heads
+        xt, k_ld = _heads(k, "k", kv, D, -1, dev)
+        T = k.shape[0]
+        vt, v_ld = _heads(v, "v", kv, D, T, dev)
+        st = _current(dev, stream)
+        if st is None:
+            with _on(dev, stream):
+                return self.append(k, v, slots, rotary, positions, q, q_out)
+        _need(slots, "slots", torch.int64, shape=(T,))
+        _on_device(slots, "slots", dev)
+        rp = pp = qp = op = None
+        q_ld = o_ld = H = 0
+        if rotary is not None:
+            _need(_given(positions, "positions"), "positions", torch.int32, shape=(T,))
+            _on_device(positions, "positions", dev)
+            _on_device(rotary.turns, "the rotary positions' table", dev)
+            rp, pp = rotary._ref, positions.data_ptr()
+        qt = xt
+        if q is not None:
+            if rotary is None:
+                raise SmoeError(-6, "q without rotary positions")
+            qt, q_ld = _heads(q, "q", -1, D, T, dev)
+            H = q.shape[1]
+            if q_out is None:
+                q_out, o_ld = _new_heads(T, H, D, self.k.dtype, q.device), H * D
+            else:
+                ot, o_ld = _heads(q_out, "q_out", H, D, T, dev)
+                if ot != self._type:
+                    raise SmoeError(-1, f"q_out is {q_out.dtype}, the cache {self.k.dtype}")
+            qp, op = q.data_ptr(), q_out.data_ptr()
+        elif q_out is not None:
+            raise SmoeError(-6, "q_out without q")
+        if vt != xt or qt != xt:
+            raise SmoeError(-1, f"q, k and v are of one type, k is {k.dtype}")
+        _check(lib().smoe_kv_append(self._ref, rp, pp, slots.data_ptr(), T, xt, qp, q_ld, H, op, o_ld, k.data_ptr(), k_ld,
+                                    v.data_ptr(), v_ld, st))
+        return q_out
+
+    def workspace_bytes(self, n_heads: int, n_tokens: int, n_seqs: int, max_len: int) -> int:
+        return int(lib().smoe_attend_workspace_bytes(self._ref, n_heads, n_tokens, n_seqs, max_len))
+
+    def attend(self, q, q_start, kv_len, pages, scale: Optional[float] = None, causal: bool = True, window: int = 0,
+               lse: bool = False, max_len: Optional[int] = None, out=None, stream=None):
+        """out (tokens, heads, head_dim): attention of q's rows q_start[b] .. q_start[b + 1] - 1 over the first kv_len[b] keys of
+        the pages pages[b] (smoe_attend), `scale` None: head_dim ** -0.5; with `lse` (out, lse (tokens, heads) f32).  q_start
+        (sequences + 1,), kv_len (sequences,) and pages (sequences, most pages) are int32 tensors; max_len bounds kv_len (None:
+        what the pages hold): the tighter, the fewer empty work-groups.  Rows of no sequence are left as they are (new outputs: any
+        values)."""
+        import torch
+        dev, D = self._device, self.head_dim
+        qt, q_ld = _heads(q, "q", -1, D, -1, dev)
+        if qt != self._type:
+            raise SmoeError(-1, f"q is {q.dtype}, the cache {self.k.dtype}")
+        st = _current(dev, stream)
+        if st is None:
+            with _on(dev, stream):
+                return self.attend(q, q_start, kv_len, pages, scale, causal, window, lse, max_len, out)
+        T, H, _ = q.shape
+        _need(kv_len, "kv_len", torch.int32)
+        if kv_len.dim() != 1:
+            raise SmoeError(-2, "kv_len must be (sequences,)")
+        B = kv_len.shape[0]
+        _need(q_start, "q_start", torch.int32, shape=(B + 1,))
+        if not isinstance(pages, torch.Tensor) or pages.dtype != torch.int32:
+            raise SmoeError(-1, "pages must be an int32 tensor")
+        if pages.dim() != 2 or pages.shape[0] != B:
+            raise SmoeError(-2, f"pages has shape {tuple(pages.shape)}, needs ({B}, most pages)")
+        if pages.stride(1) != 1 and pages.shape[1] > 1:
+            raise SmoeError(-5, "pages' rows are not contiguous")
+        for t, name in ((kv_len, "kv_len"), (q_start, "q_start"), (pages, "pages")):
+            _on_device(t, name, dev)
+        held = min(pages.shape[1] * self.page_size, 1 << 30)
+        max_len = held if max_len is None else max_len
+        if out is None:
+            out, o_ld = _new_heads(T, H, D, q.dtype, q.device), H * D
+        else:
+            ot, o_ld = _heads(out, "out", H, D, T, dev)
+            if ot != qt:
+                raise SmoeError(-1, f"out is {out.dtype}, q {q.dtype}")
+        z = torch.empty_strided((T, H), (H, 1), dtype=torch.float32, device=q.device) if lse else None
+        key = (H, T, B, max_len)
+        n = self._sizes.get(key)
+        if n is None:
+            n = self.workspace_bytes(*key)
+            if n == 0:
+                raise SmoeError(-1, lib().smoe_last_error().decode())
+            if len(self._sizes) >= 4096:
+                self._sizes.clear()
+            self._sizes[key] = n
+        # a workspace of the call's own: calls on several streams, captured or not, share none
+        ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device) if n > 256 else None
+        _check(lib().smoe_attend(self._ref, q.data_ptr(), q_ld, T, H, q_start.data_ptr(), kv_len.data_ptr(), B, pages.data_ptr(),
+                                 pages.stride(0), pages.shape[1], max_len, D ** -0.5 if scale is None else scale, int(causal), window,
+                                 out.data_ptr(), o_ld, _ptr(z), _ptr(ws), n, st))
+        return (out, z) if lse else out
 
 
 # ------------------------------------------------------------------------------------------------ stages

@@ -1,68 +1,18 @@
 // stratametal_amd/csrc/smoe_dense.cpp - the C ABI of the dense operators round the block (include/smoe.h): argument checks
-// and launches of smoe_ends.hip, smoe_linear.hip and smoe_balance.hip.  As in smoe_api.cpp every refusal happens before
+// and launches of smoe_ends.hip, smoe_linear.hip, smoe_linear4.hip and smoe_balance.hip.  As in smoe_api.cpp every refusal happens before
 // the first launch, and a zero count returns before launching.
 #include "smoe.h"
 
 #include <hip/hip_runtime.h>
 
-#include <cmath>
 #include <iterator>
 #include <string>
 
+#include "smoe_check.hpp"
 #include "smoe_launch.hpp"
 #include "smoe_rules.hpp"
 
-namespace smoe {
-smoe_status report(smoe_status s, const std::string& why);  // smoe_api.cpp: the thread's last error
-}
-
-namespace {
-
-smoe_status fail(smoe_status s, const std::string& why) { return smoe::report(s, why); }
-smoe_status ok() { return smoe::report(SMOE_OK, ""); }
-smoe_status launched(hipError_t e, const char* what) {
-    return e == hipSuccess ? ok() : fail(SMOE_EDEVICE, std::string(what) + ": " + hipGetErrorString(e));
-}
-
-bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-bool elem_type(int32_t t) { return t == SMOE_F32 || t == SMOE_F16 || t == SMOE_BF16; }
-size_t elem_size(int32_t t) { return t == SMOE_F32 ? 4 : 2; }
-bool finite(float v) { return std::isfinite(v); }
-
-// `rows` rows of `width` bytes, `step` bytes apart.
-struct Span {
-    const void* p;
-    int64_t rows, step, width;
-    uintptr_t lo() const { return (uintptr_t)p; }
-    uintptr_t hi() const { return lo() + (uintptr_t)((rows - 1) * step + width); }
-};
-Span rows_of(const void* p, int32_t type, int64_t rows, int64_t ld, int64_t n) {
-    const int64_t es = (int64_t)elem_size(type);
-    return {p, rows, rows > 1 ? ld * es : n * es, n * es};
-}
-Span bytes_of(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
-// Whether a written span shares a byte with another: columns of one matrix (the same step) that lie apart do not, nor does
-// one row between the rows of a matrix.
-bool overlap(const Span& a, const Span& b) {
-    if (!a.p || !b.p || a.hi() <= b.lo() || b.hi() <= a.lo()) return false;
-    if (a.rows == 1 && b.rows > 1) return overlap(b, a);
-    if (b.rows == 1 && a.step >= a.width) {
-        const int64_t from = (int64_t)(b.lo() - a.lo());  // of a's rows, the first that ends past b's start
-        const int64_t i = from < a.width ? 0 : (from - a.width) / a.step + 1;
-        return i < a.rows && i * a.step < from + b.width;
-    }
-    if (a.step != b.step || a.step < a.width || a.step < b.width) return true;
-    const int64_t at = ((int64_t)(b.lo() - a.lo()) % a.step + a.step) % a.step;  // b's rows within a's step
-    return at < a.width || at + b.width > a.step;
-}
-// The same rows: an element is read by the thread that then writes it.
-bool same(const Span& a, const Span& b) { return a.p == b.p && a.step == b.step && a.width == b.width; }
-
-// Row strides of 2^40 values and more cannot be those of memory (and would overflow the byte offsets).
-constexpr int64_t kMaxLd = (int64_t)1 << 40;
-bool bad_ld(int64_t ld, int64_t rows, int64_t least) { return rows > 1 && (ld < least || ld > kMaxLd); }
-
-}  // namespace
+using namespace smoe;
 
 extern "C" {
 
@@ -193,6 +143,84 @@ smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, i
     a.n_in = L->n_in, a.n_out = L->n_out, a.n_tokens = n_tokens;
     a.w_type = L->w_type, a.y_type = y_type, a.act = L->act;
     return launched(smoe::launch_linear(a, reinterpret_cast<hipStream_t>(hip_stream)), "linear");
+}
+
+// ------------------------------------------------------------------------------------------------ 4-bit weights
+
+static smoe_status check_linear4(const smoe_linear4* L) {
+    if (!L) return fail(SMOE_ENULL, "linear4: the layer is NULL");
+    if (L->n_in < 32 || L->n_in % 32 || L->n_in > smoe::kLinearMaxIn)
+        return fail(SMOE_EINVAL, "linear4: n_in must be a multiple of 32, at most " + std::to_string(smoe::kLinearMaxIn));
+    if (L->n_out < 1 || L->n_out > smoe::kLinearMaxOut)
+        return fail(SMOE_EINVAL, "linear4: n_out must be 1 to " + std::to_string(smoe::kLinearMaxOut));
+    if (L->x_type != SMOE_BF16 && L->x_type != SMOE_F16) return fail(SMOE_ETYPE, "linear4: x is SMOE_BF16 or SMOE_F16");
+    if (!elem_type(L->s_type)) return fail(SMOE_ETYPE, "linear4: scales are SMOE_F32, SMOE_F16 or SMOE_BF16");
+    if (L->group < 32 || L->group % 32) return fail(SMOE_EINVAL, "linear4: group must be a multiple of 32");
+    if (L->act < SMOE_ACT_NONE || L->act > SMOE_ACT_SIGMOID) return fail(SMOE_EINVAL, "linear4: unknown activation");
+    return SMOE_OK;
+}
+
+size_t smoe_linear4_workspace_bytes(const smoe_linear4* L, int32_t n_tokens) {
+    if (check_linear4(L) != SMOE_OK) return 0;
+    if (n_tokens < 0) {
+        fail(SMOE_EINVAL, "linear4: negative token count");
+        return 0;
+    }
+    ok();
+    return 256 + (n_tokens ? smoe::linear4_part_bytes(n_tokens, L->n_in, L->n_out, L->w2 != nullptr, L->group) : 0);
+}
+
+smoe_status smoe_linear4_run(const smoe_linear4* L, const void* x, int64_t x_ld, int32_t n_tokens, const void* residual,
+                             int64_t r_ld, void* y, int32_t y_type, int64_t y_ld, void* workspace, size_t workspace_bytes,
+                             void* hip_stream) {
+    const smoe_status s = check_linear4(L);
+    if (s != SMOE_OK) return s;
+    if (n_tokens < 0) return fail(SMOE_EINVAL, "linear4: negative token count");
+    if (!elem_type(y_type)) return fail(SMOE_ETYPE, "linear4: y is SMOE_F32, SMOE_F16 or SMOE_BF16");
+    if (n_tokens == 0) return ok();
+    if (!x || !y || !L->w || !L->scales || (L->w2 && !L->scales2)) return fail(SMOE_ENULL, "linear4: NULL buffer");
+    if ((L->bias2 || L->scales2 || L->zeros2) && !L->w2) return fail(SMOE_ENULL, "linear4: bias2, scales2 or zeros2 without w2");
+    if (bad_ld(x_ld, n_tokens, 0) || (residual && bad_ld(r_ld, n_tokens, 0)) || bad_ld(y_ld, n_tokens, L->n_out))
+        return fail(SMOE_EINVAL, "linear4: row strides must not be negative, and y's rows not overlap");
+    if (n_tokens > 1 && (x_ld % 8 || x_ld > smoe::kLinearMaxLd))
+        return fail(SMOE_EINVAL, "linear4: x's row stride must be a multiple of 8, at most " + std::to_string(smoe::kLinearMaxLd));
+    if (!aligned(x, 16) || !aligned(L->w, 16) || !aligned(L->w2, 16))
+        return fail(SMOE_EALIGN, "linear4: x, w and w2 must be 16-byte aligned");
+    if (!aligned(y, elem_size(y_type)) || !aligned(residual, elem_size(y_type)) || !aligned(L->bias, 4) || !aligned(L->bias2, 4) ||
+        !aligned(L->scales, elem_size(L->s_type)) || !aligned(L->scales2, elem_size(L->s_type)))
+        return fail(SMOE_EALIGN, "linear4: a buffer is not aligned to its values");
+    const int64_t codes = (int64_t)L->n_out * (L->n_in / 2), groups = (L->n_in + (int64_t)L->group - 1) / L->group * L->n_out;
+    const Span sy = rows_of(y, y_type, n_tokens, y_ld, L->n_out), sr = rows_of(residual, y_type, n_tokens, r_ld, L->n_out);
+    if (overlap(sy, sr) && !same(sy, sr)) return fail(SMOE_EINVAL, "linear4: y is residual's own rows or shares none with it");
+    const Span in[] = {rows_of(x, L->x_type, n_tokens, x_ld, L->n_in), bytes_of(L->w, codes), bytes_of(L->w2, codes),
+                       rows_of(L->scales, L->s_type, 1, 0, groups), rows_of(L->scales2, L->s_type, 1, 0, groups),
+                       bytes_of(L->zeros, groups), bytes_of(L->zeros2, groups), rows_of(L->bias, SMOE_F32, 1, 0, L->n_out),
+                       rows_of(L->bias2, SMOE_F32, 1, 0, L->n_out)};
+    for (const Span& i : in)
+        if (overlap(sy, i)) return fail(SMOE_EINVAL, "linear4: y overlaps x, a weight, a scale, a zero or a bias");
+    if (!smoe::linear4_fits(n_tokens, L->n_in, L->n_out, L->w2 != nullptr, L->group))
+        return fail(SMOE_EINVAL, "linear4: the product exceeds a launch's grid: split it");
+    const size_t need = smoe::linear4_part_bytes(n_tokens, L->n_in, L->n_out, L->w2 != nullptr, L->group);
+    if (need) {
+        if (!workspace) return fail(SMOE_ENULL, "linear4: the workspace is NULL");
+        if (!aligned(workspace, 256)) return fail(SMOE_EALIGN, "linear4: the workspace must be 256-byte aligned");
+        if (workspace_bytes < need)
+            return fail(SMOE_ESIZE, "linear4 workspace is " + std::to_string(workspace_bytes) + " bytes, needs " +
+                                        std::to_string(need));
+        const Span ws = bytes_of(workspace, (int64_t)need);
+        bool shared = overlap(ws, sy) || overlap(ws, sr);
+        for (const Span& i : in) shared = shared || overlap(ws, i);
+        if (shared) return fail(SMOE_EINVAL, "linear4: the workspace overlaps an operand");
+    }
+    smoe::Linear4Args a{};
+    a.x = x, a.w = L->w, a.w2 = L->w2, a.residual = residual, a.bias = L->bias, a.bias2 = L->bias2, a.y = y;
+    a.part = static_cast<float*>(workspace);
+    a.x_ld = n_tokens > 1 ? x_ld : 0, a.r_ld = n_tokens > 1 && residual ? r_ld : 0, a.y_ld = n_tokens > 1 ? y_ld : 0;
+    a.n_in = L->n_in, a.n_out = L->n_out, a.n_tokens = n_tokens;
+    a.w_type = L->x_type, a.y_type = y_type, a.act = L->act;
+    a.scales = L->scales, a.scales2 = L->scales2, a.zeros = L->zeros, a.zeros2 = L->zeros2;
+    a.group = L->group, a.s_type = L->s_type;
+    return launched(smoe::launch_linear4(a, reinterpret_cast<hipStream_t>(hip_stream)), "linear4");
 }
 
 // ------------------------------------------------------------------------------------------------ router balance

@@ -218,6 +218,15 @@ struct LinearArgs {
 size_t linear_part_bytes(int64_t n_tokens, int n_in, int n_out, bool pair);
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s);
 
+// the product with 4-bit weights (smoe_linear4.hip): w and w2 are the codes
+struct Linear4Args : LinearArgs {
+    const void *scales, *scales2;
+    const uint8_t *zeros, *zeros2;
+    int group, s_type;
+};
+size_t linear4_part_bytes(int64_t n_tokens, int n_in, int n_out, bool pair, int group);
+hipError_t launch_linear4(const Linear4Args& a, hipStream_t s);
+
 // the router's balance loss (smoe_balance.hip); dlogits and dbias may be NULL
 struct BalanceArgs {
     const float* logits;
@@ -232,6 +241,36 @@ struct BalanceArgs {
 };
 size_t balance_work_bytes(int64_t n_tokens, int n_expert);
 hipError_t launch_balance(const BalanceArgs& a, hipStream_t s);
+
+// rotary positions and the cache write (smoe_rope.hip): q_out = q turned, the pages' rows at `slots` = k turned and v; q NULL:
+// none, n_kv 0: no cache; rot 0: nothing turns
+struct RopeArgs {
+    const double* turns;
+    const int32_t* positions;
+    const int64_t* slots;
+    const void *q, *k, *v;
+    void *q_out, *k_pages, *v_pages;
+    int64_t q_ld, q_out_ld, k_ld, v_ld, n_slots;
+    int n_tokens, n_heads, n_kv, head_dim, rot, half, page_size;
+    int x_type, q_type, t_type;  // of q, k and v, of q_out, of the pages
+    float scale;
+};
+hipError_t launch_rope(const RopeArgs& a, hipStream_t s);
+
+// attention over a paged cache (smoe_attend.hip); lse may be NULL; part: the partial sums of the keys' splits
+struct AttendArgs {
+    const uint8_t *k, *v;
+    const void* q;
+    const int32_t *q_start, *kv_len, *pages;
+    void* out;
+    float *lse, *part;
+    int64_t q_ld, out_ld, pages_ld;
+    int n_tokens, n_seqs, n_heads, n_kv, head_dim, page_size, n_pages, max_len;
+    int causal, window, f16;
+    float scale;  // times log2 e
+};
+size_t attend_part_bytes(int64_t n_tokens, int n_seqs, int n_heads, int n_kv, int head_dim, int page_size, int64_t max_len);
+hipError_t launch_attend(const AttendArgs& a, hipStream_t s);
 
 hipError_t launch_synth_blocks(int type, uint64_t seed, uint64_t stream_id, int64_t n_blocks, float sigma, uint8_t* out,
                                hipStream_t s);

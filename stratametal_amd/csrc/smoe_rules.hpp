@@ -274,4 +274,7 @@ inline int64_t linear_groups(LinearPlan p, int64_t T, int64_t N, bool pair) {
     return ((pair ? 2 * N : N) + t.rows - 1) / t.rows * ((T + t.tokens - 1) / t.tokens);
 }
 
+// The product with 4-bit weights: whether a launch's grid holds it.
+inline bool linear4_fits(int64_t T, int64_t, int64_t N, bool, int) { return (N + 15) / 16 < kGridGroups && (T + 15) / 16 < 65536; }
+
 }  // namespace smoe
