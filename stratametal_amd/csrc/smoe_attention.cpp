@@ -220,8 +220,8 @@ smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t 
     a.q_start = q_start, a.kv_len = kv_len, a.pages = pages;
     a.out = out, a.lse = lse, a.part = static_cast<float*>(workspace);
     a.q_ld = n_tokens > 1 ? q_ld : 0, a.out_ld = n_tokens > 1 ? out_ld : 0, a.pages_ld = n_seqs > 1 ? pages_ld : 0;
-    a.n_tokens = n_tokens, a.n_seqs = n_seqs, a.n_heads = n_heads, a.n_kv = kv->n_kv_heads, a.head_dim = kv->head_dim;
-    a.page_size = kv->page_size, a.n_pages = kv->n_pages, a.max_len = (int)max_len;
+    a.n_tokens = n_tokens, a.n_seqs = n_seqs, a.n_heads = n_heads, a.n_kv = kv->n_kv_heads, a.group = n_heads / kv->n_kv_heads;
+    a.head_dim = kv->head_dim, a.page_size = kv->page_size, a.n_pages = kv->n_pages, a.max_len = (int)max_len;
     a.causal = causal != 0, a.window = window, a.f16 = kv->type == SMOE_F16;
     a.scale = scale * 1.44269504f;
     return launched(launch_attend(a, reinterpret_cast<hipStream_t>(hip_stream)), "attend");

@@ -265,7 +265,7 @@ struct AttendArgs {
     void* out;
     float *lse, *part;
     int64_t q_ld, out_ld, pages_ld;
-    int n_tokens, n_seqs, n_heads, n_kv, head_dim, page_size, n_pages, max_len;
+    int n_tokens, n_seqs, n_heads, n_kv, group, head_dim, page_size, n_pages, max_len;  // group: n_heads / n_kv
     int causal, window, f16;
     float scale;  // times log2 e
 };

@@ -277,4 +277,43 @@ inline int64_t linear_groups(LinearPlan p, int64_t T, int64_t N, bool pair) {
 // The product with 4-bit weights: whether a launch's grid holds it.
 inline bool linear4_fits(int64_t T, int64_t, int64_t N, bool, int) { return (N + 15) / 16 < kGridGroups && (T + 15) / 16 < 65536; }
 
+// n / d for n < 2^31 as (mulhi(n, mul) + n) >> shift: shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.
+struct Divisor {
+    uint32_t mul, shift;
+};
+constexpr Divisor divisor(uint32_t d) {
+    uint32_t shift = 0;
+    while (((uint64_t)1 << shift) < d) ++shift;
+    return {(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
+}
+
+// Attention over a paged cache: tiles of query rows, and the keys in how many splits of how many.
+constexpr int kAttendRows = 128;
+struct AttendPlan {
+    int tiles, splits, chunk;
+    int64_t part_floats;  // of the splits' tops and sums, in front of their partial outputs
+    Divisor page;
+};
+constexpr int64_t attend_tiles(int64_t T, int64_t B, int64_t group, int64_t rows) {
+    // a sequence of n tokens has ceil(n group / rows) tiles
+    const int64_t each = T * ((group + rows - 1) / rows), packed = T * group / rows + B;
+    return each < packed ? each : packed;
+}
+inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_t max_len) {
+    AttendPlan p{};
+    p.tiles = (int)attend_tiles(T, B, H / kv, kAttendRows);
+    p.splits = 1, p.chunk = (int)max_len;
+    const int64_t groups = (int64_t)p.tiles * kv;
+    if (groups < 512 && max_len > 512) {
+        int64_t splits = (1024 + groups - 1) / (groups ? groups : 1);
+        const int64_t most = (max_len + 255) / 256;
+        if (splits > most) splits = most;
+        p.chunk = (int)((max_len + splits - 1) / splits + 63) / 64 * 64;
+        p.splits = (int)((max_len + p.chunk - 1) / p.chunk);
+    }
+    p.part_floats = (2 * T * H * p.splits + 63) / 64 * 64;
+    (void)D;
+    return p;
+}
+
 }  // namespace smoe
