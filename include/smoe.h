@@ -369,7 +369,8 @@ smoe_status smoe_kv_append(const smoe_kv* kv, const smoe_rope* r, const int32_t*
  * aligned, q_ld a multiple of 8); lse [n_tokens][n_heads] f32 or NULL.  Rows before the first sequence and behind the last one
  * are left as they are.  `workspace` (256-byte aligned, apart from every operand): concurrent calls need distinct ones.  The
  * same bits in every run. */
-size_t smoe_attend_workspace_bytes(const smoe_kv* kv, int32_t n_heads, int32_t n_tokens, int32_t n_seqs, int64_t max_len);
+size_t smoe_attend_workspace_bytes(const smoe_kv* kv, int32_t n_heads, int32_t n_tokens, int32_t n_seqs, int64_t max_len,
+                                   int32_t window);
 smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t n_tokens, int32_t n_heads,
                         const int32_t* q_start, const int32_t* kv_len, int32_t n_seqs, const int32_t* pages, int64_t pages_ld,
                         int32_t max_pages, int64_t max_len, float scale, int32_t causal, int32_t window, void* out,

@@ -124,7 +124,7 @@ def lib():
             "smoe_rope_table": (i32, [i32, C.c_double, i32, C.c_double, C.c_double, C.c_double, C.c_double, vp, vp]),
             "smoe_rope_run": (i32, [vp, vp, i32, i32, vp, i32, i64, vp, i32, i64, vp]),
             "smoe_kv_append": (i32, [vp, vp, vp, vp, i32, i32, vp, i64, i32, vp, i64, vp, i64, vp, i64, vp]),
-            "smoe_attend_workspace_bytes": (C.c_size_t, [vp, i32, i32, i32, i64]),
+            "smoe_attend_workspace_bytes": (C.c_size_t, [vp, i32, i32, i32, i64, i32]),
             "smoe_attend": (i32, [vp, vp, i64, i32, i32, vp, vp, i32, vp, i64, i32, i64, f32, i32, i32, vp, i64, vp, vp,
                                   C.c_size_t, vp]),
             "smoe_router_balance_workspace_bytes": (C.c_size_t, [i32, i32]),
@@ -1048,8 +1048,8 @@ class PagedCache:
                                     v.data_ptr(), v_ld, st))
         return q_out
 
-    def workspace_bytes(self, n_heads: int, n_tokens: int, n_seqs: int, max_len: int) -> int:
-        return int(lib().smoe_attend_workspace_bytes(self._ref, n_heads, n_tokens, n_seqs, max_len))
+    def workspace_bytes(self, n_heads: int, n_tokens: int, n_seqs: int, max_len: int, window: int = 0) -> int:
+        return int(lib().smoe_attend_workspace_bytes(self._ref, n_heads, n_tokens, n_seqs, max_len, window))
 
     def attend(self, q, q_start, kv_len, pages, scale: Optional[float] = None, causal: bool = True, window: int = 0,
                lse: bool = False, max_len: Optional[int] = None, out=None, stream=None):
@@ -1090,7 +1090,7 @@ class PagedCache:
             if ot != qt:
                 raise SmoeError(-1, f"out is {out.dtype}, q {q.dtype}")
         z = torch.empty_strided((T, H), (H, 1), dtype=torch.float32, device=q.device) if lse else None
-        key = (H, T, B, max_len)
+        key = (H, T, B, max_len, window)
         n = self._sizes.get(key)
         if n is None:
             n = self.workspace_bytes(*key)

@@ -483,52 +483,80 @@ __global__ __launch_bounds__(256, 2) void k_attend_tile(const AttendArgs a, cons
         redo_row(a, p, w, wave * 32 + __builtin_ctzll(again), reinterpret_cast<float*>(lds) + wave * kMaxDim, lane);
 }
 
-// The splits' sums of a query row, a wave to a row: out = sum_s 2^(top_s - top) out_s / sum_s 2^(top_s - top) sum_s.
-__global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, const AttendPlan p) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-    if (row >= (int64_t)a.n_tokens * a.n_heads) return;
+// The splits' sums of a query row: out = sum_s 2^(top_s - top) out_s / sum_s 2^(top_s - top) sum_s.  head_dim / 4 threads to a
+// split's values; a row has as many such groups as it has splits, at most a whole work-group's, and they meet in LDS (one wave
+// to a row and its splits one by one: 170 us of 202 for 32 rows of 256 splits).
+__global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, const AttendPlan p, int per_row) {
+    __shared__ f32x4 out_s[256];
+    __shared__ float2 stats_s[256];
+    const int per = a.head_dim / 4, groups = 256 / per;  // threads of a group, groups
+    const int rows = groups / per_row, g = threadIdx.x / per, d = threadIdx.x % per;
+    const int mine = g / per_row, first = g % per_row;
+    const int64_t row = (int64_t)blockIdx.x * rows + mine;
     const int t = (int)(row / a.n_heads), head = (int)(row % a.n_heads);
-    if (sequence_of(a, t, lane).b < 0) return;
-    const float2* stats = reinterpret_cast<const float2*>(a.part) + row * p.splits;
-    float top = -__builtin_inff();
-    for (int s = lane; s < p.splits; s += 64) top = __builtin_fmaxf(top, stats[s].x);
-    top = max_halves(top);
-    for (int x = 16; x > 0; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    float out[kMaxDim / 64], sum = 0.0f;
+    const bool live = mine < rows && t >= a.q_start[0] && t < min(a.q_start[a.n_seqs], a.n_tokens);
+    float top = -__builtin_inff(), sum = 0.0f;
+    f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (live) {
+        const float2* stats = reinterpret_cast<const float2*>(a.part) + row * p.splits;
+        const float* part = part_row(a, p, row, 0) + 4 * d;
+        constexpr int AHEAD = 4;
+        for (int s = first; s < p.splits; s += AHEAD * per_row) {
+            f32x4 v[AHEAD];
+            float2 m[AHEAD];
 #pragma unroll
-    for (int i = 0; i < kMaxDim / 64; ++i) out[i] = 0.0f;
-    for (int at = 0; at < p.splits; at += 64) {
-        float w = 0.0f;
-        if (at + lane < p.splits) {
-            const float2 v = stats[at + lane];
-            w = v.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(v.x - base);
-            sum += v.x == -__builtin_inff() ? 0.0f : w * v.y;
-            w = v.x == -__builtin_inff() ? -1.0f : w;  // none
-        } else {
-            w = -1.0f;
-        }
-        for (uint64_t left = __ballot(!(w == -1.0f)); left; left &= left - 1) {
-            const int l = __builtin_ctzll(left);
-            const float wl = __shfl(w, l);
-            const float* part = part_row(a, p, row, at + l);
+            for (int i = 0; i < AHEAD; ++i) {
+                const int at = min(s + i * per_row, p.splits - 1);
+                m[i] = stats[at];
+                v[i] = *reinterpret_cast<const f32x4*>(part + (int64_t)at * a.head_dim);
+            }
+            float next = top;
 #pragma unroll
-            for (int i = 0; i < kMaxDim / 64; ++i)
-                if (lane + 64 * i < a.head_dim) out[i] = __builtin_fmaf(wl, part[lane + 64 * i], out[i]);
+            for (int i = 0; i < AHEAD; ++i) next = __builtin_fmaxf(next, m[i].x);
+            const float base = next == -__builtin_inff() ? 0.0f : next, keep = __builtin_amdgcn_exp2f(top - base);
+            top = next;
+            sum *= keep;
+            out *= keep;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                // (a split without keys has written no values)
+                const bool some = s + i * per_row < p.splits && m[i].x != -__builtin_inff();
+                const float w = some ? __builtin_amdgcn_exp2f(m[i].x - base) : 0.0f;
+                sum = some ? __builtin_fmaf(w, m[i].y, sum) : sum;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) out[k] = some ? __builtin_fmaf(w, v[i][k], out[k]) : out[k];
+            }
         }
     }
-    for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x);
+    if (per_row > 1) {
+        out_s[threadIdx.x] = out, stats_s[threadIdx.x] = make_float2(top, sum);
+        __syncthreads();
+        if (first == 0) {
+            for (int i = 1; i < per_row; ++i) top = __builtin_fmaxf(top, stats_s[threadIdx.x + i * per].x);
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+            sum = 0.0f, out = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < per_row; ++i) {
+                const float2 m = stats_s[threadIdx.x + i * per];
+                const float w = __builtin_amdgcn_exp2f(m.x - base);
+                sum = __builtin_fmaf(w, m.y, sum);
+                out += w * out_s[threadIdx.x + i * per];
+            }
+        }
+    }
+    if (!live || first != 0) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_ld + (int64_t)head * a.head_dim;
+    uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_ld + (int64_t)head * a.head_dim + 4 * d;
+    const float v[4] = {out[0] * inv, out[1] * inv, out[2] * inv, out[3] * inv};
+    const int type = a.f16 ? kF16 : kBf16;
+    if (((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_ld * 2)) & 7) == 0) store4(o, v, type);
+    else
 #pragma unroll
-    for (int i = 0; i < kMaxDim / 64; ++i)
-        if (lane + 64 * i < a.head_dim) o[lane + 64 * i] = f32_to_half_bits(out[i] * inv, a.f16 ? kF16 : kBf16);
-    if (a.lse && lane == 0) a.lse[row] = lse_of(top, sum);
+        for (int k = 0; k < 4; ++k) o[k] = f32_to_half_bits(v[k], type);
+    if (a.lse && d == 0) a.lse[row] = lse_of(top, sum);
 }
 
-size_t attend_part_bytes(int64_t n_tokens, int n_seqs, int n_heads, int n_kv, int head_dim, int, int64_t max_len) {
-    const AttendPlan p = attend_plan(n_tokens, n_seqs, n_heads, n_kv, head_dim, max_len);
+size_t attend_part_bytes(int64_t n_tokens, int n_seqs, int n_heads, int n_kv, int head_dim, int64_t max_len, int window) {
+    const AttendPlan p = attend_plan(n_tokens, n_seqs, n_heads, n_kv, head_dim, max_len, window);
     return p.splits > 1 ? (size_t)(p.part_floats + n_tokens * n_heads * p.splits * head_dim) * 4 : 0;
 }
 
@@ -544,11 +572,15 @@ hipError_t launch_attend_as(const AttendArgs& a, const AttendPlan& p, hipStream_
 }  // namespace
 
 hipError_t launch_attend(const AttendArgs& a, hipStream_t s) {
-    AttendPlan p = attend_plan(a.n_tokens, a.n_seqs, a.n_heads, a.n_kv, a.head_dim, a.max_len);
+    AttendPlan p = attend_plan(a.n_tokens, a.n_seqs, a.n_heads, a.n_kv, a.head_dim, a.max_len, a.window);
     p.page = divisor(a.page_size);
     hipError_t e = a.f16 ? launch_attend_as<true>(a, p, s) : launch_attend_as<false>(a, p, s);
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL(k_attend_join, dim3((unsigned)(((int64_t)a.n_tokens * a.n_heads + 3) / 4)), dim3(256), 0, s, a, p);
+    const int groups = 256 / (a.head_dim / 4);
+    int per_row = 1;
+    while (per_row < p.splits && 2 * per_row <= groups) per_row *= 2;
+    const int64_t rows = (int64_t)a.n_tokens * a.n_heads, each = groups / per_row;
+    hipLaunchKernelGGL(k_attend_join, dim3((unsigned)((rows + each - 1) / each)), dim3(256), 0, s, a, p, per_row);
     return hipGetLastError();
 }
 

@@ -171,10 +171,15 @@ static smoe_status check_attend(const smoe_kv* kv, int32_t n_heads, int32_t n_to
     return SMOE_OK;
 }
 
-size_t smoe_attend_workspace_bytes(const smoe_kv* kv, int32_t n_heads, int32_t n_tokens, int32_t n_seqs, int64_t max_len) {
+size_t smoe_attend_workspace_bytes(const smoe_kv* kv, int32_t n_heads, int32_t n_tokens, int32_t n_seqs, int64_t max_len,
+                                   int32_t window) {
     if (check_attend(kv, n_heads, n_tokens, n_seqs, max_len) != SMOE_OK) return 0;
+    if (window < 0) {
+        fail(SMOE_EINVAL, "attend: a window must be positive");
+        return 0;
+    }
     ok();
-    return 256 + attend_part_bytes(n_tokens, n_seqs, n_heads, kv->n_kv_heads, kv->head_dim, kv->page_size, max_len);
+    return 256 + attend_part_bytes(n_tokens, n_seqs, n_heads, kv->n_kv_heads, kv->head_dim, max_len, window);
 }
 
 smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t n_tokens, int32_t n_heads,
@@ -200,7 +205,7 @@ smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t 
     const Span in[] = {rows_of(q, kv->type, n_tokens, q_ld, n), pages_of(kv, kv->k), pages_of(kv, kv->v),
                        bytes_of(q_start, 4ll * (n_seqs + 1)), bytes_of(kv_len, 4ll * n_seqs),
                        max_pages ? rows_of(pages, SMOE_F32, n_seqs, pages_ld, max_pages) : bytes_of(nullptr, 1)};
-    const size_t need = attend_part_bytes(n_tokens, n_seqs, n_heads, kv->n_kv_heads, kv->head_dim, kv->page_size, max_len);
+    const size_t need = attend_part_bytes(n_tokens, n_seqs, n_heads, kv->n_kv_heads, kv->head_dim, max_len, window);
     if (need) {
         if (!workspace) return fail(SMOE_ENULL, "attend: the workspace is NULL");
         if (!aligned(workspace, 256)) return fail(SMOE_EALIGN, "attend: the workspace must be 256-byte aligned");

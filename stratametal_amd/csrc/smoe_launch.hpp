@@ -269,7 +269,7 @@ struct AttendArgs {
     int causal, window, f16;
     float scale;  // times log2 e
 };
-size_t attend_part_bytes(int64_t n_tokens, int n_seqs, int n_heads, int n_kv, int head_dim, int page_size, int64_t max_len);
+size_t attend_part_bytes(int64_t n_tokens, int n_seqs, int n_heads, int n_kv, int head_dim, int64_t max_len, int window);
 hipError_t launch_attend(const AttendArgs& a, hipStream_t s);
 
 hipError_t launch_synth_blocks(int type, uint64_t seed, uint64_t stream_id, int64_t n_blocks, float sigma, uint8_t* out,

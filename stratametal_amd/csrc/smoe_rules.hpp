@@ -295,24 +295,34 @@ struct AttendPlan {
     Divisor page;
 };
 constexpr int64_t attend_tiles(int64_t T, int64_t B, int64_t group, int64_t rows) {
-    // a sequence of n tokens has ceil(n group / rows) tiles
-    const int64_t each = T * ((group + rows - 1) / rows), packed = T * group / rows + B;
+    // a sequence of n tokens has ceil(n group / rows) tiles: all of them at most (T group + B (rows - 1)) / rows
+    const int64_t each = T * ((group + rows - 1) / rows), packed = (T * group + B * (rows - 1)) / rows;
     return each < packed ? each : packed;
 }
-inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_t max_len) {
+// A CU holds two work-groups.  A split costs the work-groups' rounds over those 512 places, each a start and its tiles of keys
+// (32 of them where a head is wider than 128), and beyond one split the launch that joins them and its bytes.
+constexpr int attend_keys(int D) { return D > 128 ? 32 : 64; }
+inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t rows, int D) {
+    const int64_t tile = attend_keys(D), tiles = ((keys + splits - 1) / splits + tile - 1) / tile;
+    const int64_t rounds = (groups * splits + 511) / 512;
+    return (double)rounds * (4.0 + 2.3 * (double)tiles) + (splits > 1 ? 4.0 + (double)(rows * splits * D) * 8 / 4e6 : 0.0);
+}
+inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_t max_len, int64_t window) {
     AttendPlan p{};
-    p.tiles = (int)attend_tiles(T, B, H / kv, kAttendRows);
-    p.splits = 1, p.chunk = (int)max_len;
-    const int64_t groups = (int64_t)p.tiles * kv;
-    if (groups < 512 && max_len > 512) {
-        int64_t splits = (1024 + groups - 1) / (groups ? groups : 1);
-        const int64_t most = (max_len + 255) / 256;
-        if (splits > most) splits = most;
-        p.chunk = (int)((max_len + splits - 1) / splits + 63) / 64 * 64;
-        p.splits = (int)((max_len + p.chunk - 1) / p.chunk);
+    const int64_t group = H / kv, rows = T * H;
+    p.tiles = (int)attend_tiles(T, B, group, kAttendRows);
+    // the most keys that a tile's rows see
+    const int64_t seen = window ? window + (kAttendRows + group - 1) / group : max_len, keys = seen < max_len ? seen : max_len;
+    const int64_t groups = (int64_t)p.tiles * kv, tile = attend_keys(D);
+    int64_t best = 1;
+    double least = attend_time(groups, 1, keys, rows, D);
+    for (int64_t s = 2; groups * s <= 2048 && (s - 1) * tile < keys; ++s) {
+        const double us = attend_time(groups, s, keys, rows, D);
+        if (us < least) least = us, best = s;
     }
-    p.part_floats = (2 * T * H * p.splits + 63) / 64 * 64;
-    (void)D;
+    p.chunk = (int)(((keys + best - 1) / best + tile - 1) / tile * tile);
+    p.splits = keys ? (int)((keys + p.chunk - 1) / p.chunk) : 1;
+    p.part_floats = (2 * rows * p.splits + 63) / 64 * 64;
     return p;
 }
 

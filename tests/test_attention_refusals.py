@@ -111,10 +111,10 @@ def test_attend(want, kw):
 
 
 def test_attend_workspace():
-    def size(H=4, T=4, B=2, ml=128, **c):
-        return S.lib().smoe_attend_workspace_bytes(C.byref(kv(**c)), H, T, B, ml)
+    def size(H=4, T=4, B=2, ml=128, window=0, **c):
+        return S.lib().smoe_attend_workspace_bytes(C.byref(kv(**c)), H, T, B, ml, window)
 
-    assert size() > 0 and size(T=0) > 0 and size(T=-1) == 0 and size(H=3) == 0 and size(ml=-1) == 0 and size(head_dim=7) == 0
+    assert size() > 0 and size(T=0) > 0 and size(T=-1) == 0 and size(H=3) == 0 and size(ml=-1) == 0 and size(head_dim=7) == 0 and size(window=-1) == 0
     need = size(T=1, B=1, ml=100000)
     if need > 256:
         kw = dict(T=1, B=1, mp=6250, ml=100000)
