@@ -217,6 +217,7 @@ struct LinearArgs {
 };
 size_t linear_part_bytes(int64_t n_tokens, int n_in, int n_out, bool pair);
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s);
+hipError_t launch_linear_join(const LinearArgs& a, int slices, hipStream_t s);  // the slices of `part` added, and the epilogue
 
 // the product with 4-bit weights (smoe_linear4.hip): w and w2 are the codes
 struct Linear4Args : LinearArgs {

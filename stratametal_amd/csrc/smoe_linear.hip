@@ -348,6 +348,17 @@ __global__ __launch_bounds__(256) void k_linear_join(const LinearArgs a, int sli
     }
 }
 
+hipError_t launch_linear_join(const LinearArgs& a, int slices, hipStream_t s) {
+    const bool vec = rows_vec(a) && a.n_out % 4 == 0;
+    const int64_t n = (int64_t)a.n_tokens * (vec ? a.n_out / 4 : a.n_out);
+    const dim3 grid((unsigned)((n + 255) / 256));
+    if (a.w2 && vec) hipLaunchKernelGGL((k_linear_join<true, true>), grid, dim3(256), 0, s, a, slices);
+    else if (a.w2) hipLaunchKernelGGL((k_linear_join<true, false>), grid, dim3(256), 0, s, a, slices);
+    else if (vec) hipLaunchKernelGGL((k_linear_join<false, true>), grid, dim3(256), 0, s, a, slices);
+    else hipLaunchKernelGGL((k_linear_join<false, false>), grid, dim3(256), 0, s, a, slices);
+    return hipGetLastError();
+}
+
 size_t linear_part_bytes(int64_t T, int K, int N, bool pair) {
     const int slices = linear_plan(T, K, N, pair).slices;
     return slices > 1 ? (size_t)slices * (pair ? 2 : 1) * T * ((N + 3) / 4) * 16 : 0;
@@ -381,13 +392,7 @@ hipError_t launch_linear_as(const LinearArgs& a, const LinearPlan& p, hipStream_
     if (p.kind == kLinear64) e = launch_tile<2, 2, 2, 2, 5, PAIR, F16>(a, p.slices, s);
     if (p.kind == kLinear128x64) e = launch_tile<4, 2, 2, 2, 3, PAIR, F16>(a, p.slices, s);
     if (p.kind == kLinear128) e = launch_tile<4, 4, 2, 2, 3, PAIR, F16>(a, p.slices, s);
-    if (e != hipSuccess || p.slices == 1) return e;
-    const bool vec = rows_vec(a) && a.n_out % 4 == 0;
-    const int64_t n = (int64_t)a.n_tokens * (vec ? a.n_out / 4 : a.n_out);
-    const dim3 grid((unsigned)((n + 255) / 256));
-    if (vec) hipLaunchKernelGGL((k_linear_join<PAIR, true>), grid, dim3(256), 0, s, a, p.slices);
-    else hipLaunchKernelGGL((k_linear_join<PAIR, false>), grid, dim3(256), 0, s, a, p.slices);
-    return hipGetLastError();
+    return e != hipSuccess || p.slices == 1 ? e : launch_linear_join(a, p.slices, s);
 }
 }  // namespace
 

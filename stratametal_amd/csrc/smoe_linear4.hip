@@ -35,70 +35,318 @@ __device__ __forceinline__ u32x4 expand8(uint32_t w) {
     return r;
 }
 
-__device__ __forceinline__ float scale_at(const void* p, int64_t i, int type) {
-    return type == kF32 ? static_cast<const float*>(p)[i] : elem_to_f32(static_cast<const uint16_t*>(p)[i], type);
+// The same less the row's zero, exact as well: fp16 from 1024 + code less 1024 + zero; bf16 through f32, which holds 2^23 + code.
+// `less`: minus 1024 - zero twice in fp16, or minus 2^23 - zero in f32.
+template <bool F16>
+__device__ __forceinline__ uint32_t zero_term(uint32_t z) {
+    if constexpr (F16) {
+        const uint32_t h = __builtin_bit_cast(uint16_t, (_Float16)(-1024.0f - (float)z));
+        return h | h << 16;
+    } else {
+        return f2u(-8388608.0f - (float)z);
+    }
+}
+template <bool F16>
+__device__ __forceinline__ u32x4 expand8_less(uint32_t w, uint32_t less) {
+    const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
+    u32x4 r;
+    if constexpr (F16) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        const uint32_t a = __builtin_amdgcn_perm(hi, lo, 0x05010400u), b = __builtin_amdgcn_perm(hi, lo, 0x07030602u);
+        const auto two = [&](uint32_t c) {
+            return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, c) + __builtin_bit_cast(f16x2, less));
+        };
+        r[0] = two(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)), r[1] = two(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u));
+        r[2] = two(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)), r[3] = two(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u));
+    } else {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // 0x4B0000cc: 2^23 + code
+            const uint32_t sel = 0x070C0C00u + i;
+            const f32x2 v = {u2f(__builtin_amdgcn_perm(0x4B4B4B4Bu, lo, sel)) + u2f(less),
+                             u2f(__builtin_amdgcn_perm(0x4B4B4B4Bu, hi, sel)) + u2f(less)};
+            r[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+        }
+    }
+    return r;
+}
+
+// The 16-bit or 32-bit values and bytes of a lane, as dwords in LDS (at lds + 4 lane); asynchronous, counted by vmcnt.
+__device__ __forceinline__ void scale_to_lds(uint32_t lds, const void* p, bool wide) {
+    if (wide) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void byte_to_lds(uint32_t lds, const void* p) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void codes_to_lds(uint32_t lds, const void* p) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ f32x4 four_scales(const uint32_t* p, int type) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+    return f32x4{elem_to_f32(v[0], type), elem_to_f32(v[1], type), elem_to_f32(v[2], type), elem_to_f32(v[3], type)};
 }
 
 }  // namespace
 
-// 16 outputs by 16 tokens to a work-group of eight waves, each every eighth 32 of K.
-template <bool PAIR, bool F16>
+// Up to 16 tokens: 16 outputs (of both matrices) to a work-group of eight waves, each every eighth stage of 128 of K.  A stage
+// travels to the wave's own LDS whole and asynchronously, RING stages on their way: 64 bytes of each row, so that four lanes
+// load one line's half (piece p of row r at place p ^ (r >> 2), and the dwords that a matrix instruction takes of 16 rows
+// cover the 64 banks once), the tokens' values, and the scales and zeros of its up to four groups.  Lanes past the last token
+// hold its values, and their results are dropped; the waves' sums meet in LDS, in wave order.
+template <bool PAIR, bool F16, int TOKENS>
 __global__ __launch_bounds__(512) void k_linear4_few(const Linear4Args a) {
-    constexpr int SETS = PAIR ? 2 : 1, WAVES = 8;
-    __shared__ f32x4 sum_s[WAVES][SETS][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int o0 = blockIdx.x * 16, t0 = blockIdx.y * 16, q = lane >> 4;
+    constexpr int SETS = PAIR ? 2 : 1, WAVES = 8, RING = kLinear4Ring<PAIR, TOKENS>;
+    constexpr int XS = TOKENS > 4 ? TOKENS / 4 : 1, LOADS = 3 * SETS + XS;  // a stage's loads of the tokens, and all
+    constexpr int STAGE = kLinear4Stage<PAIR, TOKENS>, X0 = SETS * 1536;
+    __shared__ __align__(1024) uint8_t lds4[WAVES * RING * STAGE];
+    static_assert(WAVES * SETS * 1024 <= WAVES * RING * STAGE, "the waves' sums");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int o0 = blockIdx.x * 16, q = lane >> 4;
+    const int groups = (a.n_in + a.group - 1) / a.group, stages = (a.n_in + 127) / 128, half_row = a.n_in / 2;
     const uint8_t* w[2] = {static_cast<const uint8_t*>(a.w), static_cast<const uint8_t*>(a.w2)};
-    const void* sc[2] = {a.scales, a.scales2};
+    const uint8_t* sc[2] = {static_cast<const uint8_t*>(a.scales), static_cast<const uint8_t*>(a.scales2)};
     const uint8_t* zr[2] = {a.zeros, a.zeros2};
-    const int64_t row = min(o0 + (lane & 15), a.n_out - 1), tok = min(t0 + (lane & 15), a.n_tokens - 1);
-    const uint16_t* x = static_cast<const uint16_t*>(a.x) + tok * a.x_ld;
-    const uint32_t one = F16 ? 0x3C003C00u : 0x3F803F80u;
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    f32x4 acc[SETS];
-#pragma unroll
-    for (int i = 0; i < SETS; ++i) acc[i] = zero;
-    for (int u = wave; u < a.n_in / 32; u += WAVES) {
-        const int k = u * 32 + 8 * q;
-        const uint4 xv = *reinterpret_cast<const uint4*>(x + k);
-        const f32x4 sx = mfma16<F16>(make_uint4(one, one, one, one), xv, zero);
-        const int64_t g = u * 32 / a.group;
+    const bool wide = a.s_type == kF32;
+    uint8_t* const mine = lds4 + wave * (RING * STAGE);
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(mine));
+    const int row = min(o0 + (lane >> 2), a.n_out - 1), piece = (lane & 3) ^ ((lane >> 4) & 3);
+    const int out = min(o0 + (lane & 15), a.n_out - 1);
+    // (a load past the row's end, or of a stage past the last, brings the row's last values: no step reads them)
+    const auto load = [&](int u, uint32_t at) {
+        u = min(u, stages - 1);
+        const int k = u * 128, g0 = k / a.group;
 #pragma unroll
         for (int i = 0; i < SETS; ++i) {
-            const uint32_t c = *reinterpret_cast<const uint32_t*>(w[i] + row * (a.n_in / 2) + k / 2);
-            const f32x4 s = mfma16<F16>(__builtin_bit_cast(uint4, expand8<F16>(c)), xv, zero);
+            codes_to_lds(at + i * 1536, w[i] + (int64_t)row * half_row + min(k / 2 + 16 * piece, half_row - 16));
+            const int64_t g = (int64_t)min(g0 + q, groups - 1) * a.n_out + out;
+            scale_to_lds(at + i * 1536 + 1024, sc[i] + g * (wide ? 4 : 2), wide);
+            byte_to_lds(at + i * 1536 + 1280, zr[i] ? zr[i] + g : sc[i]);
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t at = g * a.n_out + min(o0 + 4 * q + j, a.n_out - 1);
-                const float z = zr[i] ? (float)zr[i][at] : 8.0f;
-                acc[i][j] = __builtin_fmaf(scale_at(sc[i], at, a.s_type), __builtin_fmaf(-z, sx[j], s[j]), acc[i][j]);
+        for (int j = 0; j < XS; ++j) {
+            const int t = min(4 * j + (lane >> 4), TOKENS - 1), c = (lane & 15) ^ t;
+            codes_to_lds(at + X0 + j * 1024, static_cast<const uint16_t*>(a.x) + (int64_t)min(t, a.n_tokens - 1) * a.x_ld + min(k + 8 * c, a.n_in - 8));
+        }
+    };
+    const uint32_t one = F16 ? 0x3C003C00u : 0x3F803F80u;
+    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 acc[SETS];
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) acc[i] = none;
+#pragma unroll
+    for (int r = 0; r < RING; ++r) load(wave + r * WAVES, base + r * STAGE);
+    const int tok = min(lane & 15, TOKENS - 1);
+    const uint32_t w_at = (lane & 15) * 64 + 4 * q, w_sw = (lane >> 2) & 3;
+    uint32_t at = 0;
+    for (int u = wave; u < stages; u += WAVES) {
+        vmcnt<(RING - 1) * LOADS>();
+        const uint8_t* st = mine + at;
+        int g = 0, left = a.group - u * 128 % a.group;  // of the stage's groups, and what is left of it
+        f32x4 sum[SETS], sx = none;
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) sum[i] = none;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (u * 128 + s * 32 >= a.n_in) break;
+            const uint4 xv = *reinterpret_cast<const uint4*>(st + X0 + tok * 256 + ((4 * s + q) ^ tok) * 16);
+            sx = mfma16<F16>(make_uint4(one, one, one, one), xv, sx);
+#pragma unroll
+            for (int i = 0; i < SETS; ++i) {
+                const uint32_t c = *reinterpret_cast<const uint32_t*>(st + i * 1536 + w_at + (s ^ w_sw) * 16);
+                sum[i] = mfma16<F16>(__builtin_bit_cast(uint4, expand8<F16>(c)), xv, sum[i]);
+            }
+            left -= 32;
+            if (left == 0 || s == 3 || u * 128 + s * 32 + 32 >= a.n_in) {
+#pragma unroll
+                for (int i = 0; i < SETS; ++i) {
+                    const f32x4 scale = four_scales(reinterpret_cast<const uint32_t*>(st + i * 1536 + 1024) + g * 16 + 4 * q, a.s_type);
+                    const u32x4 z = *reinterpret_cast<const u32x4*>(st + i * 1536 + 1280 + g * 64 + 16 * q);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[i][j] = __builtin_fmaf(scale[j], __builtin_fmaf(zr[i] ? -(float)z[j] : -8.0f, sx[j], sum[i][j]), acc[i][j]);
+                    sum[i] = none;
+                }
+                sx = none;
+                ++g;
+                left = a.group;
             }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        load(u + RING * WAVES, base + at);
+        at = at + STAGE == RING * STAGE ? 0 : at + STAGE;
     }
+    vmcnt<0>();
+    __syncthreads();
+    f32x4* sum_s = reinterpret_cast<f32x4*>(lds4);  // [wave][set][lane]
 #pragma unroll
-    for (int i = 0; i < SETS; ++i) sum_s[wave][i][lane] = acc[i];
+    for (int i = 0; i < SETS; ++i) sum_s[(wave * SETS + i) * 64 + lane] = acc[i];
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
     for (int i = 0; i < SETS; ++i)
 #pragma unroll
-        for (int v = 1; v < WAVES; ++v) acc[i] = acc[i] + sum_s[v][i][lane];
-    const int t = t0 + (lane & 15), o = o0 + 4 * q;
+        for (int v = 1; v < WAVES; ++v) acc[i] = acc[i] + sum_s[(v * SETS + i) * 64 + lane];
+    const int t = lane & 15, o = o0 + 4 * q;
     if (t >= a.n_tokens || o >= a.n_out) return;
     const f32x4 g = acc[0], u = acc[SETS - 1];
     finish4<PAIR>(a, rows_vec(a), t, o, {g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]});
 }
 
-size_t linear4_part_bytes(int64_t, int, int, bool, int) { return 0; }
+// More tokens: 128 weight rows (PAIR: 64 of each matrix, 16 of each in turn) by 16 NT tokens to a work-group of four waves, 32
+// rows to a wave.  A stage is 64 of K: the wave's codes (half p of row r at place p ^ (r >> 3)), its scales and zeros of the
+// two 32-value steps, and its share of the tokens (as in k_linear_tile), through a ring of RING stages in LDS.  A wave expands
+// the codes of its rows in registers, less their zeros, for all of the tile's tokens; a group's sums are scaled into the
+// outputs' where it ends.  blockIdx.y: a slice of K, whose sums go to `part` for k_linear_join.
+template <int NT, bool PAIR, bool F16>
+__global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, int tiles_o, int tiles_t) {
+    constexpr int MT = 2, WAVES = 4, BN = 16 * NT, OUTS = PAIR ? 64 : 128, RING = 3;
+    constexpr int XS = BN / 8 / WAVES;                                  // a wave's loads of the tokens, 8 rows each
+    constexpr int LOADS = 3 + XS, X0 = WAVES * 1536, STAGE = X0 + BN * 128;
+    constexpr int NG = NT < 4 ? NT : 4;
+    static_assert(WAVES * kStoreBytes<MT, NG> <= RING * STAGE, "the waves' pieces of the epilogue");
+    __shared__ __align__(1024) uint8_t lds[RING * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
+    int to, tt;
+    tile_of(blockIdx.x, gridDim.x, tiles_o, tiles_t, to, tt);
+    const int o0 = to * OUTS, t0 = tt * BN;
+    const int n_t = min(BN, a.n_tokens - t0);
+    const int half_row = a.n_in / 2, groups = (a.n_in + a.group - 1) / a.group;
+    const int all = (a.n_in + 63) / 64;
+    const int u0 = (int)((int64_t)all * blockIdx.y / gridDim.y), u1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
+    const bool wide = a.s_type == kF32;
+    // row i (0 .. 31) of the wave: its matrix and output
+    const auto matrix = [&](int i) { return PAIR && i >= 16; };
+    const auto output = [&](int i) { return min(o0 + (PAIR ? wave * 16 + (i & 15) : wave * 32 + i), a.n_out - 1); };
+    const uint8_t* codes = static_cast<const uint8_t*>(matrix(lane >> 1) ? a.w2 : a.w) + (int64_t)output(lane >> 1) * half_row;
+    const int half = (lane & 1) ^ ((lane >> 4) & 1);
+    const bool second = matrix(lane & 31);
+    const uint8_t* scales = static_cast<const uint8_t*>(second ? a.scales2 : a.scales) + (int64_t)output(lane & 31) * (wide ? 4 : 2);
+    const uint8_t* zeros = second ? a.zeros2 : a.zeros;
+    const uint8_t* zeros_at = zeros ? zeros + output(lane & 31) : scales;
+    const int64_t zero_ld = zeros ? a.n_out : 0, scale_ld = (int64_t)a.n_out * (wide ? 4 : 2);
+    const i32x4 rx = uniform_rsrc(static_cast<const uint8_t*>(a.x) + (size_t)t0 * a.x_ld * 2, (uint32_t)((n_t - 1) * a.x_ld * 2) + 2u * a.n_in);
+    uint32_t x_off[XS];
+#pragma unroll
+    for (int i = 0; i < XS; ++i) {
+        const int r = 8 * (i * WAVES + wave) + (lane >> 3);
+        x_off[i] = r < n_t ? (uint32_t)(r * a.x_ld * 2) + 16u * ((lane & 7) ^ (lane >> 3)) : kOob;
+    }
+    const int x_lane = 8 * ((lane & 7) ^ (lane >> 3));
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds));
+    // (codes, scales and zeros past the row's end: its last; the tokens' values there are zeros)
+    const auto load = [&](int u, uint32_t at) {
+        const int k = u * 64;
+        codes_to_lds(at + wave * 1536, codes + min(k / 2 + 16 * half, half_row - 16));
+        const int g0 = min(k / a.group, groups - 1), g1 = min((k + 32) / a.group, groups - 1), g = lane < 32 ? g0 : g1;
+        scale_to_lds(at + wave * 1536 + 1024, scales + g * scale_ld, wide);
+        byte_to_lds(at + wave * 1536 + 1280, zeros_at + g * zero_ld);
+#pragma unroll
+        for (int i = 0; i < XS; ++i)
+            dma16(at + X0 + (i * WAVES + wave) * 1024, k + x_lane < a.n_in ? x_off[i] + 2u * k : kOob, rx, 0);
+    };
+    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 acc[MT][NT], sum[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = sum[m][n] = none;
+#pragma unroll
+    for (int r = 0; r < RING - 1; ++r) load(u0 + r, base + r * STAGE);
+    const int fr = lane & 15;
+    int left = a.group - u0 * 64 % a.group;  // of the group
+    const bool has_zeros = a.zeros != nullptr, has_zeros2 = PAIR ? a.zeros2 != nullptr : has_zeros;
+    uint32_t at = 0;
+    for (int u = u0; u < u1; ++u) {
+        // every wave has read the step before, and this one is there
+        vmcnt<(RING - 2) * LOADS>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        {
+            const uint32_t next = at + (RING - 1) * STAGE;
+            load(u + RING - 1, base + (next >= RING * STAGE ? next - RING * STAGE : next));
+        }
+        const uint8_t* st = lds + at;
+        const uint8_t* ws = st + wave * 1536;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int k = u * 64 + 32 * s;
+            if (s == 1 && k >= a.n_in) break;
+            u32x4 av[MT], bv[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                bv[n] = *reinterpret_cast<const u32x4*>(st + X0 + (16 * n + fr) * 128 + ((4 * s + q) ^ (fr & 7)) * 16);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const uint32_t c = *reinterpret_cast<const uint32_t*>(ws + (16 * m + fr) * 32 + (s ^ (fr >> 3)) * 16 + 4 * q);
+                const uint32_t z = *reinterpret_cast<const uint32_t*>(ws + 1280 + (32 * s + 16 * m + fr) * 4);
+                av[m] = expand8_less<F16>(c, zero_term<F16>((m ? has_zeros2 : has_zeros) ? z : 8u));
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    sum[m][n] = mfma16<F16>(__builtin_bit_cast(uint4, av[m]), __builtin_bit_cast(uint4, bv[n]), sum[m][n]);
+            left -= 32;
+            if (left == 0 || k + 32 >= a.n_in || (s == 1 && u + 1 == u1)) {
+                left = a.group;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const f32x4 scale = four_scales(reinterpret_cast<const uint32_t*>(ws + 1024) + 32 * s + 16 * m + 4 * q, a.s_type);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[m][n][j] = __builtin_fmaf(scale[j], sum[m][n][j], acc[m][n][j]);
+                        sum[m][n] = none;
+                    }
+                }
+            }
+        }
+        at = at + STAGE == RING * STAGE ? 0 : at + STAGE;
+    }
+    vmcnt<0>();
+    __syncthreads();
+    tile_store<MT, NT, NG, PAIR>(a, acc, lds + wave * kStoreBytes<MT, NG>, o0 + wave * (PAIR ? 16 : 32), t0, t0 + n_t, lane);
+}
+
+size_t linear4_part_bytes(int64_t T, int K, int N, bool pair, int) {
+    const int slices = linear4_plan(T, K, N, pair).slices;
+    return slices > 1 ? (size_t)slices * (pair ? 2 : 1) * T * ((N + 3) / 4) * 16 : 0;
+}
+
+namespace {
+template <bool PAIR, bool F16, int TOKENS>
+hipError_t launch_few(const Linear4Args& a, hipStream_t s) {
+    hipLaunchKernelGGL((k_linear4_few<PAIR, F16, TOKENS>), dim3((a.n_out + 15) / 16), dim3(512), 0, s, a);
+    return hipGetLastError();
+}
+template <int NT, bool PAIR, bool F16>
+hipError_t launch_tile4(const Linear4Args& a, int slices, hipStream_t s) {
+    constexpr int OUTS = PAIR ? 64 : 128, BN = 16 * NT;
+    const int tiles_o = (a.n_out + OUTS - 1) / OUTS, tiles_t = (a.n_tokens + BN - 1) / BN;
+    hipLaunchKernelGGL((k_linear4_tile<NT, PAIR, F16>), dim3(tiles_o * tiles_t, slices), dim3(256), 0, s, a, tiles_o, tiles_t);
+    return hipGetLastError();
+}
+template <bool PAIR, bool F16>
+hipError_t launch_linear4_as(const Linear4Args& a, hipStream_t s) {
+    const Linear4Plan p = linear4_plan(a.n_tokens, a.n_in, a.n_out, PAIR);
+    if (p.tokens == 1) return launch_few<PAIR, F16, 1>(a, s);
+    if (p.tokens == 4) return launch_few<PAIR, F16, 4>(a, s);
+    if (p.tokens == 16) return launch_few<PAIR, F16, 16>(a, s);
+    const hipError_t e = p.tokens == 32   ? launch_tile4<2, PAIR, F16>(a, p.slices, s)
+                         : p.tokens == 64 ? launch_tile4<4, PAIR, F16>(a, p.slices, s)
+                                          : launch_tile4<8, PAIR, F16>(a, p.slices, s);
+    return e != hipSuccess || p.slices == 1 ? e : launch_linear_join(a, p.slices, s);
+}
+}  // namespace
 
 hipError_t launch_linear4(const Linear4Args& a, hipStream_t s) {
-    const dim3 grid((a.n_out + 15) / 16, (a.n_tokens + 15) / 16);
     const bool f16 = a.w_type == kF16;
-    if (a.w2 && f16) hipLaunchKernelGGL((k_linear4_few<true, true>), grid, dim3(512), 0, s, a);
-    else if (a.w2) hipLaunchKernelGGL((k_linear4_few<true, false>), grid, dim3(512), 0, s, a);
-    else if (f16) hipLaunchKernelGGL((k_linear4_few<false, true>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((k_linear4_few<false, false>), grid, dim3(512), 0, s, a);
-    return hipGetLastError();
+    if (a.w2) return f16 ? launch_linear4_as<true, true>(a, s) : launch_linear4_as<true, false>(a, s);
+    return f16 ? launch_linear4_as<false, true>(a, s) : launch_linear4_as<false, false>(a, s);
 }
 
 }  // namespace smoe

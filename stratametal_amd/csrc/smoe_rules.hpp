@@ -274,8 +274,31 @@ inline int64_t linear_groups(LinearPlan p, int64_t T, int64_t N, bool pair) {
     return ((pair ? 2 * N : N) + t.rows - 1) / t.rows * ((T + t.tokens - 1) / t.tokens);
 }
 
-// The product with 4-bit weights: whether a launch's grid holds it.
-inline bool linear4_fits(int64_t T, int64_t, int64_t N, bool, int) { return (N + 15) / 16 < kGridGroups && (T + 15) / 16 < 65536; }
+// The product with 4-bit weights.  k_linear4_few: LDS of a wave's stage (codes, scales and zeros of one or two matrices, the
+// tokens' values), and stages on their way.
+template <bool PAIR, int TOKENS>
+constexpr int kLinear4Stage = (PAIR ? 2 : 1) * 1536 + (TOKENS > 4 ? TOKENS / 4 : 1) * 1024;
+template <bool PAIR, int TOKENS>
+constexpr int kLinear4Ring = TOKENS > 4 ? (PAIR ? 2 : 3) : PAIR ? 2 : 4;
+// The tokens that a work-group takes: 1, 4 and 16 k_linear4_few's, 32 to 128 a tile's, with K in slices.
+struct Linear4Plan {
+    int tokens, slices;
+};
+inline int64_t linear4_groups(Linear4Plan p, int64_t T, int64_t N, bool pair) {
+    if (p.tokens <= 16) return (N + 15) / 16;
+    const int outs = pair ? 64 : 128;
+    return (N + outs - 1) / outs * ((T + p.tokens - 1) / p.tokens);
+}
+inline Linear4Plan linear4_plan(int64_t T, int64_t K, int64_t N, bool pair) {
+    if (T <= 16) return {T <= 1 ? 1 : T <= 4 ? 4 : 16, 1};
+    Linear4Plan p{T <= 32 ? 32 : T <= 64 ? 64 : 128, 1};
+    const int64_t groups = linear4_groups(p, T, N, pair);
+    while (p.slices < 8 && groups * p.slices < 384 && K / 64 >= 8 * p.slices) p.slices *= 2;
+    return p;
+}
+inline bool linear4_fits(int64_t T, int64_t K, int64_t N, bool pair, int) {
+    return linear4_groups(linear4_plan(T, K, N, pair), T, N, pair) < kGridGroups;
+}
 
 // n / d for n < 2^31 as (mulhi(n, mul) + n) >> shift: shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.
 struct Divisor {
