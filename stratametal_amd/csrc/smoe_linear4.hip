@@ -84,9 +84,15 @@ __device__ __forceinline__ void byte_to_lds(uint32_t lds, const void* p) {
 __device__ __forceinline__ void codes_to_lds(uint32_t lds, const void* p) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 }
+// Four of them to f32, by selects: a branch for each value's type took two thirds of a step.
 __device__ __forceinline__ f32x4 four_scales(const uint32_t* p, int type) {
     const u32x4 v = *reinterpret_cast<const u32x4*>(p);
-    return f32x4{elem_to_f32(v[0], type), elem_to_f32(v[1], type), elem_to_f32(v[2], type), elem_to_f32(v[3], type)};
+    const int up = type == kF32 ? 0 : 16;
+    const bool f16 = type == kF16;
+    f32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v[i]) : u2f(v[i] << up);
+    return r;
 }
 
 }  // namespace
@@ -140,17 +146,22 @@ __global__ __launch_bounds__(512) void k_linear4_few(const Linear4Args a) {
     for (int r = 0; r < RING; ++r) load(wave + r * WAVES, base + r * STAGE);
     const int tok = min(lane & 15, TOKENS - 1);
     const uint32_t w_at = (lane & 15) * 64 + 4 * q, w_sw = (lane >> 2) & 3;
+    const bool whole = a.group % 128 == 0;
     uint32_t at = 0;
     for (int u = wave; u < stages; u += WAVES) {
         vmcnt<(RING - 1) * LOADS>();
         const uint8_t* st = mine + at;
-        int g = 0, left = a.group - u * 128 % a.group;  // of the stage's groups, and what is left of it
-        f32x4 sum[SETS], sx = none;
+        const auto scaled = [&](int g, f32x4 (&sum)[SETS], f32x4 sx) {  // the sums of the stage's group g
 #pragma unroll
-        for (int i = 0; i < SETS; ++i) sum[i] = none;
+            for (int i = 0; i < SETS; ++i) {
+                const f32x4 scale = four_scales(reinterpret_cast<const uint32_t*>(st + i * 1536 + 1024) + g * 16 + 4 * q, a.s_type);
+                const u32x4 z = *reinterpret_cast<const u32x4*>(st + i * 1536 + 1280 + g * 64 + 16 * q);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (u * 128 + s * 32 >= a.n_in) break;
+                for (int j = 0; j < 4; ++j)
+                    acc[i][j] = __builtin_fmaf(scale[j], __builtin_fmaf(zr[i] ? -(float)z[j] : -8.0f, sx[j], sum[i][j]), acc[i][j]);
+            }
+        };
+        const auto product = [&](int s, f32x4 (&sum)[SETS], f32x4& sx) {
             const uint4 xv = *reinterpret_cast<const uint4*>(st + X0 + tok * 256 + ((4 * s + q) ^ tok) * 16);
             sx = mfma16<F16>(make_uint4(one, one, one, one), xv, sx);
 #pragma unroll
@@ -158,20 +169,21 @@ __global__ __launch_bounds__(512) void k_linear4_few(const Linear4Args a) {
                 const uint32_t c = *reinterpret_cast<const uint32_t*>(st + i * 1536 + w_at + (s ^ w_sw) * 16);
                 sum[i] = mfma16<F16>(__builtin_bit_cast(uint4, expand8<F16>(c)), xv, sum[i]);
             }
-            left -= 32;
-            if (left == 0 || s == 3 || u * 128 + s * 32 + 32 >= a.n_in) {
+        };
+        if (whole && u * 128 + 128 <= a.n_in) {  // one group, straight on
+            f32x4 sum[SETS] = {}, sx = none;
 #pragma unroll
-                for (int i = 0; i < SETS; ++i) {
-                    const f32x4 scale = four_scales(reinterpret_cast<const uint32_t*>(st + i * 1536 + 1024) + g * 16 + 4 * q, a.s_type);
-                    const u32x4 z = *reinterpret_cast<const u32x4*>(st + i * 1536 + 1280 + g * 64 + 16 * q);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[i][j] = __builtin_fmaf(scale[j], __builtin_fmaf(zr[i] ? -(float)z[j] : -8.0f, sx[j], sum[i][j]), acc[i][j]);
-                    sum[i] = none;
-                }
-                sx = none;
-                ++g;
-                left = a.group;
+            for (int s = 0; s < 4; ++s) product(s, sum, sx);
+            scaled(0, sum, sx);
+        } else {
+            int g = 0, left = a.group - u * 128 % a.group;  // of the stage's groups, and what is left of it
+#pragma unroll 1
+            for (int s = 0; s < 4 && u * 128 + s * 32 < a.n_in; ++s) {
+                f32x4 sum[SETS] = {}, sx = none;
+                product(s, sum, sx);
+                scaled(g, sum, sx);
+                left -= 32;
+                if (left == 0) left = a.group, ++g;
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -199,10 +211,10 @@ __global__ __launch_bounds__(512) void k_linear4_few(const Linear4Args a) {
 // rows to a wave.  A stage is 64 of K: the wave's codes (half p of row r at place p ^ (r >> 3)), its scales and zeros of the
 // two 32-value steps, and its share of the tokens (as in k_linear_tile), through a ring of RING stages in LDS.  A wave expands
 // the codes of its rows in registers, less their zeros, for all of the tile's tokens; a group's sums are scaled into the
-// outputs' where it ends.  blockIdx.y: a slice of K, whose sums go to `part` for k_linear_join.
-template <int NT, bool PAIR, bool F16>
+// outputs' where it ends (SMALL, groups that do not hold whole steps: after every 32 values).  blockIdx.y: a slice of K, whose sums go to `part` for k_linear_join.
+template <int NT, bool PAIR, bool F16, bool SMALL>
 __global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, int tiles_o, int tiles_t) {
-    constexpr int MT = 2, WAVES = 4, BN = 16 * NT, OUTS = PAIR ? 64 : 128, RING = 3;
+    constexpr int MT = 2, WAVES = 4, BN = 16 * NT, OUTS = PAIR ? 64 : 128, RING = NT == 2 ? 7 : NT == 4 ? 5 : 3;
     constexpr int XS = BN / 8 / WAVES;                                  // a wave's loads of the tokens, 8 rows each
     constexpr int LOADS = 3 + XS, X0 = WAVES * 1536, STAGE = X0 + BN * 128;
     constexpr int NG = NT < 4 ? NT : 4;
@@ -236,13 +248,19 @@ __global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, in
     }
     const int x_lane = 8 * ((lane & 7) ^ (lane >> 3));
     const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds));
+    int next_g = u0 * 64 / a.group, next_left = a.group - u0 * 64 % a.group;  // the group of the next load's first value
     // (codes, scales and zeros past the row's end: its last; the tokens' values there are zeros)
     const auto load = [&](int u, uint32_t at) {
         const int k = u * 64;
         codes_to_lds(at + wave * 1536, codes + min(k / 2 + 16 * half, half_row - 16));
-        const int g0 = min(k / a.group, groups - 1), g1 = min((k + 32) / a.group, groups - 1), g = lane < 32 ? g0 : g1;
-        scale_to_lds(at + wave * 1536 + 1024, scales + g * scale_ld, wide);
-        byte_to_lds(at + wave * 1536 + 1280, zeros_at + g * zero_ld);
+        const int64_t first = min(next_g, groups - 1);
+        next_left -= 32;
+        if (next_left == 0) next_left = a.group, ++next_g;
+        const int64_t second = min(next_g, groups - 1);
+        next_left -= 32;
+        if (next_left == 0) next_left = a.group, ++next_g;
+        scale_to_lds(at + wave * 1536 + 1024, scales + (lane < 32 ? first * scale_ld : second * scale_ld), wide);
+        byte_to_lds(at + wave * 1536 + 1280, zeros_at + (lane < 32 ? first * zero_ld : second * zero_ld));
 #pragma unroll
         for (int i = 0; i < XS; ++i)
             dma16(at + X0 + (i * WAVES + wave) * 1024, k + x_lane < a.n_in ? x_off[i] + 2u * k : kOob, rx, 0);
@@ -271,38 +289,52 @@ __global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, in
         }
         const uint8_t* st = lds + at;
         const uint8_t* ws = st + wave * 1536;
+        u32x4 av[2][MT];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int k = u * 64 + 32 * s;
-            if (s == 1 && k >= a.n_in) break;
-            u32x4 av[MT], bv[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-                bv[n] = *reinterpret_cast<const u32x4*>(st + X0 + (16 * n + fr) * 128 + ((4 * s + q) ^ (fr & 7)) * 16);
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 const uint32_t c = *reinterpret_cast<const uint32_t*>(ws + (16 * m + fr) * 32 + (s ^ (fr >> 3)) * 16 + 4 * q);
                 const uint32_t z = *reinterpret_cast<const uint32_t*>(ws + 1280 + (32 * s + 16 * m + fr) * 4);
-                av[m] = expand8_less<F16>(c, zero_term<F16>((m ? has_zeros2 : has_zeros) ? z : 8u));
+                av[s][m] = expand8_less<F16>(c, zero_term<F16>((m ? has_zeros2 : has_zeros) ? z : 8u));
             }
+        const auto products = [&](int s, auto first) {  // (a group's first starts its sums)
+            u32x4 bv[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                bv[n] = *reinterpret_cast<const u32x4*>(st + X0 + (16 * n + fr) * 128 + ((4 * s + q) ^ (fr & 7)) * 16);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    sum[m][n] = mfma16<F16>(__builtin_bit_cast(uint4, av[m]), __builtin_bit_cast(uint4, bv[n]), sum[m][n]);
-            left -= 32;
-            if (left == 0 || k + 32 >= a.n_in || (s == 1 && u + 1 == u1)) {
+                    sum[m][n] = mfma16<F16>(__builtin_bit_cast(uint4, av[s][m]), __builtin_bit_cast(uint4, bv[n]),
+                                            decltype(first)::value ? none : sum[m][n]);
+        };
+        const auto scaled = [&](int s) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const f32x4 scale = four_scales(reinterpret_cast<const uint32_t*>(ws + 1024) + 32 * s + 16 * m + 4 * q, a.s_type);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[m][n][j] = __builtin_fmaf(scale[j], sum[m][n][j], acc[m][n][j]);
+            }
+        };
+        if constexpr (SMALL) {
+            products(0, std::true_type{});
+            scaled(0);
+            if (u * 64 + 32 < a.n_in) {
+                products(1, std::true_type{});
+                scaled(1);
+            }
+        } else {  // a step lies in one group
+            if (left == a.group || u == u0) products(0, std::true_type{});
+            else products(0, std::false_type{});
+            products(1, std::false_type{});
+            left -= 64;
+            if (left == 0 || u + 1 == u1) {
+                scaled(0);
                 left = a.group;
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const f32x4 scale = four_scales(reinterpret_cast<const uint32_t*>(ws + 1024) + 32 * s + 16 * m + 4 * q, a.s_type);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[m][n][j] = __builtin_fmaf(scale[j], sum[m][n][j], acc[m][n][j]);
-                        sum[m][n] = none;
-                    }
-                }
             }
         }
         at = at + STAGE == RING * STAGE ? 0 : at + STAGE;
@@ -323,11 +355,11 @@ hipError_t launch_few(const Linear4Args& a, hipStream_t s) {
     hipLaunchKernelGGL((k_linear4_few<PAIR, F16, TOKENS>), dim3((a.n_out + 15) / 16), dim3(512), 0, s, a);
     return hipGetLastError();
 }
-template <int NT, bool PAIR, bool F16>
+template <int NT, bool PAIR, bool F16, bool SMALL>
 hipError_t launch_tile4(const Linear4Args& a, int slices, hipStream_t s) {
     constexpr int OUTS = PAIR ? 64 : 128, BN = 16 * NT;
     const int tiles_o = (a.n_out + OUTS - 1) / OUTS, tiles_t = (a.n_tokens + BN - 1) / BN;
-    hipLaunchKernelGGL((k_linear4_tile<NT, PAIR, F16>), dim3(tiles_o * tiles_t, slices), dim3(256), 0, s, a, tiles_o, tiles_t);
+    hipLaunchKernelGGL((k_linear4_tile<NT, PAIR, F16, SMALL>), dim3(tiles_o * tiles_t, slices), dim3(256), 0, s, a, tiles_o, tiles_t);
     return hipGetLastError();
 }
 template <bool PAIR, bool F16>
@@ -336,9 +368,13 @@ hipError_t launch_linear4_as(const Linear4Args& a, hipStream_t s) {
     if (p.tokens == 1) return launch_few<PAIR, F16, 1>(a, s);
     if (p.tokens == 4) return launch_few<PAIR, F16, 4>(a, s);
     if (p.tokens == 16) return launch_few<PAIR, F16, 16>(a, s);
-    const hipError_t e = p.tokens == 32   ? launch_tile4<2, PAIR, F16>(a, p.slices, s)
-                         : p.tokens == 64 ? launch_tile4<4, PAIR, F16>(a, p.slices, s)
-                                          : launch_tile4<8, PAIR, F16>(a, p.slices, s);
+    const auto tile = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        return a.group % 64 ? launch_tile4<NT, PAIR, F16, true>(a, p.slices, s) : launch_tile4<NT, PAIR, F16, false>(a, p.slices, s);
+    };
+    const hipError_t e = p.tokens == 32   ? tile(std::integral_constant<int, 2>{})
+                         : p.tokens == 64 ? tile(std::integral_constant<int, 4>{})
+                                          : tile(std::integral_constant<int, 8>{});
     return e != hipSuccess || p.slices == 1 ? e : launch_linear_join(a, p.slices, s);
 }
 }  // namespace
