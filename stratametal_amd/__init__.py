@@ -826,7 +826,7 @@ class Linear4:
                 _on_device(t, name, w.get_device())
         self.n_in, self.n_out, self.group = n_in, n_out, group
         self.tensors = tuple(t for t, *_ in given)
-        self._act, self._cs = act, {}
+        self._act, self._cs, self._call = act, {}, lib().smoe_linear4_run
         self._device = w.get_device()
         self._s_type = _elem_type(scales.dtype)
         if self._s_type < 0:
@@ -879,7 +879,7 @@ class Linear4:
         if n is None:
             n = sizes[T] = int(lib().smoe_linear4_workspace_bytes(ref, T))
         ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=x.device) if n > 256 else None
-        _check(lib().smoe_linear4_run(ref, x.data_ptr(), x_ld, T, rp, r_ld, y.data_ptr(), yt, y_ld, _ptr(ws), n, st))
+        _check(self._call(ref, x.data_ptr(), x_ld, T, rp, r_ld, y.data_ptr(), yt, y_ld, _ptr(ws), n, st))
         return y
 
     __call__ = run
@@ -920,8 +920,21 @@ def _heads(t, name: str, heads: int, dim: int, tokens: int = -1, device: int = -
     ld, step, one = t.stride()
     if one != 1 or (step != dim and shape[1] > 1):
         raise SmoeError(-5, f"a token's values of {name} are not contiguous")
-    _on_device(t, name, device)
+    if device < 0 or t.get_device() != device:
+        _on_device(t, name, device)
     return code, ld
+
+
+def _flat(t, name: str, dtype, n: int, device: int) -> int:
+    """The address of an (n,) tensor of `dtype` on GPU `device`: _need and _on_device, most calls with less on the host."""
+    try:
+        if t.dtype is dtype and t.get_device() == device >= 0 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _need(t, name, dtype, shape=(n,))
+    _on_device(t, name, device)
+    return t.data_ptr()
 
 
 def _new_heads(tokens: int, heads: int, dim: int, dtype, device):
@@ -949,7 +962,7 @@ class Rotary:
         _on_device(self.turns, "turns")
         self.head_dim, self.rot_dim, self.scale = head_dim, rot_dim, own_scale if scale is None else scale
         self._c = _Rope(head_dim, rot_dim, layout, self.scale, self.turns.data_ptr())
-        self._ref, self._device = C.byref(self._c), self.turns.get_device()
+        self._ref, self._device, self._call = C.byref(self._c), self.turns.get_device(), lib().smoe_rope_run
         # (a call without tokens: the sizes alone are checked)
         _check(lib().smoe_rope_run(self._ref, None, 0, 1, None, F32, 0, None, F32, 0, None))
 
@@ -962,8 +975,7 @@ class Rotary:
         if st is None:
             with _on(self._device, stream):
                 return self.run(x, positions, y, y_dtype)
-        _need(positions, "positions", torch.int32, shape=(T,))
-        _on_device(positions, "positions", self._device)
+        pp = _flat(positions, "positions", torch.int32, T, self._device)
         if y is None:
             dtype = y_dtype or x.dtype
             yt, y_ld = _elem_type(dtype), H * self.head_dim
@@ -972,7 +984,7 @@ class Rotary:
             y = _new_heads(T, H, self.head_dim, dtype, x.device)
         else:
             yt, y_ld = _heads(y, "y", H, self.head_dim, T, self._device)
-        _check(lib().smoe_rope_run(self._ref, positions.data_ptr(), T, H, x.data_ptr(), xt, x_ld, y.data_ptr(), yt, y_ld, st))
+        _check(self._call(self._ref, pp, T, H, x.data_ptr(), xt, x_ld, y.data_ptr(), yt, y_ld, st))
         return y
 
     __call__ = run
@@ -995,8 +1007,9 @@ class PagedCache:
         self._c = _Kv(k.data_ptr(), v.data_ptr(), self._type, *(int(k.shape[i]) for i in (0, 2, 1, 3)))
         self._ref = C.byref(self._c)
         self._sizes: Dict = {}
+        self._append, self._attend = lib().smoe_kv_append, lib().smoe_attend
         # (a call without tokens: the sizes alone are checked)
-        _check(lib().smoe_kv_append(self._ref, None, None, None, 0, F32, None, 0, 0, None, 0, None, 0, None, 0, None))
+        _check(self._append(self._ref, None, None, None, 0, F32, None, 0, 0, None, 0, None, 0, None, 0, None))
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=None, device="cuda"):
@@ -1018,15 +1031,13 @@ class PagedCache:
         if st is None:
             with _on(dev, stream):
                 return self.append(k, v, slots, rotary, positions, q, q_out)
-        _need(slots, "slots", torch.int64, shape=(T,))
-        _on_device(slots, "slots", dev)
+        sp = _flat(slots, "slots", torch.int64, T, dev)
         rp = pp = qp = op = None
         q_ld = o_ld = H = 0
         if rotary is not None:
-            _need(_given(positions, "positions"), "positions", torch.int32, shape=(T,))
-            _on_device(positions, "positions", dev)
-            _on_device(rotary.turns, "the rotary positions' table", dev)
-            rp, pp = rotary._ref, positions.data_ptr()
+            rp, pp = rotary._ref, _flat(_given(positions, "positions"), "positions", torch.int32, T, dev)
+            if rotary._device != dev:
+                raise SmoeError(-1, f"the rotary positions' table is on cuda:{rotary._device}, the cache on cuda:{dev}")
         qt = xt
         if q is not None:
             if rotary is None:
@@ -1044,8 +1055,7 @@ class PagedCache:
             raise SmoeError(-6, "q_out without q")
         if vt != xt or qt != xt:
             raise SmoeError(-1, f"q, k and v are of one type, k is {k.dtype}")
-        _check(lib().smoe_kv_append(self._ref, rp, pp, slots.data_ptr(), T, xt, qp, q_ld, H, op, o_ld, k.data_ptr(), k_ld,
-                                    v.data_ptr(), v_ld, st))
+        _check(self._append(self._ref, rp, pp, sp, T, xt, qp, q_ld, H, op, o_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, st))
         return q_out
 
     def workspace_bytes(self, n_heads: int, n_tokens: int, n_seqs: int, max_len: int, window: int = 0) -> int:
@@ -1068,20 +1078,19 @@ class PagedCache:
             with _on(dev, stream):
                 return self.attend(q, q_start, kv_len, pages, scale, causal, window, lse, max_len, out)
         T, H, _ = q.shape
-        _need(kv_len, "kv_len", torch.int32)
-        if kv_len.dim() != 1:
-            raise SmoeError(-2, "kv_len must be (sequences,)")
-        B = kv_len.shape[0]
-        _need(q_start, "q_start", torch.int32, shape=(B + 1,))
+        B = kv_len.shape[0] if getattr(kv_len, "ndim", 0) == 1 else -1
+        lp, sp = _flat(kv_len, "kv_len", torch.int32, B, dev), _flat(q_start, "q_start", torch.int32, B + 1, dev)
         if not isinstance(pages, torch.Tensor) or pages.dtype != torch.int32:
             raise SmoeError(-1, "pages must be an int32 tensor")
-        if pages.dim() != 2 or pages.shape[0] != B:
+        width = pages.shape[1] if pages.dim() == 2 and pages.shape[0] == B else -1
+        if width < 0:
             raise SmoeError(-2, f"pages has shape {tuple(pages.shape)}, needs ({B}, most pages)")
-        if pages.stride(1) != 1 and pages.shape[1] > 1:
+        p_ld, p_step = pages.stride()
+        if p_step != 1 and width > 1:
             raise SmoeError(-5, "pages' rows are not contiguous")
-        for t, name in ((kv_len, "kv_len"), (q_start, "q_start"), (pages, "pages")):
-            _on_device(t, name, dev)
-        held = min(pages.shape[1] * self.page_size, 1 << 30)
+        if pages.get_device() != dev:
+            _on_device(pages, "pages", dev)
+        held = min(width * self.page_size, 1 << 30)
         max_len = held if max_len is None else max_len
         if out is None:
             out, o_ld = _new_heads(T, H, D, q.dtype, q.device), H * D
@@ -1101,9 +1110,8 @@ class PagedCache:
             self._sizes[key] = n
         # a workspace of the call's own: calls on several streams, captured or not, share none
         ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device) if n > 256 else None
-        _check(lib().smoe_attend(self._ref, q.data_ptr(), q_ld, T, H, q_start.data_ptr(), kv_len.data_ptr(), B, pages.data_ptr(),
-                                 pages.stride(0), pages.shape[1], max_len, D ** -0.5 if scale is None else scale, int(causal), window,
-                                 out.data_ptr(), o_ld, _ptr(z), _ptr(ws), n, st))
+        _check(self._attend(self._ref, q.data_ptr(), q_ld, T, H, sp, lp, B, pages.data_ptr(), p_ld, width, max_len,
+                            D ** -0.5 if scale is None else scale, int(causal), window, out.data_ptr(), o_ld, _ptr(z), _ptr(ws), n, st))
         return (out, z) if lse else out
 
 
