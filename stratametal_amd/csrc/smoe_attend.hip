@@ -299,19 +299,22 @@ constexpr float kLag = 8.0f;
 
 }  // namespace
 
-// Tiles of 128 query rows by KEYS keys, four waves of 32 rows.  A wave forms the transposed scores, keys by queries, with
-// v_mfma_f32_32x32x16: a lane then holds half of a query's scores, so the maximum, the exponentials and the sum are its own,
-// and its weights, in the order in which it holds them, are the second product's right operand as they are (out transposed,
-// values of the head by queries); the keys' order in that product is matched by how the values are read (read_columns).  The
-// running top moves only when a score passes it by kLag, so the sums are scaled seldom.  Keys and values of the next tile
-// travel to LDS while a tile is worked on, the page numbers of the one after with them.
+// Tiles of 128 query rows by 64 keys, four waves of 32 rows, in steps of 32 keys.  A wave forms the transposed scores, keys by
+// queries, with v_mfma_f32_32x32x16: a lane then holds half of a query's scores, so the maximum, the exponentials and the sum
+// are its own, and its weights, in the order in which it holds them, are the second product's right operand as they are (out
+// transposed, values of the head by queries); the keys' order in that product is matched by how the values are read
+// (read_columns).  The running top moves only when a score passes it by kLag, so the sums are scaled seldom.
+// The scores run a step ahead: while the next step's keys are multiplied, this step's weights are formed between the matrix
+// instructions, and while its values are, the next top; what each instruction needs of LDS is read two or three before.  A
+// tile of keys starts a step before the tile of values of the same number, so that two steps work on one tile of each while
+// the keys of the tile after next and the values of the next travel to LDS, page numbers a tile before them.
 template <int DIM, bool F16>
-__global__ __launch_bounds__(256, 2) void k_attend_tile(const AttendArgs a, const AttendPlan p) {
-    constexpr int M = kAttendRows, KEYS = DIM == 256 ? 32 : 64;
+__global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const AttendArgs a, const AttendPlan p) {
+    constexpr int M = kAttendRows, KEYS = kAttendKeys, ND = DIM / 32, NQ = DIM / 16;
     constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = KEYS / RPI / 4;  // lanes to a row, rows of a load, a wave's loads of a tile
-    constexpr int PLANE = KEYS * DIM * 2;
-    __shared__ __align__(1024) uint8_t lds[4 * PLANE];  // two tiles of keys, then values
-    __shared__ int ids[2][64];
+    constexpr int PLANE = KEYS * DIM * 2, HALF = PLANE / 2;
+    __shared__ __align__(1024) uint8_t lds[4 * PLANE];  // two tiles of keys, two of values
+    __shared__ int ids[4][64];
     __shared__ int bad_page;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Work w;
@@ -319,139 +322,254 @@ __global__ __launch_bounds__(256, 2) void k_attend_tile(const AttendArgs a, cons
     if (no_keys(a, p, w, 256)) return;
     if (threadIdx.x == 0) bad_page = 0;
     const int32_t* table = a.pages + w.s.b * a.pages_ld;
-    const int n_tiles = (w.k1 - w.k0 + KEYS - 1) / KEYS;
+    const int n_steps = (w.k1 - w.k0 + 31) / 32;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds)), ids0 = __builtin_amdgcn_readfirstlane(lds_addr(ids));
-    const auto load_ids = [&](int j) {  // a key's page number to a lane
-        const int key = min(w.k0 + j * KEYS + (lane & (KEYS - 1)), w.k1 - 1);
-        to_lds4(ids0 + (j & 1) * 256, table + divide(key, p.page));
+    // row r of key tile j: its key (before the first: the first, past the last: the last)
+    const auto key_of = [&](int j, int r) { return max(w.k0, min(w.k0 + j * KEYS - 32 + r, w.k1 - 1)); };
+    const auto load_ids = [&](int j) {  // a key's page number to a lane (every wave: the same numbers)
+        to_lds4(ids0 + (j & 3) * 256, table + divide(key_of(j, lane), p.page));
     };
-    const int r_lane = lane / LPR;
+    // the lane's rows of a tile in the cache
+    const int r_lane = wave * RPI + lane / LPR;
     bool bad = false;
-    const auto load_tile = [&](int j) {
+    const auto find_rows = [&](int j, int (&rows)[LOADS]) {
+        int page[LOADS];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) page[i] = ids[j & 3][i * 4 * RPI + r_lane];
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int r = (i * 4 + wave) * RPI + r_lane;
-            const int place = min(w.k0 + j * KEYS + r, w.k1 - 1);
-            const int off = place - divide(place, p.page) * a.page_size;
-            int page = ids[j & 1][r];
-            bad |= page < 0 || page >= a.n_pages;
-            page = page < 0 || page >= a.n_pages ? 0 : page;
-            const int c = min((lane % LPR) ^ spread<DIM>(r), a.head_dim / 8 - 1);
-            const int64_t from = ((int64_t)((page * a.n_kv + w.kvh) * a.page_size + off) * a.head_dim + 8 * c) * 2;
-            const uint32_t to = lds0 + (j & 1) * 2 * PLANE + (i * 4 + wave) * 1024;
-            to_lds16(to, a.k + from);
-            to_lds16(to + PLANE, a.v + from);
+            const int key = key_of(j, i * 4 * RPI + r_lane), off = key - divide(key, p.page) * a.page_size;
+            const bool there = (uint32_t)page[i] < (uint32_t)a.n_pages;
+            bad |= !there;
+            rows[i] = ((there ? page[i] : 0) * a.n_kv + w.kvh) * a.page_size + off;
         }
     };
-    if (wave == 0) {
-        load_ids(0);
-        if (n_tiles > 1) load_ids(1);
-    }
+    const int piece_lane = lane % LPR, last_piece = a.head_dim / 8 - 1;
+    const auto load_row = [&](const uint8_t* plane, uint32_t at, int i, int row) {
+        const int c = min(piece_lane ^ spread<DIM>(i * 4 * RPI + r_lane), last_piece);
+        to_lds16(lds0 + at + (i * 4 + wave) * 1024, plane + ((int64_t)row * (a.head_dim * 2) + 16 * c));
+    };
+    load_ids(0), load_ids(1), load_ids(2);
     // this lane's query
     const int h = lane >> 5, r_q = wave * 32 + (lane & 31);
     const int row_q = w.row0 + min(r_q, w.rows - 1);
     const int t_q = row_q / a.group, head = w.kvh * a.group + row_q % a.group;
     const int pos = w.s.len - w.s.n + t_q;
     const int hi = a.causal ? min(pos + 1, w.k1) : w.k1, lo = a.window ? max(pos - a.window + 1, w.k0) : w.k0;
-    // of the wave's queries: keys that all see lie in [lo_all, hi_all), that any sees in [lo_any, hi_any)
-    const int lo_any = __builtin_amdgcn_readfirstlane(lo), hi_all = __builtin_amdgcn_readfirstlane(hi);
-    const int lo_all = __builtin_amdgcn_readlane(lo, 31), hi_any = __builtin_amdgcn_readlane(hi, 31);
+    // keys that all of the wave's queries see: [lo_all, hi_all)
+    const int hi_all = __builtin_amdgcn_readfirstlane(hi), lo_all = __builtin_amdgcn_readlane(lo, 31);
     const bool live = wave * 32 < w.rows;
-    u32x4 qf[DIM / 16];
-    load_query<DIM / 16, 2>(a, w.s.t0 + t_q, head, h, qf);
-    f32x16 acc[DIM / 32];
+    u32x4 qf[NQ];
+    load_query<NQ, 2>(a, w.s.t0 + t_q, head, h, qf);
+    f32x16 acc[ND], even, odd;  // the sums of values, the scores of even and odd steps
 #pragma unroll
-    for (int i = 0; i < DIM / 32; ++i)
+    for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-    float top = -__builtin_inff(), base = 0.0f, sum = 0.0f;
+    float top = -__builtin_inff(), base = 0.0f, sum = 0.0f, odd_sum = 0.0f;
     const float scale = a.scale == 0.0f ? 1.0f : __builtin_fabsf(a.scale);
-    // where the lane reads: row lane & 31 of the keys, pieces h, h + 2, ...; rows 4 h + (lane & 15) / 4 of the values
+    // where the lane reads: row lane & 31 of the keys, pieces h, h + 2, ... (piece i: bits 5 on); rows 4 h + (lane & 15) / 4 and
+    // 8 on of the values, the 16 bytes of its quarter's two lanes (32 values on: bits 6 on)
     const uint32_t k_at = (lane & 31) * DIM * 2 + (h ^ spread<DIM>(lane & 31)) * 16;
     const int v_row = 4 * h + ((lane & 15) >> 2), v_piece = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    const auto value_at = [&](int x) {
+        return (uint32_t)((8 * x + v_row) * DIM * 2 + (v_piece ^ spread<DIM>(8 * x + v_row)) * 16 + 8 * (lane & 1));
+    };
+    const uint32_t v_at[2] = {value_at(0), value_at(1)};
+    const auto all_seen = [&](int key0) { return key0 >= lo_all && key0 + 32 <= hi_all; };
+    const auto mask = [&](f32x16& t, int key0) {
+        const int top_key = hi - key0 - 4 * h, low_key = lo - key0 - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int key = 8 * (i / 4) + i % 4;
+            t[i] = key < top_key && key >= low_key ? t[i] : -__builtin_inff();
+        }
+    };
+    // the top, when a score has passed it: then the sums of values are to be scaled by `keep`
+    float keep = 1.0f;
+    const auto raise = [&](float m) {
+        const float next = __builtin_fmaxf(top, max_halves(m) * scale);
+        keep = next == top ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+        top = next;
+        base = top == -__builtin_inff() ? 0.0f : top;
+        sum *= keep, odd_sum *= keep;
+    };
+    const auto passed = [&](float m) { return __ballot(m * scale > top + kLag) != 0; };
+    const auto max_of = [](const f32x16& t, int from, int to, float m) {
+#pragma unroll
+        for (int e = from; e < to; ++e) m = __builtin_fmaxf(m, t[e]);
+        return m;
+    };
+    // the scores of 32 keys at `place` in LDS into t, `slice(i)` behind matrix instruction i; the longest heads in two chains,
+    // as one wave to a SIMD would wait for each instruction's end
+    const auto scores = [&](uint32_t place, f32x16& t, auto&& slice) {
+        constexpr int AHEAD = 2;
+        constexpr bool TWO = DIM > 128;
+        uint32_t at = k_at + place;
+        asm("" : "+v"(at));  // (the places are formed here, and hold no registers through the products of the values)
+        const auto key_part = [&](int i) { return *reinterpret_cast<const u32x4*>(lds + (at ^ (32 * i))); };
+        u32x4 kf[AHEAD + 1];
+        f32x16 zero, other;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) zero[k] = 0.0f;
+        each_of<AHEAD>([&](auto i) { kf[decltype(i)::value] = key_part(decltype(i)::value); });
+        each_of<NQ>([&](auto idx) {
+            constexpr int I = decltype(idx)::value;
+            if constexpr (I + AHEAD < NQ) kf[(I + AHEAD) % (AHEAD + 1)] = key_part(I + AHEAD);
+            f32x16& sums = TWO && I % 2 ? other : t;
+            sums = mfma32<F16>(kf[I % (AHEAD + 1)], qf[I], I < (TWO ? 2 : 1) ? zero : sums);
+            slice(idx);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (TWO) t = t + other;
+    };
+    constexpr int EACH = 16 / NQ < 2 ? 2 : 16 / NQ;  // weights between two of its matrix instructions
+    u32x4 wt[2];
+    // weight e of the step (of 16 in a lane) in place of its score; two of them, e even, into the sum and the operand
+    const auto weigh = [&](f32x16& t, int e) { t[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[e], scale, -base)); };
+    const auto take = [&](const f32x16& t, int e) {
+        sum += t[e], odd_sum += t[e + 1];
+        uint32_t both = pack2<F16>(t[e], t[e + 1]);
+        asm volatile("" : "+v"(both), "+v"(sum), "+v"(odd_sum));  // here: the compiler would move them behind the mask's branch
+        wt[e / 8][e % 8 / 2] = both;
+    };
+    // the values at `place` times the weights onto the sums, which are scaled first or not, `slice(i)` behind matrix
+    // instruction i
+    const auto values = [&](auto scaled, uint32_t place, auto&& slice) {
+        constexpr int AHEAD = 3, N = 2 * ND;
+        constexpr bool SCALED = decltype(scaled)::value;
+        uint32_t at[2] = {v_at[0] + place, v_at[1] + place};
+        asm("" : "+v"(at[0]), "+v"(at[1]));
+        const auto value_part = [&](int i) {
+            u32x4 f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const u32x2 half = read_columns(lds + 16 * (i / ND) * DIM * 2 + (at[x] ^ (64 * (i % ND))));
+                f[2 * x] = half[0], f[2 * x + 1] = half[1];
+            }
+            return f;
+        };
+        const auto scale_sums = [&](int i) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[i][k] *= keep;
+        };
+        u32x4 vf[AHEAD + 1];
+        each_of<AHEAD>([&](auto i) { vf[decltype(i)::value] = value_part(decltype(i)::value); });
+        if constexpr (SCALED) scale_sums(0);
+        each_of<N>([&](auto idx) {
+            constexpr int I = decltype(idx)::value;
+            if constexpr (I + AHEAD < N) vf[(I + AHEAD) % (AHEAD + 1)] = value_part(I + AHEAD);
+            acc[I % ND] = mfma32<F16>(vf[I % (AHEAD + 1)], wt[I / ND], acc[I % ND]);
+            if constexpr (SCALED && I + 1 < ND) scale_sums(I + 1);
+            slice(idx);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    float m = 0.0f;
+    // a step, whose scores are `t`, and the scores of the next; RARE: the next is not all seen, or the sums are to be scaled
+    const auto step = [&](auto rare, f32x16& t, f32x16& next, uint32_t keys_at, uint32_t values_at, int next_key) {
+        constexpr int N = 2 * ND;
+        scores(keys_at, next, [&](auto idx) {
+            constexpr int I = decltype(idx)::value;
+#pragma unroll
+            for (int e = I * EACH; e < (I + 1) * EACH && e < 16; ++e) weigh(t, e);
+#pragma unroll
+            for (int e = (I - 1) * EACH; e < I * EACH && e < 16; e += 2)
+                if (e >= 0) take(t, e);
+        });
+#pragma unroll
+        for (int e = (NQ - 1) * EACH; e < 16; e += 2) take(t, e);
+        if constexpr (decltype(rare)::value) mask(next, next_key);
+        m = next[0];
+        values(rare, values_at, [&](auto idx) { m = max_of(next, decltype(idx)::value * 16 / N, (decltype(idx)::value + 1) * 16 / N, m); });
+    };
     vmcnt<0>();
     __syncthreads();
-    load_tile(0);
-    for (int j = 0; j < n_tiles; ++j) {
+    int behind[LOADS / 2];  // the lane's rows of the second half of the last key tile: the first half of a tile of values
+    {
+        int rows[LOADS];
+        find_rows(0, rows);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load_row(a.k, 0, i, rows[i]);
+#pragma unroll
+        for (int i = 0; i < LOADS / 2; ++i) behind[i] = rows[i + LOADS / 2];
+    }
+    // the values of tile j and the keys of tile j + 1
+    const auto load_tiles = [&](int j) {
+        int rows[LOADS];
+        find_rows(j + 1, rows);
+        const uint32_t plane = (j & 1) * PLANE;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load_row(a.k, PLANE - plane, i, rows[i]);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load_row(a.v, 2 * PLANE + plane, i, i < LOADS / 2 ? behind[i] : rows[i - LOADS / 2]);
+#pragma unroll
+        for (int i = 0; i < LOADS / 2; ++i) behind[i] = rows[i + LOADS / 2];
+    };
+    load_tiles(0);
+    // what tile j's steps read is there, and every wave is past the steps before
+    const auto turn = [&](int j) {
         vmcnt<0>();
         __syncthreads();
-        if (j + 1 < n_tiles) load_tile(j + 1);
-        if (wave == 0 && j + 2 < n_tiles) load_ids(j + 2);
-        const int key0 = w.k0 + j * KEYS;
-        if (!live || key0 >= hi_any || key0 + KEYS <= lo_any) continue;
-        const uint8_t* k_s = lds + (j & 1) * 2 * PLANE;
-        const uint8_t* v_s = k_s + PLANE;
-        f32x16 s[KEYS / 32];
-#pragma unroll
-        for (int n = 0; n < KEYS / 32; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DIM / 16; ++i)
-#pragma unroll
-            for (int n = 0; n < KEYS / 32; ++n) {
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(k_s + ((k_at ^ (32 * i)) + n * 32 * DIM * 2));
-                s[n] = mfma32<F16>(kf, qf[i], s[n]);
-            }
-        if (key0 < lo_all || key0 + KEYS > hi_all) {
-            const int top_key = hi - key0 - 4 * h, low_key = lo - key0 - 4 * h;
-#pragma unroll
-            for (int n = 0; n < KEYS / 32; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = n * 32 + 8 * (i / 4) + i % 4;
-                    s[n][i] = key < top_key && key >= low_key ? s[n][i] : -__builtin_inff();
+        load_tiles(j + 1);
+        load_ids(j + 3);
+    };
+    vmcnt<0>();
+    __syncthreads();
+    if (live) {
+        scores(HALF, even, [](auto) {});
+        mask(even, w.k0);
+        raise(max_of(even, 0, 16, -__builtin_inff()));
+        // (no branch within the plain steps that their sums would have to pass: the compiler would copy them each time)
+        int u = 0;
+        bool rare = true;
+        while (u + 1 < n_steps) {
+            if (!rare && (u & 1) == 0) {
+                for (;;) {
+                    const uint32_t plane = (u >> 1 & 1) * PLANE;
+                    turn(u >> 1);
+                    step(std::false_type{}, even, odd, PLANE - plane, 2 * PLANE + plane, 0);
+                    ++u;
+                    if (u + 1 >= n_steps || passed(m) || !all_seen(w.k0 + (u + 1) * 32)) {
+                        even = odd;
+                        break;
+                    }
+                    step(std::false_type{}, odd, even, PLANE - plane + HALF, 2 * PLANE + plane + HALF, 0);
+                    ++u;
+                    if (u + 1 >= n_steps || passed(m) || !all_seen(w.k0 + (u + 1) * 32)) break;
                 }
-        }
-        float m = s[0][0];
-#pragma unroll
-        for (int n = 0; n < KEYS / 32; ++n)
-#pragma unroll
-            for (int i = n ? 0 : 1; i < 16; ++i) m = __builtin_fmaxf(m, s[n][i]);
-        if (__ballot(m * scale > top + kLag)) {
-            const float next = __builtin_fmaxf(top, max_halves(m) * scale);
-            const float keep = next == top ? 1.0f : __builtin_amdgcn_exp2f(top - next);
-            top = next;
-            base = top == -__builtin_inff() ? 0.0f : top;
-            sum *= keep;
-#pragma unroll
-            for (int i = 0; i < DIM / 32; ++i)
-#pragma unroll
-                for (int k = 0; k < 16; ++k) acc[i][k] *= keep;
-        }
-        u32x4 wt[KEYS / 16];
-#pragma unroll
-        for (int n = 0; n < KEYS / 32; ++n) {
-            float e[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], scale, -base));
-                sum += e[i];
+            } else {
+                const uint32_t plane = (u >> 1 & 1) * PLANE, half = (u & 1) * HALF;
+                if ((u & 1) == 0) turn(u >> 1);
+                step(std::true_type{}, even, odd, PLANE - plane + half, 2 * PLANE + plane + half, w.k0 + (u + 1) * 32);
+                even = odd;
+                ++u;
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) wt[2 * n + i / 4][i % 4] = pack2<F16>(e[2 * i], e[2 * i + 1]);
+            keep = 1.0f;
+            rare = passed(m);
+            if (rare) raise(m);
+            rare = rare || !all_seen(w.k0 + (u + 1) * 32);
         }
+        vmcnt<0>();
+        __syncthreads();
 #pragma unroll
-        for (int n = 0; n < KEYS / 16; ++n)
+        for (int e = 0; e < 16; ++e) weigh(even, e);
 #pragma unroll
-            for (int i = 0; i < DIM / 32; ++i) {
-                u32x4 vf;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int r = 8 * x + v_row;
-                    const u32x2 half = read_columns(v_s + (16 * n + r) * DIM * 2 + (((4 * i + v_piece) ^ spread<DIM>(r)) * 16) + 8 * (lane & 1));
-                    vf[2 * x] = half[0], vf[2 * x + 1] = half[1];
-                }
-                acc[i] = mfma32<F16>(vf, wt[n], acc[i]);
-            }
+        for (int e = 0; e < 16; e += 2) take(even, e);
+        values(std::true_type{}, 2 * PLANE + (u >> 1 & 1) * PLANE + (u & 1) * HALF, [](auto) {});
+    } else {
+        for (int j = 0; j < n_steps / 2; ++j) turn(j);
+        vmcnt<0>();
+        __syncthreads();
     }
+    sum += odd_sum;
     sum = add_halves(sum);
     if (bad) bad_page = 1;
     __syncthreads();
     if (!live) return;
     const float inv = p.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
     // what is not finite may come of a value that the query does not see (0 times it): such rows are done anew
-    bool odd = !(__builtin_fabsf(sum) < __builtin_inff());
+    bool lost = !(__builtin_fabsf(sum) < __builtin_inff());
     const int t = w.s.t0 + t_q;
     const int64_t row = (int64_t)t * a.n_heads + head;
     const bool mine = r_q < w.rows;
@@ -467,7 +585,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_tile(const AttendArgs a, cons
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 v[x] = acc[i][k + x] * inv;
-                odd |= d < a.head_dim && !(__builtin_fabsf(v[x]) < __builtin_inff());
+                lost |= d < a.head_dim && !(__builtin_fabsf(v[x]) < __builtin_inff());
             }
             if (!mine || d >= a.head_dim) continue;
             if (part) *reinterpret_cast<f32x4*>(part + d) = f32x4{v[0], v[1], v[2], v[3]};
@@ -477,7 +595,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_tile(const AttendArgs a, cons
                 for (int x = 0; x < 4; ++x) out[d + x] = f32_to_half_bits(v[x], F16 ? kF16 : kBf16);
         }
     if (mine && h == 0) put_stats(a, p, row, w.split, top, sum);
-    uint64_t again = __ballot(mine && (odd || bad_page));
+    uint64_t again = __ballot(mine && (lost || bad_page));
     again = (again | again >> 32) & 0xFFFFFFFFull;
     for (; again; again &= again - 1)
         redo_row(a, p, w, wave * 32 + __builtin_ctzll(again), reinterpret_cast<float*>(lds) + wave * kMaxDim, lane);

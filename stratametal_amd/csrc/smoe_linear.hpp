@@ -8,9 +8,6 @@
 #include "smoe_rules.hpp"
 #include "smoe_types.hpp"
 
-#include <type_traits>
-#include <utility>
-
 namespace smoe {
 
 namespace {
@@ -339,17 +336,6 @@ __device__ __forceinline__ void tile_store(const LinearArgs& a, const f32x4 (&ac
             }
         }
     }
-}
-
-// f(0), f(1), ... as compile-time constants
-template <int N, class F, int... I>
-__device__ __forceinline__ void each_of_impl(F&& f, std::integer_sequence<int, I...>) {
-    (f(std::integral_constant<int, I>{}), ...);
-    (void)f;
-}
-template <int N, class F>
-__device__ __forceinline__ void each_of(F&& f) {
-    each_of_impl<N>(f, std::make_integer_sequence<int, N>{});
 }
 
 }  // namespace smoe

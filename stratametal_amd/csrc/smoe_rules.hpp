@@ -322,11 +322,11 @@ constexpr int64_t attend_tiles(int64_t T, int64_t B, int64_t group, int64_t rows
     const int64_t each = T * ((group + rows - 1) / rows), packed = (T * group + B * (rows - 1)) / rows;
     return each < packed ? each : packed;
 }
-// A CU holds two work-groups.  A split costs the work-groups' rounds over those 512 places, each a start and its tiles of keys
-// (32 of them where a head is wider than 128), and beyond one split the launch that joins them and its bytes.
-constexpr int attend_keys(int D) { return D > 128 ? 32 : 64; }
+// A CU holds two work-groups.  A split costs the work-groups' rounds over those 512 places, each a start and its tiles of
+// keys, and beyond one split the launch that joins them and its bytes.
+constexpr int kAttendKeys = 64;
 inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t rows, int D) {
-    const int64_t tile = attend_keys(D), tiles = ((keys + splits - 1) / splits + tile - 1) / tile;
+    const int64_t tile = kAttendKeys, tiles = ((keys + splits - 1) / splits + tile - 1) / tile;
     const int64_t rounds = (groups * splits + 511) / 512;
     return (double)rounds * (4.0 + 2.3 * (double)tiles) + (splits > 1 ? 4.0 + (double)(rows * splits * D) * 8 / 4e6 : 0.0);
 }
@@ -336,7 +336,7 @@ inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_
     p.tiles = (int)attend_tiles(T, B, group, kAttendRows);
     // the most keys that a tile's rows see
     const int64_t seen = window ? window + (kAttendRows + group - 1) / group : max_len, keys = seen < max_len ? seen : max_len;
-    const int64_t groups = (int64_t)p.tiles * kv, tile = attend_keys(D);
+    const int64_t groups = (int64_t)p.tiles * kv, tile = kAttendKeys;
     int64_t best = 1;
     double least = attend_time(groups, 1, keys, rows, D);
     for (int64_t s = 2; groups * s <= 2048 && (s - 1) * tile < keys; ++s) {

@@ -4,6 +4,9 @@
 
 #include "smoe_device.hpp"
 
+#include <type_traits>
+#include <utility>
+
 namespace smoe {
 
 // smoe.h's SMOE_F32, SMOE_F16, SMOE_BF16 (GGUF's type numbers)
@@ -54,5 +57,16 @@ __device__ __forceinline__ float exp_fast(float x) {
 }
 // (the quotient by the hardware's reciprocal: 1 ulp)
 __device__ __forceinline__ float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x)); }
+
+// f(0), f(1), ... as compile-time constants
+template <int N, class F, int... I>
+__device__ __forceinline__ void each_of_impl(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+    (void)f;
+}
+template <int N, class F>
+__device__ __forceinline__ void each_of(F&& f) {
+    each_of_impl<N>(f, std::make_integer_sequence<int, N>{});
+}
 
 }  // namespace smoe
