@@ -120,6 +120,23 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+// c += a b in accumulation registers: left to itself the compiler keeps the sums elsewhere and moves half of them at every step.
+// The hardware does not wait by itself for a matrix instruction's result where another kind of instruction reads it, nor for
+// the operands' last writes, and the compiler does not see that this is one: of a run of them the FIRST and the LAST wait
+// within themselves, so that whatever the compiler puts before or behind the run (copies of the sums too) keeps its distance.
+template <bool F16, bool FIRST, bool LAST>
+__device__ __forceinline__ void mfma32_high(f32x16& c, const u32x4& a, const u32x4& b) {
+#define SMOE_MFMA32(OP)                                                                                                   \
+    if constexpr (FIRST) asm volatile("s_nop 7\n\t" OP " %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));                     \
+    else if constexpr (LAST) asm volatile(OP " %0, %1, %2, %0\n\ts_nop 15\n\ts_nop 15" : "+a"(c) : "v"(a), "v"(b));       \
+    else asm volatile(OP " %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b))
+    if constexpr (F16) {
+        SMOE_MFMA32("v_mfma_f32_32x32x16_f16");
+    } else {
+        SMOE_MFMA32("v_mfma_f32_32x32x16_bf16");
+    }
+#undef SMOE_MFMA32
+}
 // Two f32 to the type's pair, round to nearest even.
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -313,8 +330,9 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     constexpr int M = kAttendRows, KEYS = kAttendKeys, ND = DIM / 32, NQ = DIM / 16;
     constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = KEYS / RPI / 4;  // lanes to a row, rows of a load, a wave's loads of a tile
     constexpr int PLANE = KEYS * DIM * 2, HALF = PLANE / 2;
+    constexpr bool HIGH = DIM > 128;  // the sums of values in accumulation registers
     __shared__ __align__(1024) uint8_t lds[4 * PLANE];  // two tiles of keys, two of values
-    __shared__ int ids[4][64];
+    __shared__ int ids[4][64], rows_s[4][64];  // of a tile's keys: page numbers, then rows of the cache
     __shared__ int bad_page;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Work w;
@@ -329,27 +347,30 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     const auto load_ids = [&](int j) {  // a key's page number to a lane (every wave: the same numbers)
         to_lds4(ids0 + (j & 3) * 256, table + divide(key_of(j, lane), p.page));
     };
-    // the lane's rows of a tile in the cache
-    const int r_lane = wave * RPI + lane / LPR;
+    // a lane's key of tile j: its row in the cache
     bool bad = false;
-    const auto find_rows = [&](int j, int (&rows)[LOADS]) {
-        int page[LOADS];
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) page[i] = ids[j & 3][i * 4 * RPI + r_lane];
+    const auto find_rows = [&](int j) {
+        const int page = ids[j & 3][lane], key = key_of(j, lane), off = key - divide(key, p.page) * a.page_size;
+        const bool there = (uint32_t)page < (uint32_t)a.n_pages;
+        bad |= !there;
+        rows_s[j & 3][lane] = ((there ? page : 0) * a.n_kv + w.kvh) * a.page_size + off;
+    };
+    // the lane's pieces of a tile's rows, from the half of key tile j on
+    const int r_lane = wave * RPI + lane / LPR, piece_lane = lane % LPR, last_piece = a.head_dim / 8 - 1;
+    const auto load_plane = [&](const uint8_t* plane, uint32_t at, int j, int half) {
+        int rows[LOADS];
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int key = key_of(j, i * 4 * RPI + r_lane), off = key - divide(key, p.page) * a.page_size;
-            const bool there = (uint32_t)page[i] < (uint32_t)a.n_pages;
-            bad |= !there;
-            rows[i] = ((there ? page[i] : 0) * a.n_kv + w.kvh) * a.page_size + off;
+            const int r = i * 4 * RPI + r_lane + 32 * half;
+            rows[i] = rows_s[(j + (i * 4 * RPI + 32 * half) / 64) & 3][r & 63];
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int c = min(piece_lane ^ spread<DIM>(i * 4 * RPI + r_lane), last_piece);
+            to_lds16(lds0 + at + (i * 4 + wave) * 1024, plane + ((int64_t)rows[i] * (a.head_dim * 2) + 16 * c));
         }
     };
-    const int piece_lane = lane % LPR, last_piece = a.head_dim / 8 - 1;
-    const auto load_row = [&](const uint8_t* plane, uint32_t at, int i, int row) {
-        const int c = min(piece_lane ^ spread<DIM>(i * 4 * RPI + r_lane), last_piece);
-        to_lds16(lds0 + at + (i * 4 + wave) * 1024, plane + ((int64_t)row * (a.head_dim * 2) + 16 * c));
-    };
-    load_ids(0), load_ids(1), load_ids(2);
+    load_ids(0), load_ids(1), load_ids(2), load_ids(3);
     // this lane's query
     const int h = lane >> 5, r_q = wave * 32 + (lane & 31);
     const int row_q = w.row0 + min(r_q, w.rows - 1);
@@ -453,14 +474,19 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][k] *= keep;
         };
+        if constexpr (SCALED && HIGH) {
+#pragma unroll
+            for (int i = 0; i < ND; ++i) scale_sums(i);
+        }
         u32x4 vf[AHEAD + 1];
         each_of<AHEAD>([&](auto i) { vf[decltype(i)::value] = value_part(decltype(i)::value); });
-        if constexpr (SCALED) scale_sums(0);
+        if constexpr (SCALED && !HIGH) scale_sums(0);
         each_of<N>([&](auto idx) {
             constexpr int I = decltype(idx)::value;
             if constexpr (I + AHEAD < N) vf[(I + AHEAD) % (AHEAD + 1)] = value_part(I + AHEAD);
-            acc[I % ND] = mfma32<F16>(vf[I % (AHEAD + 1)], wt[I / ND], acc[I % ND]);
-            if constexpr (SCALED && I + 1 < ND) scale_sums(I + 1);
+            if constexpr (HIGH) mfma32_high<F16, I == 0, I + 1 == N>(acc[I % ND], vf[I % (AHEAD + 1)], wt[I / ND]);
+            else acc[I % ND] = mfma32<F16>(vf[I % (AHEAD + 1)], wt[I / ND], acc[I % ND]);
+            if constexpr (SCALED && !HIGH && I + 1 < ND) scale_sums(I + 1);
             slice(idx);
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -485,26 +511,14 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     };
     vmcnt<0>();
     __syncthreads();
-    int behind[LOADS / 2];  // the lane's rows of the second half of the last key tile: the first half of a tile of values
-    {
-        int rows[LOADS];
-        find_rows(0, rows);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) load_row(a.k, 0, i, rows[i]);
-#pragma unroll
-        for (int i = 0; i < LOADS / 2; ++i) behind[i] = rows[i + LOADS / 2];
-    }
+    if (wave < 3) find_rows(wave);
+    __syncthreads();
+    load_plane(a.k, 0, 0, 0);
     // the values of tile j and the keys of tile j + 1
     const auto load_tiles = [&](int j) {
-        int rows[LOADS];
-        find_rows(j + 1, rows);
         const uint32_t plane = (j & 1) * PLANE;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) load_row(a.k, PLANE - plane, i, rows[i]);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) load_row(a.v, 2 * PLANE + plane, i, i < LOADS / 2 ? behind[i] : rows[i - LOADS / 2]);
-#pragma unroll
-        for (int i = 0; i < LOADS / 2; ++i) behind[i] = rows[i + LOADS / 2];
+        load_plane(a.k, PLANE - plane, j + 1, 0);
+        load_plane(a.v, 2 * PLANE + plane, j, 1);
     };
     load_tiles(0);
     // what tile j's steps read is there, and every wave is past the steps before
@@ -512,7 +526,8 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
         vmcnt<0>();
         __syncthreads();
         load_tiles(j + 1);
-        load_ids(j + 3);
+        if (wave == (j & 3)) find_rows(j + 3);
+        load_ids(j + 4);
     };
     vmcnt<0>();
     __syncthreads();
