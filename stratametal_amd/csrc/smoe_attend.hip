@@ -1,6 +1,7 @@
 // stratametal_amd/csrc/smoe_attend.hip - attention of each sequence's new tokens over its pages of the cache (gfx950, wave64):
 // out = sum_j w_j v_j, w = softmax of scale q k_j over the keys that the query sees.
 #include "smoe_dma.hpp"
+#include "smoe_gemv.hpp"
 #include "smoe_launch.hpp"
 #include "smoe_rules.hpp"
 #include "smoe_types.hpp"
@@ -15,27 +16,10 @@ namespace {
 constexpr float kLn2 = 0.693147181f;
 constexpr int kMaxDim = 256;
 
-// The sequence that holds query row t, and its first row and key count; b < 0: none.
+// Sequence b: its first query row, rows and keys.
 struct Sequence {
     int b, t0, n, len;
 };
-__device__ __forceinline__ Sequence sequence_at(const AttendArgs& a, int b, int t0, int t1) {
-    const int len = min(max(a.kv_len[b], 0), a.max_len);
-    return {b, t0, t1 - t0, len};
-}
-__device__ __forceinline__ Sequence sequence_of(const AttendArgs& a, int t, int lane) {
-    for (int at = 0; at < a.n_seqs; at += 64) {
-        const int b = min(at + lane, a.n_seqs - 1);
-        const int t0 = a.q_start[b], t1 = min(a.q_start[b + 1], a.n_tokens);
-        const uint64_t in = __ballot(t0 <= t && t < t1);
-        if (in) {
-            const int l = __builtin_ctzll(in);
-            return sequence_at(a, __shfl(b, l), max(__shfl(t0, l), 0), __shfl(t1, l));
-        }
-    }
-    return {-1, 0, 0, 0};
-}
-
 __device__ __forceinline__ float half_value(uint32_t bits, bool f16) { return elem_to_f32(bits, f16 ? kF16 : kBf16); }
 
 // One query row by one wave, 64 keys at a time, a key to a lane for its score and 64 values of the head to the wave for the
@@ -191,58 +175,60 @@ struct Work {
     Sequence s;
     int row0, rows, kvh, split, k0, k1;
 };
-// Tile `tile` of M rows: the sequences' tiles lie one behind the other.
-template <int M>
-__device__ __forceinline__ bool find_tile(const AttendArgs& a, int tile, int lane, Work& w) {
-    const int g = a.group;
-    int before = 0;
+// Work-group i: the key heads of a tile and split lie side by side, so that with eight of them each has an XCD (and its L2) to
+// itself; the sequences' tiles of M rows lie one behind the other, and the last, which see the most keys, come first.
+//
+// The plan's splits are made for the longest sequence that the call allows; how many keys a piece has is settled here, from
+// the lengths that are there: with sequences of about one length whose tiles are fewer than the PLACES of work-groups on the
+// card, as many pieces as fill these once; else pieces of a quarter of a place's share, at least the longest over the plan's splits.
+// (8 sequences of 4000 keys, 8 key heads: 8 pieces 37 us, 16 47; 64 sequences of up to 8192 keys: 1 piece 223 us, 7 215.)
+template <int M, int PLACES>
+__device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan& p, int lane, Work& w) {
+    const int i = blockIdx.x, g = a.group, j = i / a.n_kv, tile = p.tiles - 1 - j % p.tiles;
+    w.kvh = i % a.n_kv;
+    w.split = j / p.tiles;
+    const int seen = a.window ? min(a.window, a.max_len) + (M + g - 1) / g : a.max_len;
+    bool found = false;
+    int before = 0, most = 0;
+    float total = 0.0f;
+    int3 next = {0, 0, 0};
+    if (lane < a.n_seqs) next = {a.q_start[lane], a.q_start[lane + 1], a.kv_len[lane]};
     for (int at = 0; at < a.n_seqs; at += 64) {
-        const int b = at + lane;
-        int t0 = 0, t1 = 0;
-        if (b < a.n_seqs) {
-            t0 = min(max(a.q_start[b], 0), a.n_tokens);
-            t1 = min(max(a.q_start[b + 1], t0), a.n_tokens);
-        }
-        const int tiles = ((t1 - t0) * g + M - 1) / M;
-        int sum = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(sum, d);
-            sum += lane >= d ? v : 0;
-        }
-        const uint64_t past = __ballot(tile < before + sum);
+        const int t0 = min(max(next.x, 0), a.n_tokens), t1 = min(max(next.y, t0), a.n_tokens), len = min(max(next.z, 0), a.max_len);
+        next = {0, 0, 0};
+        if (const int b = at + 64 + lane; b < a.n_seqs) next = {a.q_start[b], a.q_start[b + 1], a.kv_len[b]};
+        const int tiles = ((t1 - t0) * g + M - 1) / M, sum = wave_inclusive_scan(tiles);
+        const uint64_t past = found ? 0 : __ballot(tile < before + sum);
         if (past) {
             const int l = __builtin_ctzll(past);
-            const int first = before + __shfl(sum - tiles, l);
-            const int s0 = __builtin_amdgcn_readfirstlane(__shfl(t0, l)), s1 = __builtin_amdgcn_readfirstlane(__shfl(t1, l));
-            w.s = sequence_at(a, __builtin_amdgcn_readfirstlane(at + l), s0, s1);
-            w.s.len = __builtin_amdgcn_readfirstlane(w.s.len);
-            w.row0 = __builtin_amdgcn_readfirstlane((tile - first) * M);
+            const int s0 = __builtin_amdgcn_readlane(t0, l), s1 = __builtin_amdgcn_readlane(t1, l);
+            w.s = {__builtin_amdgcn_readfirstlane(at + l), s0, s1 - s0, __builtin_amdgcn_readlane(len, l)};
+            w.row0 = (tile - before - __builtin_amdgcn_readlane(sum - tiles, l)) * M;
             w.rows = min(M, w.s.n * g - w.row0);
-            return true;
+            found = true;
+            if (p.splits == 1) break;
         }
-        before += __shfl(sum, 63);
+        before += __builtin_amdgcn_readlane(sum, 63);
+        const int keys = tiles ? min(len, seen) : 0;
+        most = max(most, keys);
+        total += (float)tiles * (float)keys;
     }
-    return false;
-}
-// Work-group i: the key heads of a tile and split lie side by side, so that with eight of them each has an XCD (and its L2) to
-// itself; the sequences' last tiles, which see the most keys, come first.
-template <int M>
-__device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan& p, int lane, Work& w) {
-    const int i = blockIdx.x;
-    w.kvh = i % a.n_kv;
-    const int j = i / a.n_kv;
-    w.split = j / p.tiles;
-    if (!find_tile<M>(a, p.tiles - 1 - j % p.tiles, lane, w)) return false;
+    if (!found) return false;
     // the keys that some row of the tile sees
-    const int first = w.s.len - w.s.n + w.row0 / a.group, last = w.s.len - w.s.n + (w.row0 + w.rows - 1) / a.group;
+    const int first = w.s.len - w.s.n + w.row0 / g, last = w.s.len - w.s.n + (w.row0 + w.rows - 1) / g;
     w.k0 = a.window ? max(0, first - a.window + 1) : 0;
     w.k1 = a.causal ? min(w.s.len, last + 1) : w.s.len;
     w.k0 = max(w.k0, 0), w.k1 = max(w.k1, w.k0);
     if (p.splits > 1) {
-        // equal pieces of at most p.chunk keys, counted from the first one seen
-        const int64_t from = (int64_t)w.k0 + (int64_t)w.split * p.chunk;
-        w.k1 = (int)min((int64_t)w.k1, from + p.chunk);
+        total = wave_sum_xor_fast(total), most = (int)wave_max_u32_fast((uint32_t)most);
+        const float groups = (float)before * (float)a.n_kv, all = total * (float)a.n_kv;
+        const bool one = groups <= PLACES && (float)most * groups <= 1.25f * all;
+        const float share = one ? (float)(most - 1) / __builtin_floorf(PLACES / groups) : all * (0.25f / PLACES);
+        int chunk = max((int)__builtin_fminf(share, (float)most), (most - 1) / p.splits);
+        chunk = (chunk / kAttendKeys + 1) * kAttendKeys;
+        chunk = __builtin_amdgcn_readfirstlane(chunk);
+        const int64_t from = (int64_t)w.k0 + (int64_t)w.split * chunk;
+        w.k1 = (int)min((int64_t)w.k1, from + chunk);
         w.k0 = (int)min(from, (int64_t)w.k1);
     }
     return true;
@@ -336,7 +322,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     __shared__ int bad_page;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Work w;
-    if (!find_work<M>(a, p, lane, w)) return;
+    if (!find_work<M, (DIM > 128 ? 256 : 512)>(a, p, lane, w)) return;
     if (no_keys(a, p, w, 256)) return;
     if (threadIdx.x == 0) bad_page = 0;
     const int32_t* table = a.pages + w.s.b * a.pages_ld;

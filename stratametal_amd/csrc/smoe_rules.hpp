@@ -322,13 +322,20 @@ constexpr int64_t attend_tiles(int64_t T, int64_t B, int64_t group, int64_t rows
     const int64_t each = T * ((group + rows - 1) / rows), packed = (T * group + B * (rows - 1)) / rows;
     return each < packed ? each : packed;
 }
-// A CU holds two work-groups.  A split costs the work-groups' rounds over those 512 places, each a start and its tiles of
-// keys, and beyond one split the launch that joins them and its bytes.
+// A CU holds two work-groups (one of heads wider than 128), each at 2.3 us a tile of keys (1.3 of heads up to 64) and 4 us
+// beside them.  One sequence's splits run in rounds of whole ones; those of several, whose lengths differ (by half the longest
+// on average), fill the CUs one after the other, but for the last.  Beyond one split there are the launch that joins them and
+// its bytes.  us, by splits: 1 token over 131072 keys, 4 key heads of 128: 64 75, 128 70, 256 73; 56 tokens of 64 sequences of
+// up to 8192 keys, 8 key heads: 1 223, 5 219, 7 215, 16 223; 796 tokens of 6, a window of 500 keys, heads of 64: 1 21, 2 23, 3 27;
+// 1024 tokens over 33792 keys, 32 heads, 8 key heads: 1 770, 2 627, 4 646; 8192 tokens, the same heads: 1 613, 2 755.
 constexpr int kAttendKeys = 64;
-inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t rows, int D) {
-    const int64_t tile = kAttendKeys, tiles = ((keys + splits - 1) / splits + tile - 1) / tile;
-    const int64_t rounds = (groups * splits + 511) / 512;
-    return (double)rounds * (4.0 + 2.3 * (double)tiles) + (splits > 1 ? 4.0 + (double)(rows * splits * D) * 8 / 4e6 : 0.0);
+inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t rows, int64_t B, int D) {
+    const int64_t tiles = ((keys + splits - 1) / splits + kAttendKeys - 1) / kAttendKeys, places = D > 128 ? 256 : 512;
+    const double tile = D > 64 ? 2.3 : 1.3, most = 4.0 + tile * (double)tiles;
+    const double join = splits > 1 ? 4.0 + (double)(rows * splits * D) * 8 / 4e6 : 0.0;
+    if (B == 1) return (double)((groups * splits + places - 1) / places) * most + join;
+    const double all = (double)(groups * splits) * (4.0 + tile * (double)tiles / 2) / (double)places + most / 2;
+    return (all > most ? all : most) + join;
 }
 inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_t max_len, int64_t window) {
     AttendPlan p{};
@@ -338,9 +345,9 @@ inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_
     const int64_t seen = window ? window + (kAttendRows + group - 1) / group : max_len, keys = seen < max_len ? seen : max_len;
     const int64_t groups = (int64_t)p.tiles * kv, tile = kAttendKeys;
     int64_t best = 1;
-    double least = attend_time(groups, 1, keys, rows, D);
-    for (int64_t s = 2; groups * s <= 2048 && (s - 1) * tile < keys; ++s) {
-        const double us = attend_time(groups, s, keys, rows, D);
+    double least = attend_time(groups, 1, keys, rows, B, D);
+    for (int64_t s = 2; groups * s <= 4096 && (s - 1) * tile < keys; ++s) {
+        const double us = attend_time(groups, s, keys, rows, B, D);
         if (us < least) least = us, best = s;
     }
     p.chunk = (int)(((keys + best - 1) / best + tile - 1) / tile * tile);
