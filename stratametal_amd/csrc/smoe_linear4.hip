@@ -84,15 +84,14 @@ __device__ __forceinline__ void byte_to_lds(uint32_t lds, const void* p) {
 __device__ __forceinline__ void codes_to_lds(uint32_t lds, const void* p) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 }
-// Four of them to f32, by selects: a branch for each value's type took two thirds of a step.
+// One or four of them to f32, by selects: a branch for each value's type took two thirds of a step.
+__device__ __forceinline__ float one_scale(uint32_t v, int type) {
+    const float f16 = (float)__builtin_bit_cast(_Float16, (uint16_t)v);
+    return type == kF16 ? f16 : u2f(v << (type == kF32 ? 0 : 16));
+}
 __device__ __forceinline__ f32x4 four_scales(const uint32_t* p, int type) {
     const u32x4 v = *reinterpret_cast<const u32x4*>(p);
-    const int up = type == kF32 ? 0 : 16;
-    const bool f16 = type == kF16;
-    f32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v[i]) : u2f(v[i] << up);
-    return r;
+    return f32x4{one_scale(v[0], type), one_scale(v[1], type), one_scale(v[2], type), one_scale(v[3], type)};
 }
 
 }  // namespace
@@ -207,27 +206,33 @@ __global__ __launch_bounds__(512) void k_linear4_few(const Linear4Args a) {
     finish4<PAIR>(a, rows_vec(a), t, o, {g[0], g[1], g[2], g[3]}, {u[0], u[1], u[2], u[3]});
 }
 
-// More tokens: 128 weight rows (PAIR: 64 of each matrix, 16 of each in turn) by 16 NT tokens to a work-group of four waves, 32
-// rows to a wave.  A stage is 64 of K: the wave's codes (half p of row r at place p ^ (r >> 3)), its scales and zeros of the
-// two 32-value steps, and its share of the tokens (as in k_linear_tile), through a ring of RING stages in LDS.  A wave expands
-// the codes of its rows in registers, less their zeros, for all of the tile's tokens; a group's sums are scaled into the
-// outputs' where it ends (SMALL, groups that do not hold whole steps: after every 32 values).  blockIdx.y: a slice of K, whose sums go to `part` for k_linear_join.
+// More tokens: 128 weight rows (PAIR: 64 of each matrix, 16 of each in turn) by 16 NT tokens, 32 rows to each of four waves; up to
+// 64 tokens a work-group has eight, four for each half of its slice of K, whose sums meet in LDS.  A step is 64 of K: the
+// wave's codes (half p of row r at place p ^ (r >> 3)), its scales and zeros of the two 32-value steps, and its share of the
+// tokens (as in k_linear_tile), through a ring of RING stages in LDS.  A wave expands the codes of its rows in registers, less
+// their zeros, for all of the tile's tokens; a group's sums are scaled into the outputs' where it ends (SMALL, groups that do
+// not hold whole steps: after every 32 values).  blockIdx.y: a slice of K, whose sums go to `part` for k_linear_join.
+// A step is bound by the instructions that expand and scale (180 to 290 beside 32 matrix instructions at 128 tokens) and by the
+// reads and the barrier before them: 2048 tokens, 4096 x 4096, groups of 128: 100 us, 686 TFLOP/s (groups of 32: 110); 79 without
+// the loads, 58 without expansion and scales as well.
 template <int NT, bool PAIR, bool F16, bool SMALL>
-__global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, int tiles_o, int tiles_t) {
-    constexpr int MT = 2, WAVES = 4, BN = 16 * NT, OUTS = PAIR ? 64 : 128, RING = NT == 2 ? 7 : NT == 4 ? 5 : 3;
+__global__ __launch_bounds__(256 * kLinear4Parts<NT>, 2 / kLinear4Parts<NT>) void k_linear4_tile(const Linear4Args a, int tiles_o, int tiles_t) {
+    constexpr int MT = 2, WAVES = 4, BN = 16 * NT, OUTS = PAIR ? 64 : 128, PARTS = kLinear4Parts<NT>, RING = NT == 2 ? 7 : NT == 4 ? 5 : 3;
     constexpr int XS = BN / 8 / WAVES;                                  // a wave's loads of the tokens, 8 rows each
-    constexpr int LOADS = 3 + XS, X0 = WAVES * 1536, STAGE = X0 + BN * 128;
+    constexpr int LOADS = 3 + XS, X0 = WAVES * 1536, STAGE = X0 + BN * 128, SLOT = PARTS * STAGE;
     constexpr int NG = NT < 4 ? NT : 4;
-    static_assert(WAVES * kStoreBytes<MT, NG> <= RING * STAGE, "the waves' pieces of the epilogue");
-    __shared__ __align__(1024) uint8_t lds[RING * STAGE];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
+    static_assert(WAVES * (kStoreBytes<MT, NG> + (PARTS - 1) * MT * NT * 1024) <= RING * SLOT, "the waves' pieces of the epilogue, a part's sums");
+    __shared__ __align__(1024) uint8_t lds[RING * SLOT];
+    const int lane = threadIdx.x & 63, q = lane >> 4;
+    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3);
     int to, tt;
     tile_of(blockIdx.x, gridDim.x, tiles_o, tiles_t, to, tt);
     const int o0 = to * OUTS, t0 = tt * BN;
     const int n_t = min(BN, a.n_tokens - t0);
     const int half_row = a.n_in / 2, groups = (a.n_in + a.group - 1) / a.group;
     const int all = (a.n_in + 63) / 64;
-    const int u0 = (int)((int64_t)all * blockIdx.y / gridDim.y), u1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
+    const int s0 = (int)((int64_t)all * blockIdx.y / gridDim.y), s1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
+    const int steps = (s1 - s0 + PARTS - 1) / PARTS, u0 = s0 + part * steps, u1 = min(u0 + steps, s1);
     const bool wide = a.s_type == kF32;
     // row i (0 .. 31) of the wave: its matrix and output
     const auto matrix = [&](int i) { return PAIR && i >= 16; };
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, in
         x_off[i] = r < n_t ? (uint32_t)(r * a.x_ld * 2) + 16u * ((lane & 7) ^ (lane >> 3)) : kOob;
     }
     const int x_lane = 8 * ((lane & 7) ^ (lane >> 3));
-    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds));
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + part * STAGE;
     int next_g = u0 * 64 / a.group, next_left = a.group - u0 * 64 % a.group;  // the group of the next load's first value
     // (codes, scales and zeros past the row's end: its last; the tokens' values there are zeros)
     const auto load = [&](int u, uint32_t at) {
@@ -272,23 +277,29 @@ __global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, in
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = sum[m][n] = none;
 #pragma unroll
-    for (int r = 0; r < RING - 1; ++r) load(u0 + r, base + r * STAGE);
+    for (int r = 0; r < RING - 1; ++r) load(u0 + r, base + r * SLOT);
     const int fr = lane & 15;
     int left = a.group - u0 * 64 % a.group;  // of the group
     const bool has_zeros = a.zeros != nullptr, has_zeros2 = PAIR ? a.zeros2 != nullptr : has_zeros;
     uint32_t at = 0;
-    for (int u = u0; u < u1; ++u) {
+    for (int u = u0; u < u0 + steps; ++u) {
         // every wave has read the step before, and this one is there
         vmcnt<(RING - 2) * LOADS>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         {
-            const uint32_t next = at + (RING - 1) * STAGE;
-            load(u + RING - 1, base + (next >= RING * STAGE ? next - RING * STAGE : next));
+            const uint32_t next = at + (RING - 1) * SLOT;
+            load(u + RING - 1, base + (next >= RING * SLOT ? next - RING * SLOT : next));
         }
-        const uint8_t* st = lds + at;
-        const uint8_t* ws = st + wave * 1536;
+        uint8_t* const st = lds + at + part * STAGE;
+        uint8_t* const ws = st + wave * 1536;
+        at = at + SLOT == RING * SLOT ? 0 : at + SLOT;
+        if (PARTS > 1 && u >= u1) continue;  // (the second part's last step, of an odd number)
+        {  // the step's scales to f32 where they lie, one by each lane
+            uint32_t* const own = reinterpret_cast<uint32_t*>(ws + 1024) + lane;
+            *own = f2u(one_scale(*own, a.s_type));
+        }
         u32x4 av[2][MT];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -298,22 +309,25 @@ __global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, in
                 const uint32_t z = *reinterpret_cast<const uint32_t*>(ws + 1280 + (32 * s + 16 * m + fr) * 4);
                 av[s][m] = expand8_less<F16>(c, zero_term<F16>((m ? has_zeros2 : has_zeros) ? z : 8u));
             }
-        const auto products = [&](int s, auto first) {  // (a group's first starts its sums)
-            u32x4 bv[NT];
+        const auto products = [&](int s, auto first) {  // (SMALL: a step's first starts its sums)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                bv[n] = *reinterpret_cast<const u32x4*>(st + X0 + (16 * n + fr) * 128 + ((4 * s + q) ^ (fr & 7)) * 16);
+            for (int n0 = 0; n0 < NT; n0 += NG) {
+                u32x4 bv[NG];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+                for (int n = 0; n < NG; ++n)
+                    bv[n] = *reinterpret_cast<const u32x4*>(st + X0 + (16 * (n0 + n) + fr) * 128 + ((4 * s + q) ^ (fr & 7)) * 16);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    sum[m][n] = mfma16<F16>(__builtin_bit_cast(uint4, av[s][m]), __builtin_bit_cast(uint4, bv[n]),
-                                            decltype(first)::value ? none : sum[m][n]);
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int n = 0; n < NG; ++n)
+                        sum[m][n0 + n] = mfma16<F16>(__builtin_bit_cast(uint4, av[s][m]), __builtin_bit_cast(uint4, bv[n]),
+                                                     decltype(first)::value ? none : sum[m][n0 + n]);
+            }
         };
         const auto scaled = [&](int s) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const f32x4 scale = four_scales(reinterpret_cast<const uint32_t*>(ws + 1024) + 32 * s + 16 * m + 4 * q, a.s_type);
+                const f32x4 scale = *reinterpret_cast<const f32x4*>(ws + 1024 + (32 * s + 16 * m + 4 * q) * 4);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -328,19 +342,36 @@ __global__ __launch_bounds__(256, 2) void k_linear4_tile(const Linear4Args a, in
                 scaled(1);
             }
         } else {  // a step lies in one group
-            if (left == a.group || u == u0) products(0, std::true_type{});
-            else products(0, std::false_type{});
+            products(0, std::false_type{});
             products(1, std::false_type{});
             left -= 64;
             if (left == 0 || u + 1 == u1) {
                 scaled(0);
                 left = a.group;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) sum[m][n] = none;
             }
         }
-        at = at + STAGE == RING * STAGE ? 0 : at + STAGE;
     }
     vmcnt<0>();
     __syncthreads();
+    if constexpr (PARTS == 2) {  // the second part's sums to the first
+        f32x4* const other = reinterpret_cast<f32x4*>(lds + WAVES * kStoreBytes<MT, NG>) + wave * (MT * NT * 64) + lane;
+        if (part == 1) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) other[(m * NT + n) * 64] = acc[m][n];
+        }
+        __syncthreads();
+        if (part == 1) return;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[m][n] = acc[m][n] + other[(m * NT + n) * 64];
+    }
     tile_store<MT, NT, NG, PAIR>(a, acc, lds + wave * kStoreBytes<MT, NG>, o0 + wave * (PAIR ? 16 : 32), t0, t0 + n_t, lane);
 }
 
@@ -359,7 +390,7 @@ template <int NT, bool PAIR, bool F16, bool SMALL>
 hipError_t launch_tile4(const Linear4Args& a, int slices, hipStream_t s) {
     constexpr int OUTS = PAIR ? 64 : 128, BN = 16 * NT;
     const int tiles_o = (a.n_out + OUTS - 1) / OUTS, tiles_t = (a.n_tokens + BN - 1) / BN;
-    hipLaunchKernelGGL((k_linear4_tile<NT, PAIR, F16, SMALL>), dim3(tiles_o * tiles_t, slices), dim3(256), 0, s, a, tiles_o, tiles_t);
+    hipLaunchKernelGGL((k_linear4_tile<NT, PAIR, F16, SMALL>), dim3(tiles_o * tiles_t, slices), dim3(256 * kLinear4Parts<NT>), 0, s, a, tiles_o, tiles_t);
     return hipGetLastError();
 }
 template <bool PAIR, bool F16>

@@ -280,6 +280,9 @@ template <bool PAIR, int TOKENS>
 constexpr int kLinear4Stage = (PAIR ? 2 : 1) * 1536 + (TOKENS > 4 ? TOKENS / 4 : 1) * 1024;
 template <bool PAIR, int TOKENS>
 constexpr int kLinear4Ring = TOKENS > 4 ? (PAIR ? 2 : 3) : PAIR ? 2 : 4;
+// k_linear4_tile, 16 NT tokens: the parts of a slice of K, each by four waves of a work-group.
+template <int NT>
+constexpr int kLinear4Parts = NT < 8 ? 2 : 1;
 // The tokens that a work-group takes: 1, 4 and 16 k_linear4_few's, 32 to 128 a tile's, with K in slices.
 struct Linear4Plan {
     int tokens, slices;
@@ -289,12 +292,29 @@ inline int64_t linear4_groups(Linear4Plan p, int64_t T, int64_t N, bool pair) {
     const int outs = pair ? 64 : 128;
     return (N + outs - 1) / outs * ((T + p.tokens - 1) / p.tokens);
 }
+// A tile's time: the rounds of its work-groups over the 256 CUs (two on one of 128 tokens), each 5 us and its steps of 64 of K,
+// 1.0 us of 32 tokens, 1.17 of 64 and 1.0 of 128 (1.5 where two share a CU); with slices the launch that joins them, and
+// its bytes.  us, by tokens of a tile and slices: 33 tokens, 4096 x 4096: 32/1 37, 32/4 21.5, 64/4 22, 64/8 20.5; 128 tokens, 2048 x
+// 16384: 64/1 30, 64/2 40, 128/2 35; 301 tokens, 2560 x 5003: 64/1 39, 128/2 40, 128/4 36; 512 tokens, 4096 x 4096: 64/1 46, 128/1 70,
+// 128/4 45; 2048 tokens: 64/1 167, 128/1 100, 128/2 119.
+inline double linear4_time(Linear4Plan p, int64_t T, int64_t K, int64_t N, bool pair) {
+    const int64_t groups = linear4_groups(p, T, N, pair) * p.slices, places = p.tokens == 128 ? 512 : 256;
+    const int64_t steps = (K + 63) / 64, parts = p.slices * (p.tokens == 128 ? 1 : 2), each = (steps + parts - 1) / parts;
+    const double step = p.tokens == 32 ? 1.0 : p.tokens == 64 ? 1.17 : groups <= 256 ? 1.0 : 1.5;
+    const double join = p.slices > 1 ? 4.5 + (double)(T * N * p.slices * (pair ? 2 : 1)) * 8 / 4e6 : 0.0;
+    return (double)((groups + places - 1) / places) * (5.0 + step * (double)each) + join;
+}
 inline Linear4Plan linear4_plan(int64_t T, int64_t K, int64_t N, bool pair) {
     if (T <= 16) return {T <= 1 ? 1 : T <= 4 ? 4 : 16, 1};
-    Linear4Plan p{T <= 32 ? 32 : T <= 64 ? 64 : 128, 1};
-    const int64_t groups = linear4_groups(p, T, N, pair);
-    while (p.slices < 8 && groups * p.slices < 384 && K / 64 >= 8 * p.slices) p.slices *= 2;
-    return p;
+    Linear4Plan best{32, 1};
+    double least = linear4_time(best, T, K, N, pair);
+    for (int tokens = 32; tokens <= 128; tokens *= 2)
+        for (int slices = 1; slices <= 8 && (slices == 1 || K / 64 >= 4 * slices); slices *= 2) {
+            const Linear4Plan p{tokens, slices};
+            const double us = linear4_time(p, T, K, N, pair);
+            if (us < least) least = us, best = p;
+        }
+    return best;
 }
 inline bool linear4_fits(int64_t T, int64_t K, int64_t N, bool pair, int) {
     return linear4_groups(linear4_plan(T, K, N, pair), T, N, pair) < kGridGroups;
