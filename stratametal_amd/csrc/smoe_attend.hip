@@ -106,20 +106,18 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 }
 // c += a b in accumulation registers: left to itself the compiler keeps the sums elsewhere and moves half of them at every step.
 // The hardware does not wait by itself for a matrix instruction's result where another kind of instruction reads it, nor for
-// the operands' last writes, and the compiler does not see that this is one: of a run of them the FIRST and the LAST wait
-// within themselves, so that whatever the compiler puts before or behind the run (copies of the sums too) keeps its distance.
-template <bool F16, bool FIRST, bool LAST>
+// the operands' last writes, and the compiler does not see that this is one: high_wait stands before a run of them, with all the
+// sums and the weights as its operands, and one behind it, so that copies of the sums lie outside both and keep their distance.
+template <bool F16>
 __device__ __forceinline__ void mfma32_high(f32x16& c, const u32x4& a, const u32x4& b) {
-#define SMOE_MFMA32(OP)                                                                                                   \
-    if constexpr (FIRST) asm volatile("s_nop 7\n\t" OP " %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));                     \
-    else if constexpr (LAST) asm volatile(OP " %0, %1, %2, %0\n\ts_nop 15\n\ts_nop 15" : "+a"(c) : "v"(a), "v"(b));       \
-    else asm volatile(OP " %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b))
-    if constexpr (F16) {
-        SMOE_MFMA32("v_mfma_f32_32x32x16_f16");
-    } else {
-        SMOE_MFMA32("v_mfma_f32_32x32x16_bf16");
-    }
-#undef SMOE_MFMA32
+    if constexpr (F16) asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+template <int STATES>  // 8 for operands just written, 20 for the results of 16 passes
+__device__ __forceinline__ void high_wait(f32x16 (&c)[8], u32x4 (&w)[2]) {
+    if constexpr (STATES > 8) asm volatile("s_nop 11" : "+a"(c[7]));
+    asm volatile("s_nop 7"
+                 : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]), "+v"(w[0]), "+v"(w[1]));
 }
 // Two f32 to the type's pair, round to nearest even.
 template <bool F16>
@@ -467,15 +465,17 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
         u32x4 vf[AHEAD + 1];
         each_of<AHEAD>([&](auto i) { vf[decltype(i)::value] = value_part(decltype(i)::value); });
         if constexpr (SCALED && !HIGH) scale_sums(0);
+        if constexpr (HIGH) high_wait<8>(acc, wt);
         each_of<N>([&](auto idx) {
             constexpr int I = decltype(idx)::value;
             if constexpr (I + AHEAD < N) vf[(I + AHEAD) % (AHEAD + 1)] = value_part(I + AHEAD);
-            if constexpr (HIGH) mfma32_high<F16, I == 0, I + 1 == N>(acc[I % ND], vf[I % (AHEAD + 1)], wt[I / ND]);
+            if constexpr (HIGH) mfma32_high<F16>(acc[I % ND], vf[I % (AHEAD + 1)], wt[I / ND]);
             else acc[I % ND] = mfma32<F16>(vf[I % (AHEAD + 1)], wt[I / ND], acc[I % ND]);
             if constexpr (SCALED && !HIGH && I + 1 < ND) scale_sums(I + 1);
             slice(idx);
             __builtin_amdgcn_sched_barrier(0);
         });
+        if constexpr (HIGH) high_wait<20>(acc, wt);
     };
     float m = 0.0f;
     // a step, whose scores are `t`, and the scores of the next; RARE: the next is not all seen, or the sums are to be scaled

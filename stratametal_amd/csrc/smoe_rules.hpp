@@ -317,7 +317,7 @@ inline Linear4Plan linear4_plan(int64_t T, int64_t K, int64_t N, bool pair) {
     return best;
 }
 inline bool linear4_fits(int64_t T, int64_t K, int64_t N, bool pair, int) {
-    return linear4_groups(linear4_plan(T, K, N, pair), T, N, pair) < kGridGroups;
+    return linear4_groups(linear4_plan(T, K, N, pair), T, N, pair) < kGridGroups / 2;  // (work-groups of 512 threads)
 }
 
 // n / d for n < 2^31 as (mulhi(n, mul) + n) >> shift: shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.

@@ -57,6 +57,22 @@ def test_gated_pair(T, K, N, group, t, y):
     check(x, None, layer, group, "silu", L.run(x, y_dtype=TYPES[y]), y)
 
 
+# every tile, whole and in slices of K, groups that hold whole steps and others (test_attention_rules.py)
+TILES = [(100, 1056, 300, 512, False), (100, 1056, 300, 512, True), (70, 2080, 1100, 32, False), (70, 2080, 1100, 32, True),
+         (33, 2080, 2050, 64, False), (33, 2080, 1030, 128, True), (40, 2048, 2050, 32, False), (40, 2080, 1030, 96, True),
+         (1025, 512, 1029, 128, False), (2000, 544, 515, 160, False), (300, 4096, 2049, 128, True), (300, 4128, 2049, 32, True),
+         (4100, 512, 1030, 128, False), (4100, 544, 1030, 32, False), (1025, 512, 1029, 128, True), (2000, 544, 515, 160, True),
+         (300, 4096, 2049, 128, False), (300, 4128, 2049, 32, False), (260, 8192, 2100, 64, True), (260, 4096, 4100, 32, True)]
+
+
+@pytest.mark.parametrize("T,K,N,group,pair", TILES)
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_tiles(T, K, N, group, pair, t):
+    say(f"case: linear4 tile T={T} K={K} N={N} group={group} pair={pair} {t}")
+    x, _, L, layer = make(T + N, T, K, N, group, t, zeros=t == "bf16", pair=pair, act="silu" if pair else "none", bias=True)
+    check(x, None, layer, group, "silu" if pair else "none", L.run(x, y_dtype=torch.float32), "f32")
+
+
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("s_type", list(TYPES))
 @pytest.mark.parametrize("T", [3, 90])
