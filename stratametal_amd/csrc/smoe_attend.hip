@@ -211,7 +211,8 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan&
         most = max(most, keys);
         total += (float)tiles * (float)keys;
     }
-    if (!found) return false;
+    // (starts out of order can count more tiles than 32 bits hold)
+    if (!found || w.row0 < 0 || w.rows <= 0) return false;
     // the keys that some row of the tile sees
     const int first = w.s.len - w.s.n + w.row0 / g, last = w.s.len - w.s.n + (w.row0 + w.rows - 1) / g;
     w.k0 = a.window ? max(0, first - a.window + 1) : 0;

@@ -99,6 +99,19 @@ def test_long(n, L, D, g):
     b.check(*b.run())
 
 
+@pytest.mark.parametrize("lens", [[700] * 9, [4000, 1, 130, 64, 2000, 65, 3], [1] * 70, [40, 9000], [2048] * 70])
+@pytest.mark.parametrize("n,window", [(1, 0), (5, 0), (1, 300)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_pieces_follow_the_lengths(lens, n, window, D):
+    """Tables that hold far more keys than the sequences have, which settle the pieces of the split: the same answers as from
+    tables of the longest's width."""
+    say(f"case: attend pieces {len(lens)} sequences of up to {max(lens)} n={n} window={window} D={D}")
+    b = Batch(len(lens) + n, [min(n, l) for l in lens], lens, 4, 2, D, 64)
+    b.check(*b.run(window=window), window=window)
+    b.table = np.concatenate([b.table, np.full((len(lens), 2048), -1, np.int32)], 1)
+    b.check(*b.run(window=window), window=window)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_window_far_from_the_start(n):
     say(f"case: attend window n={n}")
