@@ -102,7 +102,7 @@ __device__ __forceinline__ f32x4 four_scales(const uint32_t* p, int type) {
 // cover the 64 banks once), the tokens' values, and the scales and zeros of its up to four groups.  Lanes past the last token
 // hold its values, and their results are dropped; the waves' sums meet in LDS, in wave order.
 template <bool PAIR, bool F16, int TOKENS>
-__global__ __launch_bounds__(512) void k_linear4_few(const Linear4Args a) {
+__global__ __launch_bounds__(512, 4) void k_linear4_few(const Linear4Args a) {
     constexpr int SETS = PAIR ? 2 : 1, WAVES = 8, RING = kLinear4Ring<PAIR, TOKENS>;
     constexpr int XS = TOKENS > 4 ? TOKENS / 4 : 1, LOADS = 3 * SETS + XS;  // a stage's loads of the tokens, and all
     constexpr int STAGE = kLinear4Stage<PAIR, TOKENS>, X0 = SETS * 1536;
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(512) void k_linear4_few(const Linear4Args a) {
     for (int r = 0; r < RING; ++r) load(wave + r * WAVES, base + r * STAGE);
     const int tok = min(lane & 15, TOKENS - 1);
     const uint32_t w_at = (lane & 15) * 64 + 4 * q, w_sw = (lane >> 2) & 3;
-    const bool whole = a.group % 128 == 0;
+    const bool whole = a.group % 128 == 0, halves = a.group % 64 == 0;
     uint32_t at = 0;
     for (int u = wave; u < stages; u += WAVES) {
         vmcnt<(RING - 1) * LOADS>();
@@ -169,13 +169,31 @@ __global__ __launch_bounds__(512) void k_linear4_few(const Linear4Args a) {
                 sum[i] = mfma16<F16>(__builtin_bit_cast(uint4, expand8<F16>(c)), xv, sum[i]);
             }
         };
-        if (whole && u * 128 + 128 <= a.n_in) {  // one group, straight on
+        int g = 0, left = a.group - u * 128 % a.group;  // of the stage's groups, and what is left of it
+        const bool full = u * 128 + 128 <= a.n_in;
+        if (whole && full) {  // one group, straight on
             f32x4 sum[SETS] = {}, sx = none;
 #pragma unroll
             for (int s = 0; s < 4; ++s) product(s, sum, sx);
             scaled(0, sum, sx);
+        } else if (halves && full) {  // each half in one group
+            const int second = left == 64;
+#pragma unroll(PAIR ? 1 : 2)
+            for (int i = 0; i < 2; ++i) {
+                f32x4 sum[SETS] = {}, sx = none;
+                product(2 * i, sum, sx), product(2 * i + 1, sum, sx);
+                scaled(i ? second : 0, sum, sx);
+            }
+        } else if (!PAIR && full) {  // (of two matrices the registers would not hold it)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                f32x4 sum[SETS] = {}, sx = none;
+                product(s, sum, sx);
+                scaled(g, sum, sx);
+                left -= 32;
+                if (left == 0) left = a.group, ++g;
+            }
         } else {
-            int g = 0, left = a.group - u * 128 % a.group;  // of the stage's groups, and what is left of it
 #pragma unroll 1
             for (int s = 0; s < 4 && u * 128 + s * 32 < a.n_in; ++s) {
                 f32x4 sum[SETS] = {}, sx = none;
