@@ -180,7 +180,7 @@ struct Work {
 // the lengths that are there: with sequences of about one length whose tiles are fewer than the PLACES of work-groups on the
 // card, as many pieces as fill these once; else pieces of a quarter of a place's share, at least the longest over the plan's splits.
 // (8 sequences of 4000 keys, 8 key heads: 8 pieces 37 us, 16 47; 64 sequences of up to 8192 keys: 1 piece 223 us, 7 215.)
-template <int M, int PLACES>
+template <int M, int PLACES, int KEYS>
 __device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan& p, int lane, Work& w) {
     const int i = blockIdx.x, g = a.group, j = i / a.n_kv, tile = p.tiles - 1 - j % p.tiles;
     w.kvh = i % a.n_kv;
@@ -224,7 +224,7 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan&
         const bool one = groups <= PLACES && (float)most * groups <= 1.25f * all;
         const float share = one ? (float)(most - 1) / __builtin_floorf(PLACES / groups) : all * (0.25f / PLACES);
         int chunk = max((int)__builtin_fminf(share, (float)most), (most - 1) / p.splits);
-        chunk = (chunk / kAttendKeys + 1) * kAttendKeys;
+        chunk = (chunk / KEYS + 1) * KEYS;
         chunk = __builtin_amdgcn_readfirstlane(chunk);
         const int64_t from = (int64_t)w.k0 + (int64_t)w.split * chunk;
         w.k1 = (int)min((int64_t)w.k1, from + chunk);
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     __shared__ int bad_page;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Work w;
-    if (!find_work<M, (DIM > 128 ? 256 : 512)>(a, p, lane, w)) return;
+    if (!find_work<M, (DIM > 128 ? 256 : 512), KEYS>(a, p, lane, w)) return;
     if (no_keys(a, p, w, 256)) return;
     if (threadIdx.x == 0) bad_page = 0;
     const int32_t* table = a.pages + w.s.b * a.pages_ld;
@@ -603,6 +603,187 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
         redo_row(a, p, w, wave * 32 + __builtin_ctzll(again), reinterpret_cast<float*>(lds) + wave * kMaxDim, lane);
 }
 
+// Sequences of few query rows: tiles of 16 rows, four waves each on every fourth block of 32 keys, by itself until the waves' sums
+// meet in LDS.  A block's keys and values travel to the wave's own LDS, the next block's as soon as this one's have been
+// read, page numbers two blocks ahead.  The transposed scores (v_mfma_f32_16x16x32: keys by queries) leave a lane with 8 keys of
+// one query, which are the second product's right operand as they are, with the keys in that order (read_columns).
+template <int DIM, bool F16>
+__global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const AttendArgs a, const AttendPlan p) {
+    constexpr int M = kAttendFewRows, NQ = DIM / 32, ND = DIM / 16, PLANE = 32 * DIM * 2;
+    constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = 32 / RPI;  // lanes to a row, rows of a load, loads of a block
+    static_assert(4 * ND * 1024 <= 8 * PLANE, "the waves' sums");
+    __shared__ __align__(1024) uint8_t lds[8 * PLANE];
+    __shared__ int32_t ids[4][2][64];
+    __shared__ float2 stats_s[4][M];
+    __shared__ uint32_t again_s;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Work w;
+    if (!find_work<M, (DIM > 128 ? 256 : DIM > 64 ? 512 : 1024), kAttendFewKeys>(a, p, lane, w)) return;
+    if (no_keys(a, p, w, 256)) return;
+    if (threadIdx.x == 0) again_s = 0;
+    const int32_t* table = a.pages + (int64_t)w.s.b * a.pages_ld;
+    const int blocks = (w.k1 - w.k0 + 31) / 32;
+    uint8_t *const keys = lds + wave * 2 * PLANE, *const values = keys + PLANE;
+    const uint32_t keys_at = __builtin_amdgcn_readfirstlane(lds_addr(keys)), values_at = keys_at + PLANE;
+    const uint32_t ids_at = __builtin_amdgcn_readfirstlane(lds_addr(ids[wave]));
+    const auto key_of = [&](int j) { return min(w.k0 + 32 * j + (lane & 31), w.k1 - 1); };  // (past the last: the last)
+    const auto load_ids = [&](int j, int slot) { to_lds4(ids_at + slot * 256, table + divide(key_of(j), p.page)); };
+    bool bad = false;
+    const auto find_row = [&](int j, int slot) {  // a lane's key of block j: its row in the cache
+        const int page = ids[wave][slot][lane], key = key_of(j), off = key - divide(key, p.page) * a.page_size;
+        const bool there = (uint32_t)page < (uint32_t)a.n_pages;
+        bad |= !there;
+        return ((there ? page : 0) * a.n_kv + w.kvh) * a.page_size + off;
+    };
+    const int r_lane = lane / LPR, piece_lane = lane % LPR, last_piece = a.head_dim / 8 - 1;
+    const auto load_plane = [&](const uint8_t* plane, uint32_t at, int row) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = i * RPI + r_lane, c = min(piece_lane ^ spread<DIM>(r), last_piece);
+            to_lds16(at + i * 1024, plane + ((int64_t)__shfl(row, r) * (a.head_dim * 2) + 16 * c));
+        }
+    };
+    // this lane's query, and its quarter of the keys (of the values)
+    const int h = lane >> 4, r_q = lane & 15, row_q = w.row0 + min(r_q, w.rows - 1);
+    const int t_q = row_q / a.group, head = w.kvh * a.group + row_q % a.group;
+    const int pos = w.s.len - w.s.n + t_q;
+    const int hi = a.causal ? min(pos + 1, w.k1) : w.k1, lo = a.window ? max(pos - a.window + 1, w.k0) : w.k0;
+    if (wave < blocks) load_ids(wave, 0), load_ids(wave + 4, 1);
+    u32x4 qf[NQ];
+    load_query<NQ, 4>(a, w.s.t0 + t_q, head, h, qf);
+    f32x4 acc[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float top = -__builtin_inff(), base = 0.0f, sum = 0.0f;
+    const float scale = a.scale == 0.0f ? 1.0f : __builtin_fabsf(a.scale);
+    // rows 4 h + (lane & 15) / 4 and 16 on of the values, the 8 bytes of the lane's quarter of 16 values
+    const int v_row = 4 * h + (r_q >> 2), v_piece = (lane & 3) >> 1;
+    int row = 0;
+    if (wave < blocks) {
+        vmcnt<0>();
+        row = find_row(wave, 0);
+        load_plane(a.k, keys_at, row), load_plane(a.v, values_at, row);
+    }
+    int slot = 1;
+    for (int j = wave; j < blocks; j += 4) {
+        const bool more = j + 4 < blocks;
+        vmcnt<LOADS>();  // the keys, and the next block's page numbers
+        f32x4 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            s[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const int r = 16 * b + r_q;
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
+                s[b] = mfma16<F16>(*reinterpret_cast<const u32x4*>(keys + r * DIM * 2 + ((4 * i + h) ^ spread<DIM>(r)) * 16), qf[i], s[b]);
+        }
+        if (more) {
+            row = find_row(j + 4, slot);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the keys and these numbers have been read)
+            slot ^= 1;
+            load_ids(j + 8, slot);
+            load_plane(a.k, keys_at, row);
+        }
+        float t[8], m = -__builtin_inff();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int key = w.k0 + 32 * j + 16 * (e / 4) + 4 * h + e % 4;
+            t[e] = key < hi && key >= lo ? s[e / 4][e % 4] : -__builtin_inff();
+            m = __builtin_fmaxf(m, t[e]);
+        }
+        m = max_halves(max_quarters(m));
+        const float next = __builtin_fmaxf(top, m * scale);
+        if (__ballot(next != top)) {
+            const float keep = next == top ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+            top = next, base = top == -__builtin_inff() ? 0.0f : top;
+            sum *= keep;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) acc[i] *= keep;
+        }
+        u32x4 wt;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            t[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[e], scale, -base));
+            sum += t[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wt[e] = pack2<F16>(t[2 * e], t[2 * e + 1]);
+        if (more) vmcnt<LOADS + 1>();  // the values
+        else vmcnt<0>();
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+            u32x4 f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int r = 16 * x + v_row;
+                const u32x2 half = read_columns(values + r * DIM * 2 + ((2 * i + v_piece) ^ spread<DIM>(r)) * 16 + 8 * (lane & 1));
+                f[2 * x] = half[0], f[2 * x + 1] = half[1];
+            }
+            acc[i] = mfma16<F16>(f, wt, acc[i]);
+        }
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load_plane(a.v, values_at, row);
+        }
+    }
+    vmcnt<0>();
+    sum += __shfl_xor(sum, 16);
+    sum = add_halves(sum);
+    __syncthreads();  // (again_s is set, and every wave has read its blocks)
+    if (bad) atomicOr(&again_s, 0xFFFFu);
+    if (h == 0) stats_s[wave][r_q] = make_float2(top, sum);
+    f32x4* const sums = reinterpret_cast<f32x4*>(lds);  // [wave][16 values][lane]
+#pragma unroll
+    for (int i = 0; i < ND; ++i) sums[(wave * ND + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    float part_of[4];
+    top = -__builtin_inff();
+#pragma unroll
+    for (int v = 0; v < 4; ++v) top = __builtin_fmaxf(top, stats_s[v][r_q].x);
+    base = top == -__builtin_inff() ? 0.0f : top;
+    sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        part_of[v] = __builtin_amdgcn_exp2f(stats_s[v][r_q].x - base);
+        sum = __builtin_fmaf(part_of[v], stats_s[v][r_q].y, sum);
+    }
+    const float inv = p.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    // what is not finite may come of a value that the query does not see (0 times it): such rows are done anew
+    bool lost = !(__builtin_fabsf(sum) < __builtin_inff());
+    const int tok = w.s.t0 + t_q;
+    const int64_t out_row = (int64_t)tok * a.n_heads + head;
+    const bool mine = r_q < w.rows;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)tok * a.out_ld + (int64_t)head * a.head_dim;
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_ld * 2)) & 7) == 0;
+    float* part = p.splits > 1 ? part_row(a, p, out_row, w.split) : nullptr;
+#pragma unroll
+    for (int i = 0; i < ND / 4; ++i) {
+        const int n = 4 * i + wave, d = 16 * n + 4 * h;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o += part_of[v] * sums[(v * ND + n) * 64 + lane];
+        float y[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            y[x] = o[x] * inv;
+            lost |= d < a.head_dim && !(__builtin_fabsf(y[x]) < __builtin_inff());
+        }
+        if (!mine || d >= a.head_dim) continue;
+        if (part) *reinterpret_cast<f32x4*>(part + d) = f32x4{y[0], y[1], y[2], y[3]};
+        else if (vec) store4(out + d, y, F16 ? kF16 : kBf16);
+        else
+#pragma unroll
+            for (int x = 0; x < 4; ++x) out[d + x] = f32_to_half_bits(y[x], F16 ? kF16 : kBf16);
+    }
+    if (wave == 0 && mine && h == 0) put_stats(a, p, out_row, w.split, top, sum);
+    if (mine && lost) atomicOr(&again_s, 1u << r_q);
+    __syncthreads();
+    for (uint32_t again = again_s & ((1u << w.rows) - 1); again; again &= again - 1) {
+        const int r = __builtin_ctz(again);
+        if (r % 4 == wave) redo_row(a, p, w, r, reinterpret_cast<float*>(lds) + wave * kMaxDim, lane);
+    }
+}
+
 // The splits' sums of a query row: out = sum_s 2^(top_s - top) out_s / sum_s 2^(top_s - top) sum_s.  head_dim / 4 threads to a
 // split's values; a row has as many such groups as it has splits, at most a whole work-group's, and they meet in LDS (one wave
 // to a row and its splits one by one: 170 us of 202 for 32 rows of 256 splits).
@@ -684,7 +865,11 @@ namespace {
 template <bool F16>
 hipError_t launch_attend_as(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)p.tiles * a.n_kv * p.splits));
-    if (a.head_dim <= 64) hipLaunchKernelGGL((k_attend_tile<64, F16>), grid, dim3(256), 0, s, a, p);
+    if (p.few) {
+        if (a.head_dim <= 64) hipLaunchKernelGGL((k_attend_few<64, F16>), grid, dim3(256), 0, s, a, p);
+        else if (a.head_dim <= 128) hipLaunchKernelGGL((k_attend_few<128, F16>), grid, dim3(256), 0, s, a, p);
+        else hipLaunchKernelGGL((k_attend_few<256, F16>), grid, dim3(256), 0, s, a, p);
+    } else if (a.head_dim <= 64) hipLaunchKernelGGL((k_attend_tile<64, F16>), grid, dim3(256), 0, s, a, p);
     else if (a.head_dim <= 128) hipLaunchKernelGGL((k_attend_tile<128, F16>), grid, dim3(256), 0, s, a, p);
     else hipLaunchKernelGGL((k_attend_tile<256, F16>), grid, dim3(256), 0, s, a, p);
     return hipGetLastError();

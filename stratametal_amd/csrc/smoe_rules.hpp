@@ -331,9 +331,9 @@ constexpr Divisor divisor(uint32_t d) {
 }
 
 // Attention over a paged cache: tiles of query rows, and the keys in how many splits of how many.
-constexpr int kAttendRows = 128;
+constexpr int kAttendRows = 128, kAttendFewRows = 16, kAttendKeys = 64, kAttendFewKeys = 128;
 struct AttendPlan {
-    int tiles, splits, chunk;
+    int tiles, splits, chunk, few;
     int64_t part_floats;  // of the splits' tops and sums, in front of their partial outputs
     Divisor page;
 };
@@ -348,10 +348,10 @@ constexpr int64_t attend_tiles(int64_t T, int64_t B, int64_t group, int64_t rows
 // its bytes.  us, by splits: 1 token over 131072 keys, 4 key heads of 128: 64 75, 128 70, 256 73; 56 tokens of 64 sequences of
 // up to 8192 keys, 8 key heads: 1 223, 5 219, 7 215, 16 223; 796 tokens of 6, a window of 500 keys, heads of 64: 1 21, 2 23, 3 27;
 // 1024 tokens over 33792 keys, 32 heads, 8 key heads: 1 770, 2 627, 4 646; 8192 tokens, the same heads: 1 613, 2 755.
-constexpr int kAttendKeys = 64;
-inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t rows, int64_t B, int D) {
-    const int64_t tiles = ((keys + splits - 1) / splits + kAttendKeys - 1) / kAttendKeys, places = D > 128 ? 256 : 512;
-    const double tile = D > 64 ? 2.3 : 1.3, most = 4.0 + tile * (double)tiles;
+inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t rows, int64_t B, int D, bool few) {
+    const int64_t unit = few ? kAttendFewKeys : kAttendKeys, tiles = ((keys + splits - 1) / splits + unit - 1) / unit;
+    const int64_t places = D > 128 ? 256 : D > 64 || !few ? 512 : 1024;
+    const double tile = few ? (D > 128 ? 2.5 : D > 64 ? 1.5 : 1.0) : D > 64 ? 2.3 : 1.3, most = 4.0 + tile * (double)tiles;
     const double join = splits > 1 ? 4.0 + (double)(rows * splits * D) * 8 / 4e6 : 0.0;
     if (B == 1) return (double)((groups * splits + places - 1) / places) * most + join;
     const double all = (double)(groups * splits) * (4.0 + tile * (double)tiles / 2) / (double)places + most / 2;
@@ -360,14 +360,16 @@ inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t 
 inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_t max_len, int64_t window) {
     AttendPlan p{};
     const int64_t group = H / kv, rows = T * H;
-    p.tiles = (int)attend_tiles(T, B, group, kAttendRows);
+    p.few = T * group <= kAttendFewRows * B;
+    const int64_t m = p.few ? kAttendFewRows : kAttendRows, tile = p.few ? kAttendFewKeys : kAttendKeys;
+    p.tiles = (int)attend_tiles(T, B, group, m);
     // the most keys that a tile's rows see
-    const int64_t seen = window ? window + (kAttendRows + group - 1) / group : max_len, keys = seen < max_len ? seen : max_len;
-    const int64_t groups = (int64_t)p.tiles * kv, tile = kAttendKeys;
+    const int64_t seen = window ? window + (m + group - 1) / group : max_len, keys = seen < max_len ? seen : max_len;
+    const int64_t groups = (int64_t)p.tiles * kv;
     int64_t best = 1;
-    double least = attend_time(groups, 1, keys, rows, B, D);
+    double least = attend_time(groups, 1, keys, rows, B, D, p.few);
     for (int64_t s = 2; groups * s <= 4096 && (s - 1) * tile < keys; ++s) {
-        const double us = attend_time(groups, s, keys, rows, B, D);
+        const double us = attend_time(groups, s, keys, rows, B, D, p.few);
         if (us < least) least = us, best = s;
     }
     p.chunk = (int)(((keys + best - 1) / best + tile - 1) / tile * tile);
