@@ -179,7 +179,7 @@ struct Work {
 // The plan's splits are made for the longest sequence that the call allows; how many keys a piece has is settled here, from
 // the lengths that are there: with sequences of about one length whose tiles are fewer than the PLACES of work-groups on the
 // card, as many pieces as fill these once; else pieces of a quarter of a place's share, at least the longest over the plan's splits.
-// (8 sequences of 4000 keys, 8 key heads: 8 pieces 37 us, 16 47; 64 sequences of up to 8192 keys: 1 piece 223 us, 7 215.)
+// (8 sequences of 4000 keys, 8 key heads: 8 pieces 32 us, 32 35; 64 sequences of up to 8192 keys: 1 piece 214 us, 4 188, 32 199.)
 template <int M, int PLACES, int KEYS>
 __device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan& p, int lane, Work& w) {
     const int i = blockIdx.x, g = a.group, j = i / a.n_kv, tile = p.tiles - 1 - j % p.tiles;

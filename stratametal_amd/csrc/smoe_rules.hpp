@@ -342,16 +342,19 @@ constexpr int64_t attend_tiles(int64_t T, int64_t B, int64_t group, int64_t rows
     const int64_t each = T * ((group + rows - 1) / rows), packed = (T * group + B * (rows - 1)) / rows;
     return each < packed ? each : packed;
 }
-// A CU holds two work-groups (one of heads wider than 128), each at 2.3 us a tile of keys (1.3 of heads up to 64) and 4 us
-// beside them.  One sequence's splits run in rounds of whole ones; those of several, whose lengths differ (by half the longest
-// on average), fill the CUs one after the other, but for the last.  Beyond one split there are the launch that joins them and
-// its bytes.  us, by splits: 1 token over 131072 keys, 4 key heads of 128: 64 75, 128 70, 256 73; 56 tokens of 64 sequences of
-// up to 8192 keys, 8 key heads: 1 223, 5 219, 7 215, 16 223; 796 tokens of 6, a window of 500 keys, heads of 64: 1 21, 2 23, 3 27;
-// 1024 tokens over 33792 keys, 32 heads, 8 key heads: 1 770, 2 627, 4 646; 8192 tokens, the same heads: 1 613, 2 755.
+// Sequences of 16 query rows or fewer on average go to k_attend_few, tiles of 16 rows and keys by 128; others to k_attend_tile, 128
+// rows and keys by 64 (us, tiles of 128 rows and of 16: 8 sequences of 4000 keys, one token each, 8 key heads of 128: 37 and 32, 16 of up
+// to 8000 76 and 50, 64 of up to 8192 219 and 188, one of 1000 keys, 2 key heads of 256: 21 and 16).
+// A CU holds two work-groups (one of heads wider than 128; four of few rows and heads up to 64), each 4 us and its tiles of
+// keys.  One sequence's splits run in rounds of whole ones; those of several, whose lengths differ (by half the longest on
+// average), fill the CUs one after the other, but for the last.  Beyond one split there are the launch that joins them and its
+// bytes.  us, by splits: 1 token over 131071 keys, 4 key heads of 128: 32 53, 64 51, 128 53, 256 55; 64 sequences of up to 8192, 8
+// key heads: 1 214, 4 188, 12 191, 32 199; 8 of 4000: 1 47, 8 32, 32 35; 796 tokens of 6, a window of 500 keys, heads of 64: 1 21,
+// 2 23, 3 27; 1024 tokens over 33792 keys, 32 heads, 8 key heads: 1 770, 2 627, 4 646; 8192 tokens, the same heads: 1 613, 2 755.
 inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t rows, int64_t B, int D, bool few) {
     const int64_t unit = few ? kAttendFewKeys : kAttendKeys, tiles = ((keys + splits - 1) / splits + unit - 1) / unit;
     const int64_t places = D > 128 ? 256 : D > 64 || !few ? 512 : 1024;
-    const double tile = few ? (D > 128 ? 2.5 : D > 64 ? 1.5 : 1.0) : D > 64 ? 2.3 : 1.3, most = 4.0 + tile * (double)tiles;
+    const double tile = few ? (D > 128 ? 5.0 : D > 64 ? 4.0 : 2.0) : D > 64 ? 2.3 : 1.3, most = 4.0 + tile * (double)tiles;
     const double join = splits > 1 ? 4.0 + (double)(rows * splits * D) * 8 / 4e6 : 0.0;
     if (B == 1) return (double)((groups * splits + places - 1) / places) * most + join;
     const double all = (double)(groups * splits) * (4.0 + tile * (double)tiles / 2) / (double)places + most / 2;

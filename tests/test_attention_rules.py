@@ -16,12 +16,13 @@ HIPCC = "/opt/rocm/bin/hipcc"
 
 def test_attend_plan(ask):  # noqa: F811
     """tokens, sequences, heads, key heads, head size, longest, window -> splits within a tenth of the fastest measured."""
-    cases = [(1, 1, 32, 4, 128, 131072, 0, range(96, 257)), (56, 64, 32, 8, 128, 8193, 0, range(4, 17)), (1, 1, 16, 2, 256, 1001, 0, range(12, 33)),
+    cases = [(1, 1, 32, 4, 128, 131072, 0, range(32, 257)), (64, 64, 32, 8, 128, 8193, 0, range(4, 17)), (1, 1, 16, 2, 256, 1001, 0, range(6, 33)),
              (796, 6, 14, 2, 64, 2333, 500, (1,)), (1024, 1, 32, 8, 128, 33792, 0, range(2, 5)), (8192, 1, 32, 8, 128, 8192, 0, (1,)),
              (1, 1, 32, 8, 128, 64, 0, (1,)), (1, 1, 32, 8, 128, 0, 0, (1,)), (8, 8, 32, 8, 128, 4001, 0, range(8, 33))]
-    got = ask([f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).splits" for T, B, H, kv, D, L, w, _ in cases])
-    for g, c in zip(got, cases):
-        assert g in c[-1], (g, c)
+    got = ask([e for T, B, H, kv, D, L, w, _ in cases for e in (f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).splits",
+                                                                f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).few")])
+    for g, few, c in zip(got[::2], got[1::2], cases):
+        assert g in c[-1] and bool(few) == (c[0] <= c[1]), (g, few, c)
 
 
 def test_attend_plan_bounds(ask):  # noqa: F811
@@ -36,7 +37,7 @@ def test_attend_plan_bounds(ask):  # noqa: F811
         assert tiles * kv * splits < 2 ** 24
         assert splits == 1 or floats >= 2 * T * H * splits and floats % 64 == 0
         keys = min(L, w + 129) if w else L
-        assert splits == 1 or (splits - 1) * 64 < keys
+        assert splits == 1 or (splits - 1) * (128 if T * (H // kv) <= 16 * B else 64) < keys
 
 
 def test_attend_tiles_hold_any_batch(ask):  # noqa: F811
@@ -45,9 +46,10 @@ def test_attend_tiles_hold_any_batch(ask):  # noqa: F811
     for _ in range(300):
         group, B = rng.choice([1, 2, 3, 4, 5, 7, 8, 16, 40, 128, 129, 200, 300]), rng.randint(1, 12)
         batches.append(([rng.choice([0, 1, 1, 2, 5, 30, 128, 129, 700]) for _ in range(B)], group))
-    got = ask([f"attend_tiles({max(sum(n), 1)}, {len(n)}, {g}, 128)" for n, g in batches])
-    for (n, g), tiles in zip(batches, got):
-        assert sum((x * g + 127) // 128 for x in n) <= tiles, (n, g)
+    got = ask([f"attend_tiles({max(sum(n), 1)}, {len(n)}, {g}, {rows})" for n, g in batches for rows in (16, 128)])
+    for i, (n, g) in enumerate(batches):
+        for rows, tiles in zip((16, 128), got[2 * i:2 * i + 2]):
+            assert sum((x * g + rows - 1) // rows for x in n) <= tiles, (n, g)
 
 
 def test_divisor(ask):  # noqa: F811
