@@ -351,7 +351,8 @@ typedef struct {
  * slots[n_tokens] (page * page_size + off; one outside the cache, as -1: that token is not stored), k turned to positions, and
  * q [n_tokens][n_heads][head_dim], turned, to q_out of the cache's type.  q, k and v are of x_type (f32, fp16 or bf16), tokens
  * q_ld, k_ld and v_ld values apart (columns of one matrix, say).  r NULL: nothing turns (then q is NULL too, and positions are
- * not read); q NULL: the cache alone.  A call's slots are distinct (of two tokens' values for one slot it keeps either's).
+ * not read); q NULL: the cache alone.  A call's slots are distinct (where two tokens share one, each of its values is one of
+ * theirs).
  * q_out may be q's own rows; no other output shares a byte with an input. */
 smoe_status smoe_kv_append(const smoe_kv* kv, const smoe_rope* r, const int32_t* positions, const int64_t* slots,
                            int32_t n_tokens, int32_t x_type, const void* q, int64_t q_ld, int32_t n_heads, void* q_out,
@@ -367,8 +368,8 @@ smoe_status smoe_kv_append(const smoe_kv* kv, const smoe_rope* r, const int32_t*
  * the longest that the launch is made for).  Scores and sums are f32; the weights are rounded to the cache's type for the
  * second product.  q and out [n_tokens][n_heads][head_dim] of the cache's type, tokens q_ld and out_ld values apart (q 16-byte
  * aligned, q_ld a multiple of 8); lse [n_tokens][n_heads] f32 or NULL.  Rows before the first sequence and behind the last one
- * are left as they are.  `workspace` (256-byte aligned, apart from every operand): concurrent calls need distinct ones.  The
- * same bits in every run. */
+ * are left as they are.  `workspace` (256-byte aligned, apart from every operand, of the bytes for the call's own sizes: they do
+ * not only grow with them): concurrent calls need distinct ones.  The same bits in every run. */
 size_t smoe_attend_workspace_bytes(const smoe_kv* kv, int32_t n_heads, int32_t n_tokens, int32_t n_seqs, int64_t max_len,
                                    int32_t window);
 smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t n_tokens, int32_t n_heads,
