@@ -333,7 +333,7 @@ constexpr Divisor divisor(uint32_t d) {
 // Attention over a paged cache: tiles of query rows, and the keys in how many splits of how many.
 constexpr int kAttendRows = 128, kAttendFewRows = 16, kAttendKeys = 64, kAttendFewKeys = 128;
 struct AttendPlan {
-    int tiles, splits, chunk, few;
+    int tiles, splits, few;
     int64_t part_floats;  // of the splits' tops and sums, in front of their partial outputs
     Divisor page;
 };
@@ -342,43 +342,48 @@ constexpr int64_t attend_tiles(int64_t T, int64_t B, int64_t group, int64_t rows
     const int64_t each = T * ((group + rows - 1) / rows), packed = (T * group + B * (rows - 1)) / rows;
     return each < packed ? each : packed;
 }
-// Sequences of 16 query rows or fewer on average go to k_attend_few, tiles of 16 rows and keys by 128; others to k_attend_tile, 128
-// rows and keys by 64 (us, tiles of 128 rows and of 16: 8 sequences of 4000 keys, one token each, 8 key heads of 128: 37 and 32, 16 of up
-// to 8000 76 and 50, 64 of up to 8192 219 and 188, one of 1000 keys, 2 key heads of 256: 21 and 16).
-// A CU holds two work-groups (one of heads wider than 128; four of few rows and heads up to 64), each 4 us and its tiles of
-// keys.  One sequence's splits run in rounds of whole ones; those of several, whose lengths differ (by half the longest on
-// average), fill the CUs one after the other, but for the last.  Beyond one split there are the launch that joins them and its
-// bytes.  us, by splits: 1 token over 131071 keys, 4 key heads of 128: 32 53, 64 51, 128 53, 256 55; 64 sequences of up to 8192, 8
-// key heads: 1 214, 4 188, 12 191, 32 199; 8 of 4000: 1 47, 8 32, 32 35; 796 tokens of 6, a window of 500 keys, heads of 64: 1 21,
-// 2 23, 3 27; 1024 tokens over 33792 keys, 32 heads, 8 key heads: 1 770, 2 627, 4 646; 8192 tokens, the same heads: 1 613, 2 755.
+// k_attend_few takes tiles of 16 query rows and keys by 128, k_attend_tile 128 rows and keys by 64; a call goes to the one whose time is
+// less.  A CU holds two work-groups (one of heads wider than 128; four of few rows and heads up to 64), each its start and its
+// tiles of keys.  One sequence's splits run in rounds of whole ones; those of several, whose lengths differ (by half the longest
+// on average), fill the CUs one after the other, but for the last.  Beyond one split there are the launch that joins them and its
+// bytes.
+// us by tiles of 128 rows and of 16 (a graph's replay; 16 is the least that one takes), one token each of: 8 sequences of 4000 keys, 8 key
+// heads of 128, 37 and 32, 16 of up to 8000 76 and 50, 64 of up to 8192 219 and 188; 796 tokens of 6, a window of 500 keys, heads of 64
+// 21 and 16; 8 tokens each of 4 of up to 4000 26 and 21; 32 tokens over 20000 44 and 56; 300 each of 8 of up to 1300 57 and 61; a
+// prompt of 256 21 and 16, of 512 27 and 24, with heads of 256 40 and 28.
+// us by splits: 1 token over 131071 keys, 4 key heads of 128: 32 53, 64 51, 128 53, 256 55; 64 sequences of up to 8192, 8 key heads: 1
+// 214, 4 188, 12 191, 32 199; 8 of 4000: 1 47, 8 32, 32 35; 1024 tokens over 33792 keys, 32 heads, 8 key heads: 1 770, 2 627, 4 646;
+// 8192 tokens, the same heads: 1 613, 2 755.
 inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t rows, int64_t B, int D, bool few) {
     const int64_t unit = few ? kAttendFewKeys : kAttendKeys, tiles = ((keys + splits - 1) / splits + unit - 1) / unit;
     const int64_t places = D > 128 ? 256 : D > 64 || !few ? 512 : 1024;
-    const double tile = few ? (D > 128 ? 5.0 : D > 64 ? 4.0 : 2.0) : D > 64 ? 2.3 : 1.3, most = 4.0 + tile * (double)tiles;
+    const double tile = few ? (D > 128 ? 3.0 : D > 64 ? 2.0 : 1.2) : D > 128 ? 3.6 : D > 64 ? 2.3 : 1.3, start = few ? 4.0 : 7.0;
+    const double most = start + tile * (double)tiles;
     const double join = splits > 1 ? 4.0 + (double)(rows * splits * D) * 8 / 4e6 : 0.0;
     if (B == 1) return (double)((groups * splits + places - 1) / places) * most + join;
-    const double all = (double)(groups * splits) * (4.0 + tile * (double)tiles / 2) / (double)places + most / 2;
+    const double all = (double)(groups * splits) * (start + tile * (double)tiles / 2) / (double)places + most / 2;
     return (all > most ? all : most) + join;
 }
 inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_t max_len, int64_t window) {
-    AttendPlan p{};
     const int64_t group = H / kv, rows = T * H;
-    p.few = T * group <= kAttendFewRows * B;
-    const int64_t m = p.few ? kAttendFewRows : kAttendRows, tile = p.few ? kAttendFewKeys : kAttendKeys;
-    p.tiles = (int)attend_tiles(T, B, group, m);
-    // the most keys that a tile's rows see
-    const int64_t seen = window ? window + (m + group - 1) / group : max_len, keys = seen < max_len ? seen : max_len;
-    const int64_t groups = (int64_t)p.tiles * kv;
-    int64_t best = 1;
-    double least = attend_time(groups, 1, keys, rows, B, D, p.few);
-    for (int64_t s = 2; groups * s <= 4096 && (s - 1) * tile < keys; ++s) {
-        const double us = attend_time(groups, s, keys, rows, B, D, p.few);
-        if (us < least) least = us, best = s;
+    AttendPlan best{};
+    double least = 0.0;
+    for (int few = 1; few >= 0; --few) {
+        const int64_t m = few ? kAttendFewRows : kAttendRows, unit = few ? kAttendFewKeys : kAttendKeys;
+        const int64_t tiles = attend_tiles(T, B, group, m), groups = tiles * kv;
+        // the most keys that a tile's rows see
+        const int64_t seen = window ? window + (m + group - 1) / group : max_len, keys = seen < max_len ? seen : max_len;
+        for (int64_t s = 1; s == 1 || (groups * s <= 4096 && (s - 1) * unit < keys); s += 1 + s / 16) {
+            const double us = attend_time(groups, s, keys, rows, B, D, few);
+            if (best.tiles && us >= least) continue;
+            least = us;
+            best.few = few, best.tiles = (int)tiles;
+            const int64_t each = ((keys + s - 1) / s + unit - 1) / unit * unit;
+            best.splits = keys ? (int)((keys + each - 1) / each) : 1;
+        }
     }
-    p.chunk = (int)(((keys + best - 1) / best + tile - 1) / tile * tile);
-    p.splits = keys ? (int)((keys + p.chunk - 1) / p.chunk) : 1;
-    p.part_floats = (2 * rows * p.splits + 63) / 64 * 64;
-    return p;
+    best.part_floats = (2 * rows * best.splits + 63) / 64 * 64;
+    return best;
 }
 
 }  // namespace smoe

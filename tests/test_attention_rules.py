@@ -15,14 +15,32 @@ HIPCC = "/opt/rocm/bin/hipcc"
 
 
 def test_attend_plan(ask):  # noqa: F811
-    """tokens, sequences, heads, key heads, head size, longest, window -> splits within a tenth of the fastest measured."""
-    cases = [(1, 1, 32, 4, 128, 131072, 0, range(32, 257)), (64, 64, 32, 8, 128, 8193, 0, range(4, 17)), (1, 1, 16, 2, 256, 1001, 0, range(6, 33)),
-             (796, 6, 14, 2, 64, 2333, 500, (1,)), (1024, 1, 32, 8, 128, 33792, 0, range(2, 5)), (8192, 1, 32, 8, 128, 8192, 0, (1,)),
-             (1, 1, 32, 8, 128, 64, 0, (1,)), (1, 1, 32, 8, 128, 0, 0, (1,)), (8, 8, 32, 8, 128, 4001, 0, range(8, 33))]
-    got = ask([e for T, B, H, kv, D, L, w, _ in cases for e in (f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).splits",
-                                                                f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).few")])
-    for g, few, c in zip(got[::2], got[1::2], cases):
-        assert g in c[-1] and bool(few) == (c[0] <= c[1]), (g, few, c)
+    """tokens, sequences, heads, key heads, head size, longest, window -> tiles of few rows or not, and splits, within a tenth of the
+    fastest measured."""
+    cases = [(1, 1, 32, 4, 128, 131072, 0, 1, range(32, 257)), (64, 64, 32, 8, 128, 8193, 0, 1, range(4, 17)), (1, 1, 16, 2, 256, 1001, 0, 1, range(6, 33)),
+             (796, 6, 14, 2, 64, 2333, 500, 1, (1,)), (1024, 1, 32, 8, 128, 33792, 0, 0, range(2, 5)), (8192, 1, 32, 8, 128, 8192, 0, 0, (1,)),
+             (1, 1, 32, 8, 128, 64, 0, 1, (1,)), (1, 1, 32, 8, 128, 0, 0, 1, (1,)), (8, 8, 32, 8, 128, 4001, 0, 1, range(4, 17)),
+             (32, 4, 32, 8, 128, 4008, 0, 1, range(4, 17)), (32, 1, 32, 8, 128, 20032, 0, 0, range(20, 100)), (512, 1, 16, 2, 256, 512, 0, 1, (1,))]
+    got = ask([e for T, B, H, kv, D, L, w, *_ in cases for e in (f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).few",
+                                                                 f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).splits")])
+    for few, splits, c in zip(got[::2], got[1::2], cases):
+        assert few == c[-2] and splits in c[-1], (few, splits, c)
+
+
+def test_attend_cases_reach_both_tiles(ask):  # noqa: F811
+    from test_gpu_attend import HEADS, MANY_HEADS, MANY_LENS, MANY_NEW, MANY_SPLIT
+    plans = lambda T, B, H, kv, D, L, w: (f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).few", f"attend_plan({T}, {B}, {H}, {kv}, {D}, {L}, {w}).splits")  # noqa: E731
+    many = [(sum(MANY_NEW) + 4, len(MANY_NEW), H, kv, D, -(-max(MANY_LENS) // page + 1) * page, w) for H, kv, D in MANY_HEADS
+            for page, w in ((24, 0), (64, 37), (16, 0))]
+    got = ask([e for c in many for e in plans(*c)])
+    assert not any(got[::2]) and {c[4] for c in many} >= {64, 128, 256}
+    split = [(sum(new), len(new), H, kv, D, -(-max(lens) // 16 + 1) * 16, 0) for new, lens, H, kv, D in MANY_SPLIT]
+    got = ask([e for c in split for e in plans(*c)])
+    assert not any(got[::2]) and all(s > 1 for s in got[1::2]) and {c[4] for c in split} == {64, 128, 256}
+    ones = [(12, 10, H, kv, D, 720, 0) for H, kv, D in HEADS] + [(260, 9, H, kv, D, 224, 0) for H, kv, D in HEADS]
+    ones += [(1, 1, 4, 1, 64, 96, 0), (1, 1, 4, 1, 128, 96, 0), (1, 1, 5, 1, 256, 96, 0)]
+    got = ask([e for c in ones for e in plans(*c)])
+    assert all(got[::2]) and {(c[4], s > 1) for c, s in zip(ones, got[1::2])} >= {(D, s) for D in (64, 128, 256) for s in (False, True)}
 
 
 def test_attend_plan_bounds(ask):  # noqa: F811
@@ -37,7 +55,7 @@ def test_attend_plan_bounds(ask):  # noqa: F811
         assert tiles * kv * splits < 2 ** 24
         assert splits == 1 or floats >= 2 * T * H * splits and floats % 64 == 0
         keys = min(L, w + 129) if w else L
-        assert splits == 1 or (splits - 1) * (128 if T * (H // kv) <= 16 * B else 64) < keys
+        assert splits == 1 or (splits - 1) * 64 < keys
 
 
 def test_attend_tiles_hold_any_batch(ask):  # noqa: F811

@@ -49,15 +49,19 @@ class Batch:
         torch.cuda.synchronize()
         return o, lse
 
-    def check(self, o, lse, scale=None, causal=True, window=0, rows=None):
+    def check(self, o, lse, scale=None, causal=True, window=0, ends=False):
+        """`ends`: the first and the last key head's queries alone."""
         scale = self.D ** -0.5 if scale is None else scale
+        kv = [0, self.kv - 1] if ends else list(range(self.kv))
+        g = self.H // self.kv
+        heads = [i * g + j for i in kv for j in range(g)]
         for b in range(len(self.new)):
             if self.new[b] == 0:
                 continue
             s = slice(self.start[b], self.start[b + 1])
-            want, bound, wl, el = A.attend(host(self.q[s]), self.keys[b], self.values[b], scale, causal, window, self.t)
-            close(o[s], want, bound)
-            got = host(lse[s]).astype(np.float64)
+            want, bound, wl, el = A.attend(host(self.q[s][:, heads]), self.keys[b][:, kv], self.values[b][:, kv], scale, causal, window, self.t)
+            close(o[s][:, heads], want, bound)
+            got = host(lse[s][:, heads]).astype(np.float64)
             assert np.array_equal(np.isneginf(got), np.isneginf(wl))
             live = np.isfinite(wl)
             assert (np.abs(got[live] - wl[live]) <= el[live]).all()
@@ -90,7 +94,7 @@ def test_chunks(H, kv, D, page, window, causal, t):
     b.check(*b.run(window=window, causal=causal), window=window, causal=causal)
 
 
-@pytest.mark.parametrize("n,L", [(1, 5000), (1, 20011), (4, 9000), (100, 6000), (600, 600), (129, 4099)])
+@pytest.mark.parametrize("n,L", [(1, 70), (1, 5000), (1, 20011), (4, 9000), (100, 6000), (600, 600), (129, 4099)])
 @pytest.mark.parametrize("D,g", [(64, 4), (128, 8), (256, 5)])
 def test_long(n, L, D, g):
     """Lengths whose keys are split over work-groups."""
@@ -110,6 +114,60 @@ def test_pieces_follow_the_lengths(lens, n, window, D):
     b.check(*b.run(window=window), window=window)
     b.table = np.concatenate([b.table, np.full((len(lens), 2048), -1, np.int32)], 1)
     b.check(*b.run(window=window), window=window)
+
+
+# calls that tiles of 128 rows take (test_attention_rules.py): new tokens and lengths, heads, key heads, head size, window
+MANY_NEW, MANY_LENS = [700, 1, 0, 300, 517, 2, 130], [700, 400, 50, 900, 517, 3, 1000]
+MANY_HEADS = [(32, 4, 64), (32, 8, 128), (16, 2, 256), (40, 5, 80), (24, 4, 96), (64, 4, 8), (28, 4, 200)]
+MANY_SPLIT = [([128], [4128], 32, 8, 128), ([32], [20032], 32, 8, 128), ([33, 30, 1, 32], [4000, 100, 2000, 3333], 32, 8, 128), ([256], [8200], 32, 4, 64),
+              ([250], [4096], 16, 2, 256)]
+
+
+@pytest.mark.parametrize("H,kv,D", MANY_HEADS)
+@pytest.mark.parametrize("page,window,causal", [(24, 0, True), (64, 37, True), (16, 0, False)])
+def test_many_rows(H, kv, D, page, window, causal):
+    say(f"case: attend many rows H={H} kv={kv} D={D} page={page} window={window} {causal}")
+    b = Batch(H + D + page, MANY_NEW, MANY_LENS, H, kv, D, page, "fp16" if (H + page) % 3 == 0 else "bf16", before=1, behind=3)
+    b.check(*b.run(window=window, causal=causal), window=window, causal=causal, ends=True)
+
+
+@pytest.mark.parametrize("new,lens,H,kv,D", MANY_SPLIT)
+def test_many_rows_over_pieces_of_the_keys(new, lens, H, kv, D):
+    say(f"case: attend many rows, splits {new} {lens} D={D}")
+    b = Batch(D, new, lens, H, kv, D, 16)
+    b.check(*b.run(), ends=True)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_rows_hidden_values_and_bad_pages(D):
+    """As below for single tokens and short chunks: what a row does not see leaves it as it is, and a page outside the cache holds no
+    keys."""
+    say(f"case: attend many rows, hidden D={D}")
+    H, kv = (16, 2) if D == 256 else (32, 8) if D == 128 else (32, 4)
+    for value in (float("nan"), float("inf")):
+        b = Batch(D, MANY_NEW, MANY_LENS, H, kv, D, 16)
+        where = 650  # of the first sequence: its first 650 rows do not see it
+        page, place = b.table[0][where // 16], where % 16
+        b.cache.k[int(page), :, place] = value
+        b.cache.v[int(page), :, place] = value
+        o, lse = b.run()
+        assert not bool(torch.isfinite(o[where:700]).all(dim=2).any())
+        g, last = H // kv, kv - 1  # (the last key head's queries)
+        want, bound, _, _ = A.attend(host(b.q[:where, -g:]), b.keys[0][:where, last:], b.values[0][:where, last:], D ** -0.5, True, 0, "bf16")
+        close(o[:where, -g:], want, bound)
+        for s in range(1, len(b.new)):
+            rows = slice(b.start[s], b.start[s + 1])
+            if b.new[s]:
+                want, bound, _, _ = A.attend(host(b.q[rows, :g]), b.keys[s][:, :1], b.values[s][:, :1], D ** -0.5, True, 0, "bf16")
+                close(o[rows, :g], want, bound)
+    b = Batch(D + 1, MANY_NEW, MANY_LENS, H, kv, D, 16)
+    b.table[6, 3] = b.cache.n_pages
+    o, lse = b.run(causal=False)
+    keep = np.ones(1000, bool)
+    keep[48:64] = False
+    rows = slice(b.start[6], b.start[7])
+    want, bound, _, _ = A.attend(host(b.q[rows]), b.keys[6][keep], b.values[6][keep], D ** -0.5, False, 0, "bf16")
+    close(o[rows], want, bound)
 
 
 @pytest.mark.parametrize("n", [1, 40])
