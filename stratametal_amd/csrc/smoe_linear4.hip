@@ -227,7 +227,7 @@ __global__ __launch_bounds__(512, 4) void k_linear4_few(const Linear4Args a) {
 }
 
 // More tokens: 128 weight rows (PAIR: 64 of each matrix, 16 of each in turn) by 16 NT tokens, 32 rows to each of four waves; up to
-// 64 tokens a work-group has eight, four for each half of its slice of K, whose sums meet in LDS.  A step is 64 of K: the
+// 64 tokens a work-group has eight, four for each half of its slice of K, whose sums meet in LDS, half the tokens with each.  A step is 64 of K: the
 // wave's codes (half p of row r at place p ^ (r >> 3)), its scales and zeros of the two 32-value steps, and its share of the
 // tokens (as in k_linear_tile), through a ring of RING stages in LDS.  A wave expands the codes of its rows in registers, less
 // their zeros, for all of the tile's tokens; a group's sums are scaled into the outputs' where it ends (SMALL, groups that do
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256 * kLinear4Parts<NT>, 2 / kLinear4Parts<NT>) voi
     constexpr int XS = BN / 8 / WAVES;                                  // a wave's loads of the tokens, 8 rows each
     constexpr int LOADS = 3 + XS, X0 = WAVES * 1536, STAGE = X0 + BN * 128, SLOT = PARTS * STAGE;
     constexpr int NG = NT < 4 ? NT : 4;
-    static_assert(WAVES * (kStoreBytes<MT, NG> + (PARTS - 1) * MT * NT * 1024) <= RING * SLOT, "the waves' pieces of the epilogue, a part's sums");
+    static_assert(WAVES * (kStoreBytes<MT, NG> * PARTS + (PARTS - 1) * MT * NT * 1024) <= RING * SLOT, "the waves' pieces of the epilogue, a part's sums");
     __shared__ __align__(1024) uint8_t lds[RING * SLOT];
     const int lane = threadIdx.x & 63, q = lane >> 4;
     const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3);
@@ -377,22 +377,26 @@ __global__ __launch_bounds__(256 * kLinear4Parts<NT>, 2 / kLinear4Parts<NT>) voi
     }
     vmcnt<0>();
     __syncthreads();
-    if constexpr (PARTS == 2) {  // the second part's sums to the first
-        f32x4* const other = reinterpret_cast<f32x4*>(lds + WAVES * kStoreBytes<MT, NG>) + wave * (MT * NT * 64) + lane;
-        if (part == 1) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) other[(m * NT + n) * 64] = acc[m][n];
-        }
-        __syncthreads();
-        if (part == 1) return;
+    if constexpr (PARTS == 2) {  // each part has the other's sums of half the tokens, and writes those tokens
+        constexpr int HALF = NT / 2, STORE = kStoreBytes<MT, HALF>;
+        f32x4* const sums = reinterpret_cast<f32x4*>(lds + 2 * WAVES * STORE) + wave * (MT * NT * 64) + lane;  // [m][n]
+        f32x4 mine[MT][HALF];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[m][n] = acc[m][n] + other[(m * NT + n) * 64];
+            for (int n = 0; n < HALF; ++n) {
+                mine[m][n] = part ? acc[m][n + HALF] : acc[m][n];
+                sums[(m * NT + n + (part ? 0 : HALF)) * 64] = part ? acc[m][n] : acc[m][n + HALF];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < HALF; ++n) mine[m][n] = mine[m][n] + sums[(m * NT + n + (part ? HALF : 0)) * 64];
+        tile_store<MT, HALF, HALF, PAIR>(a, mine, lds + (part * WAVES + wave) * STORE, o0 + wave * (PAIR ? 16 : 32), t0 + part * 16 * HALF, t0 + n_t, lane);
+    } else {
+        tile_store<MT, NT, NG, PAIR>(a, acc, lds + wave * kStoreBytes<MT, NG>, o0 + wave * (PAIR ? 16 : 32), t0, t0 + n_t, lane);
     }
-    tile_store<MT, NT, NG, PAIR>(a, acc, lds + wave * kStoreBytes<MT, NG>, o0 + wave * (PAIR ? 16 : 32), t0, t0 + n_t, lane);
 }
 
 size_t linear4_part_bytes(int64_t T, int K, int N, bool pair, int) {
