@@ -227,14 +227,14 @@ __global__ __launch_bounds__(512, 4) void k_linear4_few(const Linear4Args a) {
 }
 
 // More tokens: 128 weight rows (PAIR: 64 of each matrix, 16 of each in turn) by 16 NT tokens, 32 rows to each of four waves; up to
-// 64 tokens a work-group has eight, four for each half of its slice of K, whose sums meet in LDS, half the tokens with each.  A step is 64 of K: the
-// wave's codes (half p of row r at place p ^ (r >> 3)), its scales and zeros of the two 32-value steps, and its share of the
+// 64 tokens a work-group has eight, four for each half of its slice of K, whose sums meet in LDS, half the tokens with each (301
+// tokens, 2560 x 5003: 31.5 us where one half wrote them all, 29.0).  A step is 64 of K: the wave's codes (half p of row r at place p ^ (r >> 3)), its scales and zeros of the two 32-value steps, and its share of the
 // tokens (as in k_linear_tile), through a ring of RING stages in LDS.  A wave expands the codes of its rows in registers, less
 // their zeros, for all of the tile's tokens; a group's sums are scaled into the outputs' where it ends (SMALL, groups that do
 // not hold whole steps: after every 32 values).  blockIdx.y: a slice of K, whose sums go to `part` for k_linear_join.
 // A step is bound by the instructions that expand and scale (180 to 290 beside 32 matrix instructions at 128 tokens) and by the
-// reads and the barrier before them: 2048 tokens, 4096 x 4096, groups of 128: 100 us, 686 TFLOP/s (groups of 32: 110); 79 without
-// the loads, 58 without expansion and scales as well.
+// reads and the barrier before them: 2048 tokens, 4096 x 4096, groups of 128: 100 us, 686 TFLOP/s (groups of 32: 110); of
+// 115 to 120 of a form with the conversions a step ahead, 90 without the loads, 61 without expansion and scales as well.
 template <int NT, bool PAIR, bool F16, bool SMALL>
 __global__ __launch_bounds__(256 * kLinear4Parts<NT>, 2 / kLinear4Parts<NT>) void k_linear4_tile(const Linear4Args a, int tiles_o, int tiles_t) {
     constexpr int MT = 2, WAVES = 4, BN = 16 * NT, OUTS = PAIR ? 64 : 128, PARTS = kLinear4Parts<NT>, RING = NT == 2 ? 7 : NT == 4 ? 5 : 3;
