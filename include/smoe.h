@@ -288,7 +288,8 @@ typedef struct {
     int32_t n_out;        /* 1 .. 2^24 */
     int32_t x_type;       /* SMOE_BF16 or SMOE_F16 */
     int32_t act;          /* SMOE_ACT_* */
-    int32_t group;        /* values of n_in to a scale, a multiple of 32 (the last group of a row may be shorter) */
+    int32_t group;        /* values of n_in to a scale, a multiple of 32 (the last group of a row may be shorter,
+                           * and one of n_in or more is the whole row's) */
     int32_t s_type;       /* the scales: SMOE_F32, SMOE_F16 or SMOE_BF16 */
     const void* w;        /* [n_out][n_in / 2] bytes, 16-byte aligned */
     const void* w2;       /* the same, or NULL */

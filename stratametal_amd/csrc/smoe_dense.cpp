@@ -219,7 +219,7 @@ smoe_status smoe_linear4_run(const smoe_linear4* L, const void* x, int64_t x_ld,
     a.n_in = L->n_in, a.n_out = L->n_out, a.n_tokens = n_tokens;
     a.w_type = L->x_type, a.y_type = y_type, a.act = L->act;
     a.scales = L->scales, a.scales2 = L->scales2, a.zeros = L->zeros, a.zeros2 = L->zeros2;
-    a.group = L->group, a.s_type = L->s_type;
+    a.group = smoe::linear4_group(L->group), a.s_type = L->s_type;
     return launched(smoe::launch_linear4(a, reinterpret_cast<hipStream_t>(hip_stream)), "linear4");
 }
 

@@ -320,6 +320,10 @@ inline bool linear4_fits(int64_t T, int64_t K, int64_t N, bool pair, int) {
     return linear4_groups(linear4_plan(T, K, N, pair), T, N, pair) < kGridGroups / 2;  // (work-groups of 512 threads)
 }
 
+// The values of n_in to a scale, as the kernels have them: a group as long as the longest row (a multiple of every step's width) or
+// longer is the row's one group at any length, and n_in + group stays far below 2^31.
+constexpr int linear4_group(int group) { return group < kLinearMaxIn ? group : kLinearMaxIn; }
+
 // n / d for n < 2^31 as (mulhi(n, mul) + n) >> shift: shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.
 struct Divisor {
     uint32_t mul, shift;
