@@ -204,6 +204,13 @@ def _need(t, name: str, dtype, shape=None, numel=None):
     return t
 
 
+def _int32(v, name: str):
+    """Refuse a number that the C call's 32 bits do not hold: ctypes would pass its low bits."""
+    if not -1 << 31 <= v < 1 << 31:
+        raise SmoeError(-1, f"{name} is {v}, which 32 bits do not hold")
+    return v
+
+
 def _stream(stream=None) -> int:
     import torch
     s = torch.cuda.current_stream() if stream is None else stream
@@ -813,6 +820,8 @@ class Linear4:
         import torch
         if n_in < 32 or n_in % 32 or group < 32 or group % 32:
             raise SmoeError(-1, "n_in and group must be multiples of 32")
+        for v, name in ((n_in, "n_in"), (n_out, "n_out"), (group, "group"), (act, "act")):
+            _int32(v, name)
         groups = (-(-n_in // group), n_out)
         given = [(w, "w", torch.uint8, (n_out, n_in // 2)), (scales, "scales", None, groups), (zeros, "zeros", torch.uint8, groups),
                  (bias, "bias", torch.float32, (n_out,)), (w2, "w2", torch.uint8, (n_out, n_in // 2)),
@@ -846,7 +855,8 @@ class Linear4:
         return c
 
     def workspace_bytes(self, n_tokens: int, dtype=None) -> int:
-        return int(lib().smoe_linear4_workspace_bytes(self._layer(BF16 if dtype is None else _elem_type(dtype))[1], n_tokens))
+        layer = self._layer(BF16 if dtype is None else _elem_type(dtype))[1]
+        return int(lib().smoe_linear4_workspace_bytes(layer, _int32(n_tokens, "n_tokens")))
 
     def run(self, x, residual=None, y=None, y_dtype=None, stream=None):
         """y (tokens, n_out) of `y_dtype` (None: residual's, else x's); `y` may be residual."""
@@ -860,6 +870,8 @@ class Linear4:
             with _on(dev, stream):
                 return self.run(x, residual, y, y_dtype)
         T = x.shape[0]
+        if T >> 31:
+            _int32(T, "the number of tokens")
         rp, rt, r_ld = None, -1, 0
         if residual is not None:
             rt, r_ld = _rows(residual, "residual", N, T, dev)
@@ -917,6 +929,8 @@ def _heads(t, name: str, heads: int, dim: int, tokens: int = -1, device: int = -
     if len(shape) != 3 or shape[2] != dim or (heads >= 0 and shape[1] != heads) or (tokens >= 0 and shape[0] != tokens):
         raise SmoeError(-2, f"{name} has shape {tuple(shape)}, needs ({'tokens' if tokens < 0 else tokens}, "
                             f"{'heads' if heads < 0 else heads}, {dim})")
+    if shape[0] >> 31 or shape[1] >> 31:
+        _int32(max(shape[0], shape[1]), f"a size of {name}")
     ld, step, one = t.stride()
     if one != 1 or (step != dim and shape[1] > 1):
         raise SmoeError(-5, f"a token's values of {name} are not contiguous")
@@ -952,6 +966,8 @@ class Rotary:
                  turns=None, scale: Optional[float] = None, device="cuda"):
         import torch
         rot_dim = head_dim if rot_dim is None else rot_dim
+        for v, name in ((head_dim, "head_dim"), (rot_dim, "rot_dim"), (layout, "layout")):
+            _int32(v, name)
         if turns is None:
             turns, own_scale = rope_table(rot_dim, base, scaling)
         else:
@@ -998,11 +1014,11 @@ class PagedCache:
         _given(k, "k"), _given(v, "v")
         if getattr(k, "ndim", 0) != 4:
             raise SmoeError(-2, "k must be (pages, key heads, tokens of a page, head_dim)")
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = (_int32(n, "a size of the cache") for n in k.shape)
         for t, name in ((k, "k"), (v, "v")):
             _need(t, name, k.dtype, shape=k.shape)
             _on_device(t, name, k.get_device())
         self.k, self.v = k, v
-        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self._type, self._device = _elem_type(k.dtype), k.get_device()
         self._c = _Kv(k.data_ptr(), v.data_ptr(), self._type, *(int(k.shape[i]) for i in (0, 2, 1, 3)))
         self._ref = C.byref(self._c)
@@ -1059,6 +1075,8 @@ class PagedCache:
         return q_out
 
     def workspace_bytes(self, n_heads: int, n_tokens: int, n_seqs: int, max_len: int, window: int = 0) -> int:
+        for v, name in ((n_heads, "n_heads"), (n_tokens, "n_tokens"), (n_seqs, "n_seqs"), (max_len, "max_len"), (window, "window")):
+            _int32(v, name)
         return int(lib().smoe_attend_workspace_bytes(self._ref, n_heads, n_tokens, n_seqs, max_len, window))
 
     def attend(self, q, q_start, kv_len, pages, scale: Optional[float] = None, causal: bool = True, window: int = 0,
@@ -1090,6 +1108,8 @@ class PagedCache:
             raise SmoeError(-5, "pages' rows are not contiguous")
         if pages.get_device() != dev:
             _on_device(pages, "pages", dev)
+        if width >> 31:
+            _int32(width, "the pages' width")
         held = min(width * self.page_size, 1 << 30)
         max_len = held if max_len is None else max_len
         if out is None:
@@ -1111,7 +1131,7 @@ class PagedCache:
         # a workspace of the call's own: calls on several streams, captured or not, share none
         ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device) if n > 256 else None
         _check(self._attend(self._ref, q.data_ptr(), q_ld, T, H, sp, lp, B, pages.data_ptr(), p_ld, width, max_len,
-                            D ** -0.5 if scale is None else scale, int(causal), window, out.data_ptr(), o_ld, _ptr(z), _ptr(ws), n, st))
+                            D ** -0.5 if scale is None else scale, int(bool(causal)), window, out.data_ptr(), o_ld, _ptr(z), _ptr(ws), n, st))
         return (out, z) if lse else out
 
 

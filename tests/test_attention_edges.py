@@ -1,7 +1,9 @@
 """CPU tests of the bounds that attention over a paged cache and the product with 4-bit weights keep at the edges of what their
 calls allow (test_gpu_attend_edges.py and test_gpu_linear4_edges.py run them)."""
 import pytest
+import torch
 
+import stratametal_amd as S
 from test_dispatch_rules import ask  # noqa: F401
 
 INT_MAX = 2 ** 31 - 1
@@ -16,3 +18,24 @@ def test_linear4_group_sums_stay_in_32_bits(ask):  # noqa: F811
             if group <= n_in:
                 assert got == group
         assert got % 32 == 0 and (group < 65536 or got % 128 == 0)
+
+
+def test_binding_refuses_numbers_past_32_bits():
+    """The binding passes 32-bit numbers by their low bits: a group of 2^32 + 128 would pass the shape check and run as 128."""
+    z = torch.zeros((1, 2, 64))
+    w, s = torch.zeros((4, 128), dtype=torch.uint8), torch.zeros((1, 4))
+    r, c = object.__new__(S.Rotary), object.__new__(S.PagedCache)
+    r.head_dim, r._device = 64, -1
+    c.head_dim, c.n_kv_heads, c._device, c._type, c.k, c._ref = 64, 2, -1, S.F32, z, None
+    tokens = torch.zeros(1, dtype=torch.int32).expand(2 ** 31)
+    many, pages = z.expand(2 ** 31, 2, 64), torch.empty((2 ** 32 + 1, 1, 1, 8), device="meta")
+    for fn in (lambda: S.Linear4(256, 4, w, s, group=2 ** 32 + 128), lambda: S.Linear4(2 ** 32 + 256, 4, w, s), lambda: S.Linear4(256, 2 ** 32 + 4, w, s),
+               lambda: S.Linear4(256, 4, w, s, act=2 ** 32), lambda: S.Rotary(2 ** 32 + 64, rot_dim=64, device="cpu"),
+               lambda: S.Rotary(64, rot_dim=2 ** 32 + 64, turns=[0.0], device="cpu"), lambda: S.Rotary(64, layout=2 ** 32, device="cpu"),
+               lambda: r.run(many, tokens), lambda: c.append(many, many, tokens), lambda: c.attend(many, tokens, tokens, tokens),
+               lambda: S.PagedCache(pages, pages), lambda: c.workspace_bytes(4, 1, 1, 100, window=2 ** 32 + 5),
+               lambda: c.workspace_bytes(4, 2 ** 32 + 1, 1, 100), lambda: c.workspace_bytes(2 ** 32 + 4, 1, 1, 100),
+               lambda: c.workspace_bytes(4, 1, -2 ** 31 - 1, 100), lambda: c.workspace_bytes(4, 1, 1, 2 ** 40)):
+        with pytest.raises(S.SmoeError) as err:
+            fn()
+        assert "32 bits" in str(err.value), str(err.value)
