@@ -796,12 +796,12 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
 __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, const AttendPlan p, int per_row) {
     __shared__ f32x4 out_s[256];
     __shared__ float2 stats_s[256];
-    const int per = a.head_dim / 4, groups = 256 / per;  // threads of a group, groups
-    const int rows = groups / per_row, g = threadIdx.x / per, d = threadIdx.x % per;
-    const int mine = g / per_row, first = g % per_row;
-    const int64_t row = (int64_t)blockIdx.x * rows + mine;
+    const int per = a.head_dim / 4, d = threadIdx.x % per;  // threads of a group
+    const JoinPlace place = attend_join_place(threadIdx.x, per, per_row);
+    const int first = place.group;
+    const int64_t row = (int64_t)blockIdx.x * (256 / per / per_row) + place.row;
     const int t = (int)(row / a.n_heads), head = (int)(row % a.n_heads);
-    const bool live = mine < rows && t >= a.q_start[0] && t < min(a.q_start[a.n_seqs], a.n_tokens);
+    const bool live = place.row >= 0 && t >= a.q_start[0] && t < min(a.q_start[a.n_seqs], a.n_tokens);
     float top = -__builtin_inff(), sum = 0.0f;
     f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
     if (live) {
@@ -838,7 +838,7 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, const A
     if (per_row > 1) {
         out_s[threadIdx.x] = out, stats_s[threadIdx.x] = make_float2(top, sum);
         __syncthreads();
-        if (first == 0) {
+        if (live && first == 0) {  // (of a thread past the last row the other groups' places lie past the arrays)
             for (int i = 1; i < per_row; ++i) top = __builtin_fmaxf(top, stats_s[threadIdx.x + i * per].x);
             const float base = top == -__builtin_inff() ? 0.0f : top;
             sum = 0.0f, out = f32x4{0.0f, 0.0f, 0.0f, 0.0f};

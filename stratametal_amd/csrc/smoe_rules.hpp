@@ -368,6 +368,15 @@ inline double attend_time(int64_t groups, int64_t splits, int64_t keys, int64_t 
     const double all = (double)(groups * splits) * (start + tile * (double)tiles / 2) / (double)places + most / 2;
     return (all > most ? all : most) + join;
 }
+// k_attend_join: thread i of 256, `per` threads to a split's values and per_row such groups to a query row, has a part in row
+// `row` of its work-group's, in its group `group`; the threads past the last whole row have none (-1).
+struct JoinPlace {
+    int row, group;
+};
+constexpr JoinPlace attend_join_place(int i, int per, int per_row) {
+    const int g = i / per, rows = 256 / per / per_row, row = g / per_row;
+    return {row < rows ? row : -1, g % per_row};
+}
 inline AttendPlan attend_plan(int64_t T, int64_t B, int H, int kv, int D, int64_t max_len, int64_t window) {
     const int64_t group = H / kv, rows = T * H;
     AttendPlan best{};

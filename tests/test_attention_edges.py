@@ -39,3 +39,21 @@ def test_binding_refuses_numbers_past_32_bits():
         with pytest.raises(S.SmoeError) as err:
             fn()
         assert "32 bits" in str(err.value), str(err.value)
+
+
+def test_attend_join_reads_its_arrays(ask):  # noqa: F811
+    """The threads that join a row's groups find every one of them within the work-group's 256 places, for every head size and
+    number of groups to a row; and each row has all of its groups."""
+    for dim in (8, 24, 40, 64, 80, 96, 120, 128, 168, 200, 240, 256):
+        per, per_row = dim // 4, 1
+        while per_row <= 256 // per:
+            got = ask([f"attend_join_place({i}, {per}, {per_row}).row * 1000 + attend_join_place({i}, {per}, {per_row}).group" for i in range(256)])
+            rows, seen = 256 // per // per_row, set()
+            for i, both in enumerate(got):
+                row, group = both // 1000, both % 1000
+                assert -1 <= row < rows and 0 <= group < per_row
+                if row >= 0:
+                    seen.add((row, group, i % per))
+                    assert i - group * per + (per_row - 1) * per < 256, (dim, per_row, i)
+            assert len(seen) == rows * per_row * per
+            per_row *= 2
