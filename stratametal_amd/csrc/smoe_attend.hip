@@ -826,8 +826,9 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, const A
             out *= keep;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
-                // (a split without keys has written no values)
-                const bool some = s + i * per_row < p.splits && m[i].x != -__builtin_inff();
+                // (a split without keys has a sum of 0 and has written no values; one whose scores are all NaN has a top of -inf and a
+                // sum of NaN, which 0 times it keeps)
+                const bool some = s + i * per_row < p.splits && m[i].y != 0.0f;
                 const float w = some ? __builtin_amdgcn_exp2f(m[i].x - base) : 0.0f;
                 sum = some ? __builtin_fmaf(w, m[i].y, sum) : sum;
 #pragma unroll
