@@ -20,6 +20,9 @@ constexpr int kMaxDim = 256;
 struct Sequence {
     int b, t0, n, len;
 };
+// The first key that a query at position p (below 0: before the first key) sees: p - window + 1, where that is not below 0 (and so
+// never past 32 bits), window 0: all.
+__device__ __forceinline__ int first_seen(int p, int window) { return window && p >= window ? p - window + 1 : 0; }
 __device__ __forceinline__ float half_value(uint32_t bits, bool f16) { return elem_to_f32(bits, f16 ? kF16 : kBf16); }
 
 // One query row by one wave, 64 keys at a time, a key to a lane for its score and 64 values of the head to the wave for the
@@ -33,8 +36,7 @@ __device__ __forceinline__ void row_alone(const AttendArgs& a, const Sequence& s
     const int p = s.len - s.n + (t - s.t0);
     if (a.causal) k1 = min(k1, p + 1);
     k1 = min(k1, s.len);
-    if (a.window) k0 = max(k0, p - a.window + 1);
-    k0 = max(k0, 0);
+    k0 = max(k0, first_seen(p, a.window));
     const int32_t* pages = a.pages + s.b * a.pages_ld;
     top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
@@ -215,9 +217,9 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan&
     if (!found || w.row0 < 0 || w.rows <= 0) return false;
     // the keys that some row of the tile sees
     const int first = w.s.len - w.s.n + w.row0 / g, last = w.s.len - w.s.n + (w.row0 + w.rows - 1) / g;
-    w.k0 = a.window ? max(0, first - a.window + 1) : 0;
+    w.k0 = first_seen(first, a.window);
     w.k1 = a.causal ? min(w.s.len, last + 1) : w.s.len;
-    w.k0 = max(w.k0, 0), w.k1 = max(w.k1, w.k0);
+    w.k1 = max(w.k1, w.k0);
     if (p.splits > 1) {
         total = wave_sum_xor_fast(total), most = (int)wave_max_u32_fast((uint32_t)most);
         const float groups = (float)before * (float)a.n_kv, all = total * (float)a.n_kv;
@@ -364,7 +366,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     const int row_q = w.row0 + min(r_q, w.rows - 1);
     const int t_q = row_q / a.group, head = w.kvh * a.group + row_q % a.group;
     const int pos = w.s.len - w.s.n + t_q;
-    const int hi = a.causal ? min(pos + 1, w.k1) : w.k1, lo = a.window ? max(pos - a.window + 1, w.k0) : w.k0;
+    const int hi = a.causal ? min(pos + 1, w.k1) : w.k1, lo = max(first_seen(pos, a.window), w.k0);
     // keys that all of the wave's queries see: [lo_all, hi_all)
     const int hi_all = __builtin_amdgcn_readfirstlane(hi), lo_all = __builtin_amdgcn_readlane(lo, 31);
     const bool live = wave * 32 < w.rows;
@@ -653,7 +655,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
     const int h = lane >> 4, r_q = lane & 15, row_q = w.row0 + min(r_q, w.rows - 1);
     const int t_q = row_q / a.group, head = w.kvh * a.group + row_q % a.group;
     const int pos = w.s.len - w.s.n + t_q;
-    const int hi = a.causal ? min(pos + 1, w.k1) : w.k1, lo = a.window ? max(pos - a.window + 1, w.k0) : w.k0;
+    const int hi = a.causal ? min(pos + 1, w.k1) : w.k1, lo = max(first_seen(pos, a.window), w.k0);
     if (wave < blocks) load_ids(wave, 0), load_ids(wave + 4, 1);
     u32x4 qf[NQ];
     load_query<NQ, 4>(a, w.s.t0 + t_q, head, h, qf);

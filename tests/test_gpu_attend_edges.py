@@ -47,3 +47,15 @@ def test_nan_that_a_query_sees(n, L, H, kv, split, D):
         o, lse = b.run()
         assert bool(o[:, H - g:].isnan().all()) and bool(lse[:, H - g:].isnan().all())
         assert torch.equal(o[:, :H - g], clean[:, :H - g]) and torch.equal(lse[:, :H - g], clean_lse[:, :H - g])
+
+
+@pytest.mark.parametrize("n,H,kv,D", [(1, 4, 2, 64), (4, 4, 2, 128), (60, 4, 2, 256), (200, 4, 2, 64), (700, 32, 8, 128), (1500, 16, 2, 256)])
+def test_widest_window(n, H, kv, D):
+    """A window as wide as its type holds hides nothing, in sequences with more queries than keys too."""
+    say(f"case: attend widest window n={n} H={H} kv={kv} D={D}")
+    b = Batch(n, [n, n + 5, 3], [n // 2, 3, 100], H, kv, D, 16)
+    want, want_lse = b.run()
+    for window in (2 ** 31 - 1, 2 ** 31 - 4, 2 ** 30):
+        o, lse = b.run(window=window)
+        assert torch.equal(o, want) and torch.equal(lse, want_lse), window
+    b.check(o, lse)
