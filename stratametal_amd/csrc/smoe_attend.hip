@@ -16,9 +16,10 @@ namespace {
 constexpr float kLn2 = 0.693147181f;
 constexpr int kMaxDim = 256;
 
-// Sequence b: its first query row, rows and keys.
+// Sequence b: its first query row, rows, length, and how many of its keys are there (no more than max_len).  Its query of row t
+// has position len - n + (t - t0).
 struct Sequence {
-    int b, t0, n, len;
+    int b, t0, n, len, keys;
 };
 // The first key that a query at position p (below 0: before the first key) sees: p - window + 1, where that is not below 0 (and so
 // never past 32 bits), window 0: all.
@@ -35,7 +36,7 @@ __device__ __forceinline__ void row_alone(const AttendArgs& a, const Sequence& s
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const int p = s.len - s.n + (t - s.t0);
     if (a.causal) k1 = min(k1, p + 1);
-    k1 = min(k1, s.len);
+    k1 = min(k1, s.keys);
     k0 = max(k0, first_seen(p, a.window));
     const int32_t* pages = a.pages + s.b * a.pages_ld;
     top = -__builtin_inff(), sum = 0.0f;
@@ -194,7 +195,7 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan&
     int3 next = {0, 0, 0};
     if (lane < a.n_seqs) next = {a.q_start[lane], a.q_start[lane + 1], a.kv_len[lane]};
     for (int at = 0; at < a.n_seqs; at += 64) {
-        const int t0 = min(max(next.x, 0), a.n_tokens), t1 = min(max(next.y, t0), a.n_tokens), len = min(max(next.z, 0), a.max_len);
+        const int t0 = min(max(next.x, 0), a.n_tokens), t1 = min(max(next.y, t0), a.n_tokens), len = max(next.z, 0);
         next = {0, 0, 0};
         if (const int b = at + 64 + lane; b < a.n_seqs) next = {a.q_start[b], a.q_start[b + 1], a.kv_len[b]};
         const int tiles = ((t1 - t0) * g + M - 1) / M, sum = wave_inclusive_scan(tiles);
@@ -202,14 +203,15 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan&
         if (past) {
             const int l = __builtin_ctzll(past);
             const int s0 = __builtin_amdgcn_readlane(t0, l), s1 = __builtin_amdgcn_readlane(t1, l);
-            w.s = {__builtin_amdgcn_readfirstlane(at + l), s0, s1 - s0, __builtin_amdgcn_readlane(len, l)};
+            const int s_len = __builtin_amdgcn_readlane(len, l);
+            w.s = {__builtin_amdgcn_readfirstlane(at + l), s0, s1 - s0, s_len, min(s_len, a.max_len)};
             w.row0 = (tile - before - __builtin_amdgcn_readlane(sum - tiles, l)) * M;
             w.rows = min(M, w.s.n * g - w.row0);
             found = true;
             if (p.splits == 1) break;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
-        const int keys = tiles ? min(len, seen) : 0;
+        const int keys = tiles ? min(min(len, a.max_len), seen) : 0;
         most = max(most, keys);
         total += (float)tiles * (float)keys;
     }
@@ -218,7 +220,7 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, const AttendPlan&
     // the keys that some row of the tile sees
     const int first = w.s.len - w.s.n + w.row0 / g, last = w.s.len - w.s.n + (w.row0 + w.rows - 1) / g;
     w.k0 = first_seen(first, a.window);
-    w.k1 = a.causal ? min(w.s.len, last + 1) : w.s.len;
+    w.k1 = a.causal ? min(w.s.keys, last + 1) : w.s.keys;
     w.k1 = max(w.k1, w.k0);
     if (p.splits > 1) {
         total = wave_sum_xor_fast(total), most = (int)wave_max_u32_fast((uint32_t)most);

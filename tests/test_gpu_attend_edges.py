@@ -59,3 +59,28 @@ def test_widest_window(n, H, kv, D):
         o, lse = b.run(window=window)
         assert torch.equal(o, want) and torch.equal(lse, want_lse), window
     b.check(o, lse)
+
+
+@pytest.mark.parametrize("new,lens,H,kv,D,max_len", [
+    ([10, 1, 7], [100, 2 ** 31 - 1, 93], 4, 2, 64, 90), ([1, 40, 3], [300, 130, 128], 6, 2, 128, 128), ([5, 30], [80, 70], 3, 1, 256, 64),
+    ([600, 300], [900, 500], 32, 8, 128, 400), ([300, 400], [650, 2 ** 31 - 1], 16, 2, 256, 400)])
+@pytest.mark.parametrize("window", [0, 20, 150])
+def test_positions_of_sequences_past_the_longest(new, lens, H, kv, D, max_len, window):
+    """Keys past max_len are not there; the queries' positions are those of the whole sequence."""
+    say(f"case: attend past the longest {new} {lens} H={H} D={D} max_len={max_len} window={window}")
+    there = [min(l, max_len) for l in lens]
+    b = Batch(sum(new) + D, new, there, H, kv, D, 16)
+    b.lens = lens
+    o, lse = b.run(max_len=max_len, window=window)
+    g, at = H // kv, [0, kv - 1]
+    heads = [k * g + j for k in at for j in range(g)]
+    for s in range(len(new)):
+        for i in range(0, new[s], max(1, new[s] // 9)):
+            p, t = lens[s] - new[s] + i, int(b.start[s]) + i
+            lo, hi = max(0, p - window + 1) if window else 0, min(there[s], p + 1)
+            if hi <= lo:
+                assert bool((o[t] == 0).all()) and bool(torch.isneginf(lse[t]).all())
+                continue
+            want, bound, wl, el = A.attend(host(b.q[t:t + 1, heads]), b.keys[s][lo:hi][:, at], b.values[s][lo:hi][:, at], D ** -0.5, False, 0, "bf16")
+            close(o[t:t + 1, heads], want, bound)
+            assert (np.abs(host(lse[t:t + 1, heads]) - wl) <= el).all()
