@@ -302,6 +302,12 @@ __device__ __forceinline__ void load_query(const AttendArgs& a, int t, int head,
 
 // A new key's weight may be up to 2^kLag times the top's before the sums are scaled to a new top.
 constexpr float kLag = 8.0f;
+// Weights are formed 2^LIFT times up and the sums brought back by 2^-LIFT (exact).  bf16 needs none; fp16 ones would lose a
+// weight below 2^-25 of the top's whole, and half a step of 2^-24 of others, from the values' sums but not from their own, and with
+// many equal keys behind one large score these losses add up: so as far up as the type allows (2^15 with the lag).
+template <bool F16, bool LAG>
+constexpr float kLift = !F16 ? 0.0f : LAG ? 15.0f - kLag : 15.0f;
+constexpr float power_of_half(float n) { return n < 0.5f ? 1.0f : 0.5f * power_of_half(n - 1.0f); }
 
 }  // namespace
 
@@ -323,6 +329,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = KEYS / RPI / 4;  // lanes to a row, rows of a load, a wave's loads of a tile
     constexpr int PLANE = KEYS * DIM * 2, HALF = PLANE / 2;
     constexpr bool HIGH = DIM > 128;  // the sums of values in accumulation registers
+    constexpr float LIFT = kLift<F16, true>, DROP = power_of_half(LIFT);
     __shared__ __align__(1024) uint8_t lds[4 * PLANE];  // two tiles of keys, two of values
     __shared__ int ids[4][64], rows_s[4][64];  // of a tile's keys: page numbers, then rows of the cache
     __shared__ int bad_page;
@@ -404,7 +411,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
         const float next = __builtin_fmaxf(top, max_halves(m) * scale);
         keep = next == top ? 1.0f : __builtin_amdgcn_exp2f(top - next);
         top = next;
-        base = top == -__builtin_inff() ? 0.0f : top;
+        base = top == -__builtin_inff() ? 0.0f : top - LIFT;
         sum *= keep, odd_sum *= keep;
     };
     const auto passed = [&](float m) { return __ballot(m * scale > top + kLag) != 0; };
@@ -576,7 +583,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     if (bad) bad_page = 1;
     __syncthreads();
     if (!live) return;
-    const float inv = p.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = p.splits > 1 ? DROP : sum == 0.0f ? 0.0f : 1.0f / sum;
     // what is not finite may come of a value that the query does not see (0 times it): such rows are done anew
     bool lost = !(__builtin_fabsf(sum) < __builtin_inff());
     const int t = w.s.t0 + t_q;
@@ -603,7 +610,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
 #pragma unroll
                 for (int x = 0; x < 4; ++x) out[d + x] = f32_to_half_bits(v[x], F16 ? kF16 : kBf16);
         }
-    if (mine && h == 0) put_stats(a, p, row, w.split, top, sum);
+    if (mine && h == 0) put_stats(a, p, row, w.split, top, sum * DROP);
     uint64_t again = __ballot(mine && (lost || bad_page));
     again = (again | again >> 32) & 0xFFFFFFFFull;
     for (; again; again &= again - 1)
@@ -621,6 +628,7 @@ template <int DIM, bool F16>
 __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const AttendArgs a, const AttendPlan p) {
     constexpr int M = kAttendFewRows, NQ = DIM / 32, ND = DIM / 16, PLANE = 32 * DIM * 2;
     constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = 32 / RPI;  // lanes to a row, rows of a load, loads of a block
+    constexpr float LIFT = kLift<F16, false>, DROP = power_of_half(LIFT);
     static_assert(4 * ND * 1024 <= 8 * PLANE, "the waves' sums");
     __shared__ __align__(1024) uint8_t lds[8 * PLANE];
     __shared__ int32_t ids[4][2][64];
@@ -705,7 +713,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
         const float next = __builtin_fmaxf(top, m * scale);
         if (__ballot(next != top)) {
             const float keep = next == top ? 1.0f : __builtin_amdgcn_exp2f(top - next);
-            top = next, base = top == -__builtin_inff() ? 0.0f : top;
+            top = next, base = top == -__builtin_inff() ? 0.0f : top - LIFT;
             sum *= keep;
 #pragma unroll
             for (int i = 0; i < ND; ++i) acc[i] *= keep;
@@ -757,7 +765,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
         part_of[v] = __builtin_amdgcn_exp2f(stats_s[v][r_q].x - base);
         sum = __builtin_fmaf(part_of[v], stats_s[v][r_q].y, sum);
     }
-    const float inv = p.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = p.splits > 1 ? DROP : sum == 0.0f ? 0.0f : 1.0f / sum;
     // what is not finite may come of a value that the query does not see (0 times it): such rows are done anew
     bool lost = !(__builtin_fabsf(sum) < __builtin_inff());
     const int tok = w.s.t0 + t_q;
@@ -785,7 +793,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
 #pragma unroll
             for (int x = 0; x < 4; ++x) out[d + x] = f32_to_half_bits(y[x], F16 ? kF16 : kBf16);
     }
-    if (wave == 0 && mine && h == 0) put_stats(a, p, out_row, w.split, top, sum);
+    if (wave == 0 && mine && h == 0) put_stats(a, p, out_row, w.split, top, sum * DROP);
     if (mine && lost) atomicOr(&again_s, 1u << r_q);
     __syncthreads();
     for (uint32_t again = again_s & ((1u << w.rows) - 1); again; again &= again - 1) {

@@ -84,3 +84,29 @@ def test_positions_of_sequences_past_the_longest(new, lens, H, kv, D, max_len, w
             want, bound, wl, el = A.attend(host(b.q[t:t + 1, heads]), b.keys[s][lo:hi][:, at], b.values[s][lo:hi][:, at], D ** -0.5, False, 0, "bf16")
             close(o[t:t + 1, heads], want, bound)
             assert (np.abs(host(lse[t:t + 1, heads]) - wl) <= el).all()
+
+
+@pytest.mark.parametrize("n,L,H,kv", [(1, 1000, 4, 1), (3, 9000, 4, 2), (1024, 1024, 32, 8), (1024, 2100, 16, 2)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_small_weights_in_fp16(n, L, H, kv, D):
+    """One key far above the rest, whose weights, 2^-25.2 of its own, are below half of fp16's smallest step: all that its value of
+    0 leaves is theirs.  Weights are held 2^15 (tiles of 128 rows: 2^7) times up, so at most half a step of 2^-24 over that is lost of
+    each: 2^-40 (2^-32), and half a step of those that are no subnormals, which averages over nothing here: the keys are equal."""
+    say(f"case: attend tails n={n} L={L} H={H} kv={kv} D={D}")
+    b = Batch(1, [n], [L], H, kv, D, 16, "fp16")
+    far = 17.46875  # 25.2 ln 2, a whole number of fp16's steps
+    b.q = torch.zeros_like(b.q)
+    b.q[..., 0] = 1.0
+    b.keys[0][:], b.values[0][:] = 0, 1024
+    b.keys[0][0, :, 0], b.values[0][0] = far, 0
+    for c in (b.cache.k, b.cache.v):
+        c.zero_()
+    b.cache.v.fill_(1024)
+    b.cache.k[int(b.table[0, 0]), :, 0, 0], b.cache.v[int(b.table[0, 0]), :, 0] = far, 0
+    o, lse = b.run(scale=1.0)
+    seen = np.arange(L - n + 1, L + 1, dtype=np.float64)
+    w = np.exp(-far)
+    total = 1 + (seen - 1) * w
+    want = (seen - 1) * w * 1024 / total
+    bound = want * 2.0 ** -11 + 2.0 ** -25 + 1024 * (seen - 1) * 2.0 ** -32 + want * (2.0 ** -11 + (L / 16 + 200) * 2.0 ** -24)
+    close(o, np.broadcast_to(want[:, None, None], o.shape), np.broadcast_to(bound[:, None, None], o.shape))
