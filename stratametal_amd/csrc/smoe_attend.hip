@@ -718,14 +718,17 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
 #pragma unroll
             for (int i = 0; i < ND; ++i) acc[i] *= keep;
         }
-        u32x4 wt;
+        u32x4 wt, rest;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             t[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[e], scale, -base));
             sum += t[e];
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) wt[e] = pack2<F16>(t[2 * e], t[2 * e + 1]);
+        for (int e = 0; e < 4; ++e) {
+            wt[e] = pack2<F16>(t[2 * e], t[2 * e + 1]);
+            rest[e] = pack2<F16>(t[2 * e] - half_value(wt[e] & 0xFFFFu, F16), t[2 * e + 1] - half_value(wt[e] >> 16, F16));
+        }
         if (more) vmcnt<LOADS + 1>();  // the values
         else vmcnt<0>();
 #pragma unroll
@@ -738,6 +741,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
                 f[2 * x] = half[0], f[2 * x + 1] = half[1];
             }
             acc[i] = mfma16<F16>(f, wt, acc[i]);
+            acc[i] = mfma16<F16>(f, rest, acc[i]);
         }
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -110,3 +110,21 @@ def test_many_small_weights_in_fp16(n, L, H, kv, D):
     want = (seen - 1) * w * 1024 / total
     bound = want * 2.0 ** -11 + 2.0 ** -25 + 1024 * (seen - 1) * 2.0 ** -32 + want * (2.0 ** -11 + (L / 16 + 200) * 2.0 ** -24)
     close(o, np.broadcast_to(want[:, None, None], o.shape), np.broadcast_to(bound[:, None, None], o.shape))
+
+
+@pytest.mark.parametrize("new,lens", [([1] * 6, [1, 2, 33, 100, 700, 3000]), ([1], [9000]), ([5, 20, 1], [70, 300, 2000])])
+@pytest.mark.parametrize("H,kv,D", [(8, 2, 64), (4, 1, 128), (5, 1, 256), (3, 1, 80)])
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_weights_of_few_rows_keep_two_parts(new, lens, H, kv, D, t):
+    """Tiles of 16 rows hold a weight as two numbers of the cache's type: it is off by half a step of half a step, 2^-16 in bf16
+    and less in fp16, so an output differs from the formula's by f32 arithmetic, that, and its own rounding."""
+    say(f"case: attend two parts {new} {lens} H={H} kv={kv} D={D} {t}")
+    b = Batch(D + len(new), new, lens, H, kv, D, 16, t)
+    o, lse = b.run()
+    half, tiny = {"bf16": (2.0 ** -8, 2.0 ** -134), "fp16": (2.0 ** -11, 2.0 ** -25)}[t]
+    for s in range(len(new)):
+        rows = slice(b.start[s], b.start[s + 1])
+        q = host(b.q[rows])
+        want, e, _, _ = A.attend(q, b.keys[s], b.values[s], D ** -0.5, True, 0, "f32")
+        size, *_ = A.attend(q, b.keys[s], np.abs(b.values[s]), D ** -0.5, True, 0, "f32")
+        close(o[rows], want, e + 2.0 ** -16 * size + (np.abs(want) + e) * half + tiny)
