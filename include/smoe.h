@@ -282,7 +282,7 @@ smoe_status smoe_linear_run(const smoe_linear* L, const void* x, int64_t x_ld, i
 
 /* The same product with 4-bit weights: W[o][i] = scale[i / group][o] (code[o][i] - zero[i / group][o]), the codes 0 .. 15 two to
  * a byte, the even i's low; the products are exact and summed in f32, a group's sum scaled once (no weight is rounded).
- * x is bf16 or fp16. */
+ * x is bf16 or fp16; what is not finite in a token's values gives what the formula gives, in that token alone. */
 typedef struct {
     int32_t n_in;         /* a multiple of 32, at most 65536 */
     int32_t n_out;        /* 1 .. 2^24 */

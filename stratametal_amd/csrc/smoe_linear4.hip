@@ -210,6 +210,43 @@ __global__ __launch_bounds__(512, 4) void k_linear4_few(const Linear4Args a) {
         at = at + STAGE == RING * STAGE ? 0 : at + STAGE;
     }
     vmcnt<0>();
+    // An infinite x makes sum code x and zero sum x infinite both, and so does one past 2^128 / 15: what is not finite is summed anew
+    // from codes less their zeros, as the tiles do it, so that the answer is the formula's and goes by no number of tokens.
+    bool lost = false;
+#pragma unroll
+    for (int i = 0; i < SETS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lost |= !(__builtin_fabsf(acc[i][j]) < __builtin_inff());
+    if (__ballot(lost)) {
+        f32x4 again[SETS];
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) again[i] = none;
+        const uint16_t* x = static_cast<const uint16_t*>(a.x) + (int64_t)min(lane & 15, a.n_tokens - 1) * a.x_ld + 8 * q;
+#pragma unroll 1
+        for (int u = wave; u < stages; u += WAVES)
+#pragma unroll 1
+            for (int k = u * 128; k < min(u * 128 + 128, a.n_in); k += 32) {
+                const int64_t g = (int64_t)(k / a.group) * a.n_out;
+                const uint4 xv = *reinterpret_cast<const uint4*>(x + k);
+#pragma unroll
+                for (int i = 0; i < SETS; ++i) {
+                    const uint32_t c = *reinterpret_cast<const uint32_t*>(w[i] + (int64_t)out * half_row + k / 2 + 4 * q);
+                    const u32x4 wv = expand8_less<F16>(c, zero_term<F16>(zr[i] ? zr[i][g + out] : 8u));
+                    const f32x4 sum = mfma16<F16>(__builtin_bit_cast(uint4, wv), xv, none);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int64_t at = g + min(o0 + 4 * q + j, a.n_out - 1);
+                        const float scale = wide ? static_cast<const float*>(static_cast<const void*>(sc[i]))[at]
+                                                 : one_scale(static_cast<const uint16_t*>(static_cast<const void*>(sc[i]))[at], a.s_type);
+                        again[i][j] = __builtin_fmaf(scale, sum[j], again[i][j]);
+                    }
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < SETS; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_fabsf(acc[i][j]) < __builtin_inff() ? acc[i][j] : again[i][j];
+    }
     __syncthreads();
     f32x4* sum_s = reinterpret_cast<f32x4*>(lds4);  // [wave][set][lane]
 #pragma unroll
