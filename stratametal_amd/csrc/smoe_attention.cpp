@@ -190,7 +190,8 @@ smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t 
     if (s != SMOE_OK) return s;
     if (max_pages < 0 || max_len > (int64_t)max_pages * kv->page_size)
         return fail(SMOE_EINVAL, "attend: max_len is more than max_pages hold");
-    if (!finite(scale)) return fail(SMOE_EINVAL, "attend: scale must be finite");
+    constexpr float kLog2e = 1.44269504f;
+    if (!finite(scale * kLog2e)) return fail(SMOE_EINVAL, "attend: scale must be finite, and so must scale times log2 e");
     if (window < 0 || (window && !causal)) return fail(SMOE_EINVAL, "attend: a window must be positive, and causal");
     if (n_tokens == 0 || n_seqs == 0) return ok();
     if (!kv->k || !kv->v || !q || !q_start || !kv_len || !out || (max_len && !pages)) return fail(SMOE_ENULL, "attend: NULL buffer");
@@ -228,7 +229,7 @@ smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t 
     a.n_tokens = n_tokens, a.n_seqs = n_seqs, a.n_heads = n_heads, a.n_kv = kv->n_kv_heads, a.group = n_heads / kv->n_kv_heads;
     a.head_dim = kv->head_dim, a.page_size = kv->page_size, a.n_pages = kv->n_pages, a.max_len = (int)max_len;
     a.causal = causal != 0, a.window = window, a.f16 = kv->type == SMOE_F16;
-    a.scale = scale * 1.44269504f;
+    a.scale = scale * kLog2e;
     return launched(launch_attend(a, reinterpret_cast<hipStream_t>(hip_stream)), "attend");
 }
 

@@ -4,6 +4,8 @@ import pytest
 import torch
 
 import stratametal_amd as S
+from test_attention_refusals import attend, verdict
+from test_dense_refusals import EINVAL
 from test_dispatch_rules import ask  # noqa: F401
 
 INT_MAX = 2 ** 31 - 1
@@ -57,3 +59,9 @@ def test_attend_join_reads_its_arrays(ask):  # noqa: F811
                     assert i - group * per + (per_row - 1) * per < 256, (dim, per_row, i)
             assert len(seen) == rows * per_row * per
             per_row *= 2
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, 2.4e38, float("inf")])
+def test_attend_scale_that_leaves_f32(scale):
+    """Scores travel in units of ln 2: scale times log2 e has to be a number, too."""
+    verdict(attend(scale=scale), EINVAL)
