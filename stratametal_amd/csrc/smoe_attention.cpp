@@ -10,6 +10,7 @@
 
 #include "smoe_check.hpp"
 #include "smoe_launch.hpp"
+#include "smoe_rules.hpp"
 
 using namespace smoe;
 
@@ -88,6 +89,7 @@ smoe_status smoe_rope_run(const smoe_rope* r, const int32_t* positions, int32_t 
     const smoe_status s = check_rope(r, "rope");
     if (s != SMOE_OK) return s;
     if (n_tokens < 0) return fail(SMOE_EINVAL, "rope: negative token count");
+    if (!rope_fits(n_tokens)) return fail(SMOE_EINVAL, "rope: the tokens exceed a launch's grid: split them");
     if (n_heads < 1 || n_heads > kMaxHeads) return fail(SMOE_EINVAL, "rope: n_heads must be 1 to " + std::to_string(kMaxHeads));
     if (!elem_type(x_type) || !elem_type(y_type)) return fail(SMOE_ETYPE, "rope: rows are SMOE_F32, SMOE_F16 or SMOE_BF16");
     if (n_tokens == 0) return ok();
@@ -119,6 +121,7 @@ smoe_status smoe_kv_append(const smoe_kv* kv, const smoe_rope* r, const int32_t*
     if (s != SMOE_OK) return s;
     if (r && r->head_dim != kv->head_dim) return fail(SMOE_EINVAL, "kv_append: the rotary positions' head_dim is not the cache's");
     if (n_tokens < 0) return fail(SMOE_EINVAL, "kv_append: negative token count");
+    if (!rope_fits(n_tokens)) return fail(SMOE_EINVAL, "kv_append: the tokens exceed a launch's grid: split them");
     if (!elem_type(x_type)) return fail(SMOE_ETYPE, "kv_append: rows are SMOE_F32, SMOE_F16 or SMOE_BF16");
     if (!q != !q_out) return fail(SMOE_ENULL, "kv_append: q and q_out go together");
     if (q && !r) return fail(SMOE_EINVAL, "kv_append: queries without rotary positions");

@@ -5,6 +5,7 @@
 // angle of position 10^6 would be off by 0.03), the polynomials are in 32; the pair's products are fused, one rounding to the
 // output's type.
 #include "smoe_launch.hpp"
+#include "smoe_rules.hpp"
 #include "smoe_types.hpp"
 
 namespace smoe {
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(256) void k_rope(const RopeArgs a, int per) {
 namespace {
 template <int W>
 hipError_t launch_rope_as(const RopeArgs& a, int per, hipStream_t s) {
-    const dim3 grid((a.n_tokens + per - 1) / per);
+    const dim3 grid((unsigned)rope_groups(a.n_tokens));
     const size_t lds = (size_t)per * (a.rot / 2) * sizeof(float2);
     if (a.half) hipLaunchKernelGGL((k_rope<W, true>), grid, dim3(256), lds, s, a, per);
     else hipLaunchKernelGGL((k_rope<W, false>), grid, dim3(256), lds, s, a, per);
@@ -212,7 +213,7 @@ hipError_t launch_rope(const RopeArgs& a, hipStream_t s) {
         return a.rot % (2 * w) == 0 && a.head_dim % (2 * w) == 0 && rows(a.q, a.q_ld, a.x_type) && rows(a.q_out, a.q_out_ld, a.q_type) &&
                rows(a.k, a.k_ld, a.x_type) && rows(a.v, a.v_ld, a.x_type) && rows(a.k_pages, 0, a.t_type) && rows(a.v_pages, 0, a.t_type);
     };
-    const int per = a.n_tokens >= 2048 ? 4 : 1;
+    const int per = rope_tokens(a.n_tokens);
     if (fits(8)) return launch_rope_as<8>(a, per, s);
     if (fits(4)) return launch_rope_as<4>(a, per, s);
     if (fits(2)) return launch_rope_as<2>(a, per, s);

@@ -324,6 +324,11 @@ inline bool linear4_fits(int64_t T, int64_t K, int64_t N, bool pair, int) {
 // longer is the row's one group at any length, and n_in + group stays far below 2^31.
 constexpr int linear4_group(int group) { return group < kLinearMaxIn ? group : kLinearMaxIn; }
 
+// k_rope: the tokens of a work-group (4 of many, so that its sines serve enough values), and whether a launch holds them all.
+constexpr int rope_tokens(int64_t T) { return T >= 2048 ? 4 : 1; }
+constexpr int64_t rope_groups(int64_t T) { return (T + rope_tokens(T) - 1) / rope_tokens(T); }
+constexpr bool rope_fits(int64_t T) { return rope_groups(T) < kGridGroups; }
+
 // n / d for n < 2^31 as (mulhi(n, mul) + n) >> shift: shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.
 struct Divisor {
     uint32_t mul, shift;

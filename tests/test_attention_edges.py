@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import stratametal_amd as S
-from test_attention_refusals import attend, verdict
+from test_attention_refusals import append, attend, rope, verdict
 from test_dense_refusals import EINVAL
 from test_dispatch_rules import ask  # noqa: F401
 
@@ -65,3 +65,14 @@ def test_attend_join_reads_its_arrays(ask):  # noqa: F811
 def test_attend_scale_that_leaves_f32(scale):
     """Scores travel in units of ln 2: scale times log2 e has to be a number, too."""
     verdict(attend(scale=scale), EINVAL)
+
+
+def test_rope_launch_holds_its_tokens(ask):  # noqa: F811
+    """A launch has at most 2^32 - 1 threads, 256 to a work-group: more tokens are refused before one starts."""
+    sizes = [1, 2047, 2048, 2 ** 26 - 8, 2 ** 26 - 7, 2 ** 26, INT_MAX]
+    got = ask([e for T in sizes for e in (f"rope_groups({T}) * rope_tokens({T})", f"rope_groups({T})", f"rope_fits({T})")])
+    for T, held, groups, fits in zip(sizes, got[::3], got[1::3], got[2::3]):
+        assert T <= held < T + 4 and bool(fits) == (256 * groups < 2 ** 32 - 256)
+    for T in (2 ** 26, INT_MAX):
+        verdict(rope(T=T, x=1 << 40, y=1 << 50), EINVAL)
+        verdict(append(T=T, q=1 << 40, qo=1 << 42, k=1 << 44, v=1 << 46, slots=1 << 48, pos=1 << 50), EINVAL)
