@@ -79,6 +79,7 @@ smoe_status smoe_rope_table(int32_t rot_dim, double base, int32_t scaling, doubl
             f *= g + (1 - g) / factor;
         }
         turns[i] = f / kTurn;
+        if (!std::isfinite(turns[i])) return fail(SMOE_EINVAL, "rope_table: the frequencies leave 64 bits");
     }
     *scale = scaling == SMOE_ROPE_PARTS ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
     return ok();

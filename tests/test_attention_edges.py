@@ -1,5 +1,7 @@
 """CPU tests of the bounds that attention over a paged cache and the product with 4-bit weights keep at the edges of what their
 calls allow (test_gpu_attend_edges.py and test_gpu_linear4_edges.py run them)."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -76,3 +78,10 @@ def test_rope_launch_holds_its_tokens(ask):  # noqa: F811
     for T in (2 ** 26, INT_MAX):
         verdict(rope(T=T, x=1 << 40, y=1 << 50), EINVAL)
         verdict(append(T=T, q=1 << 40, qo=1 << 42, k=1 << 44, v=1 << 46, slots=1 << 48, pos=1 << 50), EINVAL)
+
+
+@pytest.mark.parametrize("args", [(64, 1e4, 1, 1e-320, 0, 0, 0), (64, 1e4, 2, 1e-320, 0, 0, 0), (64, 1e4, 3, 1e-320, 8192.0, 1, 32)])
+def test_rope_table_that_leaves_64_bits(args):
+    """Frequencies that are no numbers would turn every head to NaN."""
+    turns, scale = (C.c_double * 32)(), C.c_float()
+    verdict(S.lib().smoe_rope_table(*args, turns, C.byref(scale)), EINVAL)
