@@ -128,3 +128,32 @@ def test_weights_of_few_rows_keep_two_parts(new, lens, H, kv, D, t):
         want, e, _, _ = A.attend(q, b.keys[s], b.values[s], D ** -0.5, True, 0, "f32")
         size, *_ = A.attend(q, b.keys[s], np.abs(b.values[s]), D ** -0.5, True, 0, "f32")
         close(o[rows], want, e + 2.0 ** -16 * size + (np.abs(want) + e) * half + tiny)
+
+
+@pytest.mark.parametrize("n,L,H,kv,D", [(2048, 2048, 32, 8, 128), (2048, 2048, 16, 2, 256), (40, 6000, 32, 8, 128), (1, 30000, 8, 1, 64)])
+def test_a_nan_score_costs_no_second_pass(n, L, H, kv, D):
+    """A key of NaN that all rows see makes them NaN where they are summed: they are not done anew one after the other, which took 10 to
+    400 times the call (the bound is 3, of a least of five)."""
+    say(f"case: attend nan's cost n={n} L={L} H={H} D={D}")
+    b = Batch(n, [n], [L], H, kv, D, 16)
+    args = b.args()
+
+    def least():
+        us = []
+        for _ in range(5):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            for _ in range(4):
+                out = b.cache.attend(*args)
+            end.record()
+            end.synchronize()
+            us.append(start.elapsed_time(end) * 250)
+        return min(us), out
+
+    least()
+    clean, _ = least()
+    b.cache.k[int(b.table[0, 0]), :, 0] = float("nan")
+    b.cache.v[int(b.table[0, 0]), :, 0] = float("nan")
+    broken, out = least()
+    say(f"{clean:.0f} us, with NaN {broken:.0f}")
+    assert bool(out.isnan().all()) and broken <= 3 * clean
