@@ -266,6 +266,41 @@ __device__ __forceinline__ void redo_row(const AttendArgs& a, const AttendPlan& 
     }
     if (lane == 0) put_stats(a, p, row, w.split, top, sum);
 }
+// Values that are not finite and that a row's sums may hold 0 times: those of keys that some row of the work-group does not see,
+// the last and the first such key, and of the last key, which fills up the last block of 32.
+struct Broken {
+    int last, first;
+    bool filling;
+    // whether a row that sees the keys lo .. hi - 1 is touched
+    __device__ __forceinline__ bool touches(int lo, int hi) const { return last >= hi || first < lo || filling; }
+};
+__device__ __forceinline__ Broken broken_values(const AttendArgs& a, const Work& w, int lane) {
+    const int first_p = w.s.len - w.s.n + w.row0 / a.group, last_p = w.s.len - w.s.n + (w.row0 + w.rows - 1) / a.group;
+    const int hi = a.causal ? max(first_p + 1, w.k0) : w.k1, lo = min(first_seen(last_p, a.window), w.k1);
+    const int32_t* pages = a.pages + w.s.b * a.pages_ld;
+    const uint32_t top_bits = a.f16 ? 0x7C00u : 0x7F80u;  // an exponent of ones
+    const auto broken = [&](int key) {
+        const int page = pages[key / a.page_size];
+        if (page < 0 || page >= a.n_pages) return false;
+        const int64_t row = ((int64_t)page * a.n_kv + w.kvh) * a.page_size + key % a.page_size;
+        const u32x4* v = reinterpret_cast<const u32x4*>(a.v + row * (a.head_dim * 2));
+        bool some = false;
+        for (int i = 0; i < a.head_dim / 8; ++i) {
+            const u32x4 q = v[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) some |= (q[j] & top_bits) == top_bits || (q[j] >> 16 & top_bits) == top_bits;
+        }
+        return some;
+    };
+    Broken b = {-1, 0x7FFFFFFF, (w.k1 - w.k0) % 32 != 0 && broken(w.k1 - 1)};
+    const auto look = [&](int from, int to) {
+        for (int key = from + lane; key < to; key += 64)
+            if (broken(key)) b.last = max(b.last, key), b.first = min(b.first, key);
+    };
+    look(w.k0, lo), look(hi, w.k1);
+    for (int x = 32; x > 0; x >>= 1) b.last = max(b.last, __shfl_xor(b.last, x)), b.first = min(b.first, __shfl_xor(b.first, x));
+    return b;
+}
 // (a work-group without keys: its rows' tops say so)
 __device__ __forceinline__ bool no_keys(const AttendArgs& a, const AttendPlan& p, const Work& w, int threads) {
     if (w.k0 < w.k1) return false;
@@ -302,12 +337,13 @@ __device__ __forceinline__ void load_query(const AttendArgs& a, int t, int head,
 
 // A new key's weight may be up to 2^kLag times the top's before the sums are scaled to a new top.
 constexpr float kLag = 8.0f;
-// Weights are formed 2^LIFT times up and the sums brought back by 2^-LIFT (exact).  bf16 needs none; fp16 ones would lose a
-// weight below 2^-25 of the top's whole, and half a step of 2^-24 of others, from the values' sums but not from their own, and with
-// many equal keys behind one large score these losses add up: so as far up as the type allows (2^15 with the lag).
+// Weights are formed 2^LIFT times up and the sums brought back by 2^-LIFT (exact).  fp16 ones would lose a weight below 2^-25 of the
+// top's whole, and half a step of 2^-24 of others, from the values' sums but not from their own, and with many equal keys behind one
+// large score these losses add up: so as far up as the type allows (2^15 with the lag).  bf16 ones lose nothing, but beside values
+// near the type's largest must not pass 1.
 template <bool F16, bool LAG>
-constexpr float kLift = !F16 ? 0.0f : LAG ? 15.0f - kLag : 15.0f;
-constexpr float power_of_half(float n) { return n < 0.5f ? 1.0f : 0.5f * power_of_half(n - 1.0f); }
+constexpr int kLift = (F16 ? 15 : 0) - (LAG ? (int)kLag : 0);
+constexpr float two_to(int n) { return n == 0 ? 1.0f : n > 0 ? 2.0f * two_to(n - 1) : 0.5f * two_to(n + 1); }
 
 }  // namespace
 
@@ -329,7 +365,8 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = KEYS / RPI / 4;  // lanes to a row, rows of a load, a wave's loads of a tile
     constexpr int PLANE = KEYS * DIM * 2, HALF = PLANE / 2;
     constexpr bool HIGH = DIM > 128;  // the sums of values in accumulation registers
-    constexpr float LIFT = kLift<F16, true>, DROP = power_of_half(LIFT);
+    constexpr float LIFT = kLift<F16, true>, DROP = two_to(-kLift<F16, true>);
+    constexpr float PART = LIFT > 0.0f ? DROP : 1.0f;  // (a piece's sums are brought down, but not up: they could leave f32)
     __shared__ __align__(1024) uint8_t lds[4 * PLANE];  // two tiles of keys, two of values
     __shared__ int ids[4][64], rows_s[4][64];  // of a tile's keys: page numbers, then rows of the cache
     __shared__ int bad_page;
@@ -583,9 +620,9 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     if (bad) bad_page = 1;
     __syncthreads();
     if (!live) return;
-    const float inv = p.splits > 1 ? DROP : sum == 0.0f ? 0.0f : 1.0f / sum;
-    // what is not finite may come of a value that the query does not see (0 times it): such rows are done anew, but not where a
-    // score is NaN, which only one that it sees can be: then all values are (a NaN key that 2048 rows see, 32 heads: 25 ms of redone rows)
+    const float inv = p.splits > 1 ? PART : sum == 0.0f ? 0.0f : 1.0f / sum;
+    // what is not finite may come of a value that the query does not see (0 times it): rows that one touches are done anew (all of
+    // 2048 tokens, 32 heads: 25 ms).  Where a score is NaN, which only one that it sees can be, all values are NaN as they stand.
     const bool settled = sum != sum;
     bool lost = false;
     const int t = w.s.t0 + t_q;
@@ -612,8 +649,12 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
 #pragma unroll
                 for (int x = 0; x < 4; ++x) out[d + x] = f32_to_half_bits(v[x], F16 ? kF16 : kBf16);
         }
-    if (mine && h == 0) put_stats(a, p, row, w.split, top, sum * DROP);
+    if (mine && h == 0) put_stats(a, p, row, w.split, p.splits > 1 && LIFT < 0.0f ? top - LIFT : top, sum * (p.splits > 1 ? PART : DROP));
     uint64_t again = __ballot(mine && (lost || bad_page));
+    if (again && !bad_page) {
+        const Broken b = broken_values(a, w, lane);
+        again = __ballot(mine && lost && b.touches(lo, hi));
+    }
     again = (again | again >> 32) & 0xFFFFFFFFull;
     for (; again; again &= again - 1)
         redo_row(a, p, w, wave * 32 + __builtin_ctzll(again), reinterpret_cast<float*>(lds) + wave * kMaxDim, lane);
@@ -630,7 +671,7 @@ template <int DIM, bool F16>
 __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const AttendArgs a, const AttendPlan p) {
     constexpr int M = kAttendFewRows, NQ = DIM / 32, ND = DIM / 16, PLANE = 32 * DIM * 2;
     constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = 32 / RPI;  // lanes to a row, rows of a load, loads of a block
-    constexpr float LIFT = kLift<F16, false>, DROP = power_of_half(LIFT);
+    constexpr float LIFT = kLift<F16, false>, DROP = two_to(-kLift<F16, false>);
     static_assert(4 * ND * 1024 <= 8 * PLANE, "the waves' sums");
     __shared__ __align__(1024) uint8_t lds[8 * PLANE];
     __shared__ int32_t ids[4][2][64];
@@ -754,7 +795,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
     sum += __shfl_xor(sum, 16);
     sum = add_halves(sum);
     __syncthreads();  // (again_s is set, and every wave has read its blocks)
-    if (bad) atomicOr(&again_s, 0xFFFFu);
+    if (bad) atomicOr(&again_s, 0x1FFFFu);  // (bit 16: a page outside the cache)
     if (h == 0) stats_s[wave][r_q] = make_float2(top, sum);
     f32x4* const sums = reinterpret_cast<f32x4*>(lds);  // [wave][16 values][lane]
 #pragma unroll
@@ -772,8 +813,8 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
         sum = __builtin_fmaf(part_of[v], stats_s[v][r_q].y, sum);
     }
     const float inv = p.splits > 1 ? DROP : sum == 0.0f ? 0.0f : 1.0f / sum;
-    // what is not finite may come of a value that the query does not see (0 times it): such rows are done anew, but not where a
-    // score is NaN, which only one that it sees can be: then all values are (a NaN key that 2048 rows see, 32 heads: 25 ms of redone rows)
+    // what is not finite may come of a value that the query does not see (0 times it): rows that one touches are done anew (all of
+    // 2048 tokens, 32 heads: 25 ms).  Where a score is NaN, which only one that it sees can be, all values are NaN as they stand.
     const bool settled = sum != sum;
     bool lost = false;
     const int tok = w.s.t0 + t_q;
@@ -804,7 +845,12 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
     if (wave == 0 && mine && h == 0) put_stats(a, p, out_row, w.split, top, sum * DROP);
     if (mine && lost) atomicOr(&again_s, 1u << r_q);
     __syncthreads();
-    for (uint32_t again = again_s & ((1u << w.rows) - 1); again; again &= again - 1) {
+    uint32_t again = again_s & ((1u << w.rows) - 1);
+    if (again && !(again_s >> 16)) {
+        const Broken b = broken_values(a, w, lane);
+        again &= (uint32_t)__ballot(b.touches(lo, hi));  // (lanes 0 .. 15 have rows 0 .. 15)
+    }
+    for (; again; again &= again - 1) {
         const int r = __builtin_ctz(again);
         if (r % 4 == wave) redo_row(a, p, w, r, reinterpret_cast<float*>(lds) + wave * kMaxDim, lane);
     }

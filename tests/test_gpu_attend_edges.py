@@ -130,6 +130,21 @@ def test_weights_of_few_rows_keep_two_parts(new, lens, H, kv, D, t):
         close(o[rows], want, e + 2.0 ** -16 * size + (np.abs(want) + e) * half + tiny)
 
 
+def least(b, args):
+    """The least of five times of a call among others, in us after one untimed, and its result."""
+    b.cache.attend(*args)
+    us = []
+    for _ in range(5):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        for _ in range(4):
+            out = b.cache.attend(*args)
+        end.record()
+        end.synchronize()
+        us.append(start.elapsed_time(end) * 250)
+    return min(us), out
+
+
 @pytest.mark.parametrize("n,L,H,kv,D", [(2048, 2048, 32, 8, 128), (2048, 2048, 16, 2, 256), (40, 6000, 32, 8, 128), (1, 30000, 8, 1, 64)])
 def test_a_nan_score_costs_no_second_pass(n, L, H, kv, D):
     """A key of NaN that all rows see makes them NaN where they are summed: they are not done anew one after the other, which took 10 to
@@ -138,22 +153,79 @@ def test_a_nan_score_costs_no_second_pass(n, L, H, kv, D):
     b = Batch(n, [n], [L], H, kv, D, 16)
     args = b.args()
 
-    def least():
-        us = []
-        for _ in range(5):
-            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
-            start.record()
-            for _ in range(4):
-                out = b.cache.attend(*args)
-            end.record()
-            end.synchronize()
-            us.append(start.elapsed_time(end) * 250)
-        return min(us), out
-
-    least()
-    clean, _ = least()
+    clean, _ = least(b, args)
     b.cache.k[int(b.table[0, 0]), :, 0] = float("nan")
     b.cache.v[int(b.table[0, 0]), :, 0] = float("nan")
-    broken, out = least()
+    broken, out = least(b, args)
     say(f"{clean:.0f} us, with NaN {broken:.0f}")
     assert bool(out.isnan().all()) and broken <= 3 * clean
+
+
+@pytest.mark.parametrize("n,L,H,kv,D", [(2048, 2048, 32, 8, 128), (2048, 2048, 16, 2, 256), (40, 6000, 32, 8, 128), (1, 30000, 8, 1, 64)])
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_a_broken_value_costs_no_second_pass(n, L, H, kv, D, t):
+    """A value of inf that all rows see, in one place of the head, makes that place inf (or NaN, with a weight of 0) as it is summed: the
+    rows are not done anew one after the other, and the head's other values are as they were."""
+    say(f"case: attend broken value's cost n={n} L={L} H={H} D={D} {t}")
+    b = Batch(n, [n], [L], H, kv, D, 16, t)
+    args = b.args()
+    clean, _ = least(b, args)
+    want = b.cache.attend(*args)
+    b.cache.v[int(b.table[0, 0]), :, 3, 5] = float("inf")
+    broken, out = least(b, args)
+    say(f"{clean:.0f} us, with inf {broken:.0f}")
+    assert not bool(torch.isfinite(out[3:, :, 5]).any()) if n > 3 else not bool(torch.isfinite(out[:, :, 5]).any())
+    keep = [d for d in range(D) if d != 5]
+    assert bool(torch.isfinite(out[..., keep]).all()) and torch.equal(out[32:, :, keep], want[32:, :, keep])
+    assert broken <= 5 * clean  # (the first rows of a prompt, which do not see the key, are done anew)
+
+
+@pytest.mark.parametrize("n,L,H,kv,D", [(200, 200, 4, 2, 64), (700, 900, 32, 8, 128), (300, 400, 16, 2, 256), (20, 5000, 8, 2, 128), (3, 77, 4, 1, 256)])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_broken_values_reach_only_those_that_see_them(n, L, H, kv, D, window, t):
+    """Infinities in single places of the values at several keys, the last among them: a row has them where it sees the key, and
+    nothing else of them."""
+    say(f"case: attend broken values n={n} L={L} H={H} D={D} window={window} {t}")
+    b = Batch(n + D, [n], [L], H, kv, D, 16, t)
+    clean = host(b.run(window=window)[0])
+    places = {L - n: 1, L - n // 2 - 1: 2, L - n // 3 - 1: 3, L - 1: 4, max(L - n - 20, 0): 5, max(L - n - 60, 0): 6}
+    for key, d in places.items():
+        b.cache.v[int(b.table[0, key // 16]), kv - 1, key % 16, d] = float("inf")
+    o = host(b.run(window=window)[0])
+    g, p = H // kv, np.arange(L - n, L)
+    for d in range(D):
+        sees = np.zeros(n, bool)
+        for key, at in places.items():
+            if at == d:
+                sees |= (p >= key) & ((p - key < window) if window else True)
+        got, was = o[:, H - g:, d], clean[:, H - g:, d]
+        assert not np.isfinite(got[sees]).any() and np.isfinite(got[~sees]).all(), d
+        assert np.array_equal(o[:, :H - g, d], clean[:, :H - g, d])
+    rows = sorted({0, n // 3, n // 2, n - 1})
+    lo = [max(0, p[r] - window + 1) if window else 0 for r in rows]
+    for r, first in zip(rows, lo):
+        want, bound, _, _ = A.attend(host(b.q[r:r + 1, H - g:]), b.keys[0][first:p[r] + 1, -1:], b.values[0][first:p[r] + 1, -1:], D ** -0.5, False, 0, t)
+        fine = np.isfinite(o[r, H - g:])
+        assert (np.abs(o[r, H - g:] - want[0])[fine] <= bound[0][fine]).all()
+
+
+@pytest.mark.parametrize("n,L,H,kv,D", [(700, 900, 32, 8, 128), (1500, 1500, 32, 8, 64), (300, 2000, 16, 2, 256), (5, 3000, 8, 2, 128), (1, 300, 4, 1, 256)])
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_largest_values(n, L, H, kv, D, t):
+    """The type's largest values, one key to a place of the head, and scores that rise along the keys, so that the running top lags:
+    finite, as the formula's are."""
+    say(f"case: attend largest values n={n} L={L} H={H} D={D} {t}")
+    b = Batch(n + D, [n], [L], H, kv, D, 16, t)
+    top = float(torch.finfo(b.cache.v.dtype).max)
+    rng = np.random.default_rng(D)
+    for d in range(0, D, 5):
+        key = int(rng.integers(0, L))
+        b.cache.v[int(b.table[0, key // 16]), kv - 1, key % 16, d] = top if d % 2 else -top
+        b.values[0][key, kv - 1, d] = top if d % 2 else -top
+    o, _ = b.run()
+    g = H // kv
+    for r in sorted({0, n // 3, n // 2, n - 1}):
+        p = L - n + r + 1
+        want, bound, _, _ = A.attend(host(b.q[r:r + 1, H - g:]), b.keys[0][:p, -1:], b.values[0][:p, -1:], D ** -0.5, True, 0, t)
+        close(o[r:r + 1, H - g:], want, bound)
