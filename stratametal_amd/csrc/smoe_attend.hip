@@ -621,9 +621,10 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     __syncthreads();
     if (!live) return;
     const float inv = p.splits > 1 ? PART : sum == 0.0f ? 0.0f : 1.0f / sum;
-    // what is not finite may come of a value that the query does not see (0 times it): rows that one touches are done anew (all of
-    // 2048 tokens, 32 heads: 25 ms).  Where a score is NaN, which only one that it sees can be, all values are NaN as they stand.
-    const bool settled = sum != sum;
+    // What is not finite may come of a value that the query does not see (0 times it): rows that one touches are done anew (all of
+    // 2048 tokens, 32 heads: 25 ms).  Where a score is NaN, which only one that it sees can be, all values are NaN as they stand, if
+    // the head fills the tile: behind a shorter one the key's last values stand again, and 0 times an infinite one is NaN as well.
+    const bool odd_score = sum != sum, settled = odd_score && a.head_dim == DIM;
     bool lost = false;
     const int t = w.s.t0 + t_q;
     const int64_t row = (int64_t)t * a.n_heads + head;
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     uint64_t again = __ballot(mine && (lost || bad_page));
     if (again && !bad_page) {
         const Broken b = broken_values(a, w, lane);
-        again = __ballot(mine && lost && b.touches(lo, hi));
+        again = __ballot(mine && lost && (odd_score || b.touches(lo, hi)));
     }
     again = (again | again >> 32) & 0xFFFFFFFFull;
     for (; again; again &= again - 1)
@@ -813,9 +814,10 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
         sum = __builtin_fmaf(part_of[v], stats_s[v][r_q].y, sum);
     }
     const float inv = p.splits > 1 ? DROP : sum == 0.0f ? 0.0f : 1.0f / sum;
-    // what is not finite may come of a value that the query does not see (0 times it): rows that one touches are done anew (all of
-    // 2048 tokens, 32 heads: 25 ms).  Where a score is NaN, which only one that it sees can be, all values are NaN as they stand.
-    const bool settled = sum != sum;
+    // What is not finite may come of a value that the query does not see (0 times it): rows that one touches are done anew (all of
+    // 2048 tokens, 32 heads: 25 ms).  Where a score is NaN, which only one that it sees can be, all values are NaN as they stand, if
+    // the head fills the tile: behind a shorter one the key's last values stand again, and 0 times an infinite one is NaN as well.
+    const bool odd_score = sum != sum, settled = odd_score && a.head_dim == DIM;
     bool lost = false;
     const int tok = w.s.t0 + t_q;
     const int64_t out_row = (int64_t)tok * a.n_heads + head;
@@ -848,7 +850,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
     uint32_t again = again_s & ((1u << w.rows) - 1);
     if (again && !(again_s >> 16)) {
         const Broken b = broken_values(a, w, lane);
-        again &= (uint32_t)__ballot(b.touches(lo, hi));  // (lanes 0 .. 15 have rows 0 .. 15)
+        again &= (uint32_t)__ballot(odd_score || b.touches(lo, hi));  // (lanes 0 .. 15 have rows 0 .. 15)
     }
     for (; again; again &= again - 1) {
         const int r = __builtin_ctz(again);

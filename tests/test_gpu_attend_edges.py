@@ -229,3 +229,31 @@ def test_largest_values(n, L, H, kv, D, t):
         p = L - n + r + 1
         want, bound, _, _ = A.attend(host(b.q[r:r + 1, H - g:]), b.keys[0][:p, -1:], b.values[0][:p, -1:], D ** -0.5, True, 0, t)
         close(o[r:r + 1, H - g:], want, bound)
+
+
+@pytest.mark.parametrize("n,L,H,kv", [(1, 90, 4, 2), (3, 5000, 4, 2), (40, 300, 4, 2), (700, 900, 32, 8), (1024, 2100, 16, 2)])
+@pytest.mark.parametrize("D", [24, 64, 80, 96, 128, 200, 256])
+def test_keys_of_minus_infinity(n, L, H, kv, D):
+    """A key that is -inf in the head's last value: a weight of 0 for queries above 0 there, NaN for those below, whatever lies between
+    the head's size and the tile's."""
+    say(f"case: attend keys of -inf n={n} L={L} H={H} kv={kv} D={D}")
+    b = Batch(n + D, [n], [L], H, kv, D, 16)
+    b.q = b.q.clone()
+    b.q[..., D - 1] = b.q[..., D - 1].abs() + 0.5
+    below = n // 2
+    if n > 1:
+        b.q[below, :, D - 1] *= -1
+    gone = [L - n, max(L - n - 40, 0)]
+    for key in gone:
+        b.cache.k[int(b.table[0, key // 16]), :, key % 16, D - 1] = -float("inf")
+    o, lse = b.run()
+    if n > 1:
+        assert bool(o[below].isnan().all()) and bool(lse[below].isnan().all())
+    g = H // kv
+    for r in sorted({0, n // 3, n - 1} - ({below} if n > 1 else set())):
+        p = L - n + r + 1
+        keep = [j for j in range(p) if j not in gone]
+        for h in ([0, kv - 1] if keep else []):
+            want, bound, wl, el = A.attend(host(b.q[r:r + 1, h * g:(h + 1) * g]), b.keys[0][keep, h:h + 1], b.values[0][keep, h:h + 1], D ** -0.5, False, 0, "bf16")
+            close(o[r:r + 1, h * g:(h + 1) * g], want, bound)
+            assert (np.abs(host(lse[r:r + 1, h * g:(h + 1) * g]) - wl) <= el).all()
