@@ -70,3 +70,18 @@ def test_groups_longer_than_any_row(T, K, N, group, pair):
     two = dict(w2=layer[1]["w"], scales2=layer[1]["scales"], zeros2=layer[1]["zeros"]) if pair else {}
     y = S.Linear4(K, N, layer[0]["w"], layer[0]["scales"], zeros=layer[0]["zeros"], group=group, **two).run(x, y_dtype=torch.float32)
     check(x, None, layer, K, "none", y, "f32")
+
+
+@pytest.mark.parametrize("T", [1, 3, 16, 40, 300])
+@pytest.mark.parametrize("first", [False, True])
+def test_zeros_and_bias_of_one_matrix_alone(T, first):
+    """A gated pair of which one matrix has zeros and a bias of its own, the other neither."""
+    say(f"case: linear4 one of two T={T} first={first}")
+    K, N, group = 416, 70, 96
+    x, r, _, layer = make(T, T, K, N, group, pair=True, bias=True, residual="f32")
+    bare = layer[1 if first else 0]
+    bare["zeros"] = bare["bias"] = None
+    a, b = layer
+    L = S.Linear4(K, N, a["w"], a["scales"], zeros=a["zeros"], group=group, bias=a["bias"], w2=b["w"], scales2=b["scales"], zeros2=b["zeros"],
+                  bias2=b["bias"], act=S.ACT_SILU)
+    check(x, r, layer, group, "silu", L.run(x, residual=r), "f32")
