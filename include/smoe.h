@@ -364,13 +364,15 @@ smoe_status smoe_kv_append(const smoe_kv* kv, const smoe_rope* r, const int32_t*
  * pages[b][j / page_size].  Its i-th query has position p = kv_len - n + i and sees, `causal`, keys j <= p, and with a window
  * (> 0) those with j > p - window; not causal, all keys (window 0).  With head h reading key head h / (n_heads / n_kv_heads):
  *   out = sum_j w_j v_j,  w = softmax of scale q k_j over the keys it sees,  lse = ln sum_j exp(scale q k_j).
- * A query that sees no key: zeros and -inf.  What a query does not see does not reach it, NaN or not; keys of a page outside
- * the cache, and those past max_len, are not there, and positions go by kv_len all the same (kv_len is read on the device; max_len, at most max_pages * page_size, is
- * the longest that the launch is made for).  Scores and sums are f32; the weights are rounded to the cache's type for the
- * second product.  q and out [n_tokens][n_heads][head_dim] of the cache's type, tokens q_ld and out_ld values apart (q 16-byte
- * aligned, q_ld a multiple of 8); lse [n_tokens][n_heads] f32 or NULL.  Rows before the first sequence and behind the last one
- * are left as they are.  `workspace` (256-byte aligned, apart from every operand, of the bytes for the call's own sizes: they do
- * not only grow with them): concurrent calls need distinct ones.  The same bits in every run. */
+ * A query that sees no key: zeros and -inf.  What a query does not see does not reach it, NaN or not; a NaN that it sees does.
+ * Keys of a page outside the cache, and those past max_len, are not there, and positions go by kv_len all the same (kv_len is read
+ * on the device; max_len, at most max_pages * page_size, is the longest that the launch is made for).  Scores and sums are f32;
+ * for the second product a weight is rounded to the cache's type where a call has many query rows, and held in two numbers of
+ * it where it has few.  scale and scale log2 e are finite.  q and out [n_tokens][n_heads][head_dim] of the cache's type,
+ * tokens q_ld and out_ld values apart (q 16-byte aligned, q_ld a multiple of 8); lse [n_tokens][n_heads] f32 or NULL.  Rows
+ * before the first sequence and behind the last one are left as they are.  `workspace` (256-byte aligned, apart from every
+ * operand, of the bytes for the call's own sizes: they do not only grow with them): concurrent calls need distinct ones.  The
+ * same bits in every run. */
 size_t smoe_attend_workspace_bytes(const smoe_kv* kv, int32_t n_heads, int32_t n_tokens, int32_t n_seqs, int64_t max_len,
                                    int32_t window);
 smoe_status smoe_attend(const smoe_kv* kv, const void* q, int64_t q_ld, int32_t n_tokens, int32_t n_heads,

@@ -1083,8 +1083,8 @@ class PagedCache:
                lse: bool = False, max_len: Optional[int] = None, out=None, stream=None):
         """out (tokens, heads, head_dim): attention of q's rows q_start[b] .. q_start[b + 1] - 1 over the first kv_len[b] keys of
         the pages pages[b] (smoe_attend), `scale` None: head_dim ** -0.5; with `lse` (out, lse (tokens, heads) f32).  q_start
-        (sequences + 1,), kv_len (sequences,) and pages (sequences, most pages) are int32 tensors; max_len bounds kv_len (None:
-        what the pages hold): the tighter, the fewer empty work-groups.  Rows of no sequence are left as they are (new outputs: any
+        (sequences + 1,), kv_len (sequences,) and pages (sequences, most pages) are int32 tensors; keys past max_len (None: what
+        the pages hold) are not there: the tighter it is, the fewer empty work-groups.  Rows of no sequence are left as they are (new outputs: any
         values)."""
         import torch
         dev, D = self._device, self.head_dim

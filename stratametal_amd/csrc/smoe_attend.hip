@@ -356,9 +356,12 @@ constexpr float two_to(int n) { return n == 0 ? 1.0f : n > 0 ? 2.0f * two_to(n -
 // instructions, and while its values are, the next top; what each instruction needs of LDS is read two or three before.  A
 // tile of keys starts a step before the tile of values of the same number, so that two steps work on one tile of each while
 // the keys of the tile after next and the values of the next travel to LDS, page numbers a tile before them.
-// 8192 tokens, 32 heads of 128, 8 key heads: 572 to 589 us, 950 TFLOP/s; bound by its parts together: without exponentials 35 us less
-// of 640, without weights 62, without the reads of LDS 103, without the second product 116, without loads 95.  Tiles of 256 rows
-// took 645 to 706 for 587 (one work-group to a CU).
+// A weight is rounded to the cache's type for the second product (its sum is not), off by half a step: the error against 64 bits grows
+// from 1.6 to 2.1 parts in 1000, where the output's own rounding is 1.6.  With what the rounding leaves as a second operand, as in
+// k_attend_few, the prompt below took 803 us for 586, 1024 tokens over 33792 keys 880 for 609.
+// 8192 tokens, 32 heads of 128, 8 key heads: 575 to 588 us, 935 to 955 TFLOP/s; bound by its parts together: without exponentials 35
+// us less of 640, without weights 62, without the reads of LDS 103, without the second product 116, without loads 95.  Tiles of 256
+// rows took 645 to 706 for 587 (one work-group to a CU).
 template <int DIM, bool F16>
 __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const AttendArgs a, const AttendPlan p) {
     constexpr int M = kAttendRows, KEYS = kAttendKeys, ND = DIM / 32, NQ = DIM / 16;
@@ -664,10 +667,11 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
 // Sequences of few query rows: tiles of 16 rows, four waves each on every fourth block of 32 keys, by itself until the waves' sums
 // meet in LDS.  A block's keys and values travel to the wave's own LDS, the next block's as soon as this one's have been
 // read, page numbers two blocks ahead.  The transposed scores (v_mfma_f32_16x16x32: keys by queries) leave a lane with 8 keys of
-// one query, which are the second product's right operand as they are, with the keys in that order (read_columns).
-// Bound by the cache's bytes where there are many (56 tokens of 64 sequences of up to 8193 keys, 8 key heads of 128: 177 us, 5.4 TB/s,
-// part of it from the Infinity Cache; one token over 131072 keys, 4 key heads 51 us), else by the trips to memory before them (one token
-// over 1001 keys, 2 key heads of 256: 9 us).  Waves that share blocks, in tiles of 128 rows, took 201, 57 and 15.
+// one query, which are the second product's right operand as they are, with the keys in that order (read_columns), in two numbers of
+// the cache's type: the matrix instructions have the time (single tokens took as long with one; 796 with a window 10.2 us for 10.7).
+// Bound by the cache's bytes where there are many (56 tokens of 64 sequences of up to 8193 keys, 8 key heads of 128: 179 us, 5.3 TB/s,
+// part of it from the Infinity Cache; one token over 131072 keys, 4 key heads 52 us), else by the trips to memory before them (one token
+// over 1001 keys, 2 key heads of 256: 10 us).  Waves that share blocks, in tiles of 128 rows, took 201, 57 and 15.
 template <int DIM, bool F16>
 __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const AttendArgs a, const AttendPlan p) {
     constexpr int M = kAttendFewRows, NQ = DIM / 32, ND = DIM / 16, PLANE = 32 * DIM * 2;

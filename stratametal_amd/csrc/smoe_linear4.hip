@@ -101,7 +101,7 @@ __device__ __forceinline__ f32x4 four_scales(const uint32_t* p, int type) {
 // load one line's half (piece p of row r at place p ^ (r >> 2), and the dwords that a matrix instruction takes of 16 rows
 // cover the 64 banks once), the tokens' values, and the scales and zeros of its up to four groups.  Lanes past the last token
 // hold its values, and their results are dropped; the waves' sums meet in LDS, in wave order.  Bound by the latency of a wave's few
-// stages: one token, 2 x 8192 rows of 2048, groups of 128, 8.1 us; 16 tokens, 2048 rows of 8192, groups of 64, 10.5 us (14.9 with
+// stages: one token, 2 x 8192 rows of 2048, groups of 128, 8.2 us; 16 tokens, 2048 rows of 8192, groups of 64, 10.6 us (14.9 with
 // stages of more than one group in a loop).
 template <bool PAIR, bool F16, int TOKENS>
 __global__ __launch_bounds__(512, 4) void k_linear4_few(const Linear4Args a) {
