@@ -81,7 +81,8 @@ __device__ __forceinline__ void row_alone(const AttendArgs& a, const Sequence& s
 }
 
 __device__ __forceinline__ float lse_of(float top, float sum) {
-    return sum == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    // (sums are up to 2^15 times those of weights of at most 1: the powers of two meet `top` by themselves)
+    return sum == 0.0f ? -__builtin_inff() : (top + (float)__builtin_amdgcn_frexp_expf(sum) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sum))) * kLn2;
 }
 
 // ------------------------------------------------------------------------------------------------ tiles
@@ -337,13 +338,15 @@ __device__ __forceinline__ void load_query(const AttendArgs& a, int t, int head,
 
 // A new key's weight may be up to 2^kLag times the top's before the sums are scaled to a new top.
 constexpr float kLag = 8.0f;
-// Weights are formed 2^LIFT times up and the sums brought back by 2^-LIFT (exact).  fp16 ones would lose a weight below 2^-25 of the
-// top's whole, and half a step of 2^-24 of others, from the values' sums but not from their own, and with many equal keys behind one
-// large score these losses add up: so as far up as the type allows (2^15 with the lag).  bf16 ones lose nothing, but beside values
-// near the type's largest must not pass 1.
+// What weights are relative to: the top less LIFT, a weight 2^LIFT times up.  fp16 ones would lose a weight below 2^-25 of the top's
+// whole, and half a step of 2^-24 of others, from the values' sums but not from their own, and with many equal keys behind one large
+// score these losses add up: so as far up as the type allows (2^15 with the lag), while a step of f32 in the scores is at most a
+// quarter.  bf16 ones lose nothing, but beside values near the type's largest must not pass 1.
 template <bool F16, bool LAG>
-constexpr int kLift = (F16 ? 15 : 0) - (LAG ? (int)kLag : 0);
-constexpr float two_to(int n) { return n == 0 ? 1.0f : n > 0 ? 2.0f * two_to(n - 1) : 0.5f * two_to(n + 1); }
+__device__ __forceinline__ float base_of(float top) {
+    constexpr float LIFT = (F16 ? 15.0f : 0.0f) - (LAG ? kLag : 0.0f);
+    return top == -__builtin_inff() ? 0.0f : F16 && !(__builtin_fabsf(top) < 4194304.0f) ? top : top - LIFT;
+}
 
 }  // namespace
 
@@ -368,8 +371,6 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = KEYS / RPI / 4;  // lanes to a row, rows of a load, a wave's loads of a tile
     constexpr int PLANE = KEYS * DIM * 2, HALF = PLANE / 2;
     constexpr bool HIGH = DIM > 128;  // the sums of values in accumulation registers
-    constexpr float LIFT = kLift<F16, true>, DROP = two_to(-kLift<F16, true>);
-    constexpr float PART = LIFT > 0.0f ? DROP : 1.0f;  // (a piece's sums are brought down, but not up: they could leave f32)
     __shared__ __align__(1024) uint8_t lds[4 * PLANE];  // two tiles of keys, two of values
     __shared__ int ids[4][64], rows_s[4][64];  // of a tile's keys: page numbers, then rows of the cache
     __shared__ int bad_page;
@@ -448,10 +449,10 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     // the top, when a score has passed it: then the sums of values are to be scaled by `keep`
     float keep = 1.0f;
     const auto raise = [&](float m) {
-        const float next = __builtin_fmaxf(top, max_halves(m) * scale);
-        keep = next == top ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+        const float next = __builtin_fmaxf(top, max_halves(m) * scale), old = base;
+        base = base_of<F16, true>(next);
+        keep = next == top ? 1.0f : top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(old - base);
         top = next;
-        base = top == -__builtin_inff() ? 0.0f : top - LIFT;
         sum *= keep, odd_sum *= keep;
     };
     const auto passed = [&](float m) { return __ballot(m * scale > top + kLag) != 0; };
@@ -623,7 +624,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
     if (bad) bad_page = 1;
     __syncthreads();
     if (!live) return;
-    const float inv = p.splits > 1 ? PART : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = p.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
     // What is not finite may come of a value that the query does not see (0 times it): rows that one touches are done anew (all of
     // 2048 tokens, 32 heads: 25 ms).  Where a score is NaN, which only one that it sees can be, all values are NaN as they stand, if
     // the head fills the tile: behind a shorter one the key's last values stand again, and 0 times an infinite one is NaN as well.
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_tile(const At
 #pragma unroll
                 for (int x = 0; x < 4; ++x) out[d + x] = f32_to_half_bits(v[x], F16 ? kF16 : kBf16);
         }
-    if (mine && h == 0) put_stats(a, p, row, w.split, p.splits > 1 && LIFT < 0.0f ? top - LIFT : top, sum * (p.splits > 1 ? PART : DROP));
+    if (mine && h == 0) put_stats(a, p, row, w.split, top == -__builtin_inff() ? top : base, sum);
     uint64_t again = __ballot(mine && (lost || bad_page));
     if (again && !bad_page) {
         const Broken b = broken_values(a, w, lane);
@@ -676,7 +677,6 @@ template <int DIM, bool F16>
 __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const AttendArgs a, const AttendPlan p) {
     constexpr int M = kAttendFewRows, NQ = DIM / 32, ND = DIM / 16, PLANE = 32 * DIM * 2;
     constexpr int LPR = DIM / 8, RPI = 64 / LPR, LOADS = 32 / RPI;  // lanes to a row, rows of a load, loads of a block
-    constexpr float LIFT = kLift<F16, false>, DROP = two_to(-kLift<F16, false>);
     static_assert(4 * ND * 1024 <= 8 * PLANE, "the waves' sums");
     __shared__ __align__(1024) uint8_t lds[8 * PLANE];
     __shared__ int32_t ids[4][2][64];
@@ -760,8 +760,10 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
         m = max_halves(max_quarters(m));
         const float next = __builtin_fmaxf(top, m * scale);
         if (__ballot(next != top)) {
-            const float keep = next == top ? 1.0f : __builtin_amdgcn_exp2f(top - next);
-            top = next, base = top == -__builtin_inff() ? 0.0f : top - LIFT;
+            const float old = base;
+            base = base_of<F16, false>(next);
+            const float keep = next == top ? 1.0f : top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(old - base);
+            top = next;
             sum *= keep;
 #pragma unroll
             for (int i = 0; i < ND; ++i) acc[i] *= keep;
@@ -801,7 +803,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
     sum = add_halves(sum);
     __syncthreads();  // (again_s is set, and every wave has read its blocks)
     if (bad) atomicOr(&again_s, 0x1FFFFu);  // (bit 16: a page outside the cache)
-    if (h == 0) stats_s[wave][r_q] = make_float2(top, sum);
+    if (h == 0) stats_s[wave][r_q] = make_float2(top == -__builtin_inff() ? top : base, sum);
     f32x4* const sums = reinterpret_cast<f32x4*>(lds);  // [wave][16 values][lane]
 #pragma unroll
     for (int i = 0; i < ND; ++i) sums[(wave * ND + i) * 64 + lane] = acc[i];
@@ -817,7 +819,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
         part_of[v] = __builtin_amdgcn_exp2f(stats_s[v][r_q].x - base);
         sum = __builtin_fmaf(part_of[v], stats_s[v][r_q].y, sum);
     }
-    const float inv = p.splits > 1 ? DROP : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = p.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
     // What is not finite may come of a value that the query does not see (0 times it): rows that one touches are done anew (all of
     // 2048 tokens, 32 heads: 25 ms).  Where a score is NaN, which only one that it sees can be, all values are NaN as they stand, if
     // the head fills the tile: behind a shorter one the key's last values stand again, and 0 times an infinite one is NaN as well.
@@ -848,7 +850,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void k_attend_few(const Att
 #pragma unroll
             for (int x = 0; x < 4; ++x) out[d + x] = f32_to_half_bits(y[x], F16 ? kF16 : kBf16);
     }
-    if (wave == 0 && mine && h == 0) put_stats(a, p, out_row, w.split, top, sum * DROP);
+    if (wave == 0 && mine && h == 0) put_stats(a, p, out_row, w.split, top, sum);
     if (mine && lost) atomicOr(&again_s, 1u << r_q);
     __syncthreads();
     uint32_t again = again_s & ((1u << w.rows) - 1);

@@ -257,3 +257,34 @@ def test_keys_of_minus_infinity(n, L, H, kv, D):
             want, bound, wl, el = A.attend(host(b.q[r:r + 1, h * g:(h + 1) * g]), b.keys[0][keep, h:h + 1], b.values[0][keep, h:h + 1], D ** -0.5, False, 0, "bf16")
             close(o[r:r + 1, h * g:(h + 1) * g], want, bound)
             assert (np.abs(host(lse[r:r + 1, h * g:(h + 1) * g]) - wl) <= el).all()
+
+
+@pytest.mark.parametrize("n,L,H,kv", [(1, 300, 4, 1), (3, 9000, 4, 2), (700, 900, 32, 8), (1024, 2100, 16, 2)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("t,size", [("fp16", 2.0 ** 8), ("fp16", 2.0 ** 9), ("fp16", 2.0 ** 10), ("bf16", 2.0 ** 9), ("bf16", 2.0 ** 11)])
+def test_far_scores(n, L, H, kv, D, t, size):
+    """Scores of 2^22 to 2^28, where a step of f32 is up to 16: keys that rise along the sequence by more than such a step to each, so
+    that a query's weight is its last key's and those equal to it, and the answer their values' mean: off by a weight's rounding and its
+    own, half a step each, and f32's sum of some hundred."""
+    say(f"case: attend far scores n={n} L={L} H={H} kv={kv} D={D} {t} {size}")
+    b = Batch(n + D, [n], [L], H, kv, D, 16, t)
+    q = torch.zeros_like(b.q)
+    q[..., :64] = size
+    b.q = q
+    k = np.zeros((L, D), np.float32)
+    steps = size * (np.linspace(0.5, 1.0, 64 * 100)[-1 - np.arange(L)[::-1] % 6400] if L > 6400 else np.linspace(0.5, 1.0, L))
+    k[:, :64] = torch.from_numpy(steps.astype(np.float32)).to(b.cache.k.dtype).float().numpy()[:, None]
+    rows = torch.from_numpy(k).to(b.cache.k.dtype).cuda()
+    slots = torch.from_numpy(np.concatenate([p * 16 + np.arange(16) for p in b.table[0][:-(-L // 16)]])[:L].astype(np.int64)).cuda()
+    v = torch.from_numpy(b.values[0]).to(b.cache.v.dtype).cuda()
+    b.cache.append(rows[:, None].expand(L, kv, D).contiguous(), v, slots)
+    o, lse = b.run(scale=1.0)
+    s = k.astype(np.float64)[:, 0] * size * 64
+    g = H // kv
+    for r in sorted({0, n // 3, n - 1}):
+        p = L - n + r + 1
+        w = np.exp(s[:p] - s[:p].max())  # (keys as near as rounding left them are equal)
+        assert np.all((w == 1) | (w < 1e-12))
+        want = np.repeat((w @ b.values[0][:p].astype(np.float64).reshape(p, -1) / w.sum()).reshape(kv, D), g, axis=0)
+        bound = np.abs(want) * 2.0 ** -7 + 2.0 ** -12
+        close(o[r], want, bound)
